@@ -43,8 +43,9 @@ const char* tfb_last_error(void);
 int64_t tfb_launch_count(void);
 /* Device-side status word of the library on the calling thread's CURRENT device (one word per GPU,
  * shared by every kernel of the library): 0, or the code of the first bounded wait that expired
- * (0x2xxx attention backward, 0x5xxx attention forward, 0x1xxx / 0x3xxx GEMM, 0x7e00 the test probe)
- * or 0x7100 for a token id outside the embedding table.  While it is non-zero the tcgen05 kernels
+ * (0x2xxx attention backward, 0x5xxx attention forward, 0x8xxx prompt mass, 0x1xxx / 0x3xxx GEMM, 0x7e00 the test probe)
+ * or 0x7100 for a token id outside the embedding table, 0x7200 / 0x7201 for a page id / a length that
+ * does not fit a paged cache (below).  While it is non-zero the tcgen05 kernels
  * (GEMM, attention) return at once without writing their outputs; the other kernels still run.
  * Synchronises the device; call it where the host synchronises anyway (the loss read-back).
  * reset != 0 clears the word; the caller must then also zero its GEMM workspaces, whose arrival
@@ -302,6 +303,72 @@ int tfb_adamw_step_many(const void* const* grads, void* const* params, float* co
  * (torch.amp.GradScaler.update's rule).  Clears *found_inf.                                                 */
 int tfb_loss_scale_update(float* state4, int* found_inf, float growth, float backoff, int interval,
                           void* stream);
+
+/* ------------------------------------------------------------------- paged key-value cache
+ * No counterpart in the reference, which trains only: what generating text with the trained model needs.
+ *
+ * The cache of a layer is a pool of pages, k_pages and v_pages (num_pages, kv_heads, page, hd) with element strides
+ * page_strides = {page, head, slot} that both share (multiples of 8, unit stride on hd, 16-byte aligned bases), and for
+ * eviction two statistics per (page, head, slot), both contiguous: the key's accumulated attention `mass` (fp32) and its
+ * position in the text `positions` (int32; NULL: a key's position is its slot's number).  Slot s of sequence b lies in page
+ * tables[b * table_ld + s / page] at row s % page; a sequence has at most width * page slots.  Entries of a table that no
+ * slot in use refers to are never read.  lengths (B,) int32 lives on the device: nothing synchronises the host.
+ * A page id outside the cache reads as rows of zeros, or is not written, and sets 0x7200 in tfb_device_status(); a length that
+ * is negative or beyond the table is taken as the nearest one that is not, and sets 0x7201.
+ * Query head h uses key head h / group.  hd is 32, 64 or 128.
+ *
+ * tfb_paged_attention: out (B, kv_heads * group, hd) = attention of one query per sequence over its lengths[b] keys.  With k_new
+ * and v_new (B, kv_heads, hd), the new token's, it is over those and the new key, whose row is written into slot lengths[b].
+ * No keys: zeros.  slopes and alibi_round as in tfb_attention_fwd, with distance query_positions[b] - position of the key
+ * (query_positions NULL: the number of the last slot); a new key's position is the query's.  With mass and mass_out (the same
+ * buffer, or another one of its shape) mass_out = mass + the key's weights, summed over the query heads of its key head, in the
+ * slots in use; a new key starts from zero.  group <= 128.  Strides {b, h} in elements, unit stride on hd, any alignment.
+ * scratch needs no initialisation.                                                                            */
+int64_t tfb_paged_attention_scratch_bytes(int64_t B, int64_t kv_heads, int64_t group, int64_t hd, int64_t capacity,
+                                          int with_mass);
+int tfb_paged_attention(const void* q, const void* k_new, const void* v_new, void* out, void* k_pages, void* v_pages,
+                        const int* tables, const int* lengths, const int* query_positions, int* positions,
+                        const float* mass, float* mass_out, const float* slopes, int alibi_round, int64_t B,
+                        int64_t kv_heads, int64_t group, int64_t hd, int64_t num_pages, int64_t page, int64_t width,
+                        int64_t table_ld, const int64_t* page_strides, const int64_t* q_strides,
+                        const int64_t* k_new_strides, const int64_t* v_new_strides, const int64_t* o_strides,
+                        void* scratch, int64_t scratch_bytes, int dtype, void* stream);
+
+/* Key and value rows of prompts into the pages: key, value (B, kv_heads, T, hd) with strides {b, h, t}; the first counts[b]
+ * (NULL: all T) of them go into the slots from lengths[b] on.  mass (may be NULL) gets key_mass (B, kv_heads, T; strides {b, h};
+ * NULL: zero), positions (may be NULL) first_positions[b] + t (NULL: the slot's number).                       */
+int tfb_cache_append(const void* key, const void* value, void* k_pages, void* v_pages, const int* tables,
+                     const int* lengths, const int* counts, const int* first_positions, float* mass, int* positions,
+                     const float* key_mass, int64_t B, int64_t kv_heads, int64_t T, int64_t hd, int64_t num_pages,
+                     int64_t page, int64_t width, int64_t table_ld, const int64_t* page_strides,
+                     const int64_t* key_strides, const int64_t* value_strides, const int64_t* key_mass_strides,
+                     int dtype, void* stream);
+
+/* The attention mass of a prompt's keys: out (B, kv_heads, T) contiguous = sum over the query heads h of the key head and
+ * the queries i with j <= i < counts[b] (NULL: T) of exp(s_hij - lse[b,h,i]), s the scaled and biased scores of
+ * tfb_attention_fwd and lse (strides {b, h}, unit stride on T) its log-sum-exp; zero for keys from counts[b] on.  q (B, kv_heads *
+ * group, T, hd) and k (B, kv_heads, T, hd) with strides {b, h, t}, positive multiples of 8, and 16-byte aligned bases.
+ * Any T from 1 to 2^23.                                                                                      */
+int64_t tfb_prompt_mass_scratch_bytes(int64_t B, int64_t kv_heads, int64_t T);
+int tfb_prompt_mass(const void* q, const void* k, const float* lse, const int* counts, const float* slopes,
+                    int alibi_round, float* out, int64_t B, int64_t kv_heads, int64_t group, int64_t T, int64_t hd,
+                    const int64_t* q_strides, const int64_t* k_strides, const int64_t* lse_strides, void* scratch,
+                    int64_t scratch_bytes, int dtype, void* stream);
+
+/* Eviction: every (sequence, key head) of more than `keep` keys keeps the `keep` of the largest mass, where a key whose position
+ * is at least next_positions[b] - recent (NULL: lengths[b] - recent) counts as one of infinite mass and a mass that is no number as
+ * one of -infinity; ties go to the lower slot.  Keys that stay and lie before slot `keep` stay in their slots; those from behind fill
+ * the slots that become free, in the order of their slots.  left[b] = min(lengths[b], keep) is the new length (left may be
+ * lengths).  The outputs, each with its statistics, are either the inputs (and out_tables = tables: in place; no page may then be
+ * part of two sequences) or other buffers of the same kv_heads and hd, which get every slot that is left.  keep >= recent. */
+int64_t tfb_cache_evict_scratch_bytes(int64_t B, int64_t kv_heads, int64_t keep);
+int tfb_cache_evict(const void* k_pages, const void* v_pages, const float* mass, const int* positions,
+                    const int* tables, const int* lengths, const int* next_positions, void* k_out, void* v_out,
+                    float* mass_out, int* positions_out, const int* out_tables, int* left, int64_t B,
+                    int64_t kv_heads, int64_t hd, int64_t keep, int64_t recent, int64_t page, int64_t num_pages,
+                    int64_t width, int64_t table_ld, const int64_t* page_strides, int64_t out_page,
+                    int64_t out_num_pages, int64_t out_width, int64_t out_table_ld, const int64_t* out_page_strides,
+                    void* scratch, int64_t scratch_bytes, int dtype, void* stream);
 
 #ifdef __cplusplus
 }

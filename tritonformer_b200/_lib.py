@@ -60,6 +60,13 @@ _SIGNATURES = {
     "tfb_attention_fwd": (_i32, [_vp] * 5 + [_i64] * 4 + [_pi64] * 4 + [_vp, _i32, _vp, _i64, _i64, _i32, _vp, _pi32]),
     "tfb_attention_bwd_scratch_bytes": (_i64, [_i64] * 4),
     "tfb_attention_bwd": (_i32, [_vp] * 9 + [_i64] * 4 + [_pi64] * 8 + [_vp, _i32, _vp, _i64, _i64, _vp, _i64, _i32, _vp, _pi32]),
+    "tfb_paged_attention_scratch_bytes": (_i64, [_i64] * 5 + [_i32]),
+    "tfb_paged_attention": (_i32, [_vp] * 13 + [_i32] + [_i64] * 8 + [_pi64] * 5 + [_vp, _i64, _i32, _vp]),
+    "tfb_cache_append": (_i32, [_vp] * 11 + [_i64] * 8 + [_pi64] * 4 + [_i32, _vp]),
+    "tfb_prompt_mass_scratch_bytes": (_i64, [_i64] * 3),
+    "tfb_prompt_mass": (_i32, [_vp] * 5 + [_i32, _vp] + [_i64] * 5 + [_pi64] * 3 + [_vp, _i64, _i32, _vp]),
+    "tfb_cache_evict_scratch_bytes": (_i64, [_i64] * 3),
+    "tfb_cache_evict": (_i32, [_vp] * 13 + [_i64] * 9 + [_pi64] + [_i64] * 4 + [_pi64, _vp, _i64, _i32, _vp]),
 }
 
 EXPORTS = tuple(sorted(_SIGNATURES))
@@ -138,12 +145,13 @@ def device_status(reset: bool = False) -> int:
     return code
 
 
-_STATUS_TEXT = {0x7100: "a token id outside the embedding table", 0x7e00: "the wait probe of the test suite"}
+_STATUS_TEXT = {0x7100: "a token id outside the embedding table", 0x7200: "a page id outside the paged cache",
+                0x7201: "a length that does not fit its sequence's pages", 0x7e00: "the wait probe of the test suite"}
 
 
 def check_status() -> None:
     """Raises RuntimeError if a kernel of the library reported a failure on the current device (a bounded wait
-    that ran out, a token id outside the embedding table).  Synchronises the device: call it where the host
+    that ran out, a token id outside the embedding table, a page table or length that does not fit the cache).  Synchronises the device: call it where the host
     waits anyway, e.g. next to the read-back of the loss.  The status stays set until device_status(reset=True)."""
     code = device_status()
     if code != 0:

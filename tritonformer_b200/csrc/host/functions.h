@@ -49,6 +49,18 @@ Tensor cross_entropy(const Tensor& logits, const Tensor& labels, bool f32);
 Tensor lm_loss(const Tensor& logits, const Tensor& labels);
 Tensor embedding(const Tensor& ids, const Tensor& tok, const Tensor& pos);
 
+// The paged key-value cache (kvcache.cpp).
+Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& tables, const Tensor& lengths,
+                       const Tensor& key, const Tensor& value, const Tensor& slopes, int64_t rounded,
+                       const Tensor& query_positions, const Tensor& mass, const Tensor& positions, const Tensor& mass_out);
+void cache_append(const Tensor& k_pages, const Tensor& v_pages, const Tensor& tables, const Tensor& lengths, const Tensor& key,
+                  const Tensor& value, const Tensor& counts, const Tensor& mass, const Tensor& positions, const Tensor& key_mass,
+                  const Tensor& first_positions);
+Tensor prompt_mass(const Tensor& q, const Tensor& k, const Tensor& lse, const Tensor& counts, const Tensor& slopes, int64_t rounded);
+Tensor cache_evict(const Tensor& k, const Tensor& v, const Tensor& mass, const Tensor& positions, const Tensor& tables,
+                   const Tensor& lengths, const Tensor& next_positions, const Tensor& k_out, const Tensor& v_out,
+                   const Tensor& mass_out, const Tensor& positions_out, const Tensor& out_tables, int64_t keep, int64_t recent);
+
 struct LayerWeights {
   Tensor ln1_w, ln1_b, wq, wk, wv, wo, ln2_w, ln2_b, w1, b1, w2, b2;
 };

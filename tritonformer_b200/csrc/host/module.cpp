@@ -164,6 +164,61 @@ TFB_PY(py_layer_and_activations) {  // (output, hidden activations): what the mo
     return Py_BuildValue("(NN)", y, THPVariable_Wrap(act));
   });
 }
+// The operators of the paged cache write into their arguments, which a recorded graph would not show.
+void refuse_tracing(const char* name) {
+  if (torch::jit::tracer::isTracing()) throw ArgumentError(std::string(name) + " cannot be recorded by torch.jit.trace");
+}
+// q, k_pages, v_pages, tables, lengths, key, value, slopes, rounded, query_positions, mass, positions, mass_out
+TFB_PY(py_paged_attention) {
+  return guarded([&]() -> PyObject* {
+    refuse_tracing("paged_attention");
+    Args a(argv, argc, 13, "paged_attention");
+    const Tensor &q = a.tensor(), &k = a.tensor(), &v = a.tensor(), &tables = a.tensor(), &lengths = a.tensor(), &key = a.tensor(),
+                 &value = a.tensor(), &slopes = a.tensor();
+    const int64_t rounded = a.integer();
+    const Tensor &at = a.tensor(), &mass = a.tensor(), &positions = a.tensor(), &mass_out = a.tensor();
+    return tensor_result(
+        [&] { return paged_attention(q, k, v, tables, lengths, key, value, slopes, rounded, at, mass, positions, mass_out); });
+  });
+}
+// k_pages, v_pages, tables, lengths, key, value, counts, mass, positions, key_mass, first_positions
+TFB_PY(py_cache_append) {
+  return guarded([&]() -> PyObject* {
+    refuse_tracing("cache_append");
+    Args a(argv, argc, 11, "cache_append");
+    const Tensor &k = a.tensor(), &v = a.tensor(), &tables = a.tensor(), &lengths = a.tensor(), &key = a.tensor(),
+                 &value = a.tensor(), &counts = a.tensor(), &mass = a.tensor(), &positions = a.tensor(), &key_mass = a.tensor(),
+                 &first = a.tensor();
+    {
+      pybind11::gil_scoped_release no_gil;
+      cache_append(k, v, tables, lengths, key, value, counts, mass, positions, key_mass, first);
+    }
+    Py_RETURN_NONE;
+  });
+}
+TFB_PY(py_prompt_mass) {  // q, k, lse, counts, slopes, rounded
+  return guarded([&]() -> PyObject* {
+    refuse_tracing("prompt_mass");
+    Args a(argv, argc, 6, "prompt_mass");
+    const Tensor &q = a.tensor(), &k = a.tensor(), &lse = a.tensor(), &counts = a.tensor(), &slopes = a.tensor();
+    const int64_t rounded = a.integer();
+    return tensor_result([&] { return prompt_mass(q, k, lse, counts, slopes, rounded); });
+  });
+}
+// k, v, mass, positions, tables, lengths, next_positions, k_out, v_out, mass_out, positions_out, out_tables, keep, recent
+TFB_PY(py_cache_evict) {
+  return guarded([&]() -> PyObject* {
+    refuse_tracing("cache_evict");
+    Args a(argv, argc, 14, "cache_evict");
+    const Tensor &k = a.tensor(), &v = a.tensor(), &mass = a.tensor(), &positions = a.tensor(), &tables = a.tensor(),
+                 &lengths = a.tensor(), &next = a.tensor(), &k_out = a.tensor(), &v_out = a.tensor(), &mass_out = a.tensor(),
+                 &positions_out = a.tensor(), &out_tables = a.tensor();
+    const int64_t keep = a.integer(), recent = a.integer();
+    return tensor_result([&] {
+      return cache_evict(k, v, mass, positions, tables, lengths, next, k_out, v_out, mass_out, positions_out, out_tables, keep, recent);
+    });
+  });
+}
 TFB_PY(py_set_grad_mode) {  // accumulating, overwrite, defer, fork
   return guarded([&]() -> PyObject* {
     Args a(argv, argc, 4, "set_grad_mode");
@@ -217,6 +272,7 @@ TFB_PY(py_reset_workspaces) {
 PyMethodDef methods[] = {TFB_METHOD(linear), TFB_METHOD(layernorm), TFB_METHOD(attention), TFB_METHOD(softmax),
                          TFB_METHOD(cross_entropy), TFB_METHOD(lm_loss), TFB_METHOD(embedding), TFB_METHOD(layer),
                          TFB_METHOD(layer_and_activations),
+                         TFB_METHOD(paged_attention), TFB_METHOD(cache_append), TFB_METHOD(prompt_mass), TFB_METHOD(cache_evict),
                          TFB_METHOD(set_grad_mode), TFB_METHOD(take_written), TFB_METHOD(join_weight_grads),
                          TFB_METHOD(gemm_workspace), TFB_METHOD(reset_workspaces), TFB_METHOD(set_recorder), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Native host path of tritonformer_b200.", -1, methods,

@@ -1,0 +1,495 @@
+// Writing prompts into a paged key-value cache, and evicting keys from it by their accumulated attention (sm_100a).
+//
+// Both move rows of 64 to 256 bytes between places that tables name; what bounds them is the bytes of the rows, so a warp takes
+// whole rows in 16-byte chunks, several at a time, and looks the places up beside the copies.
+//
+// Eviction has a selection before its copies.  A key's worth is its mass, or infinite while its position is among the
+// `recent` last ones; each (sequence, key head) keeps the `keep` worthiest, ties to the lower slot.  One block per
+// (sequence, key head) finds the worth of the keep-th by a radix selection over the bits of the worths (11, 11 and 10 of them
+// a pass: the top 11 are sign, exponent and two bits of the significand, which a long-tailed distribution fills some forty
+// values of), numbers the keys that go and those that stay behind slot `keep` in slot order, and pairs the two: the i-th
+// survivor from behind moves into the i-th slot that becomes free.  So keys that stay in front are not touched, no source of
+// a move is the goal of another, and the moves run in any order, in place, all at once.
+#include "paged.cuh"
+
+namespace tfb {
+namespace {
+
+// ------------------------------------------------------------------------------------------------------------- append
+struct AppendParams {
+  PageMap map;
+  const void *key, *value;
+  void *k, *v;
+  const int *lengths, *counts, *first;  // counts, first: may be null (all T; the slot's number)
+  float* mass;
+  int* positions;
+  const float* key_mass;
+  int64_t k_b, k_h, k_t, v_b, v_h, v_t, m_b, m_h;
+  int B, kv_heads, T;
+};
+
+constexpr int AP_ROWS = 64;  // rows of a block
+
+// One block: AP_ROWS rows of a (sequence, key head); neighbouring blocks take neighbouring heads, which lie side by side in a
+// projection's output.  VEC: 16-byte chunks; otherwise element by element.
+template <typename E, int HD, bool VEC>
+__global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
+  constexpr int W = VEC ? 8 : 1, LANES = HD / 8, PER = 256 / LANES, N = AP_ROWS / PER;
+  __shared__ int sh_page[AP_ROWS], sh_row[AP_ROWS];
+  grid_dependency_wait();
+  allow_dependents();
+  const int b = blockIdx.x / p.kv_heads, h = blockIdx.x % p.kv_heads;
+  const int cap = (int)p.map.capacity(), len = p.lengths[b];
+  const int want = p.counts ? p.counts[b] : p.T;
+  const int start = min(max(len, 0), cap), count = min(min(max(want, 0), p.T), cap - start);
+  const int t0 = blockIdx.y * AP_ROWS;
+  if (blockIdx.y == 0 && h == 0 && threadIdx.x == 0 && (len < 0 || want < 0 || want > p.T || (int64_t)len + want > cap))
+    atomicCAS(&g_dev_status, 0, kBadLength);
+  if (t0 >= count) return;
+  if (threadIdx.x < AP_ROWS) {
+    int page = -1, row = 0;
+    const int t = t0 + threadIdx.x;
+    if (t < count && find_slot(p.map, b, start + t, page, row)) {
+      const int64_t o = stat_offset(p.map, page, p.kv_heads, h, row);
+      if (p.mass) p.mass[o] = p.key_mass ? p.key_mass[b * p.m_b + h * p.m_h + t] : 0.f;
+      if (p.positions) p.positions[o] = (p.first ? p.first[b] : start) + t;
+    } else {
+      page = -1;
+    }
+    sh_page[threadIdx.x] = page;
+    sh_row[threadIdx.x] = row;
+  }
+  __syncthreads();
+  const E* key = static_cast<const E*>(p.key) + b * p.k_b + h * p.k_h;
+  const E* value = static_cast<const E*>(p.value) + b * p.v_b + h * p.v_h;
+  const int c = (threadIdx.x % LANES) * 8;
+  if constexpr (VEC) {
+    uint4 kr[N], vr[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = i * PER + threadIdx.x / LANES;
+      if (sh_page[r] >= 0) {
+        kr[i] = ld_stream16(key + (t0 + r) * p.k_t + c);
+        vr[i] = ld_stream16(value + (t0 + r) * p.v_t + c);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = i * PER + threadIdx.x / LANES;
+      if (sh_page[r] >= 0) {
+        const int64_t o = row_offset(p.map, sh_page[r], h, sh_row[r]) + c;
+        *reinterpret_cast<uint4*>(static_cast<E*>(p.k) + o) = kr[i];
+        *reinterpret_cast<uint4*>(static_cast<E*>(p.v) + o) = vr[i];
+      }
+    }
+  } else {
+    for (int i = 0; i < N; ++i) {
+      const int r = i * PER + threadIdx.x / LANES;
+      if (sh_page[r] < 0) continue;
+      const int64_t o = row_offset(p.map, sh_page[r], h, sh_row[r]) + c;
+#pragma unroll
+      for (int e = 0; e < 8; e += W) {
+        static_cast<E*>(p.k)[o + e] = key[(t0 + r) * p.k_t + c + e];
+        static_cast<E*>(p.v)[o + e] = value[(t0 + r) * p.v_t + c + e];
+      }
+    }
+  }
+}
+
+// -------------------------------------------------------------------------------------------------------------- evict
+struct EvictParams {
+  PageMap map, out_map;
+  const void *k, *v;
+  void *k_out, *v_out;
+  const float* mass;
+  const int* positions;
+  float* mass_out;
+  int* positions_out;
+  const int *lengths, *next;  // next: may be null (the length)
+  int* left;
+  int B, kv_heads, keep, recent;
+  int rows_in_place, stats_in_place;  // the outputs are the inputs, slot by slot
+  int room;                           // worths that fit shared memory
+  int* moves;   // (B * kv_heads) rows to move
+  int* to;      // (B * kv_heads, keep) in place: their goals, ascending (otherwise working space)
+  int* from;    // (B * kv_heads, keep) in place: their sources, ascending; otherwise the source of every slot
+};
+
+constexpr int EV_THREADS = 1024, EV_WARPS = 32;
+constexpr int EV_BINS = 2048;
+
+// Worths in the order of unsigned numbers; -0 is 0, a mass that is no number is -infinity.
+__device__ __forceinline__ uint32_t worth_of(float m) {
+  if (m != m) m = -INFINITY;
+  const uint32_t u = __float_as_uint(m + 0.f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+struct Stat {  // of one slot
+  int64_t at;
+  bool ok;
+};
+__device__ __forceinline__ Stat stat_at(const PageMap& m, int heads, int b, int h, int slot) {
+  int page, row;
+  const bool ok = find_slot(m, b, slot, page, row);
+  return {ok ? stat_offset(m, page, heads, h, row) : 0, ok};
+}
+__device__ __forceinline__ uint32_t worth_at(const EvictParams& p, int b, int h, int slot, int oldest) {
+  const Stat s = stat_at(p.map, p.kv_heads, b, h, slot);
+  if (!s.ok) return 0u;
+  const int at = p.positions ? p.positions[s.at] : slot;
+  return worth_of(at >= oldest ? INFINITY : p.mass[s.at]);
+}
+
+__device__ __forceinline__ void copy_stats(const EvictParams& p, int b, int h, int src, int dst) {
+  const Stat s = stat_at(p.map, p.kv_heads, b, h, src), d = stat_at(p.out_map, p.kv_heads, b, h, dst);
+  if (!s.ok || !d.ok) return;
+  p.mass_out[d.at] = p.mass[s.at];
+  if (p.positions) p.positions_out[d.at] = p.positions[s.at];
+}
+
+// Exclusive sum over the block's warps of a value that each warp has; `total` gets the whole.
+__device__ __forceinline__ int warps_before(int v, int* sh, int& total) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __syncthreads();
+  if (lane == 0) sh[warp] = v;
+  __syncthreads();
+  int x = sh[lane];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  total = __shfl_sync(0xffffffffu, x, 31);
+  const int before = __shfl_sync(0xffffffffu, x, warp) - v;
+  return before;
+}
+
+__global__ void __launch_bounds__(EV_THREADS, 1) evict_select_kernel(const EvictParams p) {
+  extern __shared__ uint32_t worths[];
+  __shared__ int bins[EV_BINS];
+  __shared__ int sh_warps[EV_WARPS];
+  __shared__ uint32_t sh_digit;
+  __shared__ int sh_want;
+  grid_dependency_wait();
+  allow_dependents();
+  const int item = blockIdx.x, b = item / p.kv_heads, h = item % p.kv_heads;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int cap = (int)p.map.capacity(), len = p.lengths[b];
+  const int n = min(max(len, 0), cap), keep = min(p.keep, n);
+  if (h == 0 && tid == 0) {
+    if (len != n) atomicCAS(&g_dev_status, 0, kBadLength);
+    p.left[b] = keep;
+  }
+  const int oldest = (int)max((int64_t)(p.next ? p.next[b] : n) - p.recent, (int64_t)INT32_MIN);
+  int* to = p.to + (int64_t)item * p.keep;
+  int* from = p.from + (int64_t)item * p.keep;
+
+  const bool in_smem = n <= p.room;  // else the worths are looked up again in every pass
+  if (n > keep) {
+    auto worth = [&](int i) { return in_smem ? worths[i] : worth_at(p, b, h, i, oldest); };
+    // ---- the worth of the keep-th, and how many of that worth stay
+    uint32_t prefix = 0, mask = 0;
+    int want = keep;
+    const int shifts[3] = {21, 10, 0}, widths[3] = {11, 11, 10};
+#pragma unroll
+    for (int pass = 0; pass < 3; ++pass) {
+      for (int i = tid; i < EV_BINS; i += EV_THREADS) bins[i] = 0;
+      __syncthreads();
+      const int sh = shifts[pass], size = 1 << widths[pass];
+      for (int i = tid; i < n; i += EV_THREADS) {
+        uint32_t u;
+        if (pass == 0 && in_smem) worths[i] = u = worth_at(p, b, h, i, oldest);
+        else u = worth(i);
+        if ((u & mask) == prefix) atomicAdd(&bins[(u >> sh) & (size - 1)], 1);
+      }
+      __syncthreads();
+      // the bin in which the want-th from the top lies: thread i has the bins size - 1 - per * i downwards
+      const int per = size / EV_THREADS;  // 2, 2, 1
+      int mine = 0;
+      for (int e = 0; e < per; ++e) mine += bins[size - 1 - per * tid - e];
+      int upto = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
+      }
+      int total;
+      int before = warps_before(__shfl_sync(0xffffffffu, upto, 31), sh_warps, total) + upto - mine;
+      for (int e = 0; e < per; ++e) {
+        const int bin = size - 1 - per * tid - e, c = bins[bin];
+        if (before < want && want <= before + c) {
+          sh_digit = (uint32_t)bin;
+          sh_want = want - before;
+        }
+        before += c;
+      }
+      __syncthreads();
+      prefix |= sh_digit << sh;
+      mask |= (uint32_t)(size - 1) << sh;
+      want = sh_want;
+    }
+    // ---- number the slots: each warp has a stretch of them, in steps of 32
+    const int steps = (n + 31) / 32, per = (steps + EV_WARPS - 1) / EV_WARPS;
+    const int lo = min(warp * per, steps), hi = min(lo + per, steps);
+    int ties = 0, over = 0, holes = 0;  // of the warp
+    for (int s = lo; s < hi; ++s) {
+      const int i = s * 32 + lane;
+      const uint32_t u = i < n ? worth(i) : 0u;
+      ties += __popc(__ballot_sync(0xffffffffu, i < n && u == prefix));
+    }
+    int total;
+    const int tie0 = warps_before(ties, sh_warps, total);
+    int tie = tie0;
+    // which of 32 slots stay; `tie` counts the slots of the keep-th's worth so far
+    auto stay = [&](int s) {
+      const int i = s * 32 + lane;
+      const uint32_t u = i < n ? worth(i) : 0u;
+      const unsigned eq = __ballot_sync(0xffffffffu, i < n && u == prefix);
+      const bool k = i < n && (u > prefix || (u == prefix && tie + __popc(eq & ((1u << lane) - 1u)) < want));
+      tie += __popc(eq);
+      return __ballot_sync(0xffffffffu, k);
+    };
+    for (int s = lo; s < hi; ++s) {
+      const unsigned k = stay(s);
+      const int front = min(max(keep - s * 32, 0), 32);  // how many of the 32 lie before slot `keep`
+      const unsigned in_front = front == 32 ? 0xffffffffu : (1u << front) - 1u;
+      holes += __popc(~k & in_front);
+      over += __popc(k & ~in_front);
+    }
+    int hole = warps_before(holes, sh_warps, total);
+    int nth = warps_before(over, sh_warps, total);
+    tie = tie0;
+    int* behind = p.rows_in_place ? from : to;  // the survivors from behind slot `keep`
+    const int hole0 = hole;
+    for (int s = lo; s < hi; ++s) {
+      const unsigned k = stay(s), below = (1u << lane) - 1u;
+      const int front = min(max(keep - s * 32, 0), 32);
+      const unsigned in_front = front == 32 ? 0xffffffffu : (1u << front) - 1u;
+      const unsigned out = ~k & in_front, in = k & ~in_front;
+      const int i = s * 32 + lane;
+      if (p.rows_in_place && (out >> lane & 1)) to[hole + __popc(out & below)] = i;
+      if (in >> lane & 1) behind[nth + __popc(in & below)] = i;
+      hole += __popc(out);
+      nth += __popc(in);
+    }
+    if (tid == 0) p.moves[item] = total;
+    __syncthreads();  // the survivors' slots are in global memory, for this block
+    tie = tie0;
+    hole = hole0;
+    for (int s = lo; s < hi && s * 32 < keep; ++s) {
+      const unsigned k = stay(s);
+      const int i = s * 32 + lane, front = min(keep - s * 32, 32);
+      const unsigned out = ~k & (front == 32 ? 0xffffffffu : (1u << front) - 1u);
+      if (i < keep) {
+        const bool stays = (k >> lane & 1) != 0;
+        const int src = stays ? i : behind[hole + __popc(out & ((1u << lane) - 1u))];
+        if (!p.rows_in_place) from[i] = src;
+        if (!(stays && p.stats_in_place)) copy_stats(p, b, h, src, i);
+      }
+      hole += __popc(out);
+    }
+  } else {
+    if (tid == 0) p.moves[item] = 0;
+    for (int i = tid; i < n; i += EV_THREADS) {
+      if (!p.rows_in_place) from[i] = i;
+      if (!p.stats_in_place) copy_stats(p, b, h, i, i);
+    }
+  }
+}
+
+constexpr int MV_ROWS = 128;
+
+// Moves rows of keys and values: in place the survivors from behind into the free slots, otherwise every slot that stays.
+template <int HD>
+__global__ void __launch_bounds__(256) evict_move_kernel(const EvictParams p) {
+  constexpr int LANES = HD / 8, PER = 256 / LANES, N = 4;
+  __shared__ int64_t sh_src[MV_ROWS], sh_dst[MV_ROWS];
+  grid_dependency_wait();
+  allow_dependents();
+  const int item = blockIdx.x, b = item / p.kv_heads, h = item % p.kv_heads;
+  const int* to = p.to + (int64_t)item * p.keep;
+  const int* from = p.from + (int64_t)item * p.keep;
+  const int count = p.rows_in_place ? p.moves[item] : p.left[b];
+  for (int i0 = blockIdx.y * MV_ROWS; i0 < count; i0 += gridDim.y * MV_ROWS) {
+    __syncthreads();
+    if (threadIdx.x < MV_ROWS) {
+      const int i = i0 + threadIdx.x;
+      int64_t src = -1, dst = 0;
+      if (i < count) {
+        const int goal = p.rows_in_place ? to[i] : i, source = from[i];
+        int page, row, page2, row2;
+        if (find_slot(p.map, b, source, page, row) && find_slot(p.out_map, b, goal, page2, row2)) {
+          src = row_offset(p.map, page, h, row);
+          dst = row_offset(p.out_map, page2, h, row2);
+        }
+      }
+      sh_src[threadIdx.x] = src;
+      sh_dst[threadIdx.x] = dst;
+    }
+    __syncthreads();
+    const int c = (threadIdx.x % LANES) * 8;
+    for (int r0 = threadIdx.x / LANES; r0 < MV_ROWS; r0 += PER * N) {
+      uint4 kr[N], vr[N];
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const int r = r0 + e * PER;
+        if (r < MV_ROWS && sh_src[r] >= 0) {
+          kr[e] = ld_stream16(static_cast<const uint16_t*>(p.k) + sh_src[r] + c);
+          vr[e] = ld_stream16(static_cast<const uint16_t*>(p.v) + sh_src[r] + c);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const int r = r0 + e * PER;
+        if (r < MV_ROWS && sh_src[r] >= 0) {
+          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.k_out) + sh_dst[r] + c) = kr[e];
+          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.v_out) + sh_dst[r] + c) = vr[e];
+        }
+      }
+    }
+  }
+}
+
+int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
+
+template <typename E, int HD, bool VEC>
+int append_launch(const AppendParams& p, cudaStream_t st) {
+  const dim3 grid((unsigned)(p.B * p.kv_heads), (unsigned)ceil_div(p.T, AP_ROWS));
+  launch_overlapped(append_kernel<E, HD, VEC>, grid, dim3(256), 0, st, p);
+  return launched("cache_append");
+}
+
+}  // namespace
+}  // namespace tfb
+
+using namespace tfb;
+
+extern "C" int tfb_cache_append(const void* key, const void* value, void* k_pages, void* v_pages, const int* tables,
+                                const int* lengths, const int* counts, const int* first_positions, float* mass, int* positions,
+                                const float* key_mass, int64_t B, int64_t kv_heads, int64_t T, int64_t hd, int64_t num_pages,
+                                int64_t page, int64_t width, int64_t table_ld, const int64_t* page_strides,
+                                const int64_t* key_strides, const int64_t* value_strides, const int64_t* key_mass_strides,
+                                int dtype, void* stream) {
+  AppendParams p = {};
+  TFB_REQUIRE(page >= 1 && page < (1LL << 31) && width >= 1 && width < (1LL << 31), "cache_append: bad page or table size");
+  p.map = {tables, table_ld, num_pages, (int)page, (int)width, page_strides[0], page_strides[1], page_strides[2]};
+  if (int rc = check_pages("cache_append", p.map, B, kv_heads, hd, dtype)) return rc;
+  TFB_REQUIRE(T >= 0 && T <= 65535 * (int64_t)AP_ROWS, "cache_append: more than %lld keys", (long long)(65535 * (int64_t)AP_ROWS));
+  TFB_REQUIRE(B * kv_heads < (1LL << 31), "cache_append: too many rows of heads");
+  if (B == 0 || T == 0) return TFB_OK;
+  TFB_REQUIRE(aligned16(k_pages) && aligned16(v_pages), "cache_append: the pages are not 16-byte aligned");
+  TFB_REQUIRE(!key_mass || mass, "cache_append: masses of the keys without masses of the cache");
+  p.key = key;
+  p.value = value;
+  p.k = k_pages;
+  p.v = v_pages;
+  p.lengths = lengths;
+  p.counts = counts;
+  p.first = first_positions;
+  p.mass = mass;
+  p.positions = positions;
+  p.key_mass = key_mass;
+  p.k_b = key_strides[0];
+  p.k_h = key_strides[1];
+  p.k_t = key_strides[2];
+  p.v_b = value_strides[0];
+  p.v_h = value_strides[1];
+  p.v_t = value_strides[2];
+  if (key_mass) {
+    p.m_b = key_mass_strides[0];
+    p.m_h = key_mass_strides[1];
+  }
+  p.B = (int)B;
+  p.kv_heads = (int)kv_heads;
+  p.T = (int)T;
+  cudaStream_t st = (cudaStream_t)stream;
+  bool vec = aligned16(key) && aligned16(value);
+  for (int i = 0; i < 3; ++i) vec = vec && key_strides[i] % 8 == 0 && value_strides[i] % 8 == 0;
+  // a copy: the type does not matter beyond its size
+  if (hd == 32) return vec ? append_launch<uint16_t, 32, true>(p, st) : append_launch<uint16_t, 32, false>(p, st);
+  if (hd == 64) return vec ? append_launch<uint16_t, 64, true>(p, st) : append_launch<uint16_t, 64, false>(p, st);
+  return vec ? append_launch<uint16_t, 128, true>(p, st) : append_launch<uint16_t, 128, false>(p, st);
+}
+
+extern "C" int64_t tfb_cache_evict_scratch_bytes(int64_t B, int64_t kv_heads, int64_t keep) {
+  if (B < 0 || kv_heads < 0 || keep < 0) return 0;
+  return up256(B * kv_heads * 4) + 2 * up256(B * kv_heads * keep * 4);
+}
+
+extern "C" int tfb_cache_evict(const void* k_pages, const void* v_pages, const float* mass, const int* positions,
+                               const int* tables, const int* lengths, const int* next_positions, void* k_out, void* v_out,
+                               float* mass_out, int* positions_out, const int* out_tables, int* left, int64_t B,
+                               int64_t kv_heads, int64_t hd, int64_t keep, int64_t recent, int64_t page, int64_t num_pages,
+                               int64_t width, int64_t table_ld, const int64_t* page_strides, int64_t out_page,
+                               int64_t out_num_pages, int64_t out_width, int64_t out_table_ld, const int64_t* out_page_strides,
+                               void* scratch, int64_t scratch_bytes, int dtype, void* stream) {
+  EvictParams p = {};
+  TFB_REQUIRE(page >= 1 && page < (1LL << 31) && width >= 1 && width < (1LL << 31), "cache_evict: bad page or table size");
+  TFB_REQUIRE(out_page >= 1 && out_page < (1LL << 31) && out_width >= 1 && out_width < (1LL << 31), "cache_evict: bad page or table size");
+  p.map = {tables, table_ld, num_pages, (int)page, (int)width, page_strides[0], page_strides[1], page_strides[2]};
+  p.out_map = {out_tables, out_table_ld, out_num_pages, (int)out_page, (int)out_width, out_page_strides[0], out_page_strides[1],
+               out_page_strides[2]};
+  if (int rc = check_pages("cache_evict", p.map, B, kv_heads, hd, dtype)) return rc;
+  if (int rc = check_pages("cache_evict", p.out_map, B, kv_heads, hd, dtype)) return rc;
+  TFB_REQUIRE(keep >= 1, "cache_evict: keep %lld: expected at least 1", (long long)keep);
+  TFB_REQUIRE(recent >= 0 && recent <= keep, "cache_evict: recent %lld: expected 0 to keep", (long long)recent);
+  if (keep > p.map.capacity()) keep = p.map.capacity();
+  if (recent > keep) recent = keep;
+  TFB_REQUIRE(keep <= p.out_map.capacity(), "cache_evict: %lld keys to keep, and room for %lld", (long long)keep,
+              (long long)p.out_map.capacity());
+  TFB_REQUIRE(B * kv_heads < (1LL << 31), "cache_evict: too many rows of heads");
+  TFB_REQUIRE(mass && mass_out, "cache_evict: no masses");
+  TFB_REQUIRE((positions == nullptr) == (positions_out == nullptr), "cache_evict: positions come with positions for the output");
+  TFB_REQUIRE((k_out == k_pages) == (v_out == v_pages), "cache_evict: keys in place and values not, or the other way round");
+  if (B == 0) return TFB_OK;
+  TFB_REQUIRE(aligned16(k_pages) && aligned16(v_pages) && aligned16(k_out) && aligned16(v_out),
+              "cache_evict: the pages are not 16-byte aligned");
+  TFB_REQUIRE(scratch && aligned16(scratch) && scratch_bytes >= tfb_cache_evict_scratch_bytes(B, kv_heads, keep),
+              "cache_evict: scratch of %lld bytes, %lld wanted", (long long)scratch_bytes,
+              (long long)tfb_cache_evict_scratch_bytes(B, kv_heads, keep));
+  p.k = k_pages;
+  p.v = v_pages;
+  p.k_out = k_out;
+  p.v_out = v_out;
+  p.mass = mass;
+  p.positions = positions;
+  p.mass_out = mass_out;
+  p.positions_out = positions_out;
+  p.lengths = lengths;
+  p.next = next_positions;
+  p.left = left;
+  p.B = (int)B;
+  p.kv_heads = (int)kv_heads;
+  p.keep = (int)keep;
+  p.recent = (int)recent;
+  const bool same_tables = out_tables == tables;
+  p.rows_in_place = same_tables && k_out == k_pages;
+  p.stats_in_place = same_tables && mass_out == mass && positions_out == positions;
+  TFB_REQUIRE(same_tables || (k_out != k_pages && mass_out != mass && (!positions || positions_out != positions)),
+              "cache_evict: tables of their own need pages of their own");
+  TFB_REQUIRE(!same_tables || (mass_out == mass) == (positions_out == positions) || !positions,
+              "cache_evict: masses in place and positions not, or the other way round");
+  char* base = static_cast<char*>(scratch);
+  p.moves = reinterpret_cast<int*>(base);
+  p.to = reinterpret_cast<int*>(base + up256(B * kv_heads * 4));
+  p.from = reinterpret_cast<int*>(base + up256(B * kv_heads * 4) + up256(B * kv_heads * keep * 4));
+  cudaStream_t st = (cudaStream_t)stream;
+  constexpr int kMost = 200 * 1024;  // beside the kernel's own arrays
+  int64_t smem = (p.map.capacity() * 4 + 15) / 16 * 16;
+  if (smem > kMost) smem = kMost;
+  p.room = (int)(smem / 4);
+  static std::atomic<uint64_t> done{0};
+  if (int rc = ensure_dynamic_smem(evict_select_kernel, kMost, done, "cache_evict")) return rc;
+  launch_overlapped(evict_select_kernel, dim3((unsigned)(B * kv_heads)), dim3(EV_THREADS), (size_t)smem, st, p);
+  if (int rc = launched("cache_evict")) return rc;
+  // a block for each MV_ROWS rows that can move, as far as that takes to fill the SMs
+  int64_t shares = ceil_div(keep, MV_ROWS);
+  const int64_t enough = ceil_div((int64_t)sm_count() * 16, B * kv_heads);
+  if (shares > enough) shares = enough;
+  const dim3 grid((unsigned)(B * kv_heads), (unsigned)shares);
+  if (hd == 32) launch_overlapped(evict_move_kernel<32>, grid, dim3(256), 0, st, p);
+  else if (hd == 64) launch_overlapped(evict_move_kernel<64>, grid, dim3(256), 0, st, p);
+  else launch_overlapped(evict_move_kernel<128>, grid, dim3(256), 0, st, p);
+  return launched("cache_evict: move");
+}
