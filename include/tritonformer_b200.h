@@ -43,7 +43,7 @@ const char* tfb_last_error(void);
 int64_t tfb_launch_count(void);
 /* Device-side status word of the library on the calling thread's CURRENT device (one word per GPU,
  * shared by every kernel of the library): 0, or the code of the first bounded wait that expired
- * (0x2xxx attention backward, 0x5xxx attention forward, 0x8xxx prompt mass, 0x1xxx / 0x3xxx GEMM, 0x7e00 the test probe)
+ * (0x2xxx attention backward, 0x5xxx attention forward, 0x8xxx prompt mass, 0x9xxx paged attention, 0x1xxx / 0x3xxx GEMM, 0x7e00 the test probe)
  * or 0x7100 for a token id outside the embedding table, 0x7200 / 0x7201 for a page id / a length that
  * does not fit a paged cache (below).  While it is non-zero the tcgen05 kernels
  * (GEMM, attention) return at once without writing their outputs; the other kernels still run.
@@ -323,16 +323,19 @@ int tfb_loss_scale_update(float* state4, int* found_inf, float growth, float bac
  * (query_positions NULL: the number of the last slot); a new key's position is the query's.  With mass and mass_out (the same
  * buffer, or another one of its shape) mass_out = mass + the key's weights, summed over the query heads of its key head, in the
  * slots in use; a new key starts from zero.  group <= 128.  Strides {b, h} in elements, unit stride on hd, any alignment.
- * scratch needs no initialisation.                                                                            */
-int64_t tfb_paged_attention_scratch_bytes(int64_t B, int64_t kv_heads, int64_t group, int64_t hd, int64_t capacity,
-                                          int with_mass);
+ * workspace: at least tfb_paged_attention_workspace_bytes(), 16-byte aligned, its first 8192 bytes ZERO on entry and zero again
+ * when the kernel has finished (the GEMM's workspace, where that is large enough, serves both); calls that share one must be
+ * stream-ordered.  scratch is for masses only and needs no initialisation; capacity = width * page.            */
+int64_t tfb_paged_attention_workspace_bytes(void);
+int64_t tfb_paged_attention_scratch_bytes(int64_t B, int64_t kv_heads, int64_t group, int64_t capacity);
 int tfb_paged_attention(const void* q, const void* k_new, const void* v_new, void* out, void* k_pages, void* v_pages,
                         const int* tables, const int* lengths, const int* query_positions, int* positions,
                         const float* mass, float* mass_out, const float* slopes, int alibi_round, int64_t B,
                         int64_t kv_heads, int64_t group, int64_t hd, int64_t num_pages, int64_t page, int64_t width,
                         int64_t table_ld, const int64_t* page_strides, const int64_t* q_strides,
                         const int64_t* k_new_strides, const int64_t* v_new_strides, const int64_t* o_strides,
-                        void* scratch, int64_t scratch_bytes, int dtype, void* stream);
+                        void* workspace, int64_t workspace_bytes, void* scratch, int64_t scratch_bytes, int dtype,
+                        void* stream);
 
 /* Key and value rows of prompts into the pages: key, value (B, kv_heads, T, hd) with strides {b, h, t}; the first counts[b]
  * (NULL: all T) of them go into the slots from lengths[b] on.  mass (may be NULL) gets key_mass (B, kv_heads, T; strides {b, h};

@@ -658,10 +658,11 @@ def _strides(*s):
 def test_argument_checks_without_device():
     pg, two, three, one = _strides(2048, 1024, 64), _strides(128, 64), _strides(4096, 2048, 64), ctypes.c_void_p(256)
 
-    def attention(hd=64, group=1, pages=4, page=16, width=2, ld=2, k_new=None, mass_out=None, scratch=None, nbytes=0, dtype=0,
-                  strides=pg, k_pages=one):
-        return L.lib.tfb_paged_attention(one, k_new, None, one, k_pages, one, one, one, None, None, None, mass_out, None, 0, 2, 2, group,
-                                         hd, pages, page, width, ld, strides, two, two, two, two, scratch, nbytes, dtype, None)
+    def attention(hd=64, group=1, pages=4, page=16, width=2, ld=2, k_new=None, mass=None, mass_out=None, scratch=None, nbytes=0,
+                  dtype=0, strides=pg, k_pages=one, workspace=None, wbytes=0):
+        return L.lib.tfb_paged_attention(one, k_new, None, one, k_pages, one, one, one, None, None, mass, mass_out, None, 0, 2, 2, group,
+                                         hd, pages, page, width, ld, strides, two, two, two, two, workspace, wbytes, scratch, nbytes,
+                                         dtype, None)
 
     def said(rc, code, text):
         assert rc == code and text in L.lib.tfb_last_error(), (rc, L.lib.tfb_last_error())
@@ -676,10 +677,10 @@ def test_argument_checks_without_device():
     said(attention(k_pages=ctypes.c_void_p(260)), -1, b"16-byte")
     said(attention(k_new=one), -1, b"without a value")
     said(attention(mass_out=one), -1, b"come together")
-    said(attention(), -1, b"scratch")
-    said(attention(scratch=one, nbytes=16), -1, b"scratch")
-    need = L.lib.tfb_paged_attention_scratch_bytes
-    assert need(2, 2, 1, 64, 32, 1) == need(2, 2, 1, 64, 32, 0) + 2 * 2 * 32 * 4
+    said(attention(), -1, b"workspace")
+    said(attention(workspace=one, wbytes=16), -1, b"workspace")
+    said(attention(mass=one, mass_out=one, workspace=one, wbytes=1 << 30, scratch=one, nbytes=16), -1, b"scratch")
+    assert L.lib.tfb_paged_attention_scratch_bytes(2, 2, 1, 32) == 256 + 2 * 2 * 32 * 4
     said(L.lib.tfb_cache_append(one, one, one, one, one, one, None, None, None, None, one, 1, 2, 5, 64, 4, 16, 2, 2, pg, three, three,
                                 two, 0, None), -1, b"masses")
     assert L.lib.tfb_cache_append(one, one, one, one, one, one, None, None, None, None, None, 1, 2, 0, 64, 4, 16, 2, 2, pg, three, three,

@@ -99,8 +99,11 @@ Tensor paged_attention(const Tensor& q_, const Tensor& k_pages, const Tensor& v_
   Tensor out = at::empty({B, heads, pool.hd}, q.options());
   if (B == 0) return out;
   const int64_t group = heads / pool.heads;
-  const int64_t bytes = tfb_paged_attention_scratch_bytes(B, pool.heads, group, pool.hd, table.width * pool.page, mass.defined());
-  Tensor scratch = at::empty({bytes}, q.options().dtype(at::kByte));
+  const int64_t bytes = mass.defined() ? tfb_paged_attention_scratch_bytes(B, pool.heads, group, table.width * pool.page) : 0;
+  Tensor scratch;
+  if (bytes) scratch = at::empty({bytes}, q.options().dtype(at::kByte));
+  const cudaStream_t stream = current_stream(q);
+  const Tensor ws = gemm_workspace(q.device(), stream);
   const int64_t sq[2] = {step(q, 0), step(q, 1)}, so[2] = {heads * pool.hd, pool.hd};
   int64_t sk[2] = {0, 0}, sv[2] = {0, 0};
   if (key.defined())
@@ -112,7 +115,8 @@ Tensor paged_attention(const Tensor& q_, const Tensor& k_pages, const Tensor& v_
                             out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), table.p, ints(lengths), ints(query_positions),
                             const_cast<int*>(ints(positions)), floats(mass), floats(mass_out), floats(slopes), (int)rounded, B,
                             pool.heads, group, pool.hd, pool.pages, pool.page, table.width, table.ld, pool.strides, sq, sk, sv, so,
-                            scratch.data_ptr(), bytes, dtype_code(q.scalar_type()), current_stream(q)));
+                            ws.data_ptr(), ws.numel(), bytes ? scratch.data_ptr() : nullptr, bytes, dtype_code(q.scalar_type()),
+                            stream));
   return out;
 }
 

@@ -10,9 +10,13 @@
 // tiles of all sequences are numbered in one line, and each warp of the grid takes an equal stretch of that line, wherever
 // sequences begin and end: lengths that differ by orders of magnitude leave no SM idle, one sequence alone fills the machine,
 // and the lengths never have to be known on the host.  A warp works by itself: its own ring of tiles in shared memory, filled
-// by cp.async two tiles ahead and across the borders of sequences, no barrier of the block anywhere in the loop.  A stretch
-// that holds a whole row of scores writes the output; otherwise the reference, sum and accumulator of the piece go to
-// scratch, and a second kernel joins the pieces in their order (no atomics: the result does not depend on timing).
+// ahead and across the borders of sequences, no barrier of the block in the loop.  A row of scores that ends in the warp it
+// began in is written out; the pieces of the others meet at the end of the block; what does not begin and end in one block goes
+// to a workspace, where the last of its blocks joins the pieces, always in their order (the result does not depend on timing).
+// Only masses need a second kernel: a key's weight is known once its row's sum is.
+//
+// Copies.  Where pages and tiles share a divisor of 8 rows or more, TMA boxes of that many rows, which also swizzle the rows
+// for ldmatrix; other page sizes take cp.async row by row.
 //
 // Products.  S^T = K Q^T and O^T = V^T P^T by mma.sync m16n8k16, keys (or head_dim) along M and query heads along N: a tile
 // of 8 heads wastes less than one of 16, and P^T comes out of the first product's registers by a transposition of 8x8
@@ -20,28 +24,40 @@
 // write P into, and nothing waits for the tensor core.
 #include "attn.cuh"
 #include "paged.cuh"
+#include "tc05.cuh"
 
 namespace tfb {
 namespace {
 
 constexpr int PG_WARPS = 8;
-constexpr int PG_STAGES = 3;
 constexpr float kLog2e = 1.4426950408889634f;
 // Probabilities are kept relative to a reference that the running maximum may pass by 2^15 before everything is rescaled
 // (they then still fit fp16); a new reference is 2^4 below the maximum, so that small ones stay clear of fp16's subnormals.
 constexpr float kAhead = 15.f, kBelow = 4.f;
 constexpr float kNone = -INFINITY;
 
-template <int HD> struct PgCfg {
+// What beginning a row of scores costs a warp, in tiles: rows of a tile or two would otherwise pile up in a few warps.
+constexpr int kRowCost = 4;
+
+template <int HD, int NT, int BIAS> struct PgCfg {
   static constexpr int KEYS = 2048 / HD;       // keys of a tile
   static constexpr int MT = KEYS / 16;
+  static constexpr int R = 8 * NT;             // query heads of a head tile
   static constexpr int CHUNKS = HD / 8;        // 16-byte chunks of a row
-  static constexpr int RPI = 32 / CHUNKS;      // rows that a warp copies with one instruction
+  static constexpr int RPI = 32 / CHUNKS;      // rows that a warp copies with one cp.async
   static constexpr int ITERS = KEYS / RPI;     // 8
   static constexpr int OWN = (KEYS + 31) / 32; // keys whose place a lane looks up
   static constexpr int TILE = KEYS * HD * 2;   // bytes of the keys of a tile (4096)
-  static constexpr int STAGE = 2 * TILE + KEYS * 4;  // keys, values, positions
-  static constexpr int SMEM = PG_WARPS * PG_STAGES * STAGE;
+  static constexpr int PANELS = HD == 128 ? 2 : 1;  // parts of a row of at most 128 bytes, one after the other
+  static constexpr int STAGES = 3;             // what 227 KB hold
+  static constexpr int OFF_POS = PG_WARPS * STAGES * 2 * TILE;   // [warp][stage][KEYS] positions
+  static constexpr int OFF_ML = OFF_POS + (BIAS ? PG_WARPS * STAGES * KEYS * 4 : 0);  // [warp][2][R] reference and sum of a piece
+  static constexpr int OFF_BAR = OFF_ML + PG_WARPS * 2 * R * 8;  // [warp][stage]
+  static constexpr int OFF_HEAD = OFF_BAR + 256;  // [warp][R][HD] the piece that a stretch begins in the middle of,
+  static constexpr bool HEAD_SMEM = OFF_HEAD + PG_WARPS * R * HD * 4 + 1024 <= 226 * 1024 + 256;  // if that fits (else in scratch)
+  static constexpr int SMEM = OFF_HEAD + (HEAD_SMEM ? PG_WARPS * R * HD * 4 : 0) + 1024;
+  static_assert(R * HD * 4 <= STAGES * 2 * TILE, "a piece fits its warp's ring");
+  static_assert(PG_WARPS * STAGES * 8 <= 256 && SMEM <= 227 * 1024 - 700, "shared memory");
 };
 
 struct PgParams {
@@ -56,14 +72,17 @@ struct PgParams {
   int bias_mode;  // as in AttnArgs: 0 none, 1 exact, 2 / 4 rounded
   int64_t q_b, q_h, kn_b, kn_h, vn_b, vn_h, o_b, o_h;
   int B, kv_heads, group, row_tiles;
-  int new_vec;    // the new rows can be copied 16 bytes at a time
-  int warps;      // of the split kernel's grid
+  int box_log2;   // rows of a TMA box
+  int q_pairs;    // the queries can be read 4 bytes at a time
+  int new_vec;    // the new rows can be read 16 bytes at a time
+  int ctas;       // of the split kernel's grid
   float scale;    // log2(e) / sqrt(hd)
-  int64_t* prefix;  // (B + 1) tiles of the sequences before b, per head tile
-  float* lse;       // (B, kv_heads * group) log2 of the sum of exponentials, rows that one warp finished
-  float2* ml;       // [2 * warps][R] reference and sum of a piece
-  float* acc;       // [2 * warps][R][hd]
-  float* scores;    // (B, kv_heads * group, capacity) in log2 units, or null
+  int* arrived;     // [ctas] how many blocks have left their pieces of the row that this one begins; zero between calls
+  float* lse;       // (B, kv_heads * group) log2 of the sum of exponentials, where masses are wanted
+  float2* ml;       // [2 * ctas][R] reference and sum of a piece
+  float* acc;       // [2 * ctas][R][hd]
+  float* heads_acc; // [ctas][warps][R][hd] the pieces that a warp's stretch begins in the middle of
+  float* scores;    // (B, kv_heads, capacity, group) in log2 units, or null
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -71,7 +90,6 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {  // the rest of the 16 is zeros
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -108,76 +126,118 @@ template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float 
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// Byte offset of 16-byte chunk `c` of row `row` of a tile: the chunk number is xor-ed with the row, so that the eight rows of
-// an ldmatrix lie in different banks.
+// Byte offset of 16-byte chunk `c` of row `row` of a tile, swizzled as TMA does it (128 bytes wide, at head_dim 32 64): the chunk
+// number is xor-ed with the row, so that the eight rows of an ldmatrix lie in different banks.
 template <int HD> __device__ __forceinline__ uint32_t tile_at(int row, int c) {
-  const int x = HD == 32 ? (row >> 1) & 3 : row & 7;
-  return (uint32_t)(row * HD * 2 + ((c ^ x) << 4));
+  if (HD == 32) return (uint32_t)(row * 64 + ((c ^ ((row >> 1) & 3)) << 4));
+  return (uint32_t)((c >> 3) * (2048 / HD) * 128 + row * 128 + (((c & 7) ^ (row & 7)) << 4));
 }
 
-// Keys of a sequence, and the slot of its new one (-1: none).
+// Keys of a sequence, and the slot of its new one (-1: none; otherwise the last).
 struct SeqKeys {
   int n, fresh;
+  __device__ __forceinline__ int cached() const { return fresh >= 0 ? fresh : n; }
 };
-__device__ __forceinline__ SeqKeys keys_of(const PgParams& p, int b) {
-  const int cap = (int)p.map.capacity(), len = p.lengths[b];
+__device__ __forceinline__ SeqKeys keys_of(const PgParams& p, int len) {
+  const int cap = (int)p.map.capacity();
   SeqKeys s;
   s.fresh = p.k_new && len >= 0 && len < cap ? len : -1;
   s.n = min(max(len, 0) + (s.fresh >= 0), cap);
   return s;
 }
 
-// The place of a warp's stretch in the line of tiles: sequence, (key head, head tile), tile.
-template <int HD>
+// A place in the line: sequence, (key head, head tile), tile, and its distance from the stretch's beginning.
+template <int KEYS>
 struct Cursor {
-  int b, hr, j, tiles;
+  int b, hr, j, tiles, at;
   SeqKeys keys;
   __device__ __forceinline__ void load(const PgParams& p) {
-    keys = keys_of(p, b);
-    tiles = (keys.n + PgCfg<HD>::KEYS - 1) / PgCfg<HD>::KEYS;
+    keys = keys_of(p, p.lengths[b]);
+    tiles = (keys.n + KEYS - 1) / KEYS;
+  }
+  // to the first tile of the next row of scores; false if there is none
+  __device__ __forceinline__ bool next_row(const PgParams& p) {
+    at += kRowCost;
+    j = 0;
+    if (++hr < p.kv_heads * p.row_tiles) return true;
+    hr = 0;
+    do {
+      if (++b >= p.B) return false;
+      load(p);
+    } while (tiles == 0);
+    return true;
   }
   // to the next tile, which there has to be
   __device__ __forceinline__ void step(const PgParams& p) {
-    if (++j < tiles) return;
-    j = 0;
-    if (++hr < p.kv_heads * p.row_tiles) return;
-    hr = 0;
-    do {
-      ++b;
-      load(p);
-    } while (tiles == 0 && b + 1 < p.B);
+    ++at;
+    if (++j == tiles) next_row(p);
   }
 };
 
-__device__ __forceinline__ float alibi_log2(int mode, float slope, int dist) {
-  const float d = (float)dist;
-  if (mode == 1) return -slope * kLog2e * d;
-  const int drop = mode == 2 ? 13 : 16;
-  return -round_significand(round_significand(d, drop) * slope, drop) * kLog2e;
+// a * b / c and a / c, rounded down, for values below 2^53
+__device__ __forceinline__ int64_t floor_div(int64_t n, int64_t d) {
+  int64_t q = (int64_t)((double)n / (double)d);
+  if (q * d > n) --q;
+  if ((q + 1) * d <= n) ++q;
+  return q;
 }
+// The line has kRowCost units and one for each tile of a row, and is cut into `parts` stretches of whole units, one for each
+// warp; with fewer units than warps, of one unit.
+struct Line {
+  int64_t units, parts;
+  __device__ __forceinline__ Line(int64_t units_, int ctas) : units(units_), parts(min(units_, (int64_t)ctas * PG_WARPS)) {}
+  __device__ __forceinline__ int64_t begin(int64_t part) const { return part < parts ? floor_div(part * units, parts) : units; }
+  // the block whose warps have unit t
+  __device__ __forceinline__ int block_of(int64_t t) const { return (int)(floor_div((t + 1) * parts - 1, units) / PG_WARPS); }
+};
+__device__ __forceinline__ int row_units(int tiles) { return tiles ? tiles + kRowCost : 0; }
+
+__device__ __forceinline__ float alibi_rounded_log2(int mode, float slope, float dist) {  // slope already rounded
+  const int drop = mode == 2 ? 13 : 16;
+  return -round_significand(round_significand(dist, drop) * slope, drop) * kLog2e;
+}
+
+// What a block knows of its warps' pieces when it joins them.
+struct Pieces {
+  int64_t begin[PG_WARPS][2];  // the piece's row's first tile in the line
+  int b[PG_WARPS][2], hr[PG_WARPS][2], tiles[PG_WARPS][2];
+  int has[PG_WARPS][2];        // [0] a piece that began before the warp's stretch, [1] one that goes on behind it
+  int ends[PG_WARPS];          // piece [0] is its row's last
+};
 
 }  // namespace
 
-template <typename T, int HD, int NT, bool BIAS>
-__global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const PgParams p) {
-  using C = PgCfg<HD>;
-  constexpr int R = 8 * NT;
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int64_t sh_scan[PG_WARPS + 1];
-  __shared__ int64_t sh_from[PG_WARPS], sh_to[PG_WARPS];
-  __shared__ int64_t sh_base[PG_WARPS];
+// BIAS: 0 none, 1 exact slopes, 2 slopes rounded as a table's
+template <typename T, int HD, int NT, int BIAS, bool TMA>
+__global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __grid_constant__ CUtensorMap tmK,
+                                                                      const __grid_constant__ CUtensorMap tmV, const PgParams p) {
+  using C = PgCfg<HD, NT, BIAS>;
+  constexpr int R = C::R, STAGES = C::STAGES, STAGE = 2 * C::TILE, KS = HD / 16;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ int64_t sh_scan[PG_WARPS], sh_from[PG_WARPS + 1], sh_base[PG_WARPS];
   __shared__ int sh_b[PG_WARPS];
+  __shared__ Pieces sh;
+  __shared__ int sh_abort, sh_last[2], sh_first[2];
+  volatile int* abort_flag = &sh_abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int heads = p.kv_heads * p.row_tiles;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR) + warp * STAGES;
 
+  if (TMA && lane == 0) {
+    for (int i = 0; i < STAGES; ++i) mbar_init(&full[i], 1);
+    mbar_fence_init();
+  }
+  if (threadIdx.x == 0) *abort_flag = 0;
+  if (lane == 0) sh.has[warp][0] = sh.has[warp][1] = 0;
   grid_dependency_wait();
   allow_dependents();
 
-  // ---- the block's stretches: a scan over the sequences' tiles
+  // ---- the warps' stretches: a scan over the sequences' tiles
   const int per = (p.B + PG_WARPS * 32 - 1) / (PG_WARPS * 32);
   const int b_lo = min((int)threadIdx.x * per, p.B), b_hi = min(b_lo + per, p.B);
   int64_t mine = 0;
-  for (int b = b_lo; b < b_hi; ++b) mine += (keys_of(p, b).n + C::KEYS - 1) / C::KEYS;
+  for (int b = b_lo; b < b_hi; ++b) mine += row_units((keys_of(p, p.lengths[b]).n + C::KEYS - 1) / C::KEYS);
   int64_t upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -193,481 +253,750 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const PgPa
     if (w < warp) base += v;
     total += v;
   }
-  // fewer tiles than warps: one tile each, the first warps of all blocks before their second ones
-  const int64_t line = total * heads, parts = min(line, (int64_t)p.warps);
-  auto part_of = [&](int w) {
-    return line < p.warps ? (int64_t)w * gridDim.x + blockIdx.x : (int64_t)blockIdx.x * PG_WARPS + w;
-  };
-  if (threadIdx.x < PG_WARPS) {
-    const int64_t x = part_of(threadIdx.x);
-    sh_from[threadIdx.x] = x < parts ? x * line / parts : 0;
-    sh_to[threadIdx.x] = x < parts ? (x + 1) * line / parts : 0;
-  }
+  const Line line(total * heads, p.ctas);
+  if (threadIdx.x <= PG_WARPS) sh_from[threadIdx.x] = line.units ? line.begin((int64_t)blockIdx.x * PG_WARPS + threadIdx.x) : 0;
   __syncthreads();
   for (int b = b_lo; b < b_hi; ++b) {
     const int len = p.lengths[b];
-    const int tiles = (keys_of(p, b).n + C::KEYS - 1) / C::KEYS;
-    if (blockIdx.x == 0) {
-      p.prefix[b] = base;
+    const int tiles = (keys_of(p, len).n + C::KEYS - 1) / C::KEYS;
+    if (b % (int)gridDim.x == (int)blockIdx.x) {
       if (len < 0 || (int64_t)len + (p.k_new ? 1 : 0) > p.map.capacity()) atomicCAS(&g_dev_status, 0, kBadLength);
+      if (tiles == 0) {  // no keys: zeros
+        T* out = static_cast<T*>(p.out) + b * p.o_b;
+        for (int h = 0; h < p.kv_heads * p.group; ++h)
+          for (int d = 0; d < HD; ++d) out[h * p.o_h + d] = Num<T>::from_f(0.f);
+      }
     }
 #pragma unroll
-    for (int w = 0; w < PG_WARPS; ++w)
-      if (sh_from[w] >= base * heads && sh_from[w] < (base + tiles) * heads) {
+    for (int w = 0; w < PG_WARPS; ++w) {
+      const int64_t f = sh_from[w];
+      if (f >= base * heads && f < (base + row_units(tiles)) * heads) {
         sh_b[w] = b;
-        sh_base[w] = base;
+        sh_base[w] = base * heads;
       }
-    base += tiles;
+    }
+    base += row_units(tiles);
   }
-  if (blockIdx.x == 0 && threadIdx.x == 0) p.prefix[p.B] = total;
+  if (sh_from[0] >= line.units) return;  // nothing for this block
   __syncthreads();
   const int64_t from = sh_from[warp];
-  const int count = (int)(sh_to[warp] - from);
-  if (count <= 0) return;  // no barrier of the block below
+  const int length = (int)(sh_from[warp + 1] - from);
 
-  uint8_t* ring = smem + warp * PG_STAGES * C::STAGE;
-  const uint32_t ring_at = smem_addr(ring);
-
-  Cursor<HD> ld;
-  {
-    ld.b = sh_b[warp];
-    ld.load(p);
-    const int64_t in = from - sh_base[warp] * heads;
-    ld.hr = (int)(in / ld.tiles);
-    ld.j = (int)(in % ld.tiles);
-  }
-  Cursor<HD> cu = ld;
-
-  // Page and row of the keys that this lane looks up, one tile ahead of the copies.
-  int page[C::OWN], row[C::OWN];
-  auto look_up = [&]() {
-#pragma unroll
-    for (int u = 0; u < C::OWN; ++u) {
-      const int kk = lane + 32 * u, slot = ld.j * C::KEYS + kk;
-      page[u] = -1;
-      row[u] = 0;
-      if (kk < C::KEYS && slot < ld.keys.n && slot != ld.keys.fresh) {
-        const int i = (int)((unsigned)slot / (unsigned)p.map.page);
-        row[u] = slot - i * p.map.page;
-        page[u] = p.map.tables[ld.b * p.map.table_ld + i];
-      }
-    }
+  uint8_t* ring = smem + warp * STAGES * STAGE;
+  const uint32_t ring_at = smem_u32(ring);
+  uint8_t* places = smem + C::OFF_POS + warp * STAGES * C::KEYS * 4;
+  float2* my_ml = reinterpret_cast<float2*>(smem + C::OFF_ML) + warp * 2 * R;
+  auto head_piece = [&](int w) {
+    return C::HEAD_SMEM ? reinterpret_cast<float*>(smem + C::OFF_HEAD) + w * (R * HD)
+                        : p.heads_acc + ((int64_t)blockIdx.x * PG_WARPS + w) * (R * HD);
   };
-  auto copy = [&](int stage) {
-    const uint32_t at = ring_at + stage * C::STAGE;
-    const int head = ld.hr / p.row_tiles;
-    int64_t off[C::OWN];
+  const int g8 = lane >> 2, j2 = 2 * (lane & 3);  // row of an 8x8 block, first of its two columns
+  // With at most four query heads the instruction's other four columns repeat them, and carry what the rounding of the
+  // probabilities to 16 bits leaves: the product then has twice the bits, for the price of that subtraction.
+  const bool fine = NT == 1 && p.group <= 4;
+  const bool rest = fine && j2 >= 4;
+
+  Cursor<C::KEYS> cu;
+  cu.at = length;
+  if (length > 0) {
+    cu.b = sh_b[warp];
+    cu.load(p);
+    const int64_t in = from - sh_base[warp];  // units of the sequence before the stretch
+    const int units = row_units(cu.tiles);
+    cu.hr = in < (1LL << 31) ? (int)((uint32_t)in / (uint32_t)units) : (int)(in / units);
+    cu.j = (int)(in - (int64_t)cu.hr * units) - kRowCost;
+    cu.at = max(-cu.j, 0);
+    cu.j = max(cu.j, 0);
+  }
+  if (cu.at < length) {
+    Cursor<C::KEYS> ld = cu;
+
+    // Page and row of what this lane looks up, one tile ahead of the copies: box `lane` of the tile, or keys lane, lane + 32.
+    int page[C::OWN], row[C::OWN];
+    auto look_up = [&]() {
 #pragma unroll
-    for (int u = 0; u < C::OWN; ++u) {
-      const int kk = lane + 32 * u, slot = ld.j * C::KEYS + kk;
-      const bool wanted = kk < C::KEYS && slot < ld.keys.n && slot != ld.keys.fresh;
-      const bool ok = wanted && page[u] >= 0 && page[u] < p.map.num_pages;
-      if (wanted && !ok) atomicCAS(&g_dev_status, 0, kBadPage);
-      off[u] = ok ? row_offset(p.map, page[u], head, row[u]) : slot == ld.keys.fresh ? -2 : -1;
-      if (BIAS && p.positions && kk < C::KEYS)
-        cp4(at + 2 * C::TILE + kk * 4, ok ? p.positions + stat_offset(p.map, page[u], p.kv_heads, head, row[u]) : p.positions,
-            ok ? 4 : 0);
-    }
-    const T* k = static_cast<const T*>(p.k) + (lane % C::CHUNKS) * 8;
-    const T* v = static_cast<const T*>(p.v) + (lane % C::CHUNKS) * 8;
-#pragma unroll
-    for (int i = 0; i < C::ITERS; ++i) {
-      const int kk = i * C::RPI + lane / C::CHUNKS;
-      const int64_t o = __shfl_sync(0xffffffffu, off[(i * C::RPI) / 32], kk & 31);
-      const uint32_t dst = at + tile_at<HD>(kk, lane % C::CHUNKS);
-      if (o != -2) {
-        cp16(dst, k + (o < 0 ? 0 : o), o < 0 ? 0 : 16);
-        cp16(dst + C::TILE, v + (o < 0 ? 0 : o), o < 0 ? 0 : 16);
-      }
-    }
-    const int kk = ld.keys.fresh - ld.j * C::KEYS;
-    if (ld.keys.fresh >= 0 && kk >= 0 && kk < C::KEYS && lane < C::CHUNKS) {  // the new token's row is not in the pages yet
-      const T* kn = static_cast<const T*>(p.k_new) + ld.b * p.kn_b + head * p.kn_h + lane * 8;
-      const T* vn = static_cast<const T*>(p.v_new) + ld.b * p.vn_b + head * p.vn_h + lane * 8;
-      const uint32_t o = stage * C::STAGE + tile_at<HD>(kk, lane);
-      if (p.new_vec) {
-        cp16(ring_at + o, kn, 16);
-        cp16(ring_at + o + C::TILE, vn, 16);
-      } else {
-        T* dk = reinterpret_cast<T*>(ring + o);
-        T* dv = reinterpret_cast<T*>(ring + o + C::TILE);
-        for (int e = 0; e < 8; ++e) {
-          dk[e] = kn[e];
-          dv[e] = vn[e];
+      for (int u = 0; u < (TMA ? 1 : C::OWN); ++u) {
+        const int kk = TMA ? lane << p.box_log2 : lane + 32 * u, slot = ld.j * C::KEYS + kk;
+        page[u] = -1;
+        row[u] = 0;
+        if (kk < C::KEYS && slot < ld.keys.cached()) {
+          const int i = (int)((unsigned)slot / (unsigned)p.map.page);
+          row[u] = slot - i * p.map.page;
+          page[u] = p.map.tables[ld.b * p.map.table_ld + i];
         }
       }
-    }
-  };
-
-  look_up();
-  int issued = 0;
-  auto issue = [&]() {  // the next tile, if there is one, and always a group
-    if (issued < count) {
-      copy(issued % PG_STAGES);
-      if (++issued < count) {
-        ld.step(p);
-        look_up();
-      }
-    }
-    cp_commit();
-  };
+    };
+    auto copy = [&](int stage) {
+      const int head = ld.hr / p.row_tiles, cached = ld.keys.cached(), slot0 = ld.j * C::KEYS;
+      if constexpr (TMA) {
+        const int box = 1 << p.box_log2;
+        const bool wanted = (lane << p.box_log2) < C::KEYS && slot0 + (lane << p.box_log2) < cached;
+        const bool ok = wanted && (unsigned)page[0] < (unsigned)p.map.num_pages;
+        const unsigned loads = __ballot_sync(0xffffffffu, ok);
+        if (lane == 0) mbar_expect_tx(&full[stage], __popc(loads) * box * HD * 4);
+        __syncwarp();
+        uint8_t* dst = ring + stage * STAGE + (lane << p.box_log2) * (HD == 32 ? 64 : 128);
+        if (ok) {
 #pragma unroll
-  for (int i = 0; i < PG_STAGES - 1; ++i) issue();
+          for (int c = 0; c < C::PANELS; ++c) {
+            tma_load_4d(dst + c * C::KEYS * 128, &tmK, c * 64, row[0], head, page[0], &full[stage]);
+            tma_load_4d(dst + C::TILE + c * C::KEYS * 128, &tmV, c * 64, row[0], head, page[0], &full[stage]);
+          }
+        } else if (wanted) {  // no such page: zeros
+          atomicCAS(&g_dev_status, 0, kBadPage);
+          for (int kk = 0; kk < box; ++kk)
+            for (int c = 0; c < C::CHUNKS; ++c) {
+              const uint32_t o = stage * STAGE + tile_at<HD>((lane << p.box_log2) + kk, c);
+              *reinterpret_cast<uint4*>(ring + o) = make_uint4(0, 0, 0, 0);
+              *reinterpret_cast<uint4*>(ring + o + C::TILE) = make_uint4(0, 0, 0, 0);
+            }
+          fence_proxy_async_smem();
+        }
+        if (BIAS && p.positions) {
+#pragma unroll
+          for (int u = 0; u < C::OWN; ++u) {
+            const int kk = lane + 32 * u, who = (kk >> p.box_log2) & 31;
+            const int pg = __shfl_sync(0xffffffffu, page[0], who), r0 = __shfl_sync(0xffffffffu, row[0], who);
+            if (kk < C::KEYS && (loads >> who & 1) != 0)
+              cp4(smem_u32(places) + (stage * C::KEYS + kk) * 4,
+                  p.positions + stat_offset(p.map, pg, p.kv_heads, head, r0 + (kk & (box - 1))), 4);
+          }
+          cp_commit();
+        }
+      } else {
+        const uint32_t at = ring_at + stage * STAGE;
+        int64_t off[C::OWN];
+#pragma unroll
+        for (int u = 0; u < C::OWN; ++u) {
+          const int kk = lane + 32 * u;
+          const bool wanted = kk < C::KEYS && slot0 + kk < cached;
+          const bool ok = wanted && (unsigned)page[u] < (unsigned)p.map.num_pages;
+          if (wanted && !ok) atomicCAS(&g_dev_status, 0, kBadPage);
+          off[u] = ok ? row_offset(p.map, page[u], head, row[u]) : -1;
+          if (BIAS && p.positions && kk < C::KEYS)
+            cp4(smem_u32(places) + (stage * C::KEYS + kk) * 4,
+                ok ? p.positions + stat_offset(p.map, page[u], p.kv_heads, head, row[u]) : p.positions, ok ? 4 : 0);
+        }
+        const T* k = static_cast<const T*>(p.k) + (lane % C::CHUNKS) * 8;
+        const T* v = static_cast<const T*>(p.v) + (lane % C::CHUNKS) * 8;
+#pragma unroll
+        for (int i = 0; i < C::ITERS; ++i) {
+          const int kk = i * C::RPI + lane / C::CHUNKS;
+          const int64_t o = __shfl_sync(0xffffffffu, off[(i * C::RPI) / 32], kk & 31);
+          const uint32_t dst = at + tile_at<HD>(kk, lane % C::CHUNKS);
+          cp16(dst, k + (o < 0 ? 0 : o), o < 0 ? 0 : 16);
+          cp16(dst + C::TILE, v + (o < 0 ? 0 : o), o < 0 ? 0 : 16);
+        }
+        cp_commit();
+      }
+    };
 
-  const int g8 = lane >> 2, j2 = 2 * (lane & 3);  // row of an 8x8 block, first of its two columns
-  uint32_t qf[NT][HD / 16][2];
-  float slope[NT][2];
-  float ref[NT][2], sum[NT][2], o[HD / 16][NT][4];
-  int here = 0, first = 0;  // the query's position; whether the piece began with its row's first tile
-  bool begin = true;
-  const int mi = lane >> 3, l8 = lane & 7;
+    look_up();
+    int into = 0;
+    auto issue = [&]() {  // the next tile, if there is one; groups of cp.async are counted either way
+      if (ld.at < length) {
+        copy(into);
+        if (++into == STAGES) into = 0;
+        ld.step(p);
+        if (ld.at < length) look_up();
+      } else if (!TMA || (BIAS && p.positions)) {
+        cp_commit();
+      }
+    };
 
-  for (int t = 0; t < count; ++t) {
-    if (begin) {
-      begin = false;
-      first = cu.j == 0;
-      const int kv = cu.hr / p.row_tiles, r0 = (cu.hr % p.row_tiles) * R;
-      const T* q = static_cast<const T*>(p.q) + cu.b * p.q_b;
-      const bool pairs = ((reinterpret_cast<uintptr_t>(p.q) | (uintptr_t)(p.q_b * 2) | (uintptr_t)(p.q_h * 2)) & 3) == 0;
+    // What a row of scores needs beside its keys is read while the row before it is worked on: the query, the slopes, the
+    // query's position, and 16 bytes of the new token's rows with the page that they go to.
+    struct Row {
+      uint32_t q[NT][KS][2];
+      float slope[NT][2];
+      int here, page;
+      uint4 fresh;
+    };
+    auto fetch = [&](const Cursor<C::KEYS>& c, Row& w) {
+      const int kv = c.hr / p.row_tiles, r0 = (c.hr - kv * p.row_tiles) * R;
+      const T* q = static_cast<const T*>(p.q) + c.b * p.q_b;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const int r = r0 + nt * 8 + g8;
+        const int r = r0 + (fine ? g8 & 3 : nt * 8 + g8);
         const T* qr = q + (int64_t)(kv * p.group + r) * p.q_h + j2;
 #pragma unroll
-        for (int ks = 0; ks < HD / 16; ++ks)
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             uint32_t v = 0;
             if (r < p.group) {
               const T* at = qr + ks * 16 + half * 8;
-              if (pairs) v = *reinterpret_cast<const uint32_t*>(at);
+              if (p.q_pairs) v = *reinterpret_cast<const uint32_t*>(at);
               else v = (uint32_t)*reinterpret_cast<const uint16_t*>(at) |
                        (uint32_t)*reinterpret_cast<const uint16_t*>(at + 1) << 16;
             }
-            qf[nt][ks][half] = v;
+            w.q[nt][ks][half] = v;
           }
+        if (BIAS)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int rr = r0 + nt * 8 + j2 + e;
-          slope[nt][e] = BIAS && rr < p.group ? p.slopes[kv * p.group + rr] : 0.f;
-          if (BIAS && p.bias_mode == 2) slope[nt][e] = __half2float(__float2half_rn(slope[nt][e]));
-          if (BIAS && p.bias_mode == 4) slope[nt][e] = __bfloat162float(__float2bfloat16_rn(slope[nt][e]));
-          ref[nt][e] = kNone;
-          sum[nt][e] = 0.f;
+          for (int e = 0; e < 2; ++e) {
+            const int rr = r0 + (fine ? (j2 + e) & 3 : nt * 8 + j2 + e);
+            w.slope[nt][e] = rr < p.group ? p.slopes[kv * p.group + rr] : 0.f;
+          }
+      }
+      if (BIAS) w.here = p.query_positions ? p.query_positions[c.b] : c.keys.n - 1;
+      w.fresh = make_uint4(0, 0, 0, 0);
+      w.page = -1;
+      if (c.keys.fresh >= 0) {
+        w.page = p.map.tables[c.b * p.map.table_ld + (unsigned)c.keys.fresh / (unsigned)p.map.page];
+        if (lane < 2 * C::CHUNKS) {
+          const T* at = lane < C::CHUNKS ? static_cast<const T*>(p.k_new) + c.b * p.kn_b + kv * p.kn_h + lane * 8
+                                         : static_cast<const T*>(p.v_new) + c.b * p.vn_b + kv * p.vn_h + (lane - C::CHUNKS) * 8;
+          if (p.new_vec) w.fresh = *reinterpret_cast<const uint4*>(at);
+          else
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              reinterpret_cast<uint32_t*>(&w.fresh)[e] = (uint32_t)*reinterpret_cast<const uint16_t*>(at + 2 * e) |
+                                                         (uint32_t)*reinterpret_cast<const uint16_t*>(at + 2 * e + 1) << 16;
         }
       }
-      if (BIAS) here = p.query_positions ? p.query_positions[cu.b] : cu.keys.n - 1;
-#pragma unroll
-      for (int m = 0; m < HD / 16; ++m)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[m][nt][e] = 0.f;
-    }
-    cp_wait<PG_STAGES - 2>();
-    __syncwarp();
-    issue();  // into the stage that the tile before this one has left
-    const uint32_t kt = ring_at + (t % PG_STAGES) * C::STAGE, vt = kt + C::TILE;
+    };
+    Row now, ahead;
+    Cursor<C::KEYS> rows = cu;  // the row of `ahead`
 
-    // ---- scores: keys g8 and g8 + 8 of each block of 16, heads j2 and j2 + 1
-    float s[C::MT][NT][4];
-#pragma unroll
-    for (int m = 0; m < C::MT; ++m) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[m][nt][e] = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < HD / 16; ++ks) {
-        uint32_t a[4];
-        ldm4(a, kt + tile_at<HD>(m * 16 + (mi & 1) * 8 + l8, ks * 2 + (mi >> 1)));
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma<T>(s[m][nt], a, qf[nt][ks][0], qf[nt][ks][1]);
-      }
-    }
-    const int slot0 = cu.j * C::KEYS;
-    const bool ragged = slot0 + C::KEYS > cu.keys.n;
-    float top[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) top[nt][0] = top[nt][1] = kNone;
-#pragma unroll
-    for (int m = 0; m < C::MT; ++m)
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int kk = m * 16 + half * 8 + g8, slot = slot0 + kk;
-        int dist = 0;
-        if (BIAS) {
-          const int at = p.positions ? reinterpret_cast<const int*>(ring + (t % PG_STAGES) * C::STAGE + 2 * C::TILE)[kk] : slot;
-          dist = slot == cu.keys.fresh ? 0 : here - at;
+    // where ldmatrix reads: chunk 0 of the lane's row; the chunk number's higher bits are xor-ed in
+    const int mi = lane >> 3, l8 = lane & 7;
+    const uint32_t k_at = tile_at<HD>((mi & 1) * 8 + l8, mi >> 1), v_at = tile_at<HD>((mi >> 1) * 8 + l8, mi & 1) + C::TILE;
+    constexpr int PER_PANEL = HD == 32 ? 2 : 4;  // k-steps in a row of at most 128 bytes
+    constexpr uint32_t BLOCK16 = 16 * (HD == 32 ? 64 : 128), PANEL = C::KEYS * 128;
+
+    float ref[NT][2], sum[NT][2], o[KS][NT][4];
+    int first = 0;  // whether the piece began with its row's first tile
+    bool begin = true;
+    int stage = 0, warm_up = STAGES - 1;  // tiles to copy before the first one is worked on
+    int fetches = 2;                      // of the next row's things; for the first row also its own
+    uint32_t phase = 0;
+
+    // (Code that runs once or twice in a short call costs its way from the L2 into the instruction cache, so the copies and
+    // the fetch stand here once each.)
+    for (;;) {
+      if (begin && warm_up == 0) {
+        begin = false;
+        first = cu.j == 0;
+#pragma unroll 1
+        for (; fetches > 0; --fetches) {
+          now = ahead;
+          if (fetches == 2 || (cu.at + cu.tiles - cu.j + kRowCost < length && rows.next_row(p))) fetch(rows, ahead);
         }
+        fetches = 1;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float x = s[m][nt][2 * half + e] * p.scale;
-            if (BIAS) x += alibi_log2(p.bias_mode, slope[nt][e], dist);
-            if (ragged && slot >= cu.keys.n) x = kNone;
-            s[m][nt][2 * half + e] = x;
-            top[nt][e] = fmaxf(top[nt][e], x);
+            if (BIAS) {
+              float& sl = now.slope[nt][e];
+              if (BIAS == 1) sl *= -kLog2e;
+              if (p.bias_mode == 2) sl = __half2float(__float2half_rn(sl));
+              if (p.bias_mode == 4) sl = __bfloat162float(__float2bfloat16_rn(sl));
+            }
+            ref[nt][e] = kNone;
+            sum[nt][e] = 0.f;
           }
+#pragma unroll
+        for (int m = 0; m < KS; ++m)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[m][nt][e] = 0.f;
       }
-    if (p.scores) {
-      const int kv = cu.hr / p.row_tiles, r0 = (cu.hr % p.row_tiles) * R;
-      const int64_t cap = p.map.capacity();
-      float* sc = p.scores + ((int64_t)(cu.b * p.kv_heads + kv) * p.group + r0) * cap + slot0;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int r = nt * 8 + j2 + e;
-          if (r0 + r < p.group)
-#pragma unroll
-            for (int m = 0; m < C::MT; ++m)
-#pragma unroll
-              for (int half = 0; half < 2; ++half) {
-                const int kk = m * 16 + half * 8 + g8;
-                if (slot0 + kk < cu.keys.n) sc[r * cap + kk] = s[m][nt][2 * half + e];
-              }
+      if (warm_up == 0) {
+        if (!TMA || (BIAS && p.positions)) cp_wait<STAGES - 2>();
+        if (TMA && !__all_sync(0xffffffffu, mbar_wait(&full[stage], phase, 0x9000 | stage, abort_flag))) break;
+        __syncwarp();
+      }
+      issue();  // into the stage that the tile before this one has left
+      if (warm_up > 0) {
+        --warm_up;
+        continue;
+      }
+      const uint32_t tile = ring_at + stage * STAGE;
+      const int slot0 = cu.j * C::KEYS, cached = cu.keys.cached();
+      const bool ragged = slot0 + C::KEYS > cached;
+      if (ragged) {  // rows behind the last cached key may hold anything; the new token's are not in the pages yet
+        const int kv = cu.hr / p.row_tiles;
+        uint8_t* at = ring + stage * STAGE;
+        for (int i = lane; i < (C::KEYS - (cached - slot0)) * C::CHUNKS; i += 32) {
+          const uint32_t dst = tile_at<HD>(cached - slot0 + i / C::CHUNKS, i % C::CHUNKS);
+          *reinterpret_cast<uint4*>(at + dst) = make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(at + dst + C::TILE) = make_uint4(0, 0, 0, 0);
         }
-    }
-    // ---- a new reference where the maximum has run away from the old one
-    bool away = false;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) away |= top[nt][0] > ref[nt][0] + kAhead || top[nt][1] > ref[nt][1] + kAhead;
-    if (__any_sync(0xffffffffu, away)) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float x = top[nt][e];
-#pragma unroll
-          for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-          if (x > ref[nt][e] + kAhead) {
-            const float f = ref[nt][e] == kNone ? 0.f : ex2(ref[nt][e] - (x - kBelow));
-            ref[nt][e] = x - kBelow;
-            sum[nt][e] *= f;
-#pragma unroll
-            for (int m = 0; m < HD / 16; ++m) {
-              o[m][nt][e] *= f;
-              o[m][nt][2 + e] *= f;
+        const int kk = cu.keys.fresh - slot0;  // at least 0, because there is a cached key in every tile before it
+        if (cu.keys.fresh >= 0 && kk < C::KEYS) {
+          __syncwarp();
+          const int c = lane % C::CHUNKS;
+          if (lane < 2 * C::CHUNKS) *reinterpret_cast<uint4*>(at + tile_at<HD>(kk, c) + (lane < C::CHUNKS ? 0 : C::TILE)) = now.fresh;
+          if (cu.hr == kv * p.row_tiles) {  // one of the row's head tiles writes it into its slot
+            const int r0 = cu.keys.fresh % p.map.page;
+            if ((unsigned)now.page < (unsigned)p.map.num_pages) {
+              if (lane < 2 * C::CHUNKS)
+                *reinterpret_cast<uint4*>(static_cast<T*>(lane < C::CHUNKS ? p.k : p.v) + row_offset(p.map, now.page, kv, r0) + c * 8) =
+                    now.fresh;
+              if (p.positions && lane == 0)
+                p.positions[stat_offset(p.map, now.page, p.kv_heads, kv, r0)] =
+                    p.query_positions ? p.query_positions[cu.b] : cu.keys.fresh;
+            } else {
+              atomicCAS(&g_dev_status, 0, kBadPage);
             }
           }
         }
-    }
-    // ---- probabilities, rounded to the values' type for the second product; the sum takes them unrounded
-    uint32_t pt[C::MT][NT][2];
+        if (TMA) fence_proxy_async_smem();
+        __syncwarp();
+      }
+
+      // ---- scores: keys g8 and g8 + 8 of each block of 16, heads j2 and j2 + 1
+      float s[C::MT][NT][4];
 #pragma unroll
-    for (int m = 0; m < C::MT; ++m)
+      for (int m = 0; m < C::MT; ++m) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[m][nt][e] = 0.f;
+      }
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int m = 0; m < C::MT; ++m) {
+          uint32_t a[4];
+          ldm4(a, tile + (k_at ^ ((ks % PER_PANEL) << 5)) + (ks / PER_PANEL) * PANEL + m * BLOCK16);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma<T>(s[m][nt], a, now.q[nt][ks][0], now.q[nt][ks][1]);
+        }
+      float top[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) top[nt][0] = top[nt][1] = kNone;
+      const int* place = reinterpret_cast<const int*>(places) + stage * C::KEYS;
+#pragma unroll
+      for (int m = 0; m < C::MT; ++m)
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          float w[2];
+          const int kk = m * 16 + half * 8 + g8;
+          float dist = 0.f;
+          if (BIAS) dist = (float)(now.here - (p.positions ? place[kk] : slot0 + kk));
+          if (BIAS && ragged && slot0 + kk == cu.keys.fresh) dist = 0.f;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float x = s[m][nt][2 * half + e] * p.scale;
+              if (BIAS == 1) x = fmaf(now.slope[nt][e], dist, x);
+              if (BIAS == 2) x += alibi_rounded_log2(p.bias_mode, now.slope[nt][e], dist);
+              s[m][nt][2 * half + e] = x;
+            }
+        }
+      if (ragged) {
+#pragma unroll
+        for (int m = 0; m < C::MT; ++m)
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+            if (slot0 + m * 16 + half * 8 + g8 >= cu.keys.n)
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) s[m][nt][2 * half] = s[m][nt][2 * half + 1] = kNone;
+      }
+#pragma unroll
+      for (int m = 0; m < C::MT; ++m)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) top[nt][e] = fmaxf(top[nt][e], fmaxf(s[m][nt][e], s[m][nt][2 + e]));
+      if (p.scores) {
+        const int kv = cu.hr / p.row_tiles, r0 = (cu.hr - kv * p.row_tiles) * R + j2;
+        float* sc = p.scores + (((int64_t)cu.b * p.kv_heads + kv) * p.map.capacity() + slot0 + g8) * p.group + r0;
+        const int left = ragged ? cu.keys.n - slot0 - g8 : C::KEYS;  // keys from this lane's first on
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (r0 + nt * 8 + e < p.group)
+#pragma unroll
+              for (int m = 0; m < C::MT; ++m)
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+                  if (m * 16 + half * 8 < left) sc[(m * 16 + half * 8) * p.group + nt * 8 + e] = s[m][nt][2 * half + e];
+      }
+      // ---- a new reference where the maximum has run away from the old one
+      bool away = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) away |= top[nt][0] > ref[nt][0] + kAhead || top[nt][1] > ref[nt][1] + kAhead;
+      if (__any_sync(0xffffffffu, away)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            w[e] = ex2(s[m][nt][2 * half + e] - (ref[nt][e] == kNone ? 0.f : ref[nt][e]));
-            sum[nt][e] += w[e];
-          }
-          pt[m][nt][half] = transpose8(pack2<T>(w[0], w[1]));
-        }
+            float x = top[nt][e];
 #pragma unroll
-    for (int m = 0; m < C::MT; ++m)
+            for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+            if (x > ref[nt][e] + kAhead) {
+              const float f = ref[nt][e] == kNone ? 0.f : ex2(ref[nt][e] - (x - kBelow));
+              ref[nt][e] = x - kBelow;
+              sum[nt][e] *= f;
 #pragma unroll
-      for (int hm = 0; hm < HD / 16; ++hm) {
-        uint32_t a[4];
-        ldm4t(a, vt + tile_at<HD>(m * 16 + (mi >> 1) * 8 + l8, hm * 2 + (mi & 1)));
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma<T>(o[hm][nt], a, pt[m][nt][0], pt[m][nt][1]);
-      }
-
-    // ---- the end of a row of scores, or of the stretch
-    const bool last = cu.j + 1 == cu.tiles;
-    if (last || t + 1 == count) {
-      begin = true;
-      const int kv = cu.hr / p.row_tiles, r0 = (cu.hr % p.row_tiles) * R;
-      const int64_t piece = 2 * part_of(warp) + first;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float l = sum[nt][e];
-#pragma unroll
-          for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-          const int r = nt * 8 + j2 + e;
-          if (r0 + r < p.group) {
-            const int64_t head = kv * p.group + r0 + r;
-            if (first && last) {
-              const float inv = l > 0.f ? 1.f / l : l;  // a row whose weights are all zero is zero; NaN stays
-              T* out = static_cast<T*>(p.out) + cu.b * p.o_b + head * p.o_h;
-#pragma unroll
-              for (int m = 0; m < HD / 16; ++m) {
-                out[m * 16 + g8] = Num<T>::from_f(o[m][nt][e] * inv);
-                out[m * 16 + 8 + g8] = Num<T>::from_f(o[m][nt][2 + e] * inv);
+              for (int m = 0; m < KS; ++m) {
+                o[m][nt][e] *= f;
+                o[m][nt][2 + e] *= f;
               }
-              if (g8 == 0) p.lse[(int64_t)cu.b * p.kv_heads * p.group + head] = ref[nt][e] + __log2f(l);
-            } else {
-              float* acc = p.acc + (piece * R + r) * HD;
-#pragma unroll
-              for (int m = 0; m < HD / 16; ++m) {
-                acc[m * 16 + g8] = o[m][nt][e];
-                acc[m * 16 + 8 + g8] = o[m][nt][2 + e];
-              }
-              if (g8 == 0) p.ml[piece * R + r] = make_float2(ref[nt][e], l);
             }
           }
-        }
-    }
-    if (t + 1 < count) cu.step(p);
-  }
-  cp_wait<0>();
-}
-
-// Joins the pieces of rows that several warps shared, adds the weights to the masses, and writes the new token's row into its
-// slot.  One block per (sequence, key head) and share of its keys (blockIdx.y; the first one joins and writes).
-template <typename T, int HD>
-__global__ void __launch_bounds__(256) paged_finish_kernel(const PgParams p, const int R) {
-  constexpr int KEYS = PgCfg<HD>::KEYS;
-  constexpr int LANES = HD, SHARES = 256 / LANES;
-  __shared__ float sh_lse[128], sh_ref[128], sh_inv[128];
-  __shared__ float sh_acc[SHARES][HD];
-  grid_dependency_wait();
-  allow_dependents();
-  const int b = blockIdx.x / p.kv_heads, kv = blockIdx.x % p.kv_heads;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const SeqKeys keys = keys_of(p, b);
-  const int heads = p.kv_heads * p.row_tiles;
-  const int64_t line = p.prefix[p.B] * heads, parts = min(line, (int64_t)p.warps), at = p.prefix[b] * heads;
-  const int tiles = (keys.n + KEYS - 1) / KEYS;
-  const bool join = blockIdx.y == 0;
-  T* out = static_cast<T*>(p.out) + b * p.o_b + (int64_t)kv * p.group * p.o_h;
-
-  if (join && keys.fresh >= 0) {
-    int page, row;
-    if (find_slot(p.map, b, keys.fresh, page, row)) {
-      const int64_t o = row_offset(p.map, page, kv, row);
-      if (threadIdx.x < HD) {
-        static_cast<T*>(p.k)[o + threadIdx.x] = static_cast<const T*>(p.k_new)[b * p.kn_b + kv * p.kn_h + threadIdx.x];
-      } else if (threadIdx.x < 2 * HD) {
-        const int e = threadIdx.x - HD;
-        static_cast<T*>(p.v)[o + e] = static_cast<const T*>(p.v_new)[b * p.vn_b + kv * p.vn_h + e];
       }
-      if (p.positions && threadIdx.x == 0)
-        p.positions[stat_offset(p.map, page, p.kv_heads, kv, row)] = p.query_positions ? p.query_positions[b] : keys.fresh;
+      // ---- probabilities, rounded to the values' type for the second product; the sum takes them unrounded
+      uint32_t pt[C::MT][NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float from_ref[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) from_ref[e] = ref[nt][e] == kNone ? 0.f : ref[nt][e];
+#pragma unroll
+        for (int m = 0; m < C::MT; ++m)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            float w[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              w[e] = ex2(s[m][nt][2 * half + e] - from_ref[e]);
+              sum[nt][e] += w[e];
+            }
+            uint32_t u = pack2<T>(w[0], w[1]);
+            if (rest) {
+              const float2 f = Num<T>::to_f2(*reinterpret_cast<const typename Num<T>::T2*>(&u));
+              u = pack2<T>(w[0] - f.x, w[1] - f.y);
+            }
+            pt[m][nt][half] = transpose8(u);
+          }
+      }
+#pragma unroll
+      for (int m = 0; m < C::MT; ++m)
+#pragma unroll
+        for (int hm = 0; hm < KS; ++hm) {
+          uint32_t a[4];
+          ldm4t(a, tile + (v_at ^ ((hm % PER_PANEL) << 5)) + (hm / PER_PANEL) * PANEL + m * BLOCK16);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma<T>(o[hm][nt], a, pt[m][nt][0], pt[m][nt][1]);
+        }
+      if (++stage == STAGES) {
+        stage = 0;
+        phase ^= 1;
+      }
+
+      // ---- the end of a row of scores, or of the stretch
+      const bool last = cu.j + 1 == cu.tiles;
+      const int row_at = cu.at - cu.j, row_b = cu.b, row_hr = cu.hr, row_tiles = cu.tiles;
+      cu.step(p);
+      const bool done = cu.at >= length;
+      if (last || done) {
+        begin = true;
+        const int kv = row_hr / p.row_tiles, r0 = (row_hr - kv * p.row_tiles) * R;
+        const bool whole = first && last;
+        // a piece: [0] one that began before the stretch, in scratch while the ring is in use; [1] the stretch's last, over the ring
+        float* acc = first ? reinterpret_cast<float*>(ring) : head_piece(warp);
+        if (!whole) {
+          __syncwarp();  // the ring has been read
+          if (lane == 0) {
+            sh.has[warp][first] = 1;
+            sh.begin[warp][first] = from + row_at;
+            sh.b[warp][first] = row_b;
+            sh.hr[warp][first] = row_hr;
+            sh.tiles[warp][first] = row_tiles;
+            if (!first) sh.ends[warp] = last;
+          }
+        }
+        if (fine) {  // the rests' products
+#pragma unroll
+          for (int m = 0; m < KS; ++m)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[m][0][e] += __shfl_xor_sync(0xffffffffu, o[m][0][e], 2);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float l = sum[nt][e];
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+            const int r = nt * 8 + j2 + e;
+            if (r0 + r < p.group) {
+              const int64_t head = kv * p.group + r0 + r;
+              if (whole) {
+                const float inv = l > 0.f ? 1.f / l : l;  // a row whose weights are all zero is zero; NaN stays
+                T* out = static_cast<T*>(p.out) + row_b * p.o_b + head * p.o_h;
+#pragma unroll
+                for (int m = 0; m < KS; ++m) {
+                  out[m * 16 + g8] = Num<T>::from_f(o[m][nt][e] * inv);
+                  out[m * 16 + 8 + g8] = Num<T>::from_f(o[m][nt][2 + e] * inv);
+                }
+                if (p.lse && g8 == 0) p.lse[(int64_t)row_b * p.kv_heads * p.group + head] = ref[nt][e] + __log2f(l);
+              } else {
+#pragma unroll
+                for (int m = 0; m < KS; ++m) {
+                  acc[r * HD + m * 16 + g8] = o[m][nt][e];
+                  acc[r * HD + m * 16 + 8 + g8] = o[m][nt][2 + e];
+                }
+                if (g8 == 0) my_ml[first * R + r] = make_float2(ref[nt][e], l);
+              }
+            }
+          }
+        if (done) break;
+      }
     }
+    cp_wait<0>();
   }
-  if (tiles == 0) {  // no keys: zeros
-    if (join)
-      for (int i = threadIdx.x; i < p.group * HD; i += 256) out[(i / HD) * p.o_h + i % HD] = Num<T>::from_f(0.f);
+
+  // ---- the block joins its warps' pieces
+  __syncthreads();
+  if (*abort_flag) {
+    for (int k = 0; k < 64; ++k) __nanosleep(1000);
     return;
   }
-  // the stretch that tile t of the line is part of
-  auto owner = [&](int64_t t) { return ((t + 1) * parts - 1) / line; };
-
-  // ---- reference and sum of every query head
-  for (int r = warp; r < p.group; r += 8) {
-    const int64_t t0 = at + ((int64_t)kv * p.row_tiles + r / R) * tiles;
-    const int64_t w0 = owner(t0), w1 = owner(t0 + tiles - 1);
-    float lse = 0.f, ref = 0.f, inv = -1.f;  // inv < 0: the split kernel has written the row
-    if (w0 == w1) {
-      if (p.mass_out) lse = p.lse[((int64_t)b * p.kv_heads + kv) * p.group + r];
-    } else {
-      float m = kNone, l = 0.f;
-      for (int64_t w = w0 + lane; w <= w1; w += 32) m = fmaxf(m, p.ml[(2 * w + (w == w0)) * R + r % R].x);
-      m = warp_max(m);
-      for (int64_t w = w0 + lane; w <= w1; w += 32) {
-        const float2 v = p.ml[(2 * w + (w == w0)) * R + r % R];
-        l += v.y * (v.x == kNone ? (v.y == v.y ? 0.f : 1.f) : ex2(v.x - m));
+  const float2* ml = reinterpret_cast<const float2*>(smem + C::OFF_ML);
+  int job = 0, open[2] = {-1, -1};  // the first warps of the chains that begin, or end, in another block
+  for (int w = 0; w < PG_WARPS; ++w) {
+#pragma unroll
+    for (int slot = 0; slot < 2; ++slot) {
+      // a chain starts with a piece [1], or with the piece [0] of the first warp
+      if (!sh.has[w][slot] || (slot == 0 && w > 0)) continue;
+      int end = w;  // its last warp
+      bool ended = slot == 0 && sh.ends[w];
+      while (!ended && end + 1 < PG_WARPS && sh.has[end + 1][0]) ended = sh.ends[++end];
+      const bool whole = slot == 1 && ended;
+      if (!whole) open[slot] = w;
+      const int b = sh.b[w][slot], hr = sh.hr[w][slot];
+      const int kv = hr / p.row_tiles, r0 = (hr - kv * p.row_tiles) * R;
+      for (int r = 0; r < R && r0 + r < p.group; ++r) {
+        if (job++ % PG_WARPS != warp) continue;
+        float m = kNone, l = 0.f, a[HD / 32];
+        for (int i = w; i <= end; ++i) m = fmaxf(m, ml[(i * 2 + (i == w ? slot : 0)) * R + r].x);
+#pragma unroll
+        for (int e = 0; e < HD / 32; ++e) a[e] = 0.f;
+#pragma unroll(C::HEAD_SMEM ? 1 : 4)
+        for (int i = w; i <= end; ++i) {
+          const int which = i == w ? slot : 0;
+          const float2 v = ml[(i * 2 + which) * R + r];
+          const float* acc = (which ? reinterpret_cast<const float*>(smem + i * STAGES * STAGE) : head_piece(i)) + r * HD;
+          const float f = v.x == kNone ? 0.f : ex2(v.x - m);
+          l += v.y == v.y ? v.y * f : v.y;
+          if (v.x != kNone)
+#pragma unroll
+            for (int e = 0; e < HD / 32; ++e) a[e] += acc[e * 32 + lane] * f;
+        }
+        const int64_t head = kv * p.group + r0 + r;
+        if (whole) {
+          const float inv = l > 0.f ? 1.f / l : l;
+          T* out = static_cast<T*>(p.out) + b * p.o_b + head * p.o_h;
+#pragma unroll
+          for (int e = 0; e < HD / 32; ++e) out[e * 32 + lane] = Num<T>::from_f(a[e] * inv);
+          if (p.lse && lane == 0) p.lse[(int64_t)b * p.kv_heads * p.group + head] = m + __log2f(l);
+        } else {
+          const int64_t piece = 2 * (int64_t)blockIdx.x + slot;
+#pragma unroll
+          for (int e = 0; e < HD / 32; ++e) p.acc[(piece * R + r) * HD + e * 32 + lane] = a[e];
+          if (lane == 0) p.ml[piece * R + r] = make_float2(m, l);
+        }
       }
-      l = warp_sum(l);
-      ref = m;
-      inv = l > 0.f ? 1.f / l : l == l ? 0.f : l;
-      lse = m + __log2f(l);
     }
-    if (lane == 0) {
-      sh_lse[r] = lse == kNone ? INFINITY : lse;  // no weight anywhere: none for the masses either
-      sh_ref[r] = ref;
-      sh_inv[r] = inv;
+  }
+  if (open[0] < 0 && open[1] < 0) return;
+
+  // ---- rows that several blocks share: the block that comes last joins their pieces.  A block begins at most one such row,
+  // whose counter is the block's.
+  __syncthreads();
+  if (warp < 2 && lane == 0) {
+    const int slot = warp, w = open[slot];
+    sh_last[slot] = 0;
+    if (w >= 0) {
+      const int64_t t0 = sh.begin[w][slot];
+      const int c0 = line.block_of(t0), c1 = line.block_of(t0 + sh.tiles[w][slot] - 1);
+      int before;
+      asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(p.arrived + c0) : "memory");
+      if (before == c1 - c0) {
+        p.arrived[c0] = 0;
+        sh_last[slot] = c1 - c0 + 1;
+        sh_first[slot] = c0;
+      }
     }
   }
   __syncthreads();
-  if (join) {
-    const int d = threadIdx.x % LANES, share = threadIdx.x / LANES;
-    for (int r = 0; r < p.group; ++r) {
-      if (sh_inv[r] < 0.f) continue;
-      const int64_t t0 = at + ((int64_t)kv * p.row_tiles + r / R) * tiles;
-      const int64_t w0 = owner(t0), w1 = owner(t0 + tiles - 1);
-      float a = 0.f;
-#pragma unroll 4
-      for (int64_t w = w0 + share; w <= w1; w += SHARES) {
-        const int64_t piece = (2 * w + (w == w0)) * R + r % R;
-        const float2 v = p.ml[piece];
-        a += v.x == kNone ? 0.f : p.acc[piece * HD + d] * ex2(v.x - sh_ref[r]);
-      }
-      sh_acc[share][d] = a;
-      __syncthreads();
-      if (share == 0) {
+#pragma unroll 1
+  for (int slot = 0; slot < 2; ++slot) {
+    const int pieces = sh_last[slot], c0 = sh_first[slot];
+    if (!pieces) continue;
+    const int w = open[slot], b = sh.b[w][slot], hr = sh.hr[w][slot];
+    const int kv = hr / p.row_tiles, r0 = (hr - kv * p.row_tiles) * R, rows = min(R, p.group - r0);
+    // threads along (row, 4 columns), and what is left of them along the pieces, up to a share for 8 pieces
+    constexpr int N = 8, THREADS = PG_WARPS * 32;
+    const int cols = rows * (HD / 4), shares = max(1, min(THREADS / cols, (pieces + N - 1) / N));
+    float4* part = reinterpret_cast<float4*>(smem);            // [THREADS]
+    float2* part_ml = reinterpret_cast<float2*>(part + THREADS);  // [THREADS]
+    for (int i0 = 0; i0 < cols; i0 += THREADS) {
+      const int i = shares > 1 ? threadIdx.x % cols : i0 + threadIdx.x, share = shares > 1 ? threadIdx.x / cols : 0;
+      const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+      float m = kNone, l = 0.f;
+      auto add = [&](const float2& v, const float4& x) {  // a piece to what there is
+        const float top = fmaxf(m, v.x);
+        const float keep = m == kNone ? 0.f : ex2(m - top), f = v.x == kNone ? 0.f : ex2(v.x - top);
+        l = (l == l ? l * keep : l) + (v.y == v.y ? v.y * f : v.y);
+        a.x = a.x * keep + (v.x == kNone ? 0.f : x.x * f);
+        a.y = a.y * keep + (v.x == kNone ? 0.f : x.y * f);
+        a.z = a.z * keep + (v.x == kNone ? 0.f : x.z * f);
+        a.w = a.w * keep + (v.x == kNone ? 0.f : x.w * f);
+        m = top;
+      };
+      if (i < cols && share < shares) {
+#pragma unroll 1
+        for (int k0 = share * N; k0 < pieces; k0 += shares * N) {
+          float2 v[N];
+          float4 x[N];
 #pragma unroll
-        for (int i = 1; i < SHARES; ++i) a += sh_acc[i][d];
-        out[r * p.o_h + d] = Num<T>::from_f(a * sh_inv[r]);
+          for (int k = 0; k < N; ++k) {
+            v[k] = make_float2(kNone, 0.f);
+            if (k0 + k < pieces) {
+              const int64_t piece = (int64_t)(2 * (c0 + k0 + k) + (k0 + k == 0)) * R + r;
+              v[k] = __ldcg(p.ml + piece);
+              x[k] = __ldcg(reinterpret_cast<const float4*>(p.acc + piece * HD + d));
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < N; ++k) add(v[k], x[k]);
+        }
       }
-      __syncthreads();
+      if (shares > 1) {
+        part[threadIdx.x] = a;
+        part_ml[threadIdx.x] = make_float2(m, l);
+        __syncthreads();
+        if (threadIdx.x < cols)
+#pragma unroll 1
+          for (int k = 1; k < shares; ++k) add(part_ml[k * cols + i], part[k * cols + i]);
+      }
+      if (i < cols && share == 0) {
+        const int64_t head = kv * p.group + r0 + r;
+        T* out = static_cast<T*>(p.out) + b * p.o_b + head * p.o_h + d;
+        const float inv = l > 0.f ? 1.f / l : l;
+        out[0] = Num<T>::from_f(a.x * inv);
+        out[1] = Num<T>::from_f(a.y * inv);
+        out[2] = Num<T>::from_f(a.z * inv);
+        out[3] = Num<T>::from_f(a.w * inv);
+        if (p.lse && d == 0) p.lse[(int64_t)b * p.kv_heads * p.group + head] = m + __log2f(l);
+      }
     }
+    __syncthreads();
   }
-  // ---- masses
-  if (!p.mass_out) return;
-  const int64_t cap = p.map.capacity();
-  const float* sc = p.scores + ((int64_t)b * p.kv_heads + kv) * p.group * cap;
+}
+
+// Adds the weights to the masses.  Blocks along (sequence, key head) and shares of its keys; V: how many of a key's scores are
+// read at once.
+template <int V>
+__global__ void __launch_bounds__(256) paged_mass_kernel(const PgParams p) {
+  __shared__ __align__(16) float sh_lse[128];
+  grid_dependency_wait();
+  allow_dependents();
+  const int b = blockIdx.x / p.kv_heads, kv = blockIdx.x % p.kv_heads;
+  const SeqKeys keys = keys_of(p, p.lengths[b]);
+  if (blockIdx.y * 256 >= keys.n) return;
+  for (int r = threadIdx.x; r < p.group; r += 256) {
+    const float lse = p.lse[((int64_t)b * p.kv_heads + kv) * p.group + r];
+    sh_lse[r] = lse == kNone ? INFINITY : lse;  // no weight anywhere: none for the masses either
+  }
+  __syncthreads();
+  const float* sc = p.scores + ((int64_t)b * p.kv_heads + kv) * p.map.capacity() * p.group;
   for (int slot = blockIdx.y * 256 + threadIdx.x; slot < keys.n; slot += gridDim.y * 256) {
     int page, row;
     if (!find_slot(p.map, b, slot, page, row)) continue;
     const int64_t o = stat_offset(p.map, page, p.kv_heads, kv, row);
+    const float had = slot == keys.fresh ? 0.f : p.mass[o];
+    const float* mine = sc + (int64_t)slot * p.group;
     float w = 0.f;
-    for (int r = 0; r < p.group; ++r) w += ex2(sc[r * cap + slot] - sh_lse[r]);
-    p.mass_out[o] = slot == keys.fresh ? w : p.mass[o] + w;
+#pragma unroll 2
+    for (int r = 0; r < p.group; r += V) {
+      float x[V], y[V];
+      if constexpr (V == 4) {
+        *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(mine + r);
+        *reinterpret_cast<float4*>(y) = *reinterpret_cast<const float4*>(sh_lse + r);
+      } else {
+        x[0] = mine[r];
+        y[0] = sh_lse[r];
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) w += ex2(x[e] - y[e]);
+    }
+    p.mass_out[o] = had + w;
   }
 }
+
+int encode_tmap_sw128(CUtensorMap* out, const void* base, int dtype, int rank, const uint64_t* dims,
+                      const uint64_t* strides_bytes, const uint32_t* box);
 
 namespace {
 
 int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 
-// Scratch: prefix, lse, pieces, scores.
-struct PgScratch {
-  int64_t lse, ml, acc, scores, bytes;
-};
 int head_tiles(int64_t group) { return group <= 8 ? 1 : 2; }  // tiles of 8 heads that a warp takes at once
-PgScratch pg_scratch(int64_t B, int64_t kv_heads, int64_t group, int64_t hd, int64_t cap, bool mass) {
-  const int64_t pieces = 2 * (int64_t)sm_count() * PG_WARPS, R = 8 * head_tiles(group);
-  PgScratch s;
-  s.lse = up256((B + 1) * 8);
-  s.ml = s.lse + up256(B * kv_heads * group * 4);
-  s.acc = s.ml + up256(pieces * R * 8);
-  s.scores = s.acc + up256(pieces * R * hd * 4);
-  s.bytes = s.scores + (mass ? up256(B * kv_heads * group * cap * 4) : 0);
+// Workspace: counters, then the pieces of blocks and warps for the widest rows.  Scratch, for the masses: log-sum-exps, scores.
+constexpr int64_t kCounterBytes = 8192;
+struct PgWorkspace {
+  int64_t ml, acc, heads_acc, bytes;
+};
+PgWorkspace pg_workspace() {
+  const int64_t n = sm_count(), R = 16, hd = 128;
+  PgWorkspace s;
+  s.ml = kCounterBytes;
+  s.acc = s.ml + up256(2 * n * R * 8);
+  s.heads_acc = s.acc + up256(2 * n * R * hd * 4);
+  s.bytes = s.heads_acc + n * PG_WARPS * R * hd * 4;
   return s;
 }
 
-template <typename T, int HD, int NT, bool BIAS>
-int pg_launch(const PgParams& p, cudaStream_t st) {
+template <typename T, int HD, int NT, int BIAS, bool TMA>
+int pg_split(const CUtensorMap& tk, const CUtensorMap& tv, const PgParams& p, cudaStream_t st) {
+  using C = PgCfg<HD, NT, BIAS>;
   static std::atomic<uint64_t> done{0};
-  if (int rc = ensure_dynamic_smem(paged_attn_kernel<T, HD, NT, BIAS>, PgCfg<HD>::SMEM, done, "paged_attention")) return rc;
-  launch_overlapped(paged_attn_kernel<T, HD, NT, BIAS>, dim3(p.warps / PG_WARPS), dim3(PG_WARPS * 32), PgCfg<HD>::SMEM, st, p);
-  if (int rc = launched("paged_attention")) return rc;
-  // enough blocks to fill the SMs, none with fewer than 1024 keys of a full table
-  int64_t shares = 1;
-  if (p.mass_out) {
-    const int64_t rows = (int64_t)p.B * p.kv_heads, most = ceil_div(p.map.capacity(), 1024);
-    shares = ceil_div((int64_t)sm_count() * 8, rows);
-    if (shares > most) shares = most;
+  if (int rc = ensure_dynamic_smem(paged_attn_kernel<T, HD, NT, BIAS, TMA>, C::SMEM, done, "paged_attention")) return rc;
+  launch_overlapped(paged_attn_kernel<T, HD, NT, BIAS, TMA>, dim3(p.ctas), dim3(PG_WARPS * 32), C::SMEM, st, tk, tv, p);
+  return launched("paged_attention");
+}
+
+template <typename T, int HD, int NT>
+int pg_launch(PgParams& p, int dtype, cudaStream_t st) {
+  // rows of a box: what divides both a page and a tile, so that a tile is whole boxes and a box lies in one page
+  int box = 2048 / HD;
+  while (p.map.page % box) box /= 2;
+  p.box_log2 = 0;
+  while ((1 << p.box_log2) < box) ++p.box_log2;
+  CUtensorMap tk = {}, tv = {};
+  int rc;
+  if (box >= 8) {
+    const uint64_t dims[4] = {(uint64_t)HD, (uint64_t)p.map.page, (uint64_t)p.kv_heads, (uint64_t)p.map.num_pages};
+    const int64_t s[3] = {p.map.s_slot, p.map.s_head, p.map.s_page};
+    uint64_t str[3];
+    for (int i = 0; i < 3; ++i) str[i] = dims[i + 1] > 1 ? (uint64_t)s[i] * 2 : (uint64_t)HD * 2;
+    const uint32_t shape[4] = {HD < 64 ? (uint32_t)HD : 64u, (uint32_t)box, 1, 1};
+    const auto encode = HD == 32 ? encode_tmap_sw64 : encode_tmap_sw128;
+    if ((rc = encode(&tk, p.k, dtype, 4, dims, str, shape)) || (rc = encode(&tv, p.v, dtype, 4, dims, str, shape))) return rc;
+    rc = p.bias_mode == 0   ? pg_split<T, HD, NT, 0, true>(tk, tv, p, st)
+         : p.bias_mode == 1 ? pg_split<T, HD, NT, 1, true>(tk, tv, p, st)
+                            : pg_split<T, HD, NT, 2, true>(tk, tv, p, st);
+  } else {
+    rc = p.bias_mode == 0   ? pg_split<T, HD, NT, 0, false>(tk, tv, p, st)
+         : p.bias_mode == 1 ? pg_split<T, HD, NT, 1, false>(tk, tv, p, st)
+                            : pg_split<T, HD, NT, 2, false>(tk, tv, p, st);
   }
-  launch_overlapped(paged_finish_kernel<T, HD>, dim3((unsigned)(p.B * p.kv_heads), (unsigned)shares), dim3(256), 0, st, p, 8 * NT);
-  return launched("paged_attention: join");
+  if (rc) return rc;
+  if (!p.mass_out) return TFB_OK;
+  // enough blocks to fill the SMs, none with fewer than 1024 keys of a full table
+  const int64_t rows = (int64_t)p.B * p.kv_heads, most = ceil_div(p.map.capacity(), 1024);
+  int64_t shares = ceil_div((int64_t)sm_count() * 8, rows);
+  if (shares > most) shares = most;
+  const dim3 grid((unsigned)rows, (unsigned)shares);
+  if (p.group % 4 == 0) launch_overlapped(paged_mass_kernel<4>, grid, dim3(256), 0, st, p);
+  else launch_overlapped(paged_mass_kernel<1>, grid, dim3(256), 0, st, p);
+  return launched("paged_attention: masses");
 }
 
 template <typename T, int HD>
-int pg_dispatch(const PgParams& p, cudaStream_t st) {
-  if (p.bias_mode) return head_tiles(p.group) == 1 ? pg_launch<T, HD, 1, true>(p, st) : pg_launch<T, HD, 2, true>(p, st);
-  return head_tiles(p.group) == 1 ? pg_launch<T, HD, 1, false>(p, st) : pg_launch<T, HD, 2, false>(p, st);
+int pg_dispatch(PgParams& p, int dtype, cudaStream_t st) {
+  return head_tiles(p.group) == 1 ? pg_launch<T, HD, 1>(p, dtype, st) : pg_launch<T, HD, 2>(p, dtype, st);
 }
 
 }  // namespace
@@ -675,10 +1004,11 @@ int pg_dispatch(const PgParams& p, cudaStream_t st) {
 
 using namespace tfb;
 
-extern "C" int64_t tfb_paged_attention_scratch_bytes(int64_t B, int64_t kv_heads, int64_t group, int64_t hd, int64_t capacity,
-                                                     int with_mass) {
-  if (B < 0 || kv_heads < 0 || group < 0 || hd < 0 || capacity < 0) return 0;
-  return pg_scratch(B, kv_heads, group, hd, capacity, with_mass != 0).bytes;
+extern "C" int64_t tfb_paged_attention_workspace_bytes(void) { return pg_workspace().bytes; }
+
+extern "C" int64_t tfb_paged_attention_scratch_bytes(int64_t B, int64_t kv_heads, int64_t group, int64_t capacity) {
+  if (B < 0 || kv_heads < 0 || group < 0 || capacity < 0) return 0;
+  return up256(B * kv_heads * group * 4) + B * kv_heads * group * capacity * 4;
 }
 
 extern "C" int tfb_paged_attention(const void* q, const void* k_new, const void* v_new, void* out, void* k_pages, void* v_pages,
@@ -687,7 +1017,8 @@ extern "C" int tfb_paged_attention(const void* q, const void* k_new, const void*
                                    int64_t kv_heads, int64_t group, int64_t hd, int64_t num_pages, int64_t page, int64_t width,
                                    int64_t table_ld, const int64_t* page_strides, const int64_t* q_strides,
                                    const int64_t* k_new_strides, const int64_t* v_new_strides, const int64_t* o_strides,
-                                   void* scratch, int64_t scratch_bytes, int dtype, void* stream) {
+                                   void* workspace, int64_t workspace_bytes, void* scratch, int64_t scratch_bytes, int dtype,
+                                   void* stream) {
   PgParams p = {};
   TFB_REQUIRE(page >= 1 && page < (1LL << 31) && width >= 1 && width < (1LL << 31), "paged_attention: bad page or table size");
   p.map = {tables, table_ld, num_pages, (int)page, (int)width, page_strides[0], page_strides[1], page_strides[2]};
@@ -699,9 +1030,14 @@ extern "C" int tfb_paged_attention(const void* q, const void* k_new, const void*
   TFB_REQUIRE(alibi_round >= 0 && alibi_round <= 2, "paged_attention: alibi_round %d", alibi_round);
   if (B == 0) return TFB_OK;
   TFB_REQUIRE(aligned16(k_pages) && aligned16(v_pages), "paged_attention: the pages are not 16-byte aligned");
-  const PgScratch s = pg_scratch(B, kv_heads, group, hd, p.map.capacity(), mass != nullptr);
-  TFB_REQUIRE(scratch && aligned16(scratch) && scratch_bytes >= s.bytes, "paged_attention: scratch of %lld bytes, %lld wanted",
-              (long long)scratch_bytes, (long long)s.bytes);
+  const PgWorkspace s = pg_workspace();
+  TFB_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= s.bytes, "paged_attention: workspace of %lld bytes, %lld wanted",
+              (long long)workspace_bytes, (long long)s.bytes);
+  if (mass) {
+    const int64_t want = tfb_paged_attention_scratch_bytes(B, kv_heads, group, p.map.capacity());
+    TFB_REQUIRE(scratch && aligned16(scratch) && scratch_bytes >= want, "paged_attention: scratch of %lld bytes, %lld wanted",
+                (long long)scratch_bytes, (long long)want);
+  }
   p.q = q;
   p.k_new = k_new;
   p.v_new = v_new;
@@ -730,18 +1066,22 @@ extern "C" int tfb_paged_attention(const void* q, const void* k_new, const void*
   p.kv_heads = (int)kv_heads;
   p.group = (int)group;
   p.row_tiles = (int)ceil_div(group, 8 * head_tiles(group));
-  p.warps = sm_count() * PG_WARPS;
+  p.ctas = sm_count();
   p.scale = kLog2e / sqrtf((float)hd);
-  char* base = static_cast<char*>(scratch);
-  p.prefix = reinterpret_cast<int64_t*>(base);
-  p.lse = reinterpret_cast<float*>(base + s.lse);
+  p.q_pairs = ((reinterpret_cast<uintptr_t>(q) | (uintptr_t)(p.q_b * 2) | (uintptr_t)(p.q_h * 2)) & 3) == 0;
+  char* base = static_cast<char*>(workspace);
+  p.arrived = reinterpret_cast<int*>(base);
   p.ml = reinterpret_cast<float2*>(base + s.ml);
   p.acc = reinterpret_cast<float*>(base + s.acc);
-  p.scores = mass ? reinterpret_cast<float*>(base + s.scores) : nullptr;
+  p.heads_acc = reinterpret_cast<float*>(base + s.heads_acc);
+  if (mass) {
+    p.lse = static_cast<float*>(scratch);
+    p.scores = reinterpret_cast<float*>(static_cast<char*>(scratch) + up256(B * kv_heads * group * 4));
+  }
   cudaStream_t st = (cudaStream_t)stream;
   TFB_DISPATCH_16(dtype, T, {
-    if (hd == 32) return pg_dispatch<T, 32>(p, st);
-    if (hd == 64) return pg_dispatch<T, 64>(p, st);
-    return pg_dispatch<T, 128>(p, st);
+    if (hd == 32) return pg_dispatch<T, 32>(p, dtype, st);
+    if (hd == 64) return pg_dispatch<T, 64>(p, dtype, st);
+    return pg_dispatch<T, 128>(p, dtype, st);
   })
 }
