@@ -351,12 +351,12 @@ int tfb_cache_append(const void* key, const void* value, void* k_pages, void* v_
  * the queries i with j <= i < counts[b] (NULL: T) of exp(s_hij - lse[b,h,i]), s the scaled and biased scores of
  * tfb_attention_fwd and lse (strides {b, h}, unit stride on T) its log-sum-exp; zero for keys from counts[b] on.  q (B, kv_heads *
  * group, T, hd) and k (B, kv_heads, T, hd) with strides {b, h, t}, positive multiples of 8, and 16-byte aligned bases.
- * Any T from 1 to 2^23.                                                                                      */
-int64_t tfb_prompt_mass_scratch_bytes(int64_t B, int64_t kv_heads, int64_t T);
+ * Any T from 1 to 2^23.  workspace as in tfb_paged_attention, of at least tfb_prompt_mass_workspace_bytes().       */
+int64_t tfb_prompt_mass_workspace_bytes(void);
 int tfb_prompt_mass(const void* q, const void* k, const float* lse, const int* counts, const float* slopes,
                     int alibi_round, float* out, int64_t B, int64_t kv_heads, int64_t group, int64_t T, int64_t hd,
-                    const int64_t* q_strides, const int64_t* k_strides, const int64_t* lse_strides, void* scratch,
-                    int64_t scratch_bytes, int dtype, void* stream);
+                    const int64_t* q_strides, const int64_t* k_strides, const int64_t* lse_strides, void* workspace,
+                    int64_t workspace_bytes, int dtype, void* stream);
 
 /* Eviction: every (sequence, key head) of more than `keep` keys keeps the `keep` of the largest mass, where a key whose position
  * is at least next_positions[b] - recent (NULL: lengths[b] - recent) counts as one of infinite mass and a mass that is no number as

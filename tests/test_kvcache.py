@@ -687,7 +687,7 @@ def test_argument_checks_without_device():
                                   two, 0, None) == 0  # no keys
     said(L.lib.tfb_prompt_mass(one, one, one, None, None, 0, one, 1, 2, 1, 8, 64, _strides(0, 64, 64), three, two, one, 1 << 30, 0, None),
          -1, b"positive multiples")
-    said(L.lib.tfb_prompt_mass(one, one, one, None, None, 0, one, 1, 2, 1, 8, 64, three, three, two, None, 0, 0, None), -1, b"scratch")
+    said(L.lib.tfb_prompt_mass(one, one, one, None, None, 0, one, 1, 2, 1, 8, 64, three, three, two, None, 0, 0, None), -1, b"workspace")
     assert L.lib.tfb_prompt_mass(one, one, one, None, None, 0, one, 1, 2, 1, 0, 64, three, three, two, None, 0, 0, None) == 0
 
     def evict(keep=4, recent=0, k_out=one, out_tables=one, mass_out=one, out_width=2, nbytes=1 << 20):

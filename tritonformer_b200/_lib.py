@@ -64,7 +64,7 @@ _SIGNATURES = {
     "tfb_paged_attention_scratch_bytes": (_i64, [_i64] * 4),
     "tfb_paged_attention": (_i32, [_vp] * 13 + [_i32] + [_i64] * 8 + [_pi64] * 5 + [_vp, _i64, _vp, _i64, _i32, _vp]),
     "tfb_cache_append": (_i32, [_vp] * 11 + [_i64] * 8 + [_pi64] * 4 + [_i32, _vp]),
-    "tfb_prompt_mass_scratch_bytes": (_i64, [_i64] * 3),
+    "tfb_prompt_mass_workspace_bytes": (_i64, []),
     "tfb_prompt_mass": (_i32, [_vp] * 5 + [_i32, _vp] + [_i64] * 5 + [_pi64] * 3 + [_vp, _i64, _i32, _vp]),
     "tfb_cache_evict_scratch_bytes": (_i64, [_i64] * 3),
     "tfb_cache_evict": (_i32, [_vp] * 13 + [_i64] * 9 + [_pi64] + [_i64] * 4 + [_pi64, _vp, _i64, _i32, _vp]),

@@ -192,11 +192,10 @@ Tensor prompt_mass(const Tensor& q_, const Tensor& k_, const Tensor& lse_, const
   if (!mapped(q, sq)) mapped(q = q.clone(at::MemoryFormat::Contiguous), sq);
   if (!mapped(k, sk)) mapped(k = k.clone(at::MemoryFormat::Contiguous), sk);
   const int64_t sl[2] = {step(lse, 0), step(lse, 1)};
-  const int64_t bytes = tfb_prompt_mass_scratch_bytes(B, kv_heads, T);
-  Tensor scratch = at::empty({bytes}, q.options().dtype(at::kByte));
+  const cudaStream_t stream = current_stream(q);
+  const Tensor ws = gemm_workspace(q.device(), stream);
   check(tfb_prompt_mass(q.data_ptr(), k.data_ptr(), floats(lse), ints(counts), floats(slopes), (int)rounded, floats(out), B, kv_heads,
-                        heads / kv_heads, T, hd, sq, sk, sl, scratch.data_ptr(), bytes, dtype_code(q.scalar_type()),
-                        current_stream(q)));
+                        heads / kv_heads, T, hd, sq, sk, sl, ws.data_ptr(), ws.numel(), dtype_code(q.scalar_type()), stream));
   return out;
 }
 

@@ -82,7 +82,7 @@ Tensor gemm_workspace(c10::Device device, cudaStream_t stream) {
   }
   // allocated and cleared in the order of the stream that uses it
   c10::cuda::CUDAStreamGuard on(c10::cuda::getStreamFromExternal(stream, device.index()));
-  const int64_t bytes = std::max(tfb_gemm_workspace_bytes(), tfb_paged_attention_workspace_bytes());
+  const int64_t bytes = std::max({tfb_gemm_workspace_bytes(), tfb_paged_attention_workspace_bytes(), tfb_prompt_mass_workspace_bytes()});
   Tensor buf = at::zeros({bytes}, at::TensorOptions().device(device).dtype(at::kByte));
   l.push_back({device.index(), stream, buf});
   if (l.size() > kMaxWorkspaces) l.pop_front();

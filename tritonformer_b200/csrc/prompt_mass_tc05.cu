@@ -6,14 +6,20 @@
 // product is taken with the keys along the 128 lanes of tensor memory and the queries along its columns, so that a thread
 // owns one key and its sum stays in a register from the key tile's first query tile to its last.
 //
-//   warp 0      TMA producer (K tile of 128 keys into one of two buffers, Q tiles of 128 queries through a ring)
-//   warp 1      MMA issuer
-//   warp 2      the columns' terms: -lse * log2(e) of 128 queries, -inf for those past the prompt's end, through a ring
-//   warps 4-11  exponentials and sums: two per lane quarter, each with 64 of the 128 queries of a tile
+//   warp 0      TMA producer (K tile of 128 keys into one of two buffers, Q tiles of 256 queries through a ring)
+//   warp 1      MMA issuer: M 128 (keys), N 256 (queries), into one of two score buffers of 256 columns
+//   warps 4-19  exponentials and sums: four per lane quarter, each with 64 of the 256 queries of a tile.  A lane reads the
+//               log-sum-exp of two of the queries, a tile ahead; the warp shares them through shared memory.
 //
 // Split.  The (key tile, head, query tile) triples of all prompts are numbered in one line, key tile by key tile, and each CTA
 // takes an equal stretch of it: the causal triangle and prompts of different lengths leave no CTA with more than one tile
-// over another.  Key tiles that several CTAs share leave their sums in scratch, and a second kernel adds them in order.
+// over another.  Key tiles that several CTAs share leave their sums in a workspace; the last of the CTAs adds them, in order.
+//
+// Bound: the exponentials, one per score, 16 a clock and SM: 2048 clocks for a tile of 128 x 256, against 512 of the product at
+// head_dim 64.  One pair in four goes to the FMA pipe (a polynomial of degree 5 for 2^f, |f| <= 1/2, relative error 2.1e-7 in 32
+// bits, the SFU's own being 2.4e-7).  A tile of 128 x 128, with a warp for the terms, was bound by the
+// issuing warps' 1.2 k clocks a tile instead.  Measured: 4 prompts of 2048 tokens, 16 heads of 64, exact slopes 64 us (88 with
+// 128 x 128); one of 8192, 12 query heads of 128 on 4 key heads 143 us (264): 72% of what the SFU alone could do.
 #include "attn.cuh"
 #include "paged.cuh"
 #include "tc05.cuh"
@@ -22,20 +28,27 @@
 namespace tfb {
 namespace {
 
-constexpr int PM_TILE = 128;
-constexpr int PM_BUFS = 4;  // score buffers of 128 columns
+constexpr int PM_TILE = 128;             // keys of a tile
+constexpr int PM_QUERIES = 2 * PM_TILE;  // queries of a tile
+constexpr int PM_PARTS = 4;              // warps per lane quarter; each has PM_COLS columns of a tile
+constexpr int PM_COLS = PM_QUERIES / PM_PARTS;
+// A warp is at most two tiles ahead of another, which may still read the sums of the key tile that ended before those: each of
+// the last PM_TURNS key tiles has a place and a barrier of its own.
+constexpr int PM_TURNS = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int HD> struct PmCfg {
   static constexpr int PANELS = HD / 64;
-  static constexpr int TILE_BYTES = PANELS * 16384;
-  static constexpr int STAGES = HD == 64 ? 4 : 3;
+  static constexpr int K_BYTES = PANELS * 16384, Q_BYTES = 2 * K_BYTES;
+  static constexpr int STAGES = HD == 64 ? 4 : 2;
   static constexpr int OFF_K = 0;
-  static constexpr int OFF_Q = 2 * TILE_BYTES;
-  static constexpr int OFF_C = OFF_Q + STAGES * TILE_BYTES;  // [PM_BUFS][128] column terms
-  static constexpr int OFF_BAR = OFF_C + PM_BUFS * 512;
-  static constexpr int SMEM_BYTES = OFF_BAR + 256 + 1024;
-  static constexpr int THREADS = 384;
+  static constexpr int OFF_Q = 2 * K_BYTES;
+  static constexpr int OFF_C = OFF_Q + STAGES * Q_BYTES;         // [warp][2][PM_COLS] column terms
+  static constexpr int OFF_SUM = OFF_C + 4 * PM_PARTS * 2 * PM_COLS * 4;  // [PM_TURNS][PM_PARTS][128] sums of a key tile
+  static constexpr int OFF_BAR = OFF_SUM + PM_TURNS * PM_PARTS * 512;
+  static constexpr int SMEM_BYTES = OFF_BAR + 512 + 1024;
+  static constexpr int THREADS = 128 + 128 * PM_PARTS;
+  static_assert(SMEM_BYTES <= 226 * 1024, "shared memory");
 };
 
 struct PmParams {
@@ -47,40 +60,43 @@ struct PmParams {
   int B, kv_heads, group, T;
   float scale;  // log2(e) / sqrt(hd)
   int ctas;
-  int64_t* prefix;  // (B + 1)
-  float* halves;    // [2][B][kv_heads][T]
-  float* pieces;    // [ctas][2][2][128]
+  int* arrived;     // [ctas] how many CTAs have left their pieces of the key tile that this one begins; zero between calls
+  float* pieces;    // [ctas][2][128]
 };
 
 __device__ __forceinline__ int pm_count(const PmParams& p, int b) { return p.counts ? min(max(p.counts[b], 0), p.T) : p.T; }
+// Query tiles of all m last key tiles of a head: m, m - 1, .. 1 tiles of 128 queries, in pairs.
+__device__ __forceinline__ int64_t pm_pairs(int64_t m) { return (m + 1) * (m + 1) / 4; }
 __device__ __forceinline__ int64_t pm_tiles(const PmParams& p, int count) {
-  const int64_t n = (count + PM_TILE - 1) / PM_TILE;
-  return n * (n + 1) / 2 * p.kv_heads * p.group;
+  return pm_pairs((count + PM_TILE - 1) / PM_TILE) * p.kv_heads * p.group;
 }
 
-// A place in the line of tiles.
+// A place in the line of tiles.  A run is what a key tile and a head have in common: the query tiles i, i + 2, .. below n.
 struct PmCursor {
-  int b, kv, j, r, i, n;  // prompt, key head, key tile, query head of the group, query tile, tiles of the prompt
+  int b, kv, j, r, i, n;  // prompt, key head, key tile, query head of the group, query tile (of 128), tiles of the prompt
+  __device__ __forceinline__ int64_t start(int64_t j) const { return pm_pairs(n) - pm_pairs(n - j); }  // per head
+  __device__ __forceinline__ int64_t key_tile() const { return (int64_t)(n - j + 1) / 2; }            // pairs in a run
   __device__ __forceinline__ void seek(const PmParams& p, int b_, int64_t in) {
     b = b_;
     n = (pm_count(p, b) + PM_TILE - 1) / PM_TILE;
-    const int64_t per = (int64_t)n * (n + 1) / 2 * p.group;
+    const int64_t per = pm_pairs(n) * p.group;
     kv = (int)(in / per);
-    const int64_t rest = in % per, x = rest / p.group;  // key tile j begins at group * (j n - j (j - 1) / 2)
-    const double w = 2.0 * n + 1.0;
-    j = (int)((w - sqrt(fmax(w * w - 8.0 * (double)x, 0.0))) * 0.5);
+    const int64_t rest = in % per, x = rest / p.group;  // key tile j begins at group * start(j)
+    j = n - (int)sqrt(fmax(4.0 * (double)(pm_pairs(n) - x), 0.0));
     j = min(max(j, 0), n - 1);
     while (j > 0 && start(j) > x) --j;
     while (j + 1 < n && start(j + 1) <= x) ++j;
     const int64_t left = rest - start(j) * p.group;
-    r = (int)(left / (n - j));
-    i = j + (int)(left % (n - j));
+    r = (int)(left / key_tile());
+    i = j + 2 * (int)(left % key_tile());
   }
-  __device__ __forceinline__ int64_t start(int64_t j) const { return j * n - j * (j - 1) / 2; }
+  __device__ __forceinline__ int run(int64_t left) const { return (int)min((int64_t)(n - i + 1) / 2, left); }  // tiles of the run
   __device__ __forceinline__ bool begins() const { return r == 0 && i == j; }
-  __device__ __forceinline__ bool ends(const PmParams& p) const { return i + 1 == n && r + 1 == p.group; }
-  __device__ __forceinline__ void step(const PmParams& p) {
-    if (++i < n) return;
+  __device__ __forceinline__ bool ends(const PmParams& p, int tiles) const { return i + 2 * tiles >= n && r + 1 == p.group; }
+  // past `tiles` tiles of the run; what follows has to be there
+  __device__ __forceinline__ void skip(const PmParams& p, int tiles) {
+    i += 2 * tiles;
+    if (i < n) return;
     i = j;
     if (++r < p.group) return;
     r = 0;
@@ -101,6 +117,28 @@ __device__ __forceinline__ float pm_ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float at_least(float x, float low) {  // NaN stays
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(low));
+  return y;
+}
+// 2^x of a pair on the FMA pipe: 2^f by a polynomial (minimax of the relative error), times 2^n by its exponent field.
+__device__ __forceinline__ uint64_t pm_ex2_fma(uint64_t xp) {
+  float x0, x1;
+  f2_unpack(xp, x0, x1);
+  const uint64_t x = f2_pack(at_least(x0, -127.f), at_least(x1, -127.f));  // 2^-127 is an exponent field of 0: zero
+  const uint64_t xr = f2_add(x, f2_pack(12582912.f, 12582912.f));  // n in the low bits
+  const uint64_t f = f2_fma(f2_add(xr, f2_pack(-12582912.f, -12582912.f)), f2_pack(-1.f, -1.f), x);
+  auto both = [](float c) { return f2_pack(c, c); };
+  uint64_t q = f2_fma(f, both(0.0013276472454890609f), both(0.009675540961325169f));
+  q = f2_fma(q, f, both(0.05550713092088699f));
+  q = f2_fma(q, f, both(0.24022120237350464f));
+  q = f2_fma(q, f, both(0.6931469440460205f));
+  q = f2_fma(q, f, both(1.0000001192092896f));
+  float n0, n1;
+  f2_unpack(xr, n0, n1);
+  return f2_mul(q, f2_pack(__int_as_float((__float_as_int(n0) << 23) + 0x3f800000), __int_as_float((__float_as_int(n1) << 23) + 0x3f800000)));
+}
 
 }  // namespace
 
@@ -116,33 +154,29 @@ __global__ void __launch_bounds__(PmCfg<HD>::THREADS, 1) prompt_mass_kernel(cons
   uint64_t* k_empty = k_full + 2;           // [2]
   uint64_t* q_full = k_empty + 2;           // [STAGES]
   uint64_t* q_empty = q_full + C::STAGES;   // [STAGES]
-  uint64_t* s_full = q_empty + C::STAGES;   // [PM_BUFS] scores are in tensor memory
-  uint64_t* s_empty = s_full + PM_BUFS;     // [PM_BUFS] and have been read (8 warps)
-  uint64_t* c_full = s_empty + PM_BUFS;     // [PM_BUFS] column terms are in shared memory
-  uint64_t* c_empty = c_full + PM_BUFS;     // [PM_BUFS]
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(c_empty + PM_BUFS);
+  uint64_t* s_full = q_empty + C::STAGES;   // [2] scores are in tensor memory
+  uint64_t* s_empty = s_full + 2;           // [2] and have been read (every warp)
+  uint64_t* sum_full = s_empty + 2;         // [PM_TURNS][4 lane quarters] a key tile's sums are in shared memory (PM_PARTS warps)
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(sum_full + 4 * PM_TURNS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
-  static_assert((2 * 2 + 2 * 4 + 4 * PM_BUFS) * 8 + 8 <= 256, "barriers");
+  static_assert((2 * 2 + 2 * 4 + 2 * 2 + 4 * PM_TURNS) * 8 + 8 <= 512, "barriers");
   __shared__ int64_t sh_scan[C::THREADS / 32];
-  __shared__ int64_t sh_base;
-  __shared__ int sh_b;
+  __shared__ int64_t sh_base, sh_tile[2], sh_row[2];
+  __shared__ int sh_b, sh_open[2], sh_key[2], sh_left[2], sh_tiles[2], sh_last[2], sh_first[2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&k_empty[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_empty[i], 4 * PM_PARTS);
     }
     for (int i = 0; i < C::STAGES; ++i) {
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
     }
-    for (int i = 0; i < PM_BUFS; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&s_empty[i], 8);
-      mbar_init(&c_full[i], 1);
-      mbar_init(&c_empty[i], 8);
-    }
+    for (int i = 0; i < 4 * PM_TURNS; ++i) mbar_init(&sum_full[i], PM_PARTS);
     mbar_fence_init();
   }
   if (warp == 1) {
@@ -152,6 +186,7 @@ __global__ void __launch_bounds__(PmCfg<HD>::THREADS, 1) prompt_mass_kernel(cons
   grid_dependency_wait();
   allow_dependents();
   if (threadIdx.x == 0) *abort_flag = (*(volatile int*)&g_dev_status != 0) ? 1 : 0;
+  if (threadIdx.x < 2) sh_open[threadIdx.x] = 0;
 
   // ---- the CTA's stretch of the line
   const int per = (p.B + C::THREADS - 1) / C::THREADS;
@@ -180,22 +215,21 @@ __global__ void __launch_bounds__(PmCfg<HD>::THREADS, 1) prompt_mass_kernel(cons
   const int64_t count = blockIdx.x < parts ? (blockIdx.x + 1) * total / parts - from : 0;
   for (int b = b_lo; b < b_hi; ++b) {
     const int64_t tiles = pm_tiles(p, pm_count(p, b));
-    if (blockIdx.x == 0) {
-      p.prefix[b] = base;
-      if (p.counts && (p.counts[b] < 0 || p.counts[b] > p.T)) atomicCAS(dev_status(), 0, kBadLength);
-    }
+    if (blockIdx.x == 0 && p.counts && (p.counts[b] < 0 || p.counts[b] > p.T)) atomicCAS(dev_status(), 0, kBadLength);
     if (from >= base && from < base + tiles) {
       sh_b = b;
       sh_base = base;
     }
     base += tiles;
   }
-  if (blockIdx.x == 0 && threadIdx.x == 0) p.prefix[p.B] = total;
   __syncthreads();
   const uint32_t tmem_base = *tmem_holder;
   const bool live = *abort_flag == 0 && count > 0;
   PmCursor cu;
   if (live) cu.seek(p, sh_b, from - sh_base);
+  if (*abort_flag == 0 && p.counts)  // keys past the prompts' ends
+    for (int row = blockIdx.x; row < p.B * p.kv_heads; row += gridDim.x)
+      for (int key = pm_count(p, row / p.kv_heads) + threadIdx.x; key < p.T; key += C::THREADS) p.out[(int64_t)row * p.T + key] = 0.f;
 
   if (!live) {
   } else if (warp == 0) {
@@ -205,162 +239,247 @@ __global__ void __launch_bounds__(PmCfg<HD>::THREADS, 1) prompt_mass_kernel(cons
       tma_prefetch_desc(&tmK);
       int st = 0, nk = 0;
       uint32_t ph = 0;
-      for (int64_t t = 0; t < count; ++t) {
-        if (t == 0 || cu.begins()) {
+      bool ok = true, fresh = true;  // fresh: the key tile has to be read
+      for (int64_t left = count; left > 0 && ok;) {
+        const int tiles = cu.run(left), head = cu.kv * p.group + cu.r;
+        if (fresh || cu.begins()) {
+          fresh = false;
           const int kb = nk & 1;
           if (!mbar_wait(&k_empty[kb], ((nk >> 1) & 1) ^ 1, 0x8000 | kb, abort_flag)) break;
-          mbar_expect_tx(&k_full[kb], C::TILE_BYTES);
+          mbar_expect_tx(&k_full[kb], C::K_BYTES);
 #pragma unroll
           for (int c = 0; c < C::PANELS; ++c)
-            tma_load_4d(smem + C::OFF_K + kb * C::TILE_BYTES + c * 16384, &tmK, c * 64, cu.j * PM_TILE, cu.kv, cu.b, &k_full[kb]);
+            tma_load_4d(smem + C::OFF_K + kb * C::K_BYTES + c * 16384, &tmK, c * 64, cu.j * PM_TILE, cu.kv, cu.b, &k_full[kb]);
           ++nk;
         }
-        if (!mbar_wait(&q_empty[st], ph ^ 1, 0x8100 | st, abort_flag)) break;
-        mbar_expect_tx(&q_full[st], C::TILE_BYTES);
+        for (int k = 0; k < tiles; ++k) {
+          ok = mbar_wait(&q_empty[st], ph ^ 1, 0x8100 | st, abort_flag);
+          if (!ok) break;
+          mbar_expect_tx(&q_full[st], C::Q_BYTES);
 #pragma unroll
-        for (int c = 0; c < C::PANELS; ++c)
-          tma_load_4d(smem + C::OFF_Q + st * C::TILE_BYTES + c * 16384, &tmQ, c * 64, cu.i * PM_TILE, cu.kv * p.group + cu.r, cu.b,
-                      &q_full[st]);
-        if (++st == C::STAGES) { st = 0; ph ^= 1; }
-        if (t + 1 < count) cu.step(p);
+          for (int c = 0; c < C::PANELS; ++c)
+            tma_load_4d(smem + C::OFF_Q + st * C::Q_BYTES + c * 32768, &tmQ, c * 64, (cu.i + 2 * k) * PM_TILE, head, cu.b, &q_full[st]);
+          if (++st == C::STAGES) { st = 0; ph ^= 1; }
+        }
+        left -= tiles;
+        if (left > 0) cu.skip(p, tiles);
       }
     }
   } else if (warp == 1) {
     // ----------------------------------------------------------------------- MMA issuer
     constexpr int fmt = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
-    constexpr uint32_t idesc = instr_desc_f16(PM_TILE, PM_TILE, fmt, 0, 0);
+    constexpr uint32_t idesc = instr_desc_f16(PM_TILE, PM_QUERIES, fmt, 0, 0);
     const uint32_t tb = __shfl_sync(0xffffffffu, tmem_base, 0);
     const uint32_t s0 = smem_u32(smem);
-    int st = 0, nk = -1;
-    uint32_t ph = 0;
-    for (int64_t t = 0; t < count; ++t) {
-      const int buf = (int)(t % PM_BUFS);
-      bool ok = true;
-      if (t == 0 || cu.begins()) {
+    int st = 0, nk = -1, buf = 0;
+    uint32_t ph = 0, sph = 1;
+    bool ok = true, fresh = true;
+    for (int64_t left = count; left > 0 && ok;) {
+      const int tiles = cu.run(left);
+      if (fresh || cu.begins()) {
+        fresh = false;
         ++nk;
-        ok = mbar_wait(&k_full[nk & 1], (nk >> 1) & 1, 0x8200 | (nk & 1), abort_flag);
+        if (!__all_sync(0xffffffffu, mbar_wait(&k_full[nk & 1], (nk >> 1) & 1, 0x8200 | (nk & 1), abort_flag))) break;
       }
-      ok = ok && mbar_wait(&q_full[st], ph, 0x8300 | st, abort_flag);
-      ok = ok && mbar_wait(&s_empty[buf], (uint32_t)((t / PM_BUFS) & 1) ^ 1, 0x8400 | buf, abort_flag);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      tc_fence_after();
-      const uint64_t dk = smem_desc_sw128(s0 + C::OFF_K + (nk & 1) * C::TILE_BYTES, 16, 1024);
-      const uint64_t dq = smem_desc_sw128(s0 + C::OFF_Q + st * C::TILE_BYTES, 16, 1024);
+      const bool last = cu.ends(p, tiles);
+      const uint64_t dk = smem_desc_sw128(s0 + C::OFF_K + (nk & 1) * C::K_BYTES, 16, 1024);
+      for (int k = 0; k < tiles; ++k) {
+        ok = mbar_wait(&q_full[st], ph, 0x8300 | st, abort_flag) && mbar_wait(&s_empty[buf], sph, 0x8400 | buf, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t dq = smem_desc_sw128(s0 + C::OFF_Q + st * C::Q_BYTES, 16, 1024);
 #pragma unroll
-      for (int s = 0; s < HD / 16; ++s) {
-        const uint32_t off = (s / 4) * 16384 + (s % 4) * 32;
-        if (elect_one()) tc_mma_ss(tb + buf * PM_TILE, desc_advance(dk, off), desc_advance(dq, off), idesc, s ? 1u : 0u);
-      }
-      if (elect_one()) {
-        tc_commit(&s_full[buf]);
-        tc_commit(&q_empty[st]);
-        if (cu.ends(p)) tc_commit(&k_empty[nk & 1]);
-      }
-      __syncwarp();
-      if (++st == C::STAGES) { st = 0; ph ^= 1; }
-      if (t + 1 < count) cu.step(p);
-    }
-  } else if (warp == 2) {
-    // ------------------------------------------------------------------------ column terms
-    float v[4];
-    auto fetch = [&]() {  // of the cursor's tile
-      const float* lse = p.lse + cu.b * p.lse_b + (int64_t)(cu.kv * p.group + cu.r) * p.lse_h;
-      const int n = pm_count(p, cu.b);
-      float slope = 0.f;
-      if (MODE == 1) slope = p.slopes[cu.kv * p.group + cu.r] * kLog2e;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int c = e * 32 + lane, q = cu.i * PM_TILE + c;
-        float x = -INFINITY;  // past the end, or a row that gives no weight
-        if (q < n) {
-          const float l = lse[q];
-          x = l == -INFINITY ? -INFINITY : -l * kLog2e - slope * (float)c;
+        for (int s = 0; s < HD / 16; ++s)
+          if (elect_one())
+            tc_mma_ss(tb + buf * PM_QUERIES, desc_advance(dk, (s / 4) * 16384 + (s % 4) * 32),
+                      desc_advance(dq, (s / 4) * 32768 + (s % 4) * 32), idesc, s ? 1u : 0u);
+        if (elect_one()) {
+          tc_commit(&s_full[buf]);
+          tc_commit(&q_empty[st]);
+          if (last && k + 1 == tiles) tc_commit(&k_empty[nk & 1]);
         }
-        v[e] = x;
+        __syncwarp();
+        if (++st == C::STAGES) { st = 0; ph ^= 1; }
+        if (++buf == 2) { buf = 0; sph ^= 1; }
       }
-    };
-    fetch();
-    for (int64_t t = 0; t < count; ++t) {
-      const int buf = (int)(t % PM_BUFS);
-      const bool ok = mbar_wait(&c_empty[buf], (uint32_t)((t / PM_BUFS) & 1) ^ 1, 0x8500 | buf, abort_flag);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      float* dst = reinterpret_cast<float*>(smem + C::OFF_C) + buf * PM_TILE;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) dst[e * 32 + lane] = v[e];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&c_full[buf]);
-      if (t + 1 < count) {
-        cu.step(p);
-        fetch();
-      }
+      left -= tiles;
+      if (left > 0) cu.skip(p, tiles);
     }
   } else if (warp >= 4) {
     // ---------------------------------------------------------------- exponentials and sums
-    const int quarter = warp & 3, half = (warp - 4) >> 2;
-    const int row = quarter * 32 + lane;  // key of the tile
+    const int quarter = warp & 3, part = (warp - 4) >> 2;
+    // A thread has rows (keys) g8, g8 + 8, g8 + 16 and g8 + 24 of its quarter and of every 8 columns two: it needs a quarter of
+    // the columns' terms, whose way from shared memory would otherwise cost as much as the scores'.
+    const int g8 = lane >> 2, j2 = 2 * (lane & 3);
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const uint64_t scale2 = f2_pack(p.scale, p.scale);
-    float sum = 0.f;
-    bool first = cu.begins();
-    for (int64_t t = 0; t < count; ++t) {
-      const int buf = (int)(t % PM_BUFS);
-      const uint32_t par = (uint32_t)((t / PM_BUFS) & 1);
-      bool ok = mbar_wait(&c_full[buf], par, 0x8600 | buf, abort_flag);
-      ok = ok && mbar_wait(&s_full[buf], par, 0x8700 | buf, abort_flag);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      tc_fence_after();
-      uint32_t s[64];
-      tmem_ld64(tmem_base + lane_base + buf * PM_TILE + half * 64, s);
-      tc_wait_ld();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s_empty[buf]);
-      const float4* col = reinterpret_cast<const float4*>(smem + C::OFF_C + buf * 512 + half * 256);
-      const int dist = (cu.i - cu.j) * PM_TILE + half * 64 - row;  // of the first of the 64 queries from this thread's key
-      float slope = 0.f;
-      if (MODE != 0) slope = p.slopes[cu.kv * p.group + cu.r];
-      const AlibiLog2<MODE> alibi(slope);
-      // exact slopes: the query's place in its tile is in the column's term, the rest is the thread's
-      const float shift = MODE == 1 ? -slope * kLog2e * (float)((cu.i - cu.j) * PM_TILE - row) : 0.f;
-      const bool diagonal = cu.i == cu.j;
-      uint64_t part0 = f2_pack(0.f, 0.f), part1 = part0;
+    float* terms = reinterpret_cast<float*>(smem + C::OFF_C) + (warp - 4) * 2 * PM_COLS;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    int turn = 0, buf = 0;
+    uint32_t parity = 0;
+    bool first = cu.begins(), ok = true;
+    int64_t tile_at = from - (cu.r * cu.key_tile() + (cu.i - cu.j) / 2);  // where the key tile begins in the line
+    // The log-sum-exps of the next tile are read while a tile is worked on, over the ends of runs too.
+    struct Run {
+      const float* lse;  // of this lane's first query of the run's first tile
+      int left;          // queries from there on to the prompt's end
+      float slope;
+    };
+    auto run_of = [&](const PmCursor& c) {
+      const int h = c.kv * p.group + c.r, q = c.i * PM_TILE + part * PM_COLS + lane;
+      return Run{p.lse + c.b * p.lse_b + h * p.lse_h + q, pm_count(p, c.b) - q, MODE == 0 ? 0.f : p.slopes[h]};
+    };
+    float lse[PM_COLS / 32];
+    auto fetch = [&](const Run& run, int k) {
 #pragma unroll
-      for (int c4 = 0; c4 < 16; ++c4) {
-        const float4 a = col[c4];
+      for (int e = 0; e < PM_COLS / 32; ++e)
+        lse[e] = k * PM_QUERIES + e * 32 < run.left ? run.lse[k * PM_QUERIES + e * 32] : -INFINITY;
+    };
+    Run run = run_of(cu);
+    fetch(run, 0);
+    for (int64_t left = count; left > 0 && ok;) {
+      const int tiles = cu.run(left);
+      const bool last = cu.ends(p, tiles);
+      PmCursor next = cu;
+      left -= tiles;
+      Run after = run;
+      if (left > 0) {
+        next.skip(p, tiles);
+        after = run_of(next);
+      }
+      const AlibiLog2<MODE> alibi(run.slope);
+      const float k1 = run.slope * kLog2e;
+      // exact slopes: the query's place in its tile is in the column's term, the rest is the row's
+      float shift = -k1 * (float)((cu.i - cu.j) * PM_TILE - quarter * 32 - g8);
+      int dist = (cu.i - cu.j) * PM_TILE + part * PM_COLS + j2 - quarter * 32 - g8;  // of the first query from the first key
+      bool diagonal = cu.i == cu.j;
+      for (int k = 0; k < tiles; ++k) {
+        // The term of a query's column: -lse * log2(e), with exact slopes also its place in the tile; -inf past the prompt's end,
+        // or where the row gives no weight.
+        float* mine = terms + (k & 1) * PM_COLS;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int c = c4 * 4 + e * 2;
-          uint64_t x = f2_fma(f2_pack(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), scale2, e ? f2_pack(a.z, a.w) : f2_pack(a.x, a.y));
-          if (MODE == 1) x = f2_add(x, f2_pack(shift, shift));
-          if (MODE > 1) x = alibi.sub_pair(x, (float)(dist + c), (float)(dist + c + 1));
-          float x0, x1;
-          f2_unpack(x, x0, x1);
-          if (diagonal) {
-            if (dist + c < 0) x0 = -INFINITY;
-            if (dist + c + 1 < 0) x1 = -INFINITY;
+        for (int e = 0; e < PM_COLS / 32; ++e) {
+          const float x = MODE == 1 ? fmaf(lse[e], -kLog2e, -k1 * (float)(part * PM_COLS + e * 32 + lane)) : lse[e] * -kLog2e;
+          mine[e * 32 + lane] = lse[e] == -INFINITY ? -INFINITY : x;
+        }
+        if (k + 1 < tiles) fetch(run, k + 1);
+        else if (left > 0) fetch(after, 0);
+        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[buf], parity, 0x8500 | buf, abort_flag));
+        if (!ok) break;
+        tc_fence_after();
+        uint64_t acc[4] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f), f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
+        // Of a tile whose queries begin before its keys end a warp may have nothing, and has to mask what is below the diagonal.
+        const bool none = diagonal && (part + 1) * PM_COLS <= quarter * 32, masked = diagonal && part * PM_COLS < quarter * 32 + 32;
+#pragma unroll
+        for (int cc = 0; cc < PM_COLS / 32; ++cc) {  // 32 columns at a time
+          uint32_t s[2][16];
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            tmem_ld_half32(tmem_base + lane_base + ((uint32_t)(16 * h) << 16) + buf * PM_QUERIES + part * PM_COLS + cc * 32, s[h]);
+          tc_wait_ld();
+          if (cc + 1 == PM_COLS / 32) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_empty[buf]);
           }
-          const uint64_t w = f2_pack(pm_ex2(x0), pm_ex2(x1));
-          if (e) part1 = f2_add(part1, w);
-          else part0 = f2_add(part0, w);
+          uint64_t term[4];  // of the thread's columns 8 c + j2, 8 c + j2 + 1
+#pragma unroll
+          for (int c = 0; c < 4; ++c) term[c] = *reinterpret_cast<const uint64_t*>(mine + cc * 32 + c * 8 + j2);
+          // the exponents of the columns of block c in row g8 + 8 a
+          auto exponent = [&](int c, int a) {
+            const uint32_t* v = &s[a / 2][c * 4 + (a % 2) * 2];
+            uint64_t x = f2_fma(f2_pack(__uint_as_float(v[0]), __uint_as_float(v[1])), scale2, term[c]);
+            if (MODE == 1) {
+              const float r = fmaf(k1, (float)(8 * a), shift);
+              x = f2_add(x, f2_pack(r, r));
+            }
+            if (MODE > 1) x = alibi.sub_pair(x, (float)(dist + cc * 32 + c * 8 - 8 * a), (float)(dist + cc * 32 + c * 8 - 8 * a + 1));
+            return x;
+          };
+          if (!masked) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int a = 0; a < 4; ++a) {
+                uint64_t x = exponent(c, a);
+                constexpr unsigned kFma = 0x22;  // of eight pairs, those that take the FMA pipe
+                if (kFma >> ((c * 4 + a) % 8) & 1) {
+                  x = pm_ex2_fma(x);
+                } else {
+                  float x0, x1;
+                  f2_unpack(x, x0, x1);
+                  x = f2_pack(pm_ex2(x0), pm_ex2(x1));
+                }
+                acc[a] = f2_add(acc[a], x);
+              }
+          } else if (!none) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int a = 0; a < 4; ++a) {
+                float x0, x1;
+                f2_unpack(exponent(c, a), x0, x1);
+                const int d = dist + cc * 32 + c * 8 - 8 * a;
+                if (d < 0) x0 = -INFINITY;
+                if (d + 1 < 0) x1 = -INFINITY;
+                acc[a] = f2_add(acc[a], f2_pack(pm_ex2(x0), pm_ex2(x1)));
+              }
+          }
         }
+        if (++buf == 2) {
+          buf = 0;
+          parity ^= 1;
+        }
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+          float w0, w1;
+          f2_unpack(acc[a], w0, w1);
+          sum[a] += w0 + w1;
+        }
+        diagonal = false;
+        dist += PM_QUERIES;
+        shift -= k1 * (float)PM_QUERIES;
       }
-      float w0, w1;
-      f2_unpack(f2_add(part0, part1), w0, w1);
-      sum += w0 + w1;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&c_empty[buf]);
-      const bool last = cu.ends(p);
-      if (last || t + 1 == count) {
-        const int key = cu.j * PM_TILE + row;
-        if (first && last) {
-          if (key < p.T) p.halves[((int64_t)half * p.B * p.kv_heads + (int64_t)cu.b * p.kv_heads + cu.kv) * p.T + key] = sum;
-        } else {
-          p.pieces[(((int64_t)blockIdx.x * 2 + first) * 2 + half) * PM_TILE + row] = sum;
+      if (ok && (last || left == 0)) {
+        // the sums of a key's warps
+        const int place = turn % PM_TURNS;
+        uint64_t* bar = &sum_full[place * 4 + quarter];
+        float* sums = reinterpret_cast<float*>(smem + C::OFF_SUM) + place * PM_PARTS * PM_TILE;
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+          sum[a] += __shfl_xor_sync(0xffffffffu, sum[a], 1);
+          sum[a] += __shfl_xor_sync(0xffffffffu, sum[a], 2);
+          if (j2 == 0) sums[part * PM_TILE + quarter * 32 + g8 + 8 * a] = sum[a];
+          sum[a] = 0.f;
         }
-        sum = 0.f;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
+        if (part == 0) {
+          if (!__all_sync(0xffffffffu, mbar_wait(bar, turn / PM_TURNS & 1, 0x8600 | quarter, abort_flag))) break;
+          const int row = quarter * 32 + lane;
+          float whole = sums[row];
+#pragma unroll
+          for (int e = 1; e < PM_PARTS; ++e) whole += sums[e * PM_TILE + row];
+          const int key = cu.j * PM_TILE + row, count_of = pm_count(p, cu.b);
+          if (first && last) {
+            if (key < count_of) p.out[((int64_t)cu.b * p.kv_heads + cu.kv) * p.T + key] = whole;
+          } else {
+            p.pieces[((int64_t)blockIdx.x * 2 + first) * PM_TILE + row] = whole;
+            sh_open[first] = 1;
+            sh_row[first] = (int64_t)cu.b * p.kv_heads + cu.kv;
+            sh_key[first] = cu.j * PM_TILE;
+            sh_left[first] = count_of - cu.j * PM_TILE;
+            sh_tile[first] = tile_at;
+            sh_tiles[first] = (int)cu.key_tile() * p.group;
+          }
+        }
+        ++turn;
         first = true;  // whatever follows begins with a key tile's first tile
+        tile_at += cu.key_tile() * p.group;
       }
-      if (t + 1 < count) cu.step(p);
+      cu = next;
+      run = after;
     }
   }
 
@@ -375,34 +494,33 @@ __global__ void __launch_bounds__(PmCfg<HD>::THREADS, 1) prompt_mass_kernel(cons
     tc_fence_after();
     tmem_dealloc(tmem_base, 512);
   }
-}
-
-// Adds the two halves of each key's sum, or the pieces of a key tile that several CTAs shared; zero past the prompt's end.
-__global__ void __launch_bounds__(256) prompt_mass_finish_kernel(const PmParams p) {
-  grid_dependency_wait();
-  allow_dependents();
-  if (*(volatile int*)&g_dev_status != 0) return;
-  const int b = blockIdx.x / p.kv_heads, kv = blockIdx.x % p.kv_heads;
-  const int key = blockIdx.y * 256 + threadIdx.x;
-  if (key >= p.T) return;
-  const int count = pm_count(p, b);
-  float sum = 0.f;
-  const int64_t plane = (int64_t)p.B * p.kv_heads * p.T, at = (int64_t)blockIdx.x * p.T + key;
-  if (key < count) {
-    const int64_t total = p.prefix[p.B], parts = min(total, (int64_t)p.ctas), n = (count + PM_TILE - 1) / PM_TILE, j = key / PM_TILE;
-    const int64_t t0 = p.prefix[b] + (kv * (n * (n + 1) / 2) + j * n - j * (j - 1) / 2) * p.group;
-    const int64_t t1 = t0 + (n - j) * p.group - 1;
-    const int64_t c0 = ((t0 + 1) * parts - 1) / total, c1 = ((t1 + 1) * parts - 1) / total;
-    if (c0 == c1) {
-      sum = p.halves[at] + p.halves[plane + at];
-    } else {
-      for (int64_t c = c0; c <= c1; ++c) {
-        const float* piece = p.pieces + (c * 2 + (c == c0)) * 2 * PM_TILE + key % PM_TILE;
-        sum += piece[0] + piece[PM_TILE];
+  // ---- key tiles that several CTAs share: the last of them adds the pieces.  A CTA begins at most one such tile, whose counter
+  // is the CTA's.
+  if (*abort_flag || !(sh_open[0] || sh_open[1])) return;
+  if (threadIdx.x < 2) {
+    const int slot = threadIdx.x;
+    sh_last[slot] = 0;
+    if (sh_open[slot]) {
+      const int64_t t0 = sh_tile[slot], t1 = t0 + sh_tiles[slot] - 1;
+      const int c0 = (int)(((t0 + 1) * parts - 1) / total), c1 = (int)(((t1 + 1) * parts - 1) / total);
+      int before;
+      asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(p.arrived + c0) : "memory");
+      if (before == c1 - c0) {
+        p.arrived[c0] = 0;
+        sh_last[slot] = c1 - c0 + 1;
+        sh_first[slot] = c0;
       }
     }
   }
-  p.out[at] = sum;
+  __syncthreads();
+  const int slot = threadIdx.x / PM_TILE, row = threadIdx.x % PM_TILE;
+  if (slot < 2 && sh_last[slot] && row < sh_left[slot]) {
+    const int c0 = sh_first[slot];
+    float sum = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < sh_last[slot]; ++i) sum += __ldcg(p.pieces + ((int64_t)(c0 + i) * 2 + (i == 0)) * PM_TILE + row);
+    p.out[sh_row[slot] * p.T + sh_key[slot] + row] = sum;
+  }
 }
 
 int encode_tmap_sw128(CUtensorMap* out, const void* base, int dtype, int rank, const uint64_t* dims,
@@ -410,17 +528,7 @@ int encode_tmap_sw128(CUtensorMap* out, const void* base, int dtype, int rank, c
 
 namespace {
 
-int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
-struct PmScratch {
-  int64_t halves, pieces, bytes;
-};
-PmScratch pm_scratch(int64_t B, int64_t kv_heads, int64_t T) {
-  PmScratch s;
-  s.halves = up256((B + 1) * 8);
-  s.pieces = s.halves + up256(2 * B * kv_heads * T * 4);
-  s.bytes = s.pieces + (int64_t)sm_count() * 4 * PM_TILE * 4;
-  return s;
-}
+constexpr int64_t kCounterBytes = 8192;  // of the workspace; the pieces follow
 
 template <typename T, int HD, int MODE>
 int pm_launch(const CUtensorMap& tq, const CUtensorMap& tk, const PmParams& p, cudaStream_t st) {
@@ -442,15 +550,12 @@ int pm_dispatch(int mode, const CUtensorMap& tq, const CUtensorMap& tk, const Pm
 
 using namespace tfb;
 
-extern "C" int64_t tfb_prompt_mass_scratch_bytes(int64_t B, int64_t kv_heads, int64_t T) {
-  if (B < 0 || kv_heads < 0 || T < 0) return 0;
-  return pm_scratch(B, kv_heads, T).bytes;
-}
+extern "C" int64_t tfb_prompt_mass_workspace_bytes(void) { return kCounterBytes + (int64_t)sm_count() * 2 * PM_TILE * 4; }
 
 extern "C" int tfb_prompt_mass(const void* q, const void* k, const float* lse, const int* counts, const float* slopes,
                                int alibi_round, float* out, int64_t B, int64_t kv_heads, int64_t group, int64_t T, int64_t hd,
-                               const int64_t* q_strides, const int64_t* k_strides, const int64_t* lse_strides, void* scratch,
-                               int64_t scratch_bytes, int dtype, void* stream) {
+                               const int64_t* q_strides, const int64_t* k_strides, const int64_t* lse_strides, void* workspace,
+                               int64_t workspace_bytes, int dtype, void* stream) {
   TFB_REQUIRE(dtype == TFB_F16 || dtype == TFB_BF16, "prompt_mass: dtype %d: expected fp16 or bf16", dtype);
   if (hd != 32 && hd != 64 && hd != 128) return fail(TFB_ERR_UNSUPPORTED, "prompt_mass: Only head_dims of [32,64,128] are supported.");
   TFB_REQUIRE(B >= 0 && B < (1 << 20) && kv_heads >= 1 && group >= 1 && kv_heads * group <= 65535, "prompt_mass: bad batch or head count");
@@ -463,20 +568,19 @@ extern "C" int tfb_prompt_mass(const void* q, const void* k, const float* lse, c
   for (int i = 0; i < 3; ++i)
     TFB_REQUIRE(q_strides[i] > 0 && q_strides[i] % 8 == 0 && k_strides[i] > 0 && k_strides[i] % 8 == 0,
                 "prompt_mass: strides of q and k are positive multiples of 8 elements");
-  const PmScratch s = pm_scratch(B, kv_heads, T);
-  TFB_REQUIRE(scratch && aligned16(scratch) && scratch_bytes >= s.bytes, "prompt_mass: scratch of %lld bytes, %lld wanted",
-              (long long)scratch_bytes, (long long)s.bytes);
+  TFB_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= tfb_prompt_mass_workspace_bytes(),
+              "prompt_mass: workspace of %lld bytes, %lld wanted", (long long)workspace_bytes, (long long)tfb_prompt_mass_workspace_bytes());
   CUtensorMap tq, tk;
-  const uint32_t box[4] = {64, PM_TILE, 1, 1};
+  const uint32_t box_q[4] = {64, PM_QUERIES, 1, 1}, box_k[4] = {64, PM_TILE, 1, 1};
   {
     const uint64_t dims[4] = {(uint64_t)hd, (uint64_t)T, (uint64_t)(kv_heads * group), (uint64_t)B};
     const uint64_t st[3] = {(uint64_t)q_strides[2] * 2, (uint64_t)q_strides[1] * 2, (uint64_t)q_strides[0] * 2};
-    if (int rc = encode_tmap_sw128(&tq, q, dtype, 4, dims, st, box)) return rc;
+    if (int rc = encode_tmap_sw128(&tq, q, dtype, 4, dims, st, box_q)) return rc;
   }
   {
     const uint64_t dims[4] = {(uint64_t)hd, (uint64_t)T, (uint64_t)kv_heads, (uint64_t)B};
     const uint64_t st[3] = {(uint64_t)k_strides[2] * 2, (uint64_t)k_strides[1] * 2, (uint64_t)k_strides[0] * 2};
-    if (int rc = encode_tmap_sw128(&tk, k, dtype, 4, dims, st, box)) return rc;
+    if (int rc = encode_tmap_sw128(&tk, k, dtype, 4, dims, st, box_k)) return rc;
   }
   PmParams p = {};
   p.lse = lse;
@@ -490,19 +594,11 @@ extern "C" int tfb_prompt_mass(const void* q, const void* k, const float* lse, c
   p.group = (int)group;
   p.T = (int)T;
   p.scale = kLog2e / sqrtf((float)hd);
-  const int64_t n = ceil_div(T, PM_TILE), tiles = n * (n + 1) / 2 * kv_heads * group * B;
+  const int64_t n = ceil_div(T, PM_TILE), tiles = (n + 1) * (n + 1) / 4 * kv_heads * group * B;
   p.ctas = (int)(tiles < sm_count() ? tiles : sm_count());
-  char* base = static_cast<char*>(scratch);
-  p.prefix = reinterpret_cast<int64_t*>(base);
-  p.halves = reinterpret_cast<float*>(base + s.halves);
-  p.pieces = reinterpret_cast<float*>(base + s.pieces);
+  p.arrived = static_cast<int*>(workspace);
+  p.pieces = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes);
   const int mode = !slopes ? 0 : alibi_round == 0 ? 1 : alibi_round == 1 ? 2 : 4;
   cudaStream_t st = (cudaStream_t)stream;
-  int rc = TFB_OK;
-  TFB_DISPATCH_16(dtype, E, {
-    rc = hd <= 64 ? pm_dispatch<E, 64>(mode, tq, tk, p, st) : pm_dispatch<E, 128>(mode, tq, tk, p, st);
-  })
-  if (rc) return rc;
-  launch_overlapped(prompt_mass_finish_kernel, dim3((unsigned)(B * kv_heads), (unsigned)ceil_div(T, 256)), dim3(256), 0, st, p);
-  return launched("prompt_mass: join");
+  TFB_DISPATCH_16(dtype, E, { return hd <= 64 ? pm_dispatch<E, 64>(mode, tq, tk, p, st) : pm_dispatch<E, 128>(mode, tq, tk, p, st); })
 }
