@@ -4,16 +4,20 @@
 // whole rows in 16-byte chunks, several at a time, and looks the places up beside the copies.
 //
 // Eviction has a selection before its copies.  A key's worth is its mass, or infinite while its position is among the
-// `recent` last ones; each (sequence, key head) keeps the `keep` worthiest, ties to the lower slot.  One block per
-// (sequence, key head) finds the worth of the keep-th by a radix selection over the bits of the worths (11, 11 and 10 of them
-// a pass: the top 11 are sign, exponent and two bits of the significand, which a long-tailed distribution fills some forty
-// values of), numbers the keys that go and those that stay behind slot `keep` in slot order, and pairs the two: the i-th
-// survivor from behind moves into the i-th slot that becomes free.  So keys that stay in front are not touched, no source of
-// a move is the goal of another, and the moves run in any order, in place, all at once.
+// `recent` last ones; each (sequence, key head) keeps the `keep` worthiest, ties to the lower slot.  A cluster of one to eight
+// blocks finds the worth of the keep-th by a radix selection over the bits of the worths (11, 11 and 10 of them a pass: the top 11
+// are sign, exponent and two bits of the significand, which a long-tailed distribution fills some forty values of), its blocks
+// adding their histograms through distributed shared memory; then it numbers the keys that go and those that stay behind slot
+// `keep`, in slot order.  A second kernel pairs the two: the i-th survivor from behind moves into the i-th slot that becomes
+// free.  So keys that stay in front are not touched, no source of a move is the goal of another, and the moves run in any order,
+// in place, all at once.
+#include <cooperative_groups.h>
 #include "paged.cuh"
 
 namespace tfb {
 namespace {
+
+namespace cg = cooperative_groups;
 
 // ------------------------------------------------------------------------------------------------------------- append
 struct AppendParams {
@@ -110,13 +114,17 @@ struct EvictParams {
   int B, kv_heads, keep, recent;
   int rows_in_place, stats_in_place;  // the outputs are the inputs, slot by slot
   int room;                           // worths that fit shared memory
-  int* moves;   // (B * kv_heads) rows to move
-  int* to;      // (B * kv_heads, keep) in place: their goals, ascending (otherwise working space)
-  int* from;    // (B * kv_heads, keep) in place: their sources, ascending; otherwise the source of every slot
+  int cluster;   // blocks of a (sequence, key head)
+  int* moves;    // (B * kv_heads) rows to move
+  int* to;       // (B * kv_heads, keep) their goals, ascending
+  int* from;     // (B * kv_heads, keep) their sources, ascending
+  uint32_t* stay;  // (B * kv_heads, words) bit d: slot d of the first `keep` stays (unset where nothing moves)
+  int words;
 };
 
-constexpr int EV_THREADS = 1024, EV_WARPS = 32;
+constexpr int EV_THREADS = 512, EV_WARPS = EV_THREADS / 32;
 constexpr int EV_BINS = 2048;
+constexpr int EV_BATCH = 8;  // worths that a thread looks up at a time
 
 // Worths in the order of unsigned numbers; -0 is 0, a mass that is no number is -infinity.
 __device__ __forceinline__ uint32_t worth_of(float m) {
@@ -141,166 +149,175 @@ __device__ __forceinline__ uint32_t worth_at(const EvictParams& p, int b, int h,
   return worth_of(at >= oldest ? INFINITY : p.mass[s.at]);
 }
 
-__device__ __forceinline__ void copy_stats(const EvictParams& p, int b, int h, int src, int dst) {
-  const Stat s = stat_at(p.map, p.kv_heads, b, h, src), d = stat_at(p.out_map, p.kv_heads, b, h, dst);
-  if (!s.ok || !d.ok) return;
-  p.mass_out[d.at] = p.mass[s.at];
-  if (p.positions) p.positions_out[d.at] = p.positions[s.at];
-}
-
 // Exclusive sum over the block's warps of a value that each warp has; `total` gets the whole.
 __device__ __forceinline__ int warps_before(int v, int* sh, int& total) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   __syncthreads();
   if (lane == 0) sh[warp] = v;
   __syncthreads();
-  int x = sh[lane];
+  int x = lane < EV_WARPS ? sh[lane] : 0;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int y = __shfl_up_sync(0xffffffffu, x, o);
     if (lane >= o) x += y;
   }
   total = __shfl_sync(0xffffffffu, x, 31);
-  const int before = __shfl_sync(0xffffffffu, x, warp) - v;
-  return before;
+  return __shfl_sync(0xffffffffu, x, warp) - v;
 }
 
-__global__ void __launch_bounds__(EV_THREADS, 1) evict_select_kernel(const EvictParams p) {
+__global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(const EvictParams p) {
   extern __shared__ uint32_t worths[];
   __shared__ int bins[EV_BINS];
   __shared__ int sh_warps[EV_WARPS];
+  __shared__ int sh_ties, sh_holes, sh_over;
   __shared__ uint32_t sh_digit;
   __shared__ int sh_want;
+  cg::cluster_group cluster = cg::this_cluster();
   grid_dependency_wait();
   allow_dependents();
-  const int item = blockIdx.x, b = item / p.kv_heads, h = item % p.kv_heads;
+  const int blocks = p.cluster, rank = blockIdx.x % blocks;
+  const int item = blockIdx.x / blocks, b = item / p.kv_heads, h = item % p.kv_heads;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cap = (int)p.map.capacity(), len = p.lengths[b];
   const int n = min(max(len, 0), cap), keep = min(p.keep, n);
-  if (h == 0 && tid == 0) {
+  if (h == 0 && rank == 0 && tid == 0) {
     if (len != n) atomicCAS(&g_dev_status, 0, kBadLength);
     p.left[b] = keep;
+  }
+  if (n <= keep) {
+    if (rank == 0 && tid == 0) p.moves[item] = 0;
+    return;
   }
   const int oldest = (int)max((int64_t)(p.next ? p.next[b] : n) - p.recent, (int64_t)INT32_MIN);
   int* to = p.to + (int64_t)item * p.keep;
   int* from = p.from + (int64_t)item * p.keep;
-
-  const bool in_smem = n <= p.room;  // else the worths are looked up again in every pass
-  if (n > keep) {
-    auto worth = [&](int i) { return in_smem ? worths[i] : worth_at(p, b, h, i, oldest); };
-    // ---- the worth of the keep-th, and how many of that worth stay
-    uint32_t prefix = 0, mask = 0;
-    int want = keep;
-    const int shifts[3] = {21, 10, 0}, widths[3] = {11, 11, 10};
+  // the block's slots [base, base + size): whole steps of 32
+  const int share = ((n + 31) / 32 + blocks - 1) / blocks * 32;
+  const int base = min(rank * share, n), size = min(share, n - base);
+  const bool in_smem = share <= p.room;  // else the worths are looked up again in every pass
+  if (in_smem)
+    for (int i0 = tid; i0 < size; i0 += EV_THREADS * EV_BATCH) {
+      uint32_t u[EV_BATCH];
 #pragma unroll
-    for (int pass = 0; pass < 3; ++pass) {
-      for (int i = tid; i < EV_BINS; i += EV_THREADS) bins[i] = 0;
-      __syncthreads();
-      const int sh = shifts[pass], size = 1 << widths[pass];
-      for (int i = tid; i < n; i += EV_THREADS) {
-        uint32_t u;
-        if (pass == 0 && in_smem) worths[i] = u = worth_at(p, b, h, i, oldest);
-        else u = worth(i);
-        if ((u & mask) == prefix) atomicAdd(&bins[(u >> sh) & (size - 1)], 1);
-      }
-      __syncthreads();
-      // the bin in which the want-th from the top lies: thread i has the bins size - 1 - per * i downwards
-      const int per = size / EV_THREADS;  // 2, 2, 1
-      int mine = 0;
-      for (int e = 0; e < per; ++e) mine += bins[size - 1 - per * tid - e];
-      int upto = mine;
+      for (int k = 0; k < EV_BATCH; ++k) u[k] = i0 + k * EV_THREADS < size ? worth_at(p, b, h, base + i0 + k * EV_THREADS, oldest) : 0u;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += y;
-      }
-      int total;
-      int before = warps_before(__shfl_sync(0xffffffffu, upto, 31), sh_warps, total) + upto - mine;
-      for (int e = 0; e < per; ++e) {
-        const int bin = size - 1 - per * tid - e, c = bins[bin];
-        if (before < want && want <= before + c) {
-          sh_digit = (uint32_t)bin;
-          sh_want = want - before;
-        }
-        before += c;
-      }
-      __syncthreads();
-      prefix |= sh_digit << sh;
-      mask |= (uint32_t)(size - 1) << sh;
-      want = sh_want;
+      for (int k = 0; k < EV_BATCH; ++k)
+        if (i0 + k * EV_THREADS < size) worths[i0 + k * EV_THREADS] = u[k];
     }
-    // ---- number the slots: each warp has a stretch of them, in steps of 32
-    const int steps = (n + 31) / 32, per = (steps + EV_WARPS - 1) / EV_WARPS;
-    const int lo = min(warp * per, steps), hi = min(lo + per, steps);
-    int ties = 0, over = 0, holes = 0;  // of the warp
-    for (int s = lo; s < hi; ++s) {
-      const int i = s * 32 + lane;
-      const uint32_t u = i < n ? worth(i) : 0u;
-      ties += __popc(__ballot_sync(0xffffffffu, i < n && u == prefix));
+  auto worth = [&](int i) { return in_smem ? worths[i] : worth_at(p, b, h, base + i, oldest); };
+  // ---- the worth of the keep-th, and how many of that worth stay
+  uint32_t prefix = 0, mask = 0;
+  int want = keep;
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+    const int sh = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11, count = 1 << bits;
+    for (int i = tid; i < EV_BINS; i += EV_THREADS) bins[i] = 0;
+    __syncthreads();
+    for (int i = tid; i < size; i += EV_THREADS) {
+      const uint32_t u = worth(i);
+      if ((u & mask) == prefix) atomicAdd(&bins[(u >> sh) & (count - 1)], 1);
+    }
+    cluster.sync();
+    // the bin in which the want-th from the top lies, of all blocks' histograms: thread i has the bins count - 1 - per * i downwards
+    constexpr int MOST = EV_BINS / EV_THREADS;
+    const int per = count / EV_THREADS;
+    int c[MOST], mine = 0;
+#pragma unroll
+    for (int e = 0; e < MOST; ++e) {
+      c[e] = 0;
+      if (e < per)
+        for (int r = 0; r < blocks; ++r) c[e] += cluster.map_shared_rank(bins, r)[count - 1 - per * tid - e];
+      mine += c[e];
+    }
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += y;
     }
     int total;
-    const int tie0 = warps_before(ties, sh_warps, total);
-    int tie = tie0;
-    // which of 32 slots stay; `tie` counts the slots of the keep-th's worth so far
-    auto stay = [&](int s) {
-      const int i = s * 32 + lane;
-      const uint32_t u = i < n ? worth(i) : 0u;
-      const unsigned eq = __ballot_sync(0xffffffffu, i < n && u == prefix);
-      const bool k = i < n && (u > prefix || (u == prefix && tie + __popc(eq & ((1u << lane) - 1u)) < want));
-      tie += __popc(eq);
-      return __ballot_sync(0xffffffffu, k);
-    };
-    for (int s = lo; s < hi; ++s) {
-      const unsigned k = stay(s);
-      const int front = min(max(keep - s * 32, 0), 32);  // how many of the 32 lie before slot `keep`
-      const unsigned in_front = front == 32 ? 0xffffffffu : (1u << front) - 1u;
-      holes += __popc(~k & in_front);
-      over += __popc(k & ~in_front);
-    }
-    int hole = warps_before(holes, sh_warps, total);
-    int nth = warps_before(over, sh_warps, total);
-    tie = tie0;
-    int* behind = p.rows_in_place ? from : to;  // the survivors from behind slot `keep`
-    const int hole0 = hole;
-    for (int s = lo; s < hi; ++s) {
-      const unsigned k = stay(s), below = (1u << lane) - 1u;
-      const int front = min(max(keep - s * 32, 0), 32);
-      const unsigned in_front = front == 32 ? 0xffffffffu : (1u << front) - 1u;
-      const unsigned out = ~k & in_front, in = k & ~in_front;
-      const int i = s * 32 + lane;
-      if (p.rows_in_place && (out >> lane & 1)) to[hole + __popc(out & below)] = i;
-      if (in >> lane & 1) behind[nth + __popc(in & below)] = i;
-      hole += __popc(out);
-      nth += __popc(in);
-    }
-    if (tid == 0) p.moves[item] = total;
-    __syncthreads();  // the survivors' slots are in global memory, for this block
-    tie = tie0;
-    hole = hole0;
-    for (int s = lo; s < hi && s * 32 < keep; ++s) {
-      const unsigned k = stay(s);
-      const int i = s * 32 + lane, front = min(keep - s * 32, 32);
-      const unsigned out = ~k & (front == 32 ? 0xffffffffu : (1u << front) - 1u);
-      if (i < keep) {
-        const bool stays = (k >> lane & 1) != 0;
-        const int src = stays ? i : behind[hole + __popc(out & ((1u << lane) - 1u))];
-        if (!p.rows_in_place) from[i] = src;
-        if (!(stays && p.stats_in_place)) copy_stats(p, b, h, src, i);
+    int before = warps_before(__shfl_sync(0xffffffffu, upto, 31), sh_warps, total) + upto - mine;
+#pragma unroll
+    for (int e = 0; e < MOST; ++e)
+      if (e < per) {
+        if (before < want && want <= before + c[e]) {
+          sh_digit = (uint32_t)(count - 1 - per * tid - e);
+          sh_want = want - before;
+        }
+        before += c[e];
       }
-      hole += __popc(out);
-    }
-  } else {
-    if (tid == 0) p.moves[item] = 0;
-    for (int i = tid; i < n; i += EV_THREADS) {
-      if (!p.rows_in_place) from[i] = i;
-      if (!p.stats_in_place) copy_stats(p, b, h, i, i);
-    }
+    cluster.sync();  // and every block has read the histograms
+    prefix |= sh_digit << sh;
+    mask |= (uint32_t)(count - 1) << sh;
+    want = sh_want;
   }
+  // ---- number the slots: each warp has a stretch of them, in steps of 32
+  const int steps = (size + 31) / 32, per = (steps + EV_WARPS - 1) / EV_WARPS;
+  const int lo = min(warp * per, steps), hi = min(lo + per, steps);
+  int ties = 0, over = 0, holes = 0;  // of the warp
+  for (int s = lo; s < hi; ++s) {
+    const int i = s * 32 + lane;
+    const uint32_t u = i < size ? worth(i) : 0u;
+    ties += __popc(__ballot_sync(0xffffffffu, i < size && u == prefix));
+  }
+  int total;
+  int tie0 = warps_before(ties, sh_warps, total);
+  if (tid == 0) sh_ties = total;
+  cluster.sync();
+  for (int r = 0; r < rank; ++r) tie0 += *cluster.map_shared_rank(&sh_ties, r);
+  int tie = tie0;
+  // which of 32 slots stay; `tie` counts the slots of the keep-th's worth so far
+  auto stay = [&](int s) {
+    const int i = s * 32 + lane;
+    const uint32_t u = i < size ? worth(i) : 0u;
+    const unsigned eq = __ballot_sync(0xffffffffu, i < size && u == prefix);
+    const bool k = i < size && (u > prefix || (u == prefix && tie + __popc(eq & ((1u << lane) - 1u)) < want));
+    tie += __popc(eq);
+    return __ballot_sync(0xffffffffu, k);
+  };
+  // those of step s that lie before slot `keep`
+  auto front = [&](int s) {
+    const int f = min(max(keep - base - s * 32, 0), 32);
+    return f == 32 ? 0xffffffffu : (1u << f) - 1u;
+  };
+  for (int s = lo; s < hi; ++s) {
+    const unsigned k = stay(s), in_front = front(s);
+    holes += __popc(~k & in_front);
+    over += __popc(k & ~in_front);
+  }
+  int hole = warps_before(holes, sh_warps, total);
+  if (tid == 0) sh_holes = total;
+  int nth = warps_before(over, sh_warps, total);
+  if (tid == 0) sh_over = total;
+  cluster.sync();
+  int all = 0;
+  for (int r = 0; r < blocks; ++r) {
+    const int y = *cluster.map_shared_rank(&sh_holes, r);
+    if (r < rank) {
+      hole += y;
+      nth += *cluster.map_shared_rank(&sh_over, r);
+    }
+    all += y;
+  }
+  if (rank == 0 && tid == 0) p.moves[item] = all;
+  tie = tie0;
+  for (int s = lo; s < hi; ++s) {
+    const unsigned k = stay(s), in_front = front(s), below = (1u << lane) - 1u;
+    const unsigned out = ~k & in_front, in = k & ~in_front;
+    const int i = base + s * 32 + lane;
+    if (out >> lane & 1) to[hole + __popc(out & below)] = i;
+    if (in >> lane & 1) from[nth + __popc(in & below)] = i;
+    if (lane == 0 && in_front) p.stay[(int64_t)item * p.words + (base / 32 + s)] = k;
+    hole += __popc(out);
+    nth += __popc(in);
+  }
+  cluster.sync();  // no block ends while another reads its counts
 }
 
 constexpr int MV_ROWS = 128;
 
-// Moves rows of keys and values: in place the survivors from behind into the free slots, otherwise every slot that stays.
+// Moves keys, values and statistics: the survivors from behind into the free slots, and where the output is another buffer the
+// slots that stay as well.
 template <int HD>
 __global__ void __launch_bounds__(256) evict_move_kernel(const EvictParams p) {
   constexpr int LANES = HD / 8, PER = 256 / LANES, N = 4;
@@ -308,25 +325,41 @@ __global__ void __launch_bounds__(256) evict_move_kernel(const EvictParams p) {
   grid_dependency_wait();
   allow_dependents();
   const int item = blockIdx.x, b = item / p.kv_heads, h = item % p.kv_heads;
+  const int moves = p.moves[item], left = p.left[b];
   const int* to = p.to + (int64_t)item * p.keep;
   const int* from = p.from + (int64_t)item * p.keep;
-  const int count = p.rows_in_place ? p.moves[item] : p.left[b];
-  for (int i0 = blockIdx.y * MV_ROWS; i0 < count; i0 += gridDim.y * MV_ROWS) {
+  const int batches = (moves + MV_ROWS - 1) / MV_ROWS;
+  const int all = batches + (p.rows_in_place && p.stats_in_place ? 0 : (left + MV_ROWS - 1) / MV_ROWS);
+  for (int batch = blockIdx.y; batch < all; batch += gridDim.y) {
+    const bool move = batch < batches;  // otherwise slots that stay
+    const bool rows = move || !p.rows_in_place, stats = move || !p.stats_in_place;
     __syncthreads();
     if (threadIdx.x < MV_ROWS) {
-      const int i = i0 + threadIdx.x;
+      const int i = (move ? batch : batch - batches) * MV_ROWS + threadIdx.x;
       int64_t src = -1, dst = 0;
-      if (i < count) {
-        const int goal = p.rows_in_place ? to[i] : i, source = from[i];
-        int page, row, page2, row2;
-        if (find_slot(p.map, b, source, page, row) && find_slot(p.out_map, b, goal, page2, row2)) {
-          src = row_offset(p.map, page, h, row);
-          dst = row_offset(p.out_map, page2, h, row2);
+      int source = -1, goal = -1;
+      if (move) {
+        if (i < moves) {
+          source = from[i];
+          goal = to[i];
+        }
+      } else if (i < left && (moves == 0 || (p.stay[(int64_t)item * p.words + i / 32] >> (i % 32) & 1) != 0)) {
+        source = goal = i;
+      }
+      int page, row, page2, row2;
+      if (source >= 0 && find_slot(p.map, b, source, page, row) && find_slot(p.out_map, b, goal, page2, row2)) {
+        src = row_offset(p.map, page, h, row);
+        dst = row_offset(p.out_map, page2, h, row2);
+        if (stats) {
+          const int64_t at = stat_offset(p.map, page, p.kv_heads, h, row), out = stat_offset(p.out_map, page2, p.kv_heads, h, row2);
+          p.mass_out[out] = p.mass[at];
+          if (p.positions) p.positions_out[out] = p.positions[at];
         }
       }
       sh_src[threadIdx.x] = src;
       sh_dst[threadIdx.x] = dst;
     }
+    if (!rows) continue;
     __syncthreads();
     const int c = (threadIdx.x % LANES) * 8;
     for (int r0 = threadIdx.x / LANES; r0 < MV_ROWS; r0 += PER * N) {
@@ -414,7 +447,7 @@ extern "C" int tfb_cache_append(const void* key, const void* value, void* k_page
 
 extern "C" int64_t tfb_cache_evict_scratch_bytes(int64_t B, int64_t kv_heads, int64_t keep) {
   if (B < 0 || kv_heads < 0 || keep < 0) return 0;
-  return up256(B * kv_heads * 4) + 2 * up256(B * kv_heads * keep * 4);
+  return up256(B * kv_heads * 4) + 2 * up256(B * kv_heads * keep * 4) + up256(B * kv_heads * ((keep + 31) / 32) * 4);
 }
 
 extern "C" int tfb_cache_evict(const void* k_pages, const void* v_pages, const float* mass, const int* positions,
@@ -438,7 +471,7 @@ extern "C" int tfb_cache_evict(const void* k_pages, const void* v_pages, const f
   if (recent > keep) recent = keep;
   TFB_REQUIRE(keep <= p.out_map.capacity(), "cache_evict: %lld keys to keep, and room for %lld", (long long)keep,
               (long long)p.out_map.capacity());
-  TFB_REQUIRE(B * kv_heads < (1LL << 31), "cache_evict: too many rows of heads");
+  TFB_REQUIRE(B * kv_heads < (1LL << 28), "cache_evict: too many rows of heads");
   TFB_REQUIRE(mass && mass_out, "cache_evict: no masses");
   TFB_REQUIRE((positions == nullptr) == (positions_out == nullptr), "cache_evict: positions come with positions for the output");
   TFB_REQUIRE((k_out == k_pages) == (v_out == v_pages), "cache_evict: keys in place and values not, or the other way round");
@@ -474,17 +507,37 @@ extern "C" int tfb_cache_evict(const void* k_pages, const void* v_pages, const f
   p.moves = reinterpret_cast<int*>(base);
   p.to = reinterpret_cast<int*>(base + up256(B * kv_heads * 4));
   p.from = reinterpret_cast<int*>(base + up256(B * kv_heads * 4) + up256(B * kv_heads * keep * 4));
+  p.stay = reinterpret_cast<uint32_t*>(base + up256(B * kv_heads * 4) + 2 * up256(B * kv_heads * keep * 4));
+  p.words = (int)((keep + 31) / 32);
   cudaStream_t st = (cudaStream_t)stream;
+  // as many blocks for a (sequence, key head) as the SMs have room for, none with fewer than 2048 slots of a full table
+  p.cluster = 1;
+  while (p.cluster < 8 && B * kv_heads * p.cluster * 2 <= sm_count() * 2 && p.map.capacity() >= (int64_t)p.cluster * 2 * 2048) p.cluster *= 2;
   constexpr int kMost = 200 * 1024;  // beside the kernel's own arrays
-  int64_t smem = (p.map.capacity() * 4 + 15) / 16 * 16;
+  int64_t smem = (ceil_div(ceil_div(p.map.capacity(), 32), p.cluster) * 32 * 4 + 15) / 16 * 16;
   if (smem > kMost) smem = kMost;
   p.room = (int)(smem / 4);
   static std::atomic<uint64_t> done{0};
   if (int rc = ensure_dynamic_smem(evict_select_kernel, kMost, done, "cache_evict")) return rc;
-  launch_overlapped(evict_select_kernel, dim3((unsigned)(B * kv_heads)), dim3(EV_THREADS), (size_t)smem, st, p);
+  {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(B * kv_heads * p.cluster));
+    cfg.blockDim = dim3(EV_THREADS);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)p.cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = g_plain_launch.load(std::memory_order_relaxed) ? 1 : 2;
+    (void)cudaLaunchKernelEx(&cfg, evict_select_kernel, static_cast<const EvictParams>(p));  // error read by launched()
+  }
   if (int rc = launched("cache_evict")) return rc;
-  // a block for each MV_ROWS rows that can move, as far as that takes to fill the SMs
-  int64_t shares = ceil_div(keep, MV_ROWS);
+  // a block for each MV_ROWS rows that can move or stay, as far as that takes to fill the SMs
+  int64_t shares = ceil_div(keep, MV_ROWS) * (p.rows_in_place && p.stats_in_place ? 1 : 2);
   const int64_t enough = ceil_div((int64_t)sm_count() * 16, B * kv_heads);
   if (shares > enough) shares = enough;
   const dim3 grid((unsigned)(B * kv_heads), (unsigned)shares);

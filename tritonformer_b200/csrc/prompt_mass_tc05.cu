@@ -349,26 +349,23 @@ __global__ void __launch_bounds__(PmCfg<HD>::THREADS, 1) prompt_mass_kernel(cons
         after = run_of(next);
       }
       const AlibiLog2<MODE> alibi(run.slope);
-      const float k1 = run.slope * kLog2e;
-      // exact slopes: the query's place in its tile is in the column's term, the rest is the row's
-      float shift = -k1 * (float)((cu.i - cu.j) * PM_TILE - quarter * 32 - g8);
       int dist = (cu.i - cu.j) * PM_TILE + part * PM_COLS + j2 - quarter * 32 - g8;  // of the first query from the first key
       bool diagonal = cu.i == cu.j;
       for (int k = 0; k < tiles; ++k) {
-        // The term of a query's column: -lse * log2(e), with exact slopes also its place in the tile; -inf past the prompt's end,
-        // or where the row gives no weight.
+        // The term of a query's column: -lse * log2(e); -inf past the prompt's end, or where the row gives no weight.
         float* mine = terms + (k & 1) * PM_COLS;
 #pragma unroll
-        for (int e = 0; e < PM_COLS / 32; ++e) {
-          const float x = MODE == 1 ? fmaf(lse[e], -kLog2e, -k1 * (float)(part * PM_COLS + e * 32 + lane)) : lse[e] * -kLog2e;
-          mine[e * 32 + lane] = lse[e] == -INFINITY ? -INFINITY : x;
-        }
+        for (int e = 0; e < PM_COLS / 32; ++e) mine[e * 32 + lane] = lse[e] == -INFINITY ? -INFINITY : lse[e] * -kLog2e;
         if (k + 1 < tiles) fetch(run, k + 1);
         else if (left > 0) fetch(after, 0);
         ok = __all_sync(0xffffffffu, mbar_wait(&s_full[buf], parity, 0x8500 | buf, abort_flag));
         if (!ok) break;
         tc_fence_after();
         uint64_t acc[4] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f), f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
+        // Distances are exact integers, and one rounding takes their product with the slope into the exponent: parts of it for rows
+        // and columns would cancel near the diagonal, where the weights are.
+        const float dist_f = (float)dist;
+        const uint64_t dist2 = f2_pack(dist_f, dist_f + 1.f);
         // Of a tile whose queries begin before its keys end a warp may have nothing, and has to mask what is below the diagonal.
         const bool none = diagonal && (part + 1) * PM_COLS <= quarter * 32, masked = diagonal && part * PM_COLS < quarter * 32 + 32;
 #pragma unroll
@@ -390,11 +387,12 @@ __global__ void __launch_bounds__(PmCfg<HD>::THREADS, 1) prompt_mass_kernel(cons
           auto exponent = [&](int c, int a) {
             const uint32_t* v = &s[a / 2][c * 4 + (a % 2) * 2];
             uint64_t x = f2_fma(f2_pack(__uint_as_float(v[0]), __uint_as_float(v[1])), scale2, term[c]);
-            if (MODE == 1) {
-              const float r = fmaf(k1, (float)(8 * a), shift);
-              x = f2_add(x, f2_pack(r, r));
+            if (MODE != 0) {
+              const float k = (float)(cc * 32 + c * 8 - 8 * a);
+              float d0, d1;
+              f2_unpack(f2_add(dist2, f2_pack(k, k)), d0, d1);
+              x = alibi.sub_pair(x, d0, d1);
             }
-            if (MODE > 1) x = alibi.sub_pair(x, (float)(dist + cc * 32 + c * 8 - 8 * a), (float)(dist + cc * 32 + c * 8 - 8 * a + 1));
             return x;
           };
           if (!masked) {
@@ -439,7 +437,6 @@ __global__ void __launch_bounds__(PmCfg<HD>::THREADS, 1) prompt_mass_kernel(cons
         }
         diagonal = false;
         dist += PM_QUERIES;
-        shift -= k1 * (float)PM_QUERIES;
       }
       if (ok && (last || left == 0)) {
         // the sums of a key's warps
