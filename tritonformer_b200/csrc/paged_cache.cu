@@ -4,11 +4,12 @@
 // whole rows in 16-byte chunks, several at a time, and looks the places up beside the copies.
 //
 // Eviction has a selection before its copies.  A key's worth is its mass, or infinite while its position is among the
-// `recent` last ones; each (sequence, key head) keeps the `keep` worthiest, ties to the lower slot.  A cluster of one to eight
-// blocks finds the worth of the keep-th by a radix selection over the bits of the worths (11, 11 and 10 of them a pass: the top 11
-// are sign, exponent and two bits of the significand, which a long-tailed distribution fills some forty values of), its blocks
-// adding their histograms through distributed shared memory; then it numbers the keys that go and those that stay behind slot
-// `keep`, in slot order.  A second kernel pairs the two: the i-th survivor from behind moves into the i-th slot that becomes
+// `recent` last ones; each (sequence, key head) keeps the `keep` worthiest, ties to the lower slot.  With the worth in the upper and
+// the inverted slot in the lower half all keys are different 64-bit numbers, and a cluster of one to eight blocks finds the
+// keep-th largest by a radix selection, 11 bits a pass.  The passes end as soon as all that is left in a bin stays: after two,
+// unless masses are equal.  The blocks add their histograms through distributed shared memory, each a slice of the bins (every
+// block reading every histogram took 5 us a pass of eight blocks, five times as long).  Then the keys that go and those that stay behind slot `keep` are numbered
+// in slot order, and a second kernel pairs the two: the i-th survivor from behind moves into the i-th slot that becomes
 // free.  So keys that stay in front are not touched, no source of a move is the goal of another, and the moves run in any order,
 // in place, all at once.
 #include <cooperative_groups.h>
@@ -133,45 +134,40 @@ __device__ __forceinline__ uint32_t worth_of(float m) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-struct Stat {  // of one slot
-  int64_t at;
-  bool ok;
-};
-__device__ __forceinline__ Stat stat_at(const PageMap& m, int heads, int b, int h, int slot) {
-  int page, row;
-  const bool ok = find_slot(m, b, slot, page, row);
-  return {ok ? stat_offset(m, page, heads, h, row) : 0, ok};
-}
-__device__ __forceinline__ uint32_t worth_at(const EvictParams& p, int b, int h, int slot, int oldest) {
-  const Stat s = stat_at(p.map, p.kv_heads, b, h, slot);
-  if (!s.ok) return 0u;
-  const int at = p.positions ? p.positions[s.at] : slot;
-  return worth_of(at >= oldest ? INFINITY : p.mass[s.at]);
-}
-
-// Exclusive sum over the block's warps of a value that each warp has; `total` gets the whole.
-__device__ __forceinline__ int warps_before(int v, int* sh, int& total) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  __syncthreads();
-  if (lane == 0) sh[warp] = v;
-  __syncthreads();
-  int x = lane < EV_WARPS ? sh[lane] : 0;
+// The worths of EV_BATCH slots `EV_THREADS` apart, those from `end` on left out: all lookups of a kind together.
+__device__ __forceinline__ void worths_at(const EvictParams& p, int b, int h, int slot, int end, int oldest, uint32_t (&u)[EV_BATCH]) {
+  int page[EV_BATCH], row[EV_BATCH], at[EV_BATCH];
+  float mass[EV_BATCH];
+  const int* table = p.map.tables + b * p.map.table_ld;
+  bool bad = false;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
+  for (int k = 0; k < EV_BATCH; ++k) {
+    const int s = min(slot + k * EV_THREADS, end - 1), i = (int)((unsigned)s / (unsigned)p.map.page);
+    row[k] = s - i * p.map.page;
+    page[k] = table[i];
   }
-  total = __shfl_sync(0xffffffffu, x, 31);
-  return __shfl_sync(0xffffffffu, x, warp) - v;
+#pragma unroll
+  for (int k = 0; k < EV_BATCH; ++k) {
+    const bool ok = (unsigned)page[k] < (unsigned)p.map.num_pages;
+    bad |= !ok;
+    const int64_t o = ok ? stat_offset(p.map, page[k], p.kv_heads, h, row[k]) : 0;
+    mass[k] = p.mass[o];
+    at[k] = p.positions ? p.positions[o] : slot + k * EV_THREADS;
+    if (!ok) at[k] = INT32_MIN, mass[k] = -INFINITY;
+  }
+#pragma unroll
+  for (int k = 0; k < EV_BATCH; ++k) u[k] = worth_of(at[k] >= oldest ? INFINITY : mass[k]);
+  if (bad) atomicCAS(&g_dev_status, 0, kBadPage);
 }
 
-__global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(const EvictParams p) {
+__global__ void __launch_bounds__(EV_THREADS, 2) evict_select_kernel(const EvictParams p) {
   extern __shared__ uint32_t worths[];
-  __shared__ int bins[EV_BINS];
+  __shared__ __align__(16) int bins[EV_BINS];
   __shared__ int sh_warps[EV_WARPS];
-  __shared__ int sh_ties, sh_holes, sh_over;
-  __shared__ uint32_t sh_digit;
-  __shared__ int sh_want;
+  __shared__ int slice_bins[EV_BINS];  // of this block's slice, all blocks' counts
+  __shared__ int sh_slices[2];         // and their sum, in turn: another block may still read the last pass's
+  __shared__ int64_t sh_pairs[EV_WARPS], sh_total;
+  __shared__ int sh_digit, sh_want, sh_count;
   cg::cluster_group cluster = cg::this_cluster();
   grid_dependency_wait();
   allow_dependents();
@@ -188,45 +184,94 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(const EvictPar
     if (rank == 0 && tid == 0) p.moves[item] = 0;
     return;
   }
-  const int oldest = (int)max((int64_t)(p.next ? p.next[b] : n) - p.recent, (int64_t)INT32_MIN);
-  int* to = p.to + (int64_t)item * p.keep;
-  int* from = p.from + (int64_t)item * p.keep;
+  auto sync = [&]() {
+    if (blocks == 1) __syncthreads();
+    else cluster.sync();
+  };
+  const int oldest = (int)max((int64_t)(p.next ? p.next[b] : n) - p.recent, (int64_t)INT32_MIN + 1);
   // the block's slots [base, base + size): whole steps of 32
   const int share = ((n + 31) / 32 + blocks - 1) / blocks * 32;
-  const int base = min(rank * share, n), size = min(share, n - base);
+  const int base = min(rank * share, n), size = min(share, n - base), end = base + size;
   const bool in_smem = share <= p.room;  // else the worths are looked up again in every pass
   if (in_smem)
     for (int i0 = tid; i0 < size; i0 += EV_THREADS * EV_BATCH) {
       uint32_t u[EV_BATCH];
-#pragma unroll
-      for (int k = 0; k < EV_BATCH; ++k) u[k] = i0 + k * EV_THREADS < size ? worth_at(p, b, h, base + i0 + k * EV_THREADS, oldest) : 0u;
+      worths_at(p, b, h, base + i0, end, oldest, u);
 #pragma unroll
       for (int k = 0; k < EV_BATCH; ++k)
         if (i0 + k * EV_THREADS < size) worths[i0 + k * EV_THREADS] = u[k];
     }
-  auto worth = [&](int i) { return in_smem ? worths[i] : worth_at(p, b, h, base + i, oldest); };
-  // ---- the worth of the keep-th, and how many of that worth stay
-  uint32_t prefix = 0, mask = 0;
+  // the key of the block's i-th slot; worth and inverted slot
+  const int slot_bits = 32 - __clz(n - 1);  // n >= 2
+  auto key_of = [&](int i) {
+    uint32_t u;
+    if (in_smem) {
+      u = worths[i];
+    } else {
+      uint32_t v[EV_BATCH];
+      worths_at(p, b, h, base + i, base + i + 1, oldest, v);
+      u = v[0];
+    }
+    return (uint64_t)u << slot_bits | (uint64_t)(n - 1 - (base + i));
+  };
+  // ---- the keep-th key, as far as it takes: a key stays if its bits in `mask` are at least `prefix`
+  uint64_t prefix = 0, mask = 0;
   int want = keep;
 #pragma unroll 1
-  for (int pass = 0; pass < 3; ++pass) {
-    const int sh = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11, count = 1 << bits;
+  for (int top = 32 + slot_bits, turn = 0; top > 0; turn ^= 1) {  // top: bits that are not decided yet
+    const int shift = max(top - 11, 0), digits = (1 << (top - shift)) - 1;
+    top = shift;
     for (int i = tid; i < EV_BINS; i += EV_THREADS) bins[i] = 0;
+    if (tid == 0) sh_slices[turn] = 0;
     __syncthreads();
     for (int i = tid; i < size; i += EV_THREADS) {
-      const uint32_t u = worth(i);
-      if ((u & mask) == prefix) atomicAdd(&bins[(u >> sh) & (count - 1)], 1);
+      const uint64_t key = key_of(i);
+      if ((key & mask) == prefix) atomicAdd(&bins[(int)(key >> shift) & digits], 1);
     }
-    cluster.sync();
-    // the bin in which the want-th from the top lies, of all blocks' histograms: thread i has the bins count - 1 - per * i downwards
-    constexpr int MOST = EV_BINS / EV_THREADS;
-    const int per = count / EV_THREADS;
-    int c[MOST], mine = 0;
+    sync();
+    const int slice = EV_BINS / blocks;
+    int below = 0;  // keys in the slices above the one that the want-th from the top lies in
+    int* from_bins = bins;
+    if (blocks > 1) {
+      int sum = 0;
+      for (int i = tid; i < slice; i += EV_THREADS) {
+        int c = 0;
 #pragma unroll
-    for (int e = 0; e < MOST; ++e) {
-      c[e] = 0;
-      if (e < per)
-        for (int r = 0; r < blocks; ++r) c[e] += cluster.map_shared_rank(bins, r)[count - 1 - per * tid - e];
+        for (int r = 0; r < 8; ++r)
+          if (r < blocks) c += cluster.map_shared_rank(bins, r)[rank * slice + i];
+        slice_bins[i] = c;
+        sum += c;
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane == 0 && sum) atomicAdd(&sh_slices[turn], sum);
+      sync();
+      int sums[8], owner = 0;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) sums[r] = r < blocks ? *cluster.map_shared_rank(&sh_slices[turn], r) : 0;
+      bool found = false;
+#pragma unroll
+      for (int r = 7; r >= 0; --r)
+        if (r < blocks && !found) {
+          if (want <= below + sums[r]) {
+            owner = r;
+            found = true;
+          } else {
+            below += sums[r];
+          }
+        }
+      from_bins = cluster.map_shared_rank(slice_bins, owner);
+      if (tid == 0) sh_digit = owner * slice;
+    } else if (tid == 0) {
+      sh_digit = 0;
+    }
+    // the bin in that slice: a thread has up to four, the first thread the top ones
+    static_assert(EV_BINS == 4 * EV_THREADS, "bins of a thread");
+    const int each = max(slice / EV_THREADS, 1), top_bin = slice - 1 - each * tid;
+    int c[4], mine = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      c[e] = e < each && top_bin - e >= 0 ? from_bins[top_bin - e] : 0;
       mine += c[e];
     }
     int upto = mine;
@@ -235,72 +280,65 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(const EvictPar
       const int y = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += y;
     }
-    int total;
-    int before = warps_before(__shfl_sync(0xffffffffu, upto, 31), sh_warps, total) + upto - mine;
+    if (lane == 31) sh_warps[warp] = upto;
+    __syncthreads();
+    int before = below + upto - mine;
 #pragma unroll
-    for (int e = 0; e < MOST; ++e)
-      if (e < per) {
-        if (before < want && want <= before + c[e]) {
-          sh_digit = (uint32_t)(count - 1 - per * tid - e);
-          sh_want = want - before;
-        }
-        before += c[e];
+    for (int w = 0; w < EV_WARPS; ++w)
+      if (w < warp) before += sh_warps[w];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (before < want && want <= before + c[e]) {
+        sh_digit += top_bin - e;
+        sh_want = want - before;
+        sh_count = c[e];
       }
-    cluster.sync();  // and every block has read the histograms
-    prefix |= sh_digit << sh;
-    mask |= (uint32_t)(count - 1) << sh;
+      before += c[e];
+    }
+    __syncthreads();
+    prefix |= (uint64_t)sh_digit << shift;
+    mask |= (uint64_t)digits << shift;
     want = sh_want;
+    if (sh_count == want) break;  // the whole bin stays
   }
   // ---- number the slots: each warp has a stretch of them, in steps of 32
   const int steps = (size + 31) / 32, per = (steps + EV_WARPS - 1) / EV_WARPS;
   const int lo = min(warp * per, steps), hi = min(lo + per, steps);
-  int ties = 0, over = 0, holes = 0;  // of the warp
-  for (int s = lo; s < hi; ++s) {
+  auto stay = [&](int s) {  // which of 32 slots stay
     const int i = s * 32 + lane;
-    const uint32_t u = i < size ? worth(i) : 0u;
-    ties += __popc(__ballot_sync(0xffffffffu, i < size && u == prefix));
-  }
-  int total;
-  int tie0 = warps_before(ties, sh_warps, total);
-  if (tid == 0) sh_ties = total;
-  cluster.sync();
-  for (int r = 0; r < rank; ++r) tie0 += *cluster.map_shared_rank(&sh_ties, r);
-  int tie = tie0;
-  // which of 32 slots stay; `tie` counts the slots of the keep-th's worth so far
-  auto stay = [&](int s) {
-    const int i = s * 32 + lane;
-    const uint32_t u = i < size ? worth(i) : 0u;
-    const unsigned eq = __ballot_sync(0xffffffffu, i < size && u == prefix);
-    const bool k = i < size && (u > prefix || (u == prefix && tie + __popc(eq & ((1u << lane) - 1u)) < want));
-    tie += __popc(eq);
-    return __ballot_sync(0xffffffffu, k);
+    return __ballot_sync(0xffffffffu, i < size && (key_of(min(i, size - 1)) & mask) >= prefix);
   };
-  // those of step s that lie before slot `keep`
-  auto front = [&](int s) {
+  auto front = [&](int s) {  // those of step s that lie before slot `keep`
     const int f = min(max(keep - base - s * 32, 0), 32);
     return f == 32 ? 0xffffffffu : (1u << f) - 1u;
   };
+  int64_t pair = 0;  // slots that become free, and above them (32 bits up) survivors from behind
   for (int s = lo; s < hi; ++s) {
     const unsigned k = stay(s), in_front = front(s);
-    holes += __popc(~k & in_front);
-    over += __popc(k & ~in_front);
+    pair += __popc(~k & in_front) + ((int64_t)__popc(k & ~in_front) << 32);
   }
-  int hole = warps_before(holes, sh_warps, total);
-  if (tid == 0) sh_holes = total;
-  int nth = warps_before(over, sh_warps, total);
-  if (tid == 0) sh_over = total;
-  cluster.sync();
-  int all = 0;
-  for (int r = 0; r < blocks; ++r) {
-    const int y = *cluster.map_shared_rank(&sh_holes, r);
-    if (r < rank) {
-      hole += y;
-      nth += *cluster.map_shared_rank(&sh_over, r);
+  if (lane == 0) sh_pairs[warp] = pair;
+  __syncthreads();
+  int64_t before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < EV_WARPS; ++w) {
+    if (w < warp) before += sh_pairs[w];
+    total += sh_pairs[w];
+  }
+  if (blocks > 1) {
+    if (tid == 0) sh_total = total;
+    cluster.sync();
+    total = 0;
+    for (int r = 0; r < blocks; ++r) {
+      const int64_t y = *cluster.map_shared_rank(&sh_total, r);
+      if (r < rank) before += y;
+      total += y;
     }
-    all += y;
   }
-  if (rank == 0 && tid == 0) p.moves[item] = all;
-  tie = tie0;
+  if (rank == 0 && tid == 0) p.moves[item] = (int)total;
+  int hole = (int)before, nth = (int)(before >> 32);
+  int* to = p.to + (int64_t)item * p.keep;
+  int* from = p.from + (int64_t)item * p.keep;
   for (int s = lo; s < hi; ++s) {
     const unsigned k = stay(s), in_front = front(s), below = (1u << lane) - 1u;
     const unsigned out = ~k & in_front, in = k & ~in_front;
@@ -311,7 +349,7 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(const EvictPar
     hole += __popc(out);
     nth += __popc(in);
   }
-  cluster.sync();  // no block ends while another reads its counts
+  if (blocks > 1) cluster.sync();  // no block ends while another reads what it counted
 }
 
 constexpr int MV_ROWS = 128;
@@ -531,8 +569,9 @@ extern "C" int tfb_cache_evict(const void* k_pages, const void* v_pages, const f
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = g_plain_launch.load(std::memory_order_relaxed) ? 1 : 2;
+    const int skip = p.cluster == 1 ? 1 : 0;  // a block alone needs no cluster
+    cfg.attrs = attr + skip;
+    cfg.numAttrs = (g_plain_launch.load(std::memory_order_relaxed) ? 1 : 2) - skip;
     (void)cudaLaunchKernelEx(&cfg, evict_select_kernel, static_cast<const EvictParams>(p));  // error read by launched()
   }
   if (int rc = launched("cache_evict")) return rc;
