@@ -99,6 +99,18 @@ __device__ __forceinline__ void cp4(uint32_t dst, const void* src, int bytes) {
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
+// A box that is read once: it leaves the L2 before the scores do, which are read again.
+__device__ __forceinline__ uint64_t read_once() {
+  uint64_t policy;
+  asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+  return policy;
+}
+__device__ __forceinline__ void load_box(void* dst, const CUtensorMap* m, int c0, int c1, int c2, int c3, uint64_t* bar, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, %5, %6}], [%2], %7;"
+      ::"r"(smem_u32(dst)), "l"(m), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "l"(policy)
+      : "memory");
+}
 __device__ __forceinline__ void ldm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -174,21 +186,23 @@ struct Cursor {
   }
 };
 
-// a * b / c and a / c, rounded down, for values below 2^53
-__device__ __forceinline__ int64_t floor_div(int64_t n, int64_t d) {
-  int64_t q = (int64_t)((double)n / (double)d);
-  if (q * d > n) --q;
-  if ((q + 1) * d <= n) ++q;
-  return q;
+__device__ __forceinline__ int64_t divide(int64_t n, int64_t d) {  // of values that are not negative
+  return ((n | d) >> 32) == 0 ? (int64_t)((uint32_t)n / (uint32_t)d) : n / d;
 }
-// The line has kRowCost units and one for each tile of a row, and is cut into `parts` stretches of whole units, one for each
-// warp; with fewer units than warps, of one unit.
+// The line has kRowCost units and one for each tile of a row, and is cut into equal stretches, one for each warp (with fewer
+// units than warps, of one unit): the first `more` have a unit more than `each`.
 struct Line {
-  int64_t units, parts;
-  __device__ __forceinline__ Line(int64_t units_, int ctas) : units(units_), parts(min(units_, (int64_t)ctas * PG_WARPS)) {}
-  __device__ __forceinline__ int64_t begin(int64_t part) const { return part < parts ? floor_div(part * units, parts) : units; }
+  int64_t units, each, more, parts;
+  __device__ __forceinline__ Line(int64_t units_, int ctas) : units(units_), parts(min(units_, (int64_t)ctas * PG_WARPS)) {
+    each = parts ? divide(units, parts) : 0;
+    more = units - each * parts;
+  }
+  __device__ __forceinline__ int64_t begin(int64_t part) const { return part < parts ? part * each + min(part, more) : units; }
   // the block whose warps have unit t
-  __device__ __forceinline__ int block_of(int64_t t) const { return (int)(floor_div((t + 1) * parts - 1, units) / PG_WARPS); }
+  __device__ __forceinline__ int block_of(int64_t t) const {
+    const int64_t wide = more * (each + 1);
+    return (int)((t < wide ? divide(t, each + 1) : more + divide(t - wide, each)) / PG_WARPS);
+  }
 };
 __device__ __forceinline__ int row_units(int tiles) { return tiles ? tiles + kRowCost : 0; }
 
@@ -201,9 +215,8 @@ __device__ __forceinline__ float alibi_rounded_log2(int mode, float slope, float
 struct Pieces {
   int64_t begin[PG_WARPS][2];  // the piece's row's first tile in the line
   int b[PG_WARPS][2], hr[PG_WARPS][2], tiles[PG_WARPS][2];
-  int has[PG_WARPS][2];        // [0] a piece that began before the warp's stretch, [1] one that goes on behind it
-  int ends[PG_WARPS];          // piece [0] is its row's last
-};
+  uint8_t flags[PG_WARPS];  // bit 0: there is a piece [0], which began before the warp's stretch; 1: a piece [1], which goes on
+};                          // behind it; 2: piece [0] is its row's last
 
 }  // namespace
 
@@ -217,7 +230,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ int64_t sh_scan[PG_WARPS], sh_from[PG_WARPS + 1], sh_base[PG_WARPS];
   __shared__ int sh_b[PG_WARPS];
-  __shared__ Pieces sh;
+  __shared__ __align__(8) Pieces sh;
   __shared__ int sh_abort, sh_last[2], sh_first[2];
   volatile int* abort_flag = &sh_abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -229,7 +242,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
     mbar_fence_init();
   }
   if (threadIdx.x == 0) *abort_flag = 0;
-  if (lane == 0) sh.has[warp][0] = sh.has[warp][1] = 0;
+  if (lane == 0) sh.flags[warp] = 0;
   grid_dependency_wait();
   allow_dependents();
 
@@ -326,6 +339,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
         }
       }
     };
+    const uint64_t once = read_once();
     auto copy = [&](int stage) {
       const int head = ld.hr / p.row_tiles, cached = ld.keys.cached(), slot0 = ld.j * C::KEYS;
       if constexpr (TMA) {
@@ -339,8 +353,8 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
         if (ok) {
 #pragma unroll
           for (int c = 0; c < C::PANELS; ++c) {
-            tma_load_4d(dst + c * C::KEYS * 128, &tmK, c * 64, row[0], head, page[0], &full[stage]);
-            tma_load_4d(dst + C::TILE + c * C::KEYS * 128, &tmV, c * 64, row[0], head, page[0], &full[stage]);
+            load_box(dst + c * C::KEYS * 128, &tmK, c * 64, row[0], head, page[0], &full[stage], once);
+            load_box(dst + C::TILE + c * C::KEYS * 128, &tmV, c * 64, row[0], head, page[0], &full[stage], once);
           }
         } else if (wanted) {  // no such page: zeros
           atomicCAS(&g_dev_status, 0, kBadPage);
@@ -695,12 +709,11 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
         if (!whole) {
           __syncwarp();  // the ring has been read
           if (lane == 0) {
-            sh.has[warp][first] = 1;
+            sh.flags[warp] |= first ? 2 : last ? 5 : 1;
             sh.begin[warp][first] = from + row_at;
             sh.b[warp][first] = row_b;
             sh.hr[warp][first] = row_hr;
             sh.tiles[warp][first] = row_tiles;
-            if (!first) sh.ends[warp] = last;
           }
         }
         if (fine) {  // the rests' products
@@ -751,21 +764,43 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
     return;
   }
   const float2* ml = reinterpret_cast<const float2*>(smem + C::OFF_ML);
-  int job = 0, open[2] = {-1, -1};  // the first warps of the chains that begin, or end, in another block
-  for (int w = 0; w < PG_WARPS; ++w) {
-#pragma unroll
-    for (int slot = 0; slot < 2; ++slot) {
-      // a chain starts with a piece [1], or with the piece [0] of the first warp
-      if (!sh.has[w][slot] || (slot == 0 && w > 0)) continue;
-      int end = w;  // its last warp
-      bool ended = slot == 0 && sh.ends[w];
-      while (!ended && end + 1 < PG_WARPS && sh.has[end + 1][0]) ended = sh.ends[++end];
-      const bool whole = slot == 1 && ended;
-      if (!whole) open[slot] = w;
+  const uint64_t flags = *reinterpret_cast<const uint64_t*>(sh.flags);
+  // bit w: of warp w
+  auto bits = [&](int bit) {  // bit `bit` of each byte, gathered
+    return (unsigned)(((flags >> bit & 0x0101010101010101ull) * 0x0102040810204080ull) >> 56);
+  };
+  const unsigned has0 = bits(0), has1 = bits(1), ends = bits(2);
+  // A chain of pieces starts with a piece [1], or with the piece [0] that has none before it in this block: only the first can.
+  const unsigned lead = has0 & (0u - has0);                             // the first warp with a piece [0]
+  const bool leads = lead != 0 && (has1 & (lead - 1u)) == 0;            // and nothing goes on into it
+  const int chains = __popc(has1) + leads, rows_most = min(R, p.group);
+  int open0 = -1, open1 = -1;  // the first warps of the chains that begin, or end, in another block
+  auto end_of = [&](int w, int slot) {  // a chain's last warp
+    int end = w;
+    bool ended = slot == 0 && (ends >> w & 1) != 0;
+    while (!ended && end + 1 < PG_WARPS && (has0 >> (end + 1) & 1) != 0) ended = (ends >> ++end & 1) != 0;
+    return ended ? end : end | 64;  // 64: the row goes on in the next block
+  };
+  if (leads) open0 = __ffs(lead) - 1;
+  if (has1 != 0) {  // only the last chain can go on
+    const int w = 31 - __clz(has1);
+    if (end_of(w, 1) & 64) open1 = w;
+  }
+  for (int job = warp; job < chains * rows_most; job += PG_WARPS) {
+    const int chain = job / rows_most, r = job - chain * rows_most;
+    const int slot = leads && chain == 0 ? 0 : 1;
+    int w = open0;
+    if (slot == 1) {
+      unsigned left = has1;
+      for (int i = chain - leads; i > 0; --i) left &= left - 1u;
+      w = __ffs(left) - 1;
+    }
+    const int end = end_of(w, slot) & 63;
+    const bool whole = slot == 1 && w != open1;
+    {
       const int b = sh.b[w][slot], hr = sh.hr[w][slot];
       const int kv = hr / p.row_tiles, r0 = (hr - kv * p.row_tiles) * R;
-      for (int r = 0; r < R && r0 + r < p.group; ++r) {
-        if (job++ % PG_WARPS != warp) continue;
+      if (r0 + r < p.group) {
         float m = kNone, l = 0.f, a[HD / 32];
         for (int i = w; i <= end; ++i) m = fmaxf(m, ml[(i * 2 + (i == w ? slot : 0)) * R + r].x);
 #pragma unroll
@@ -797,13 +832,13 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
       }
     }
   }
-  if (open[0] < 0 && open[1] < 0) return;
+  if (open0 < 0 && open1 < 0) return;
 
   // ---- rows that several blocks share: the block that comes last joins their pieces.  A block begins at most one such row,
   // whose counter is the block's.
   __syncthreads();
   if (warp < 2 && lane == 0) {
-    const int slot = warp, w = open[slot];
+    const int slot = warp, w = slot ? open1 : open0;
     sh_last[slot] = 0;
     if (w >= 0) {
       const int64_t t0 = sh.begin[w][slot];
@@ -822,7 +857,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
   for (int slot = 0; slot < 2; ++slot) {
     const int pieces = sh_last[slot], c0 = sh_first[slot];
     if (!pieces) continue;
-    const int w = open[slot], b = sh.b[w][slot], hr = sh.hr[w][slot];
+    const int w = slot ? open1 : open0, b = sh.b[w][slot], hr = sh.hr[w][slot];
     const int kv = hr / p.row_tiles, r0 = (hr - kv * p.row_tiles) * R, rows = min(R, p.group - r0);
     // threads along (row, 4 columns), and what is left of them along the pieces, up to a share for 8 pieces
     constexpr int N = 8, THREADS = PG_WARPS * 32;
