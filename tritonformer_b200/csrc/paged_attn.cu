@@ -83,6 +83,7 @@ struct PgParams {
   float* acc;       // [2 * ctas][R][hd]
   float* heads_acc; // [ctas][warps][R][hd] the pieces that a warp's stretch begins in the middle of
   float* scores;    // (B, kv_heads, capacity, group) in log2 units, or null
+  int scores_stay;  // they fit the L2
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -99,11 +100,13 @@ __device__ __forceinline__ void cp4(uint32_t dst, const void* src, int bytes) {
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// A box that is read once: it leaves the L2 before the scores do, which are read again.
-__device__ __forceinline__ uint64_t read_once() {
-  uint64_t policy;
-  asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
-  return policy;
+// A box is read once.  Where the scores stay in the L2 until they are read again, it leaves the L2 before they do (24 sequences of
+// up to 2048 keys: 35.1 us without, 33.6 with it); elsewhere that costs (2 of 49157 keys: 100.5 without, 102.4 with it).
+__device__ __forceinline__ uint64_t read_once(bool leave) {
+  uint64_t first, normal;
+  asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(first));
+  asm("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(normal));
+  return leave ? first : normal;
 }
 __device__ __forceinline__ void load_box(void* dst, const CUtensorMap* m, int c0, int c1, int c2, int c3, uint64_t* bar, uint64_t policy) {
   asm volatile(
@@ -339,7 +342,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
         }
       }
     };
-    const uint64_t once = read_once();
+    const uint64_t once = read_once(p.scores_stay);
     auto copy = [&](int stage) {
       const int head = ld.hr / p.row_tiles, cached = ld.keys.cached(), slot0 = ld.j * C::KEYS;
       if constexpr (TMA) {
@@ -923,36 +926,41 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
 // Adds the weights to the masses.  Blocks along (sequence, key head) and shares of its keys; a thread takes MASS_BATCH keys at a
 // time, all lookups of a kind together (one after the other the kernel waited for them: 25 us for 2.1 M keys of 8 heads).  V: how
 // many of a key's scores are read at once.
-constexpr int MASS_BATCH = 4, MASS_THREADS = 256;
+constexpr int MASS_BATCH = 4, MASS_THREADS = 128;
 template <int V>
 __global__ void __launch_bounds__(MASS_THREADS) paged_mass_kernel(const PgParams p) {
   __shared__ __align__(16) float sh_lse[128];
   grid_dependency_wait();
   allow_dependents();
-  const int b = blockIdx.x / p.kv_heads, kv = blockIdx.x % p.kv_heads;
-  const SeqKeys keys = keys_of(p, p.lengths[b]);
+  const int b = blockIdx.x / p.kv_heads, kv = blockIdx.x % p.kv_heads, cap = (int)p.map.capacity();
   constexpr int SPAN = MASS_BATCH * MASS_THREADS;
-  if (blockIdx.y * SPAN >= keys.n) return;
+  const int* table = p.map.tables + b * p.map.table_ld;
+  int page[MASS_BATCH], row[MASS_BATCH];
+  auto look_up = [&](int slot0) {  // does not wait for the length: entries behind it are read, not used
+#pragma unroll
+    for (int k = 0; k < MASS_BATCH; ++k) {
+      const int slot = min(slot0 + k * MASS_THREADS, cap - 1), i = (int)((unsigned)slot / (unsigned)p.map.page);
+      row[k] = slot - i * p.map.page;
+      page[k] = table[i];
+    }
+  };
+  const int len = p.lengths[b];
+  look_up(blockIdx.y * SPAN + threadIdx.x);
   for (int r = threadIdx.x; r < p.group; r += MASS_THREADS) {
     const float lse = p.lse[((int64_t)b * p.kv_heads + kv) * p.group + r];
     sh_lse[r] = lse == kNone ? INFINITY : lse;  // no weight anywhere: none for the masses either
   }
+  const SeqKeys keys = keys_of(p, len);
+  if (blockIdx.y * SPAN >= keys.n) return;
   const float* sc = p.scores + ((int64_t)b * p.kv_heads + kv) * p.map.capacity() * p.group;
-  const int* table = p.map.tables + b * p.map.table_ld;
   __syncthreads();
   for (int slot0 = blockIdx.y * SPAN + threadIdx.x; slot0 < keys.n; slot0 += gridDim.y * SPAN) {
     int64_t at[MASS_BATCH];
     float had[MASS_BATCH], w[MASS_BATCH];
-    int page[MASS_BATCH], row[MASS_BATCH];
 #pragma unroll
     for (int k = 0; k < MASS_BATCH; ++k) {
-      const int slot = min(slot0 + k * MASS_THREADS, keys.n - 1), i = (int)((unsigned)slot / (unsigned)p.map.page);
-      row[k] = slot - i * p.map.page;
-      page[k] = table[i];
-    }
-#pragma unroll
-    for (int k = 0; k < MASS_BATCH; ++k) {
-      const bool ok = (unsigned)page[k] < (unsigned)p.map.num_pages;  // the attention has reported a bad one
+      // of a slot in use the attention has reported a bad page
+      const bool ok = slot0 + k * MASS_THREADS < keys.n && (unsigned)page[k] < (unsigned)p.map.num_pages;
       at[k] = ok ? stat_offset(p.map, page[k], p.kv_heads, kv, row[k]) : -1;
       had[k] = ok ? p.mass[at[k]] : 0.f;
       w[k] = 0.f;
@@ -975,9 +983,9 @@ __global__ void __launch_bounds__(MASS_THREADS) paged_mass_kernel(const PgParams
     }
 #pragma unroll
     for (int k = 0; k < MASS_BATCH; ++k) {
-      const int slot = slot0 + k * MASS_THREADS;
-      if (slot < keys.n && at[k] >= 0) p.mass_out[at[k]] = slot == keys.fresh ? w[k] : had[k] + w[k];
+      if (at[k] >= 0) p.mass_out[at[k]] = slot0 + k * MASS_THREADS == keys.fresh ? w[k] : had[k] + w[k];
     }
+    look_up(slot0 + gridDim.y * SPAN);
   }
 }
 
@@ -1042,7 +1050,7 @@ int pg_launch(PgParams& p, int dtype, cudaStream_t st) {
   if (!p.mass_out) return TFB_OK;
   // enough blocks to fill the SMs, none with fewer keys of a full table than its threads take at once
   const int64_t rows = (int64_t)p.B * p.kv_heads, most = ceil_div(p.map.capacity(), MASS_BATCH * MASS_THREADS);
-  int64_t shares = ceil_div((int64_t)sm_count() * 8, rows);
+  int64_t shares = ceil_div((int64_t)sm_count() * 32, rows);
   if (shares > most) shares = most;
   const dim3 grid((unsigned)rows, (unsigned)shares);
   if (p.group % 4 == 0) launch_overlapped(paged_mass_kernel<4>, grid, dim3(MASS_THREADS), 0, st, p);
@@ -1132,6 +1140,7 @@ extern "C" int tfb_paged_attention(const void* q, const void* k_new, const void*
   p.heads_acc = reinterpret_cast<float*>(base + s.heads_acc);
   if (mass) {
     p.lse = static_cast<float*>(scratch);
+    p.scores_stay = B * kv_heads * group * p.map.capacity() * 4 <= (32 << 20);
     p.scores = reinterpret_cast<float*>(static_cast<char*>(scratch) + up256(B * kv_heads * group * 4));
   }
   cudaStream_t st = (cudaStream_t)stream;
