@@ -311,8 +311,8 @@ int tfb_loss_scale_update(float* state4, int* found_inf, float growth, float bac
  * page_strides = {page, head, slot} that both share (multiples of 8, unit stride on hd, 16-byte aligned bases), and for
  * eviction two statistics per (page, head, slot), both contiguous: the key's accumulated attention `mass` (fp32) and its
  * position in the text `positions` (int32; NULL: a key's position is its slot's number).  Slot s of sequence b lies in page
- * tables[b * table_ld + s / page] at row s % page; a sequence has at most width * page slots.  Entries of a table that no
- * slot in use refers to are never read.  lengths (B,) int32 lives on the device: nothing synchronises the host.
+ * tables[b * table_ld + s / page] at row s % page; a sequence has at most width * page slots.  What entries of
+ * a table hold that no slot in use refers to does not matter.  lengths (B,) int32 lives on the device: nothing synchronises the host.
  * A page id outside the cache reads as rows of zeros, or is not written, and sets 0x7200 in tfb_device_status(); a length that
  * is negative or beyond the table is taken as the nearest one that is not, and sets 0x7201.
  * Query head h uses key head h / group.  hd is 32, 64 or 128.

@@ -1,7 +1,7 @@
 """A paged key-value cache: what generating text with a trained model needs of attention (the reference trains only).
 
 The keys and values of a layer lie in a pool of pages, (pages, heads, page, head_dim).  Slot s of sequence b is row s % page of
-page `tables[b, s // page]`; entries of a table beyond the slots in use are never read.  `tables` (batch, pages of a sequence)
+page `tables[b, s // page]`; what a table holds beyond the slots in use does not matter.  `tables` (batch, pages of a sequence)
 and `lengths` (batch,) are int32 tensors on the GPU, so no call waits for the host and all of them can be captured in a CUDA
 graph.  For eviction every (page, head, slot) has two statistics: the attention that its key has got so far (`mass`, fp32), and
 the position of its token (`positions`, int32), because a key that moves to another slot keeps its distance for ALiBi.
@@ -69,9 +69,9 @@ def cache_append(k_pages, v_pages, tables, lengths, key, value, counts=None, mas
 
 def cache_evict(k_pages, v_pages, mass, positions, tables, lengths, keep, recent=0, next_positions=None, out=None,
                 out_tables=None):
-    """Every head of every sequence that has more than `keep` keys keeps `keep`: those whose position is at least
-    next_positions[b] - recent (positions and next_positions None: the slot's number and the length), then those of the largest
-    mass, ties to the lower slot.  Keys before slot `keep` that stay do not move; those from behind fill the free slots.
+    """Every head of every sequence that has more than `keep` keys keeps the `keep` of the largest mass, ties to the lower slot,
+    where a key whose position is at least next_positions[b] - recent (positions and next_positions None: the slot's number and
+    the length) counts as one of infinite mass.  Keys before slot `keep` that stay do not move; those from behind fill the free slots.
     Returns the new lengths.  In place, unless `out` = (k_pages, v_pages, mass, positions) of other buffers is given, and where
     their pages are others, `out_tables`; in place, no page may be part of two sequences."""
     k_out, v_out, mass_out, positions_out = (None,) * 4 if out is None else out
