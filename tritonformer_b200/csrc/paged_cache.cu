@@ -7,7 +7,7 @@
 // `recent` last ones; each (sequence, key head) keeps the `keep` worthiest, ties to the lower slot.  With the worth in the upper and
 // the inverted slot in the lower half all keys are different 64-bit numbers, and a cluster of one to eight blocks finds the
 // keep-th largest by a radix selection, 11 bits a pass.  The passes end as soon as all that is left in a bin stays: after two,
-// unless masses are equal.  The blocks add their histograms through distributed shared memory, each a slice of the bins (every
+// unless masses are equal, and of a block alone when few are left to be ranked.  The blocks add their histograms through distributed shared memory, each a slice of the bins (every
 // block reading every histogram took 5 us a pass of eight blocks, five times as long).  Then the keys that go and those that stay behind slot `keep` are numbered
 // in slot order, and a second kernel pairs the two: the i-th survivor from behind moves into the i-th slot that becomes
 // free.  So keys that stay in front are not touched, no source of a move is the goal of another, and the moves run in any order,
@@ -125,7 +125,8 @@ struct EvictParams {
 
 constexpr int EV_THREADS = 512, EV_WARPS = EV_THREADS / 32;
 constexpr int EV_BINS = 2048;
-constexpr int EV_BATCH = 8;  // worths that a thread looks up at a time
+constexpr int EV_BATCH = 4;  // worths that a thread looks up at a time
+constexpr int EV_RANKED = 256;  // of so many keys left, a block alone counts for each how many are above it (a pass saved, with ties three)
 
 // Worths in the order of unsigned numbers; -0 is 0, a mass that is no number is -infinity.
 __device__ __forceinline__ uint32_t worth_of(float m) {
@@ -160,6 +161,121 @@ __device__ __forceinline__ void worths_at(const EvictParams& p, int b, int h, in
   if (bad) atomicCAS(&g_dev_status, 0, kBadPage);
 }
 
+struct Slot {
+  int page, row;
+  bool ok;
+};
+__device__ __forceinline__ Slot slot_at(const PageMap& m, int b, int slot) {  // without a report
+  const int i = (int)((unsigned)slot / (unsigned)m.page), page = m.tables[b * m.table_ld + i];
+  return {page, slot - i * m.page, (unsigned)page < (unsigned)m.num_pages};
+}
+
+// Moves keys, values and statistics of a (sequence, key head): the survivors from behind into the free slots, and where the output
+// is another buffer the slots that stay as well.  The block takes every `step`-th batch from `first` on.
+template <int HD, int THREADS>
+__device__ __forceinline__ void move_rows(const EvictParams& p, int item, int b, int h, int moves, int left, int first, int step) {
+  constexpr int ROWS = THREADS / 2, LANES = HD / 8, PER = THREADS / LANES, N = ROWS / PER < 4 ? ROWS / PER : 4;  // N rows at a time
+  __shared__ int64_t sh_src[ROWS], sh_dst[ROWS];
+  const int* to = p.to + (int64_t)item * p.keep;
+  const int* from = p.from + (int64_t)item * p.keep;
+  const int batches = (moves + ROWS - 1) / ROWS;
+  const int all = batches + (p.rows_in_place ? 0 : (left + ROWS - 1) / ROWS);
+  auto stays = [&](int i) { return i < left && (moves == 0 || (p.stay[(int64_t)item * p.words + i / 32] >> (i % 32) & 1) != 0); };
+  if (p.rows_in_place && !p.stats_in_place) {  // of slots that stay the statistics alone, all lookups of a kind together
+    constexpr int K = 4;
+    for (int i0 = first * THREADS * K + threadIdx.x; i0 < left; i0 += step * THREADS * K) {
+      int64_t src[K], dst[K];
+      float mass[K];
+      int position[K];
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int i = i0 + k * THREADS;
+        const Slot a = slot_at(p.map, b, min(i, left - 1)), d = slot_at(p.out_map, b, min(i, left - 1));
+        const bool ok = stays(i) && a.ok && d.ok;
+        if (i < left && !(a.ok && d.ok)) atomicCAS(&g_dev_status, 0, kBadPage);
+        src[k] = ok ? stat_offset(p.map, a.page, p.kv_heads, h, a.row) : -1;
+        dst[k] = stat_offset(p.out_map, d.page, p.kv_heads, h, d.row);
+      }
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        mass[k] = src[k] >= 0 ? p.mass[src[k]] : 0.f;
+        position[k] = src[k] >= 0 && p.positions ? p.positions[src[k]] : 0;
+      }
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        if (src[k] >= 0) {
+          p.mass_out[dst[k]] = mass[k];
+          if (p.positions) p.positions_out[dst[k]] = position[k];
+        }
+    }
+  }
+  for (int batch = first; batch < all; batch += step) {
+    const bool move = batch < batches;  // otherwise slots that stay
+    const bool stats = move || !p.stats_in_place;
+    int64_t stat_src = -1, stat_dst = 0;
+    __syncthreads();
+    if (threadIdx.x < ROWS) {
+      const int i = (move ? batch : batch - batches) * ROWS + threadIdx.x;
+      int64_t src = -1, dst = 0;
+      int source = -1, goal = -1;
+      if (move) {
+        if (i < moves) {
+          source = from[i];
+          goal = to[i];
+        }
+      } else if (stays(i)) {
+        source = goal = i;
+      }
+      int page, row, page2, row2;
+      if (source >= 0 && find_slot(p.map, b, source, page, row) && find_slot(p.out_map, b, goal, page2, row2)) {
+        src = row_offset(p.map, page, h, row);
+        dst = row_offset(p.out_map, page2, h, row2);
+        stat_src = stat_offset(p.map, page, p.kv_heads, h, row);
+        stat_dst = stat_offset(p.out_map, page2, p.kv_heads, h, row2);
+      }
+      sh_src[threadIdx.x] = src;
+      sh_dst[threadIdx.x] = dst;
+    }
+    // the statistics' loads go out beside the rows'
+    const bool mine = stats && stat_src >= 0;
+    float mass = 0.f;
+    int position = 0;
+    if (mine) {
+      mass = p.mass[stat_src];
+      if (p.positions) position = p.positions[stat_src];
+    }
+    __syncthreads();
+    const int c = (threadIdx.x % LANES) * 8;
+#pragma unroll
+    for (int r0 = 0; r0 < ROWS; r0 += PER * N) {
+      uint4 kr[N], vr[N];
+      int64_t from_row[N];
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        from_row[e] = sh_src[r0 + e * PER + threadIdx.x / LANES];
+        if (from_row[e] >= 0) {
+          kr[e] = ld_stream16(static_cast<const uint16_t*>(p.k) + from_row[e] + c);
+          vr[e] = ld_stream16(static_cast<const uint16_t*>(p.v) + from_row[e] + c);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const int64_t to_row = sh_dst[r0 + e * PER + threadIdx.x / LANES];
+        if (from_row[e] >= 0) {
+          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.k_out) + to_row + c) = kr[e];
+          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.v_out) + to_row + c) = vr[e];
+        }
+      }
+    }
+    if (mine) {
+      p.mass_out[stat_dst] = mass;
+      if (p.positions) p.positions_out[stat_dst] = position;
+    }
+  }
+}
+
+// MOVE: the head_dim where the blocks move the rows as well, otherwise 0.
+template <int MOVE>
 __global__ void __launch_bounds__(EV_THREADS, 2) evict_select_kernel(const EvictParams p) {
   extern __shared__ uint32_t worths[];
   __shared__ __align__(16) int bins[EV_BINS];
@@ -167,7 +283,8 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_select_kernel(const Evict
   __shared__ int slice_bins[EV_BINS];  // of this block's slice, all blocks' counts
   __shared__ int sh_slices[2];         // and their sum, in turn: another block may still read the last pass's
   __shared__ int64_t sh_pairs[EV_WARPS], sh_total;
-  __shared__ int sh_digit, sh_want, sh_count;
+  __shared__ int sh_digit, sh_want, sh_count, sh_found;
+  __shared__ uint64_t ranked[EV_RANKED], sh_key;
   cg::cluster_group cluster = cg::this_cluster();
   grid_dependency_wait();
   allow_dependents();
@@ -181,7 +298,8 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_select_kernel(const Evict
     p.left[b] = keep;
   }
   if (n <= keep) {
-    if (rank == 0 && tid == 0) p.moves[item] = 0;
+    if constexpr (MOVE != 0) move_rows<MOVE, EV_THREADS>(p, item, b, h, 0, keep, rank, blocks);
+    else if (rank == 0 && tid == 0) p.moves[item] = 0;
     return;
   }
   auto sync = [&]() {
@@ -222,7 +340,7 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_select_kernel(const Evict
     const int shift = max(top - 11, 0), digits = (1 << (top - shift)) - 1;
     top = shift;
     for (int i = tid; i < EV_BINS; i += EV_THREADS) bins[i] = 0;
-    if (tid == 0) sh_slices[turn] = 0;
+    if (tid == 0) sh_slices[turn] = sh_found = 0;
     __syncthreads();
     for (int i = tid; i < size; i += EV_THREADS) {
       const uint64_t key = key_of(i);
@@ -299,7 +417,25 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_select_kernel(const Evict
     prefix |= (uint64_t)sh_digit << shift;
     mask |= (uint64_t)digits << shift;
     want = sh_want;
-    if (sh_count == want) break;  // the whole bin stays
+    const int left = sh_count;
+    if (left == want) break;  // the whole bin stays
+    if (blocks == 1 && left <= EV_RANKED) {  // few enough to be ranked against one another
+      for (int i = tid; i < size; i += EV_THREADS) {
+        const uint64_t key = key_of(i);
+        if ((key & mask) == prefix) ranked[atomicAdd(&sh_found, 1)] = key;
+      }
+      __syncthreads();
+      if (tid < left) {
+        const uint64_t key = ranked[tid];
+        int above = 0;
+        for (int i = 0; i < left; ++i) above += ranked[i] > key;
+        if (above == want - 1) sh_key = key;
+      }
+      __syncthreads();
+      prefix = sh_key;
+      mask = ~0ull;
+      break;
+    }
   }
   // ---- number the slots: each warp has a stretch of them, in steps of 32
   const int steps = (size + 31) / 32, per = (steps + EV_WARPS - 1) / EV_WARPS;
@@ -335,7 +471,7 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_select_kernel(const Evict
       total += y;
     }
   }
-  if (rank == 0 && tid == 0) p.moves[item] = (int)total;
+  if (MOVE == 0 && rank == 0 && tid == 0) p.moves[item] = (int)total;
   int hole = (int)before, nth = (int)(before >> 32);
   int* to = p.to + (int64_t)item * p.keep;
   int* from = p.from + (int64_t)item * p.keep;
@@ -350,79 +486,46 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_select_kernel(const Evict
     nth += __popc(in);
   }
   if (blocks > 1) cluster.sync();  // no block ends while another reads what it counted
-}
-
-constexpr int MV_ROWS = 128;
-
-// Moves keys, values and statistics: the survivors from behind into the free slots, and where the output is another buffer the
-// slots that stay as well.
-template <int HD>
-__global__ void __launch_bounds__(256) evict_move_kernel(const EvictParams p) {
-  constexpr int LANES = HD / 8, PER = 256 / LANES, N = 4;
-  __shared__ int64_t sh_src[MV_ROWS], sh_dst[MV_ROWS];
-  grid_dependency_wait();
-  allow_dependents();
-  const int item = blockIdx.x, b = item / p.kv_heads, h = item % p.kv_heads;
-  const int moves = p.moves[item], left = p.left[b];
-  const int* to = p.to + (int64_t)item * p.keep;
-  const int* from = p.from + (int64_t)item * p.keep;
-  const int batches = (moves + MV_ROWS - 1) / MV_ROWS;
-  const int all = batches + (p.rows_in_place && p.stats_in_place ? 0 : (left + MV_ROWS - 1) / MV_ROWS);
-  for (int batch = blockIdx.y; batch < all; batch += gridDim.y) {
-    const bool move = batch < batches;  // otherwise slots that stay
-    const bool rows = move || !p.rows_in_place, stats = move || !p.stats_in_place;
-    __syncthreads();
-    if (threadIdx.x < MV_ROWS) {
-      const int i = (move ? batch : batch - batches) * MV_ROWS + threadIdx.x;
-      int64_t src = -1, dst = 0;
-      int source = -1, goal = -1;
-      if (move) {
-        if (i < moves) {
-          source = from[i];
-          goal = to[i];
-        }
-      } else if (i < left && (moves == 0 || (p.stay[(int64_t)item * p.words + i / 32] >> (i % 32) & 1) != 0)) {
-        source = goal = i;
-      }
-      int page, row, page2, row2;
-      if (source >= 0 && find_slot(p.map, b, source, page, row) && find_slot(p.out_map, b, goal, page2, row2)) {
-        src = row_offset(p.map, page, h, row);
-        dst = row_offset(p.out_map, page2, h, row2);
-        if (stats) {
-          const int64_t at = stat_offset(p.map, page, p.kv_heads, h, row), out = stat_offset(p.out_map, page2, p.kv_heads, h, row2);
-          p.mass_out[out] = p.mass[at];
-          if (p.positions) p.positions_out[out] = p.positions[at];
-        }
-      }
-      sh_src[threadIdx.x] = src;
-      sh_dst[threadIdx.x] = dst;
-    }
-    if (!rows) continue;
-    __syncthreads();
-    const int c = (threadIdx.x % LANES) * 8;
-    for (int r0 = threadIdx.x / LANES; r0 < MV_ROWS; r0 += PER * N) {
-      uint4 kr[N], vr[N];
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const int r = r0 + e * PER;
-        if (r < MV_ROWS && sh_src[r] >= 0) {
-          kr[e] = ld_stream16(static_cast<const uint16_t*>(p.k) + sh_src[r] + c);
-          vr[e] = ld_stream16(static_cast<const uint16_t*>(p.v) + sh_src[r] + c);
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const int r = r0 + e * PER;
-        if (r < MV_ROWS && sh_src[r] >= 0) {
-          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.k_out) + sh_dst[r] + c) = kr[e];
-          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.v_out) + sh_dst[r] + c) = vr[e];
-        }
-      }
-    }
+  if constexpr (MOVE != 0) {
+    if (blocks == 1) __syncthreads();  // the lists are written
+    move_rows<MOVE, EV_THREADS>(p, item, b, h, (int)total, keep, rank, blocks);
   }
 }
 
+// The moves as a kernel of their own, on more blocks than have selected.
+template <int HD>
+__global__ void __launch_bounds__(256, 4) evict_move_kernel(const EvictParams p) {
+  grid_dependency_wait();
+  allow_dependents();
+  const int item = blockIdx.x, b = item / p.kv_heads;
+  move_rows<HD, 256>(p, item, b, item % p.kv_heads, p.moves[item], p.left[b], blockIdx.y, gridDim.y);
+}
+
 int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
+
+constexpr int EV_SMEM = 200 * 1024;  // worths, beside the kernel's own arrays
+
+template <int MOVE>
+int evict_select(const EvictParams& p, int64_t smem, cudaStream_t st) {
+  static std::atomic<uint64_t> done{0};
+  if (int rc = ensure_dynamic_smem(evict_select_kernel<MOVE>, EV_SMEM, done, "cache_evict")) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(p.B * p.kv_heads * p.cluster));
+  cfg.blockDim = dim3(EV_THREADS);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)p.cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  const int skip = p.cluster == 1 ? 1 : 0;  // a block alone needs no cluster
+  cfg.attrs = attr + skip;
+  cfg.numAttrs = (g_plain_launch.load(std::memory_order_relaxed) ? 1 : 2) - skip;
+  (void)cudaLaunchKernelEx(&cfg, evict_select_kernel<MOVE>, static_cast<const EvictParams>(p));  // error read by launched()
+  return launched("cache_evict");
+}
 
 template <typename E, int HD, bool VEC>
 int append_launch(const AppendParams& p, cudaStream_t st) {
@@ -551,32 +654,22 @@ extern "C" int tfb_cache_evict(const void* k_pages, const void* v_pages, const f
   // as many blocks for a (sequence, key head) as the SMs have room for, none with fewer than 2048 slots of a full table
   p.cluster = 1;
   while (p.cluster < 8 && B * kv_heads * p.cluster * 2 <= sm_count() * 2 && p.map.capacity() >= (int64_t)p.cluster * 2 * 2048) p.cluster *= 2;
-  constexpr int kMost = 200 * 1024;  // beside the kernel's own arrays
   int64_t smem = (ceil_div(ceil_div(p.map.capacity(), 32), p.cluster) * 32 * 4 + 15) / 16 * 16;
-  if (smem > kMost) smem = kMost;
+  if (smem > EV_SMEM) smem = EV_SMEM;
   p.room = (int)(smem / 4);
-  static std::atomic<uint64_t> done{0};
-  if (int rc = ensure_dynamic_smem(evict_select_kernel, kMost, done, "cache_evict")) return rc;
-  {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(B * kv_heads * p.cluster));
-    cfg.blockDim = dim3(EV_THREADS);
-    cfg.dynamicSmemBytes = (size_t)smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)p.cluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    const int skip = p.cluster == 1 ? 1 : 0;  // a block alone needs no cluster
-    cfg.attrs = attr + skip;
-    cfg.numAttrs = (g_plain_launch.load(std::memory_order_relaxed) ? 1 : 2) - skip;
-    (void)cudaLaunchKernelEx(&cfg, evict_select_kernel, static_cast<const EvictParams>(p));  // error read by launched()
-  }
-  if (int rc = launched("cache_evict")) return rc;
-  // a block for each MV_ROWS rows that can move or stay, as far as that takes to fill the SMs
-  int64_t shares = ceil_div(keep, MV_ROWS) * (p.rows_in_place && p.stats_in_place ? 1 : 2);
+  // Where single blocks select and fill half the SMs they move the rows too: blocks that are done early move while others
+  // select, and there is one launch (256 heads of up to 2048 keys into other pages 24.5 us, with two launches 26.3; 96 heads of 1088
+  // keys 8 us of the host's time against 13).  Clusters leave the moves to a grid of their own (32 heads of 32768 keys: 68 us, with
+  // one launch 71).
+  const bool fused = p.cluster == 1 && B * kv_heads * 2 >= sm_count();
+  int rc;
+  if (!fused) rc = evict_select<0>(p, smem, st);
+  else if (hd == 32) rc = evict_select<32>(p, smem, st);
+  else if (hd == 64) rc = evict_select<64>(p, smem, st);
+  else rc = evict_select<128>(p, smem, st);
+  if (rc || fused) return rc;
+  // a block for each 128 rows that can move or stay, as far as that takes to fill the SMs
+  int64_t shares = ceil_div(keep, 128) * (p.rows_in_place && p.stats_in_place ? 1 : 2);
   const int64_t enough = ceil_div((int64_t)sm_count() * 16, B * kv_heads);
   if (shares > enough) shares = enough;
   const dim3 grid((unsigned)(B * kv_heads), (unsigned)shares);
