@@ -83,8 +83,8 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
       const int r = i * PER + threadIdx.x / LANES;
       if (sh_page[r] >= 0) {
         const int64_t o = row_offset(p.map, sh_page[r], h, sh_row[r]) + c;
-        *reinterpret_cast<uint4*>(static_cast<E*>(p.k) + o) = kr[i];
-        *reinterpret_cast<uint4*>(static_cast<E*>(p.v) + o) = vr[i];
+        st_stream16(static_cast<E*>(p.k) + o, kr[i]);
+        st_stream16(static_cast<E*>(p.v) + o, vr[i]);
       }
     }
   } else {
@@ -262,8 +262,8 @@ __device__ __forceinline__ void move_rows(const EvictParams& p, int item, int b,
       for (int e = 0; e < N; ++e) {
         const int64_t to_row = sh_dst[r0 + e * PER + threadIdx.x / LANES];
         if (from_row[e] >= 0) {
-          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.k_out) + to_row + c) = kr[e];
-          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.v_out) + to_row + c) = vr[e];
+          st_stream16(static_cast<uint16_t*>(p.k_out) + to_row + c, kr[e]);
+          st_stream16(static_cast<uint16_t*>(p.v_out) + to_row + c, vr[e]);
         }
       }
     }
