@@ -314,7 +314,8 @@ int tfb_loss_scale_update(float* state4, int* found_inf, float growth, float bac
  * tables[b * table_ld + s / page] at row s % page; a sequence has at most width * page slots.  What entries of
  * a table hold that no slot in use refers to does not matter.  lengths (B,) int32 lives on the device: nothing synchronises the host.
  * A page id outside the cache reads as rows of zeros, or is not written, and sets 0x7200 in tfb_device_status(); a length that
- * is negative or beyond the table is taken as the nearest one that is not, and sets 0x7201.
+ * is negative or beyond the table is taken as the nearest one that is not, and sets 0x7201.  Results of such a call are not to
+ * be used.
  * Query head h uses key head h / group.  hd is 32, 64 or 128.
  *
  * tfb_paged_attention: out (B, kv_heads * group, hd) = attention of one query per sequence over its lengths[b] keys.  With k_new
@@ -322,7 +323,7 @@ int tfb_loss_scale_update(float* state4, int* found_inf, float growth, float bac
  * No keys: zeros.  slopes and alibi_round as in tfb_attention_fwd, with distance query_positions[b] - position of the key
  * (query_positions NULL: the number of the last slot); a new key's position is the query's.  With mass and mass_out (the same
  * buffer, or another one of its shape) mass_out = mass + the key's weights, summed over the query heads of its key head, in the
- * slots in use; a new key starts from zero.  group <= 128.  Strides {b, h} in elements, unit stride on hd, any alignment.
+ * slots in use; a new key starts from zero; no page may then be part of two sequences.  group <= 128.  Strides {b, h} in elements, unit stride on hd, any alignment.
  * workspace: at least tfb_paged_attention_workspace_bytes(), 16-byte aligned, its first 8192 bytes ZERO on entry and zero again
  * when the kernel has finished (the GEMM's workspace, where that is large enough, serves both); calls that share one must be
  * stream-ordered.  scratch is for masses only and needs no initialisation; capacity = width * page.            */
@@ -361,8 +362,8 @@ int tfb_prompt_mass(const void* q, const void* k, const float* lse, const int* c
 /* Eviction: every (sequence, key head) of more than `keep` keys keeps the `keep` of the largest mass, where a key whose position
  * is at least next_positions[b] - recent (NULL: lengths[b] - recent) counts as one of infinite mass and a mass that is no number as
  * one of -infinity; ties go to the lower slot.  Keys that stay and lie before slot `keep` stay in their slots; those from behind fill
- * the slots that become free, in the order of their slots.  left[b] = min(lengths[b], keep) is the new length (left may be
- * lengths).  The outputs, each with its statistics, are either the inputs (and out_tables = tables: in place; no page may then be
+ * the slots that become free, in the order of their slots.  left[b] = min(lengths[b], keep) is the new length (in an array of
+ * its own: lengths is still read).  The outputs, each with its statistics, are either the inputs (and out_tables = tables: in place; no page may then be
  * part of two sequences) or other buffers of the same kv_heads and hd, which get every slot that is left.  keep >= recent. */
 int64_t tfb_cache_evict_scratch_bytes(int64_t B, int64_t kv_heads, int64_t keep);
 int tfb_cache_evict(const void* k_pages, const void* v_pages, const float* mass, const int* positions,

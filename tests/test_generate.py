@@ -62,6 +62,14 @@ def test_a_budget_that_is_never_reached_changes_nothing():
     assert torch.equal(plain, kept)
 
 
+def test_inside_an_autocast_region():
+    model = _model(dtype=torch.float16)
+    ids = torch.randint(0, 1000, (1, 70), device="cuda")
+    plain = _teacher(model, ids, 60, Generator(model, 1, 128, budget=64))
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        assert torch.equal(plain, _teacher(model, ids, 60, Generator(model, 1, 128, budget=64)))
+
+
 def test_prompts_of_different_lengths():
     """A sequence's logits do not depend on what it shares the batch with."""
     model = _model()

@@ -364,6 +364,17 @@ def test_mass_lengths(T, hd, dtype):
 
 
 @gpu
+def test_mass_reports_bad_counts():
+    q, k = (torch.randn((2, 2, 40, 64), device="cuda", generator=_gen(s)).half() for s in (1, 2))
+    lse = _mass_reference(q, k, None)[1]
+    for bad in (-1, 41):
+        counts = torch.tensor([bad, 40], dtype=torch.int32, device="cuda")
+        kvcache.prompt_mass(q, k, lse, counts)
+        assert L.device_status(reset=True) == 0x7201
+    assert torch.equal(kvcache.prompt_mass(q, k, lse), kvcache.prompt_mass(q, k, lse, torch.full((2,), 40, dtype=torch.int32, device="cuda")))
+
+
+@gpu
 def test_mass_prompts_of_all_lengths():
     _check_mass(7, 2, 2, 400, 64, torch.float16, counts=[0, 400, 1, 128, 129, 0, 256])
     _check_mass(3, 1, 1, 40, 64, torch.float16, counts=[0, 0, 0])
@@ -691,10 +702,13 @@ def test_argument_checks_without_device():
     assert L.lib.tfb_prompt_mass(one, one, one, None, None, 0, one, 1, 2, 1, 0, 64, three, three, two, None, 0, 0, None) == 0
 
     def evict(keep=4, recent=0, k_out=one, out_tables=one, mass_out=one, out_width=2, nbytes=1 << 20):
-        return L.lib.tfb_cache_evict(one, one, one, None, one, one, None, k_out, k_out, mass_out, None, out_tables, one, 1, 2, 64, keep,
+        return L.lib.tfb_cache_evict(one, one, one, None, one, one, None, k_out, k_out, mass_out, None, out_tables, two, 1, 2, 64, keep,
                                      recent, 16, 4, 2, 2, pg, 16, 4, out_width, 2, pg, one, nbytes, 0, None)
 
     other = ctypes.c_void_p(1 << 20)
+    rc = L.lib.tfb_cache_evict(one, one, one, None, one, one, None, one, one, one, None, one, one, 1, 2, 64, 4, 0, 16, 4, 2, 2, pg, 16, 4,
+                               2, 2, pg, one, 1 << 20, 0, None)
+    said(rc, -1, b"array of their own")
     said(evict(keep=0), -1, b"at least 1")
     said(evict(recent=5), -1, b"0 to keep")
     said(evict(out_tables=other), -1, b"pages of their own")

@@ -614,6 +614,7 @@ extern "C" int tfb_cache_evict(const void* k_pages, const void* v_pages, const f
               (long long)p.out_map.capacity());
   TFB_REQUIRE(B * kv_heads < (1LL << 28), "cache_evict: too many rows of heads");
   TFB_REQUIRE(mass && mass_out, "cache_evict: no masses");
+  TFB_REQUIRE(left && left != lengths, "cache_evict: the new lengths need an array of their own");
   TFB_REQUIRE((positions == nullptr) == (positions_out == nullptr), "cache_evict: positions come with positions for the output");
   TFB_REQUIRE((k_out == k_pages) == (v_out == v_pages), "cache_evict: keys in place and values not, or the other way round");
   if (B == 0) return TFB_OK;

@@ -215,7 +215,6 @@ __global__ void __launch_bounds__(PmCfg<HD>::THREADS, 1) prompt_mass_kernel(cons
   const int64_t count = blockIdx.x < parts ? (blockIdx.x + 1) * total / parts - from : 0;
   for (int b = b_lo; b < b_hi; ++b) {
     const int64_t tiles = pm_tiles(p, pm_count(p, b));
-    if (blockIdx.x == 0 && p.counts && (p.counts[b] < 0 || p.counts[b] > p.T)) atomicCAS(dev_status(), 0, kBadLength);
     if (from >= base && from < base + tiles) {
       sh_b = b;
       sh_base = base;
@@ -491,6 +490,9 @@ __global__ void __launch_bounds__(PmCfg<HD>::THREADS, 1) prompt_mass_kernel(cons
     tc_fence_after();
     tmem_dealloc(tmem_base, 512);
   }
+  if (blockIdx.x == 0 && p.counts)  // at the end, because no CTA begins while the status is set
+    for (int b = b_lo; b < b_hi; ++b)
+      if (p.counts[b] < 0 || p.counts[b] > p.T) atomicCAS(dev_status(), 0, kBadLength);
   // ---- key tiles that several CTAs share: the last of them adds the pieces.  A CTA begins at most one such tile, whose counter
   // is the CTA's.
   if (*abort_flag || !(sh_open[0] || sh_open[1])) return;

@@ -5,7 +5,7 @@
     logits = gen.prefill(prompts, lengths); logits = gen.step(tokens) # or token by token
 
 The prompts' attention is the training forward; their keys and values (and with a budget their attention masses) go into the
-cache's pages.  A step writes each sequence's new key and value and attends over its pages in one call per layer.  With a budget every
+cache's pages.  Everything runs in the model's own type, also inside an autocast region.  A step writes each sequence's new key and value and attends over its pages in one call per layer.  With a budget every
 head of every layer keeps the `recent` last keys and those that have got most attention, after the prompt and then every
 `interval` tokens.  The reference has no counterpart: it trains only.
 """
@@ -60,6 +60,7 @@ class Generator:
                                  mlp.dense_4h_to_h.bias, x)
 
     @torch.no_grad()
+    @torch.autocast("cuda", enabled=False)
     def prefill(self, prompts, lengths=None):
         """Starts the sequences: prompts (batch, T) int64, the first lengths[b] of each (all by default).  Returns the logits
         (batch, vocab) of the tokens that follow."""
@@ -128,6 +129,7 @@ class Generator:
         self.next += 1
 
     @torch.no_grad()
+    @torch.autocast("cuda", enabled=False)
     def step(self, tokens):
         """Appends one token per sequence, (batch,) int64.  Returns the logits (batch, vocab) of those that follow, in a buffer
         that the next step writes again."""

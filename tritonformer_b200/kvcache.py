@@ -38,7 +38,7 @@ def paged_attention(query, k_pages, v_pages, tables, lengths, key=None, value=No
     """Attention of one query per sequence, (batch, heads, head_dim), over the lengths[b] keys in its pages; with `key` and
     `value` (batch, cache heads, head_dim) over those and the new key, which is written into slot lengths[b] (`lengths` itself
     stays).  A sequence without keys gets zeros.  With `mass` every key's weights, summed over the query heads of its head, are
-    added to it, in place or into `mass_out`; with `positions` the new key's entry is set.  The query's position is
+    added to it, in place or into `mass_out` (no page may then be part of two sequences); with `positions` the new key's entry is set.  The query's position is
     query_positions[b], or the number of the last slot."""
     bias = _NO_BIAS if attn_bias is None else _slopes(attn_bias, query.shape[1])
     return _host.paged_attention(query, k_pages, v_pages, tables, lengths, key, value, bias.slopes, int(bias.rounded),
