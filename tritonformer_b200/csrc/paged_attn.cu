@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
   constexpr int R = C::R, STAGES = C::STAGES, STAGE = 2 * C::TILE, KS = HD / 16;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ int64_t sh_scan[PG_WARPS], sh_from[PG_WARPS + 1], sh_base[PG_WARPS];
+  __shared__ int64_t sh_scan[PG_WARPS], sh_base[PG_WARPS];
   __shared__ int sh_b[PG_WARPS];
   __shared__ __align__(8) Pieces sh;
   __shared__ int sh_abort, sh_last[2], sh_first[2];
@@ -246,57 +246,86 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
   }
   if (threadIdx.x == 0) *abort_flag = 0;
   if (lane == 0) sh.flags[warp] = 0;
+  if (TMA && threadIdx.x == 32) {
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  __syncthreads();
   grid_dependency_wait();
   allow_dependents();
 
-  // ---- the warps' stretches: a scan over the sequences' tiles
-  const int per = (p.B + PG_WARPS * 32 - 1) / (PG_WARPS * 32);
-  const int b_lo = min((int)threadIdx.x * per, p.B), b_hi = min(b_lo + per, p.B);
-  int64_t mine = 0;
-  for (int b = b_lo; b < b_hi; ++b) mine += row_units((keys_of(p, p.lengths[b]).n + C::KEYS - 1) / C::KEYS);
-  int64_t upto = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += v;
-  }
-  if (lane == 31) sh_scan[warp] = upto;
-  __syncthreads();
-  int64_t base = upto - mine, total = 0;
-#pragma unroll
-  for (int w = 0; w < PG_WARPS; ++w) {
-    const int64_t v = sh_scan[w];
-    if (w < warp) base += v;
-    total += v;
-  }
-  const Line line(total * heads, p.ctas);
-  if (threadIdx.x <= PG_WARPS) sh_from[threadIdx.x] = line.units ? line.begin((int64_t)blockIdx.x * PG_WARPS + threadIdx.x) : 0;
-  __syncthreads();
-  for (int b = b_lo; b < b_hi; ++b) {
-    const int len = p.lengths[b];
-    const int tiles = (keys_of(p, len).n + C::KEYS - 1) / C::KEYS;
-    if (b % (int)gridDim.x == (int)blockIdx.x) {
-      if (len < 0 || (int64_t)len + (p.k_new ? 1 : 0) > p.map.capacity()) atomicCAS(&g_dev_status, 0, kBadLength);
-      if (tiles == 0) {  // no keys: zeros
-        T* out = static_cast<T*>(p.out) + b * p.o_b;
-        for (int h = 0; h < p.kv_heads * p.group; ++h)
-          for (int d = 0; d < HD; ++d) out[h * p.o_h + d] = Num<T>::from_f(0.f);
-      }
+  // What one block of the grid does beside its stretches for sequence b: a report, zeros where there are no keys.
+  auto look_over = [&](int b, int len, int tiles) {
+    if (b % (int)gridDim.x != (int)blockIdx.x) return;
+    if (len < 0 || (int64_t)len + (p.k_new ? 1 : 0) > p.map.capacity()) atomicCAS(&g_dev_status, 0, kBadLength);
+    if (tiles == 0) {
+      T* out = static_cast<T*>(p.out) + b * p.o_b;
+      for (int h = 0; h < p.kv_heads * p.group; ++h)
+        for (int d = 0; d < HD; ++d) out[h * p.o_h + d] = Num<T>::from_f(0.f);
     }
+  };
+  // ---- the warps' stretches: a scan over the sequences' units
+  const int64_t part = (int64_t)blockIdx.x * PG_WARPS + warp;
+  Line line(0, 0);
+  int start_b = 0;
+  int64_t start_base = 0;  // the units before it
+  if (p.B <= 32) {         // each warp by itself: no barrier, one load (one user 10.0 us, with the scan below 10.9)
+    const int len = lane < p.B ? p.lengths[lane] : 0;
+    const int tiles = lane < p.B ? (keys_of(p, len).n + C::KEYS - 1) / C::KEYS : 0;
+    const uint32_t mine = row_units(tiles);
+    uint32_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    line = Line((int64_t)__shfl_sync(0xffffffffu, upto, 31) * heads, p.ctas);
+    const unsigned behind = __ballot_sync(0xffffffffu, (int64_t)upto * heads > line.begin(part));
+    start_b = behind ? __ffs(behind) - 1 : 0;
+    start_base = (int64_t)__shfl_sync(0xffffffffu, upto - mine, start_b) * heads;
+    if (warp == 0 && lane < p.B) look_over(lane, len, tiles);
+  } else {
+    const int per = (p.B + PG_WARPS * 32 - 1) / (PG_WARPS * 32);
+    const int b_lo = min((int)threadIdx.x * per, p.B), b_hi = min(b_lo + per, p.B);
+    int64_t mine = 0;
+    for (int b = b_lo; b < b_hi; ++b) mine += row_units((keys_of(p, p.lengths[b]).n + C::KEYS - 1) / C::KEYS);
+    int64_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    if (lane == 31) sh_scan[warp] = upto;
+    __syncthreads();
+    int64_t base = upto - mine, total = 0;
 #pragma unroll
     for (int w = 0; w < PG_WARPS; ++w) {
-      const int64_t f = sh_from[w];
-      if (f >= base * heads && f < (base + row_units(tiles)) * heads) {
-        sh_b[w] = b;
-        sh_base[w] = base * heads;
-      }
+      const int64_t v = sh_scan[w];
+      if (w < warp) base += v;
+      total += v;
     }
-    base += row_units(tiles);
+    line = Line(total * heads, p.ctas);
+    for (int b = b_lo; b < b_hi; ++b) {
+      const int len = p.lengths[b];
+      const int tiles = (keys_of(p, len).n + C::KEYS - 1) / C::KEYS;
+      look_over(b, len, tiles);
+#pragma unroll 1
+      for (int w = 0; w < PG_WARPS; ++w) {
+        const int64_t f = line.begin((int64_t)blockIdx.x * PG_WARPS + w);
+        if (f >= base * heads && f < (base + row_units(tiles)) * heads) {
+          sh_b[w] = b;
+          sh_base[w] = base * heads;
+        }
+      }
+      base += row_units(tiles);
+    }
+    __syncthreads();
+    start_b = sh_b[warp];
+    start_base = sh_base[warp];
   }
-  if (sh_from[0] >= line.units) return;  // nothing for this block
-  __syncthreads();
-  const int64_t from = sh_from[warp];
-  const int length = (int)(sh_from[warp + 1] - from);
+  if (line.begin((int64_t)blockIdx.x * PG_WARPS) >= line.units) return;  // nothing for this block
+  const int64_t from = line.begin(part);
+  const int length = (int)(line.begin(part + 1) - from);
 
   uint8_t* ring = smem + warp * STAGES * STAGE;
   const uint32_t ring_at = smem_u32(ring);
@@ -315,9 +344,9 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
   Cursor<C::KEYS> cu;
   cu.at = length;
   if (length > 0) {
-    cu.b = sh_b[warp];
+    cu.b = start_b;
     cu.load(p);
-    const int64_t in = from - sh_base[warp];  // units of the sequence before the stretch
+    const int64_t in = from - start_base;  // units of the sequence before the stretch
     const int units = row_units(cu.tiles);
     cu.hr = in < (1LL << 31) ? (int)((uint32_t)in / (uint32_t)units) : (int)(in / units);
     cu.j = (int)(in - (int64_t)cu.hr * units) - kRowCost;
