@@ -3,15 +3,19 @@
 // Both move rows of 64 to 256 bytes between places that tables name; what bounds them is the bytes of the rows, so a warp takes
 // whole rows in 16-byte chunks, several at a time, and looks the places up beside the copies.
 //
+// Measured: prompts of up to 4096 keys, 16 x 8 heads of 128 with statistics, 272 MB in and out, 46.0 us (5.9 TB/s; rows stored so that
+// they leave the caches first, 48.9 without).  Eviction in place of 4 x 8 heads of 128 from 32768 to 8192 keys 66 us, of which the
+// selection takes 32; of 16 x 16 heads of 64 from up to 2048 to 512 keys into other pages 23.6; from 1088 to 1024 keys 10.6.
+//
 // Eviction has a selection before its copies.  A key's worth is its mass, or infinite while its position is among the
 // `recent` last ones; each (sequence, key head) keeps the `keep` worthiest, ties to the lower slot.  With the worth in the upper and
 // the inverted slot in the lower half all keys are different 64-bit numbers, and a cluster of one to eight blocks finds the
 // keep-th largest by a radix selection, 11 bits a pass.  The passes end as soon as all that is left in a bin stays: after two,
-// unless masses are equal, and of a block alone when few are left to be ranked.  The blocks add their histograms through distributed shared memory, each a slice of the bins (every
-// block reading every histogram took 5 us a pass of eight blocks, five times as long).  Then the keys that go and those that stay behind slot `keep` are numbered
-// in slot order, and a second kernel pairs the two: the i-th survivor from behind moves into the i-th slot that becomes
-// free.  So keys that stay in front are not touched, no source of a move is the goal of another, and the moves run in any order,
-// in place, all at once.
+// unless masses are equal, and of a block alone when few are left to be ranked.  The blocks add their histograms through
+// distributed shared memory, each a slice of the bins (every block reading every histogram took 5 us a pass of eight blocks, five
+// times as long).  Then the keys that go and those that stay behind slot `keep` are numbered in slot order, and a second kernel
+// pairs the two: the i-th survivor from behind moves into the i-th slot that becomes free.  So keys that stay in front are not
+// touched, no source of a move is the goal of another, and the moves run in any order, in place, all at once.
 #include <cooperative_groups.h>
 #include "paged.cuh"
 

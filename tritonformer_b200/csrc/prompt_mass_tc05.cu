@@ -18,8 +18,8 @@
 // Bound: the exponentials, one per score, 16 a clock and SM: 2048 clocks for a tile of 128 x 256, against 512 of the product at
 // head_dim 64.  One pair in four goes to the FMA pipe (a polynomial of degree 5 for 2^f, |f| <= 1/2, relative error 2.1e-7 in 32
 // bits, the SFU's own being 2.4e-7).  A tile of 128 x 128, with a warp for the terms, was bound by the
-// issuing warps' 1.2 k clocks a tile instead.  Measured: 4 prompts of 2048 tokens, 16 heads of 64, exact slopes 64 us (88 with
-// 128 x 128); one of 8192, 12 query heads of 128 on 4 key heads 143 us (264): 72% of what the SFU alone could do.
+// issuing warps' 1.2 k clocks a tile instead.  Measured: 4 prompts of 2048 tokens, 16 heads of 64, exact slopes 62 us (89 with
+// 128 x 128); one of 8192, 12 query heads of 128 on 4 key heads 152 us (264).
 #include "attn.cuh"
 #include "paged.cuh"
 #include "tc05.cuh"
