@@ -1,0 +1,30 @@
+"""The paged key-value cache where values, lengths and layouts are at their limits.  Bounds as in test_kvcache.py, unless a test
+says otherwise."""
+import math
+
+import pytest
+import torch
+
+from test_kvcache import U, Cache, _attend_reference, _gen
+from tritonformer_b200 import kvcache
+
+gpu = pytest.mark.gpu
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("group", [1, 4, 5, 8, 9, 16, 24])
+def test_attention_is_rounded_once_whatever_the_group(group, hd, dtype):
+    """The weights enter the second product in two parts, so u^2 of them is lost and not u; 32-bit sums of a few tiles lose 2^-17."""
+    c = Cache([129, 40, 700], 2, hd, 32, dtype)
+    q = (2 * torch.randn((3, 2 * group, hd), device="cuda", generator=_gen(1))).to(dtype)
+    ref, _, weights = _attend_reference(q, c.copy(), None)
+    bound = []
+    for b, n in enumerate(c.lengths):
+        p, r = c.at(b, torch.arange(n, device="cuda"))
+        v = c.v[p, :, r].double().abs().repeat_interleave(group, 1)  # (n, heads, hd)
+        scale = torch.einsum("hn,nhd->hd", weights[b], v)
+        bound.append(U[dtype] * ref[b].abs() + (1e-5 + 2.0 ** -17 + U[dtype] ** 2) * scale + n * 2.0 ** -29 * v.amax() + 1e-7)
+    out = kvcache.paged_attention(q, c.k, c.v, c.tables, c.len)
+    assert ((out.double() - ref).abs() <= torch.stack(bound)).all()

@@ -16,7 +16,7 @@
 // Only masses need a second kernel: a key's weight is known once its row's sum is.
 //
 // Measured (bf16, head_dim 128): 2 sequences of 49157 keys, 12 heads, 99.7 us, 6.06 TB/s (93% of a copy); 64 sequences of up to 8192
-// keys, 8 key heads of 8 query heads, with masses, 223 us, of which the first kernel takes 189 at 5.8 TB/s.  Head_dim 64, fp16: 24
+// keys, 8 key heads of 8 query heads, with masses, 214 us, of which the first kernel takes most.  Head_dim 64, fp16: 24
 // sequences of up to 2048 keys, 16 heads, slopes and masses 32.7 us; one of 700 keys, 12 heads, 10.0 us.
 //
 // Copies.  Where pages and tiles share a divisor of 8 rows or more, TMA boxes of that many rows, which also swizzle the rows
@@ -26,6 +26,7 @@
 // of 8 heads wastes less than one of 16, and P^T comes out of the first product's registers by a transposition of 8x8
 // blocks (movmatrix).  tcgen05 has no place here: its smallest M would be fed from shared memory that the CUDA cores have to
 // write P into, and nothing waits for the tensor core.
+#include <cfloat>
 #include "attn.cuh"
 #include "paged.cuh"
 #include "tc05.cuh"
@@ -43,7 +44,9 @@ constexpr float kNone = -INFINITY;
 // What beginning a row of scores costs a warp, in tiles: rows of a tile or two would otherwise pile up in a few warps.
 constexpr int kRowCost = 4;
 
-template <int HD, int NT, int BIAS> struct PgCfg {
+// G: query heads that a warp takes at once, 4, 8 or 16.
+template <int HD, int G, int BIAS> struct PgCfg {
+  static constexpr int NT = G == 16 ? 2 : 1;   // blocks of 8 columns in the products
   static constexpr int KEYS = 2048 / HD;       // keys of a tile
   static constexpr int MT = KEYS / 16;
   static constexpr int R = 8 * NT;             // query heads of a head tile
@@ -140,6 +143,8 @@ template <> __device__ __forceinline__ void mma<__nv_bfloat16>(float (&c)[4], co
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// An infinite or missing number as the nearest finite one or the lowest: on top of a sum that is not finite either it changes nothing.
+__device__ __forceinline__ float finite(float x) { return fminf(fmaxf(x, -FLT_MAX), FLT_MAX); }
 template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   const typename Num<T>::T2 v = Num<T>::from_f2(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
@@ -228,11 +233,11 @@ struct Pieces {
 }  // namespace
 
 // BIAS: 0 none, 1 exact slopes, 2 slopes rounded as a table's
-template <typename T, int HD, int NT, int BIAS, bool TMA>
+template <typename T, int HD, int G, int BIAS, bool TMA>
 __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __grid_constant__ CUtensorMap tmK,
                                                                       const __grid_constant__ CUtensorMap tmV, const PgParams p) {
-  using C = PgCfg<HD, NT, BIAS>;
-  constexpr int R = C::R, STAGES = C::STAGES, STAGE = 2 * C::TILE, KS = HD / 16;
+  using C = PgCfg<HD, G, BIAS>;
+  constexpr int NT = C::NT, R = C::R, STAGES = C::STAGES, STAGE = 2 * C::TILE, KS = HD / 16;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ int64_t sh_scan[PG_WARPS], sh_base[PG_WARPS];
@@ -340,10 +345,12 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
                         : p.heads_acc + ((int64_t)blockIdx.x * PG_WARPS + w) * (R * HD);
   };
   const int g8 = lane >> 2, j2 = 2 * (lane & 3);  // row of an 8x8 block, first of its two columns
-  // With at most four query heads the instruction's other four columns repeat them, and carry what the rounding of the
-  // probabilities to 16 bits leaves: the product then has twice the bits, for the price of that subtraction.
-  const bool fine = NT == 1 && p.group <= 4;
-  const bool rest = fine && j2 >= 4;
+  // The second product takes the probabilities in two parts of 16 bits: rounded, and what that leaves (64 sequences of 8 query heads a
+  // key head: 1.2e-3 off in bf16, its own rounding; 1.6e-3 with the first part alone).  Up to four query heads the instruction's other
+  // four columns repeat them and carry the rest; more heads take a second product (that case: 214 us, 219 without it, from a kernel
+  // that chose between the two while it ran).
+  constexpr bool FINE = G == 4, APART = G == 8;  // APART: in sums of its own, for more than 8 heads there are no registers
+  const bool rest = FINE && j2 >= 4;
 
   Cursor<C::KEYS> cu;
   cu.at = length;
@@ -467,7 +474,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
       const T* q = static_cast<const T*>(p.q) + c.b * p.q_b;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const int r = r0 + (fine ? g8 & 3 : nt * 8 + g8);
+        const int r = r0 + (FINE ? g8 & 3 : nt * 8 + g8);
         const T* qr = q + (int64_t)(kv * p.group + r) * p.q_h + j2;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
@@ -485,7 +492,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
         if (BIAS)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const int rr = r0 + (fine ? (j2 + e) & 3 : nt * 8 + j2 + e);
+            const int rr = r0 + (FINE ? (j2 + e) & 3 : nt * 8 + j2 + e);
             w.slope[nt][e] = rr < p.group ? p.slopes[kv * p.group + rr] : 0.f;
           }
       }
@@ -515,7 +522,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
     constexpr int PER_PANEL = HD == 32 ? 2 : 4;  // k-steps in a row of at most 128 bytes
     constexpr uint32_t BLOCK16 = 16 * (HD == 32 ? 64 : 128), PANEL = C::KEYS * 128;
 
-    float ref[NT][2], sum[NT][2], o[KS][NT][4];
+    float ref[NT][2], sum[NT][2], o[KS][NT][4], o_rest[APART ? KS : 1][4];
     int first = 0;  // whether the piece began with its row's first tile
     bool begin = true;
     int stage = 0, warm_up = STAGES - 1;  // tiles to copy before the first one is worked on
@@ -553,6 +560,11 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[m][nt][e] = 0.f;
+        if (APART)
+#pragma unroll
+          for (int m = 0; m < KS; ++m)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o_rest[m][e] = 0.f;
       }
       if (warm_up == 0) {
         if (!TMA || (BIAS && p.positions)) cp_wait<STAGES - 2>();
@@ -688,12 +700,17 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
               for (int m = 0; m < KS; ++m) {
                 o[m][nt][e] *= f;
                 o[m][nt][2 + e] *= f;
+                if (APART) {
+                  o_rest[m][e] *= f;
+                  o_rest[m][2 + e] *= f;
+                }
               }
             }
           }
       }
-      // ---- probabilities, rounded to the values' type for the second product; the sum takes them unrounded
-      uint32_t pt[C::MT][NT][2];
+      // ---- probabilities for the second product: rounded to the values' type (pt), and what that leaves, rounded too (rt); the sum
+      // takes them unrounded
+      uint32_t pt[C::MT][NT][2], rt[C::MT][NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float from_ref[2];
@@ -709,12 +726,14 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
               w[e] = ex2(s[m][nt][2 * half + e] - from_ref[e]);
               sum[nt][e] += w[e];
             }
-            uint32_t u = pack2<T>(w[0], w[1]);
-            if (rest) {
+            const uint32_t u = pack2<T>(w[0], w[1]);
+            uint32_t left = u;
+            if (!FINE || rest) {
               const float2 f = Num<T>::to_f2(*reinterpret_cast<const typename Num<T>::T2*>(&u));
-              u = pack2<T>(w[0] - f.x, w[1] - f.y);
+              left = pack2<T>(w[0] - f.x, w[1] - f.y);
             }
-            pt[m][nt][half] = transpose8(u);
+            pt[m][nt][half] = transpose8(FINE ? left : u);
+            if (!FINE) rt[m][nt][half] = transpose8(left);
           }
       }
 #pragma unroll
@@ -725,7 +744,28 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
           ldm4t(a, tile + (v_at ^ ((hm % PER_PANEL) << 5)) + (hm / PER_PANEL) * PANEL + m * BLOCK16);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) mma<T>(o[hm][nt], a, pt[m][nt][0], pt[m][nt][1]);
+          if (APART) mma<T>(o_rest[hm], a, rt[m][0][0], rt[m][0][1]);
         }
+      if (!APART && !FINE) {
+        // The rests' products on top, unless a value is infinite: a rest of zero or below would make NaN of that.
+        float zero = 0.f;  // NaN if a sum is not finite
+#pragma unroll
+        for (int m = 0; m < KS; ++m)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) zero = fmaf(o[m][nt][e], 0.f, zero);
+        if (!__any_sync(0xffffffffu, zero != zero))
+#pragma unroll
+          for (int m = 0; m < C::MT; ++m)
+#pragma unroll
+            for (int hm = 0; hm < KS; ++hm) {
+              uint32_t a[4];
+              ldm4t(a, tile + (v_at ^ ((hm % PER_PANEL) << 5)) + (hm / PER_PANEL) * PANEL + m * BLOCK16);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma<T>(o[hm][nt], a, rt[m][nt][0], rt[m][nt][1]);
+            }
+      }
       if (++stage == STAGES) {
         stage = 0;
         phase ^= 1;
@@ -752,11 +792,16 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
             sh.tiles[warp][first] = row_tiles;
           }
         }
-        if (fine) {  // the rests' products
+        if (FINE) {  // the rests' products
 #pragma unroll
           for (int m = 0; m < KS; ++m)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[m][0][e] += __shfl_xor_sync(0xffffffffu, o[m][0][e], 2);
+        } else if (APART) {
+#pragma unroll
+          for (int m = 0; m < KS; ++m)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[m][0][e] += finite(o_rest[m][e]);
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -1029,7 +1074,6 @@ namespace {
 
 int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 
-int head_tiles(int64_t group) { return group <= 8 ? 1 : 2; }  // tiles of 8 heads that a warp takes at once
 // Workspace: counters, then the pieces of blocks and warps for the widest rows.  Scratch, for the masses: log-sum-exps, scores.
 constexpr int64_t kCounterBytes = 8192;
 struct PgWorkspace {
@@ -1045,16 +1089,16 @@ PgWorkspace pg_workspace() {
   return s;
 }
 
-template <typename T, int HD, int NT, int BIAS, bool TMA>
+template <typename T, int HD, int G, int BIAS, bool TMA>
 int pg_split(const CUtensorMap& tk, const CUtensorMap& tv, const PgParams& p, cudaStream_t st) {
-  using C = PgCfg<HD, NT, BIAS>;
+  using C = PgCfg<HD, G, BIAS>;
   static std::atomic<uint64_t> done{0};
-  if (int rc = ensure_dynamic_smem(paged_attn_kernel<T, HD, NT, BIAS, TMA>, C::SMEM, done, "paged_attention")) return rc;
-  launch_overlapped(paged_attn_kernel<T, HD, NT, BIAS, TMA>, dim3(p.ctas), dim3(PG_WARPS * 32), C::SMEM, st, tk, tv, p);
+  if (int rc = ensure_dynamic_smem(paged_attn_kernel<T, HD, G, BIAS, TMA>, C::SMEM, done, "paged_attention")) return rc;
+  launch_overlapped(paged_attn_kernel<T, HD, G, BIAS, TMA>, dim3(p.ctas), dim3(PG_WARPS * 32), C::SMEM, st, tk, tv, p);
   return launched("paged_attention");
 }
 
-template <typename T, int HD, int NT>
+template <typename T, int HD, int G>
 int pg_launch(PgParams& p, int dtype, cudaStream_t st) {
   // rows of a box: what divides both a page and a tile, so that a tile is whole boxes and a box lies in one page
   int box = 2048 / HD;
@@ -1071,13 +1115,13 @@ int pg_launch(PgParams& p, int dtype, cudaStream_t st) {
     const uint32_t shape[4] = {HD < 64 ? (uint32_t)HD : 64u, (uint32_t)box, 1, 1};
     const auto encode = HD == 32 ? encode_tmap_sw64 : encode_tmap_sw128;
     if ((rc = encode(&tk, p.k, dtype, 4, dims, str, shape)) || (rc = encode(&tv, p.v, dtype, 4, dims, str, shape))) return rc;
-    rc = p.bias_mode == 0   ? pg_split<T, HD, NT, 0, true>(tk, tv, p, st)
-         : p.bias_mode == 1 ? pg_split<T, HD, NT, 1, true>(tk, tv, p, st)
-                            : pg_split<T, HD, NT, 2, true>(tk, tv, p, st);
+    rc = p.bias_mode == 0   ? pg_split<T, HD, G, 0, true>(tk, tv, p, st)
+         : p.bias_mode == 1 ? pg_split<T, HD, G, 1, true>(tk, tv, p, st)
+                            : pg_split<T, HD, G, 2, true>(tk, tv, p, st);
   } else {
-    rc = p.bias_mode == 0   ? pg_split<T, HD, NT, 0, false>(tk, tv, p, st)
-         : p.bias_mode == 1 ? pg_split<T, HD, NT, 1, false>(tk, tv, p, st)
-                            : pg_split<T, HD, NT, 2, false>(tk, tv, p, st);
+    rc = p.bias_mode == 0   ? pg_split<T, HD, G, 0, false>(tk, tv, p, st)
+         : p.bias_mode == 1 ? pg_split<T, HD, G, 1, false>(tk, tv, p, st)
+                            : pg_split<T, HD, G, 2, false>(tk, tv, p, st);
   }
   if (rc) return rc;
   if (!p.mass_out) return TFB_OK;
@@ -1093,7 +1137,8 @@ int pg_launch(PgParams& p, int dtype, cudaStream_t st) {
 
 template <typename T, int HD>
 int pg_dispatch(PgParams& p, int dtype, cudaStream_t st) {
-  return head_tiles(p.group) == 1 ? pg_launch<T, HD, 1>(p, dtype, st) : pg_launch<T, HD, 2>(p, dtype, st);
+  if (p.group <= 4) return pg_launch<T, HD, 4>(p, dtype, st);
+  return p.group <= 8 ? pg_launch<T, HD, 8>(p, dtype, st) : pg_launch<T, HD, 16>(p, dtype, st);
 }
 
 }  // namespace
@@ -1162,7 +1207,7 @@ extern "C" int tfb_paged_attention(const void* q, const void* k_new, const void*
   p.B = (int)B;
   p.kv_heads = (int)kv_heads;
   p.group = (int)group;
-  p.row_tiles = (int)ceil_div(group, 8 * head_tiles(group));
+  p.row_tiles = (int)ceil_div(group, 16);
   p.ctas = sm_count();
   p.scale = kLog2e / sqrtf((float)hd);
   p.q_pairs = ((reinterpret_cast<uintptr_t>(q) | (uintptr_t)(p.q_b * 2) | (uintptr_t)(p.q_h * 2)) & 3) == 0;
