@@ -28,3 +28,25 @@ def test_attention_is_rounded_once_whatever_the_group(group, hd, dtype):
         bound.append(U[dtype] * ref[b].abs() + (1e-5 + 2.0 ** -17 + U[dtype] ** 2) * scale + n * 2.0 ** -29 * v.amax() + 1e-7)
     out = kvcache.paged_attention(q, c.k, c.v, c.tables, c.len)
     assert ((out.double() - ref).abs() <= torch.stack(bound)).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("group", [1, 4, 5, 8, 16])
+def test_attention_of_an_infinite_value_is_infinite(group, hd, dtype):
+    """A weight times infinity is infinity, in this value's column alone; equal weights, in tiles before and behind it as well."""
+    n = 600
+    c = Cache([n], 1, hd, 16, dtype)
+    p, r = c.at(0, torch.tensor([7, 300], device="cuda"))
+    c.v[p, 0, r, 3] = torch.tensor([math.inf, 1.0], device="cuda", dtype=dtype)
+    c.v[p, 0, r, 9] = torch.tensor([1.0, -math.inf], device="cuda", dtype=dtype)
+    q = torch.zeros((1, group, hd), device="cuda", dtype=dtype)
+    out = kvcache.paged_attention(q, c.k, c.v, c.tables, c.len)[0].double()
+    p, r = c.at(0, torch.arange(n, device="cuda"))
+    v = c.v[p, 0, r].double()
+    want = v.mean(0)
+    plain = want.isfinite()
+    assert torch.equal(out[:, ~plain], want[~plain].expand(group, -1)) and int((~plain).sum()) == 2
+    bound = 2 * U[dtype] * v.abs().mean(0) + 1e-5  # the rests of the finite columns may go with the infinite one
+    assert ((out - want).abs() <= bound)[:, plain].all()

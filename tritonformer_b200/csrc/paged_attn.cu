@@ -796,7 +796,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
 #pragma unroll
           for (int m = 0; m < KS; ++m)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[m][0][e] += __shfl_xor_sync(0xffffffffu, o[m][0][e], 2);
+            for (int e = 0; e < 4; ++e) o[m][0][e] += finite(__shfl_xor_sync(0xffffffffu, o[m][0][e], 2));
         } else if (APART) {
 #pragma unroll
           for (int m = 0; m < KS; ++m)
