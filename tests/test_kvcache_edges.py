@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_kvcache import U, Cache, _attend_reference, _gen
+from test_kvcache import U, Cache, _attend_reference, _check_mass, _gen, _mass_reference
 from tritonformer_b200 import kvcache
 
 gpu = pytest.mark.gpu
@@ -50,3 +50,21 @@ def test_attention_of_an_infinite_value_is_infinite(group, hd, dtype):
     assert torch.equal(out[:, ~plain], want[~plain].expand(group, -1)) and int((~plain).sum()) == 2
     bound = 2 * U[dtype] * v.abs().mean(0) + 1e-5  # the rests of the finite columns may go with the infinite one
     assert ((out - want).abs() <= bound)[:, plain].all()
+
+
+# ------------------------------------------------------------------------------------------------------- prompt mass
+
+
+@gpu
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("T", [100, 256, 640, 1300])
+def test_mass_of_heads_that_follow_one_another(T, hd):
+    """Runs of one tile, or of an odd number, each with the log-sum-exps of another query head: none sees its neighbour's."""
+    q = (2 * torch.randn((2, 6, T, hd), device="cuda", generator=_gen(T))).half()
+    q *= torch.tensor([0.1, 1.5, 1.0, 2.0, 0.2, 1.0], device="cuda").half()[:, None, None]  # sums far apart
+    k = torch.randn((2, 2, T, hd), device="cuda", generator=_gen(T + 1)).half()
+    slopes = torch.rand((6,), device="cuda", generator=_gen(0)) * 0.3
+    first = _check_mass(2, 2, 3, T, hd, torch.float16, slopes=slopes, q=q, k=k)
+    lse = _mass_reference(q, k, None, slopes)[1]
+    for _ in range(20):
+        assert torch.equal(first, kvcache.prompt_mass(q, k, lse, attn_bias=slopes))

@@ -351,10 +351,12 @@ __global__ void __launch_bounds__(PmCfg<HD>::THREADS, 1) prompt_mass_kernel(cons
       int dist = (cu.i - cu.j) * PM_TILE + part * PM_COLS + j2 - quarter * 32 - g8;  // of the first query from the first key
       bool diagonal = cu.i == cu.j;
       for (int k = 0; k < tiles; ++k) {
-        // The term of a query's column: -lse * log2(e); -inf past the prompt's end, or where the row gives no weight.
-        float* mine = terms + (k & 1) * PM_COLS;
+        // The term of a query's column: -lse * log2(e); -inf past the prompt's end, or where the row gives no weight.  Two buffers in
+        // turn, over the ends of runs too: between a tile's reads and the writes two tiles on lies the barrier of the tile between.
+        float* mine = terms + buf * PM_COLS;
 #pragma unroll
         for (int e = 0; e < PM_COLS / 32; ++e) mine[e * 32 + lane] = lse[e] == -INFINITY ? -INFINITY : lse[e] * -kLog2e;
+        __syncwarp();
         if (k + 1 < tiles) fetch(run, k + 1);
         else if (left > 0) fetch(after, 0);
         ok = __all_sync(0xffffffffu, mbar_wait(&s_full[buf], parity, 0x8500 | buf, abort_flag));
