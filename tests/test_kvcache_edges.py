@@ -5,6 +5,8 @@ import math
 import pytest
 import torch
 
+import tritonformer_b200._lib as L
+
 from test_kvcache import U, Cache, _attend_reference, _check_mass, _gen, _mass_reference
 from tritonformer_b200 import kvcache
 
@@ -68,3 +70,30 @@ def test_mass_of_heads_that_follow_one_another(T, hd):
     lse = _mass_reference(q, k, None, slopes)[1]
     for _ in range(20):
         assert torch.equal(first, kvcache.prompt_mass(q, k, lse, attn_bias=slopes))
+
+
+@gpu
+@pytest.mark.parametrize("alibi", [False, True])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("T,counts", [(200, [150, 1, 0]), (512, [300, 256, 511]), (700, [129, 640, 500])])
+def test_mass_does_not_see_what_lies_behind_a_prompt(T, counts, hd, alibi):
+    """Padding may be NaN or infinite, in the queries, the keys and the log-sum-exps; so may a query whose row gives no weight."""
+    q = (2 * torch.randn((3, 4, T, hd), device="cuda", generator=_gen(T))).to(torch.bfloat16)
+    k = torch.randn((3, 2, T, hd), device="cuda", generator=_gen(T + 1)).to(torch.bfloat16)
+    slopes = torch.rand((4,), device="cuda", generator=_gen(0)) * 0.3 if alibi else None
+    clean = _check_mass(3, 2, 2, T, hd, torch.bfloat16, counts=counts, slopes=slopes, q=q, k=k)
+    lse = _mass_reference(q, k, counts, slopes)[1]
+    n = torch.tensor(counts, dtype=torch.int32, device="cuda")
+    for value in (math.nan, math.inf, -math.inf):
+        bad = q.clone(), k.clone(), lse.clone()
+        for b, count in enumerate(counts):
+            for x in bad:
+                x[b, :, count:] = value
+        assert torch.equal(clean, kvcache.prompt_mass(*bad, n, attn_bias=slopes))
+    lse[:, :, 40:60] = -math.inf
+    want = kvcache.prompt_mass(q, k, lse, n, attn_bias=slopes)
+    for value in (math.nan, math.inf):
+        bad = q.clone()
+        bad[:, :, 40:60] = value
+        assert torch.equal(want, kvcache.prompt_mass(bad, k, lse, n, attn_bias=slopes))
+    assert want.isfinite().all() and L.device_status() == 0

@@ -23,6 +23,7 @@
 #include "attn.cuh"
 #include "paged.cuh"
 #include "tc05.cuh"
+#include <cfloat>
 #include <type_traits>
 
 namespace tfb {
@@ -351,11 +352,19 @@ __global__ void __launch_bounds__(PmCfg<HD>::THREADS, 1) prompt_mass_kernel(cons
       int dist = (cu.i - cu.j) * PM_TILE + part * PM_COLS + j2 - quarter * 32 - g8;  // of the first query from the first key
       bool diagonal = cu.i == cu.j;
       for (int k = 0; k < tiles; ++k) {
-        // The term of a query's column: -lse * log2(e); -inf past the prompt's end, or where the row gives no weight.  Two buffers in
-        // turn, over the ends of runs too: between a tile's reads and the writes two tiles on lies the barrier of the tile between.
+        // The term of a query's column: -lse * log2(e).  It is -inf, and the column is left out, past the prompt's end and where the
+        // row gives no weight; any other one is finite or NaN.  Two buffers in turn, over the ends of runs too: between a tile's reads
+        // and the writes two tiles on lies the barrier of the tile between.
         float* mine = terms + buf * PM_COLS;
+        bool out = false, in = false;
 #pragma unroll
-        for (int e = 0; e < PM_COLS / 32; ++e) mine[e * 32 + lane] = lse[e] == -INFINITY ? -INFINITY : lse[e] * -kLog2e;
+        for (int e = 0; e < PM_COLS / 32; ++e) {
+          const bool none = lse[e] == -INFINITY;
+          mine[e * 32 + lane] = none ? -INFINITY : at_least(lse[e] * -kLog2e, -FLT_MAX);
+          out |= none;
+          in |= !none;
+        }
+        const bool holes = __any_sync(0xffffffffu, out), any = __any_sync(0xffffffffu, in);
         __syncwarp();
         if (k + 1 < tiles) fetch(run, k + 1);
         else if (left > 0) fetch(after, 0);
@@ -367,8 +376,10 @@ __global__ void __launch_bounds__(PmCfg<HD>::THREADS, 1) prompt_mass_kernel(cons
         // and columns would cancel near the diagonal, where the weights are.
         const float dist_f = (float)dist;
         const uint64_t dist2 = f2_pack(dist_f, dist_f + 1.f);
-        // Of a tile whose queries begin before its keys end a warp may have nothing, and has to mask what is below the diagonal.
-        const bool none = diagonal && (part + 1) * PM_COLS <= quarter * 32, masked = diagonal && part * PM_COLS < quarter * 32 + 32;
+        // Of a tile whose queries begin before its keys end a warp may have nothing, and has to mask what is below the diagonal.  What is
+        // masked or left out is so by selection: its score may be anything, and a NaN or infinite one would outlast a term of -inf.
+        const bool none = !any || (diagonal && (part + 1) * PM_COLS <= quarter * 32);
+        const bool masked = holes || (diagonal && part * PM_COLS < quarter * 32 + 32);
 #pragma unroll
         for (int cc = 0; cc < PM_COLS / 32; ++cc) {  // 32 columns at a time
           uint32_t s[2][16];
@@ -420,8 +431,10 @@ __global__ void __launch_bounds__(PmCfg<HD>::THREADS, 1) prompt_mass_kernel(cons
                 float x0, x1;
                 f2_unpack(exponent(c, a), x0, x1);
                 const int d = dist + cc * 32 + c * 8 - 8 * a;
-                if (d < 0) x0 = -INFINITY;
-                if (d + 1 < 0) x1 = -INFINITY;
+                float t0, t1;
+                f2_unpack(term[c], t0, t1);
+                if (d < 0 || t0 == -INFINITY) x0 = -INFINITY;
+                if (d + 1 < 0 || t1 == -INFINITY) x1 = -INFINITY;
                 acc[a] = f2_add(acc[a], f2_pack(pm_ex2(x0), pm_ex2(x1)));
               }
           }
