@@ -60,7 +60,8 @@ std::vector<uintptr_t> take_written();
 inline cudaStream_t current_stream(const Tensor& t) {
   return c10::cuda::getCurrentCUDAStream(t.device().index()).stream();
 }
-// Scratch of the GEMM and of the paged attention, one per device and stream, cleared once (the kernels keep its counters zero).
+// Scratch of the GEMM, the paged attention and the prompt mass, one per device and stream, cleared once (the kernels keep its
+// counters zero); a call that is captured into a graph gets one that belongs to the graph.
 Tensor gemm_workspace(c10::Device device, cudaStream_t stream);
 void reset_workspaces();
 

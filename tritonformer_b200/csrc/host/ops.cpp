@@ -60,20 +60,58 @@ std::vector<uintptr_t> take_written() {
 // ------------------------------------------------------------------------------------------------ workspaces
 // Newest last; at most kMaxWorkspaces per process.  An entry that falls out goes back to the caching allocator, which
 // hands it out again only in the order of the stream it was allocated on, so kernels still in flight keep it.
+//
+// What is captured into a graph runs when nobody calls here, on a stream of the replay's choice.  So a graph has workspaces of its
+// own, one for each stream of its capture, in memory that the graph owns, and clears their counters itself.  Their tensors are held
+// only so that the rest of the capture does not get the memory: until their stream is met again outside it, or kMaxCaptured later.
 struct Workspace {
   c10::DeviceIndex device;
   cudaStream_t stream;
+  unsigned long long capture;  // id of the capture; 0 of those outside one
   Tensor buf;
 };
-constexpr size_t kMaxWorkspaces = 8;
+constexpr size_t kMaxWorkspaces = 8, kMaxCaptured = 64;
+constexpr size_t kCounterBytes = 8192;  // head of a workspace: zero between kernels
 static std::mutex g_ws_lock;
 static std::list<Workspace>& workspaces() {
   static auto* l = new std::list<Workspace>();  // never destroyed: the CUDA context may be gone by then
   return *l;
 }
+static std::list<Workspace>& captured_workspaces() {
+  static auto* l = new std::list<Workspace>();
+  return *l;
+}
+
+static unsigned long long capture_of(cudaStream_t stream) {
+  if (stream == nullptr || stream == cudaStreamLegacy) return 0;  // never part of a capture
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  TORCH_CHECK(cudaStreamGetCaptureInfo(stream, &status, &id) == cudaSuccess, "cudaStreamGetCaptureInfo failed");
+  return status == cudaStreamCaptureStatusActive ? id : 0;
+}
+
+static int64_t workspace_bytes() {
+  return std::max({tfb_gemm_workspace_bytes(), tfb_paged_attention_workspace_bytes(), tfb_prompt_mass_workspace_bytes()});
+}
+
+static Tensor captured_workspace(c10::Device device, cudaStream_t stream, unsigned long long capture) {  // lock held
+  auto& l = captured_workspaces();
+  for (auto& w : l)
+    if (w.stream == stream && w.device == device.index()) return w.buf;  // of this capture: others' have been dropped
+  c10::cuda::CUDAStreamGuard on(c10::cuda::getStreamFromExternal(stream, device.index()));
+  Tensor buf = at::empty({workspace_bytes()}, at::TensorOptions().device(device).dtype(at::kByte));
+  TORCH_CHECK(cudaMemsetAsync(buf.data_ptr(), 0, kCounterBytes, stream) == cudaSuccess, "cudaMemsetAsync failed");
+  l.push_back({device.index(), stream, capture, buf});
+  if (l.size() > kMaxCaptured) l.pop_front();
+  return buf;
+}
 
 Tensor gemm_workspace(c10::Device device, cudaStream_t stream) {
+  const unsigned long long capture = capture_of(stream);
   std::lock_guard<std::mutex> g(g_ws_lock);
+  captured_workspaces().remove_if(
+      [&](const Workspace& w) { return w.stream == stream && w.device == device.index() && w.capture != capture; });
+  if (capture) return captured_workspace(device, stream, capture);
   auto& l = workspaces();
   for (auto it = l.rbegin(); it != l.rend(); ++it) {
     if (it->stream != stream || it->device != device.index()) continue;
@@ -82,9 +120,8 @@ Tensor gemm_workspace(c10::Device device, cudaStream_t stream) {
   }
   // allocated and cleared in the order of the stream that uses it
   c10::cuda::CUDAStreamGuard on(c10::cuda::getStreamFromExternal(stream, device.index()));
-  const int64_t bytes = std::max({tfb_gemm_workspace_bytes(), tfb_paged_attention_workspace_bytes(), tfb_prompt_mass_workspace_bytes()});
-  Tensor buf = at::zeros({bytes}, at::TensorOptions().device(device).dtype(at::kByte));
-  l.push_back({device.index(), stream, buf});
+  Tensor buf = at::zeros({workspace_bytes()}, at::TensorOptions().device(device).dtype(at::kByte));
+  l.push_back({device.index(), stream, 0, buf});
   if (l.size() > kMaxWorkspaces) l.pop_front();
   return buf;
 }

@@ -133,7 +133,7 @@ def _collect_written():
 def _gemm_workspace(device, stream):
     """Scratch the GEMM uses to share the contraction of a tile between SMs: arrival counters (kept zero by
     the kernels, so cleared only once) and one fp32 partial tile per SM.  One per device and stream, since calls
-    that share it must be stream-ordered."""
+    that share it must be stream-ordered; in a capture one that belongs to the graph."""
     return _host.gemm_workspace(device.index if device.index is not None else torch.cuda.current_device(), stream)
 
 
