@@ -1,0 +1,44 @@
+"""Prompts as they come: lengths that do not fit, padding of any kind, models in other types."""
+import pytest
+import torch
+
+import tritonformer_b200._lib as L
+from test_generate import _model
+from tritonformer_b200.generate import Generator, _prompt_lengths
+
+gpu = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("bad", [[0, 5], [5, 9], [-1, 5], [5], [5, 5, 5], [1.0, 2.0], [True, True], [[5, 5]]])
+def test_lengths_that_the_host_refuses(bad):
+    for lengths in (bad, torch.tensor(bad)):
+        with pytest.raises(AssertionError, match="tokens"):
+            _prompt_lengths(lengths, 2, 8, "cpu")
+
+
+def test_lengths_that_the_host_takes():
+    for lengths in ([1, 8], (1, 8), torch.tensor([1, 8]), torch.tensor([1, 8], dtype=torch.int16)):
+        counts, bad = _prompt_lengths(lengths, 2, 8, "cpu")
+        assert counts.tolist() == [1, 8] and counts.dtype is torch.int32 and bad is None
+    assert _prompt_lengths(None, 2, 8, "cpu")[0].tolist() == [8, 8]
+
+
+@gpu
+@pytest.mark.parametrize("budget", [None, 20])
+def test_lengths_on_the_gpu_that_do_not_fit(budget):
+    """They are taken as the nearest that do, here where the model has no position behind the prompt's padding; it is reported."""
+    model = _model(layers=1, positions=64)
+    ids = torch.randint(0, 1000, (4, 50), device="cuda")
+    gen = Generator(model, 4, 64, budget=budget)
+    want = gen.prefill(ids, [1, 50, 50, 7])
+    assert L.device_status() == 0
+    got = gen.prefill(ids, torch.tensor([0, 64, 2 ** 40, 7], device="cuda"))
+    assert L.device_status(reset=True) == 0x7201
+    assert torch.equal(want, got)
+    assert gen.next.tolist() == [1, 50, 50, 7]
+    for value in (torch.tensor([1, 50, 50, 7], device="cuda"), torch.tensor([1, 50, 50, 7], device="cuda", dtype=torch.int16)):
+        assert torch.equal(want, gen.prefill(ids, value)) and L.device_status() == 0
+    for _ in range(14):
+        logits = gen.step(ids[:, 0])
+    assert logits.isfinite().all() and gen.next.tolist() == [15, 64, 64, 21]
+    L.check_status()

@@ -14,7 +14,22 @@ import torch
 from .attention import _resolve_bias
 from .embedding import Embedding
 from .fused import LinearResidual, MLPResidual, QKVProjection
-from .kvcache import PagedKVCache, cache_evict, prompt_attention, prompt_mass
+from .kvcache import PagedKVCache, cache_append, cache_evict, prompt_attention, prompt_mass
+
+
+def _prompt_lengths(lengths, batch, tokens, device):
+    """(lengths as int32 on the device, each from 1 to `tokens`; which of them were not, or None where the host has looked)."""
+    if lengths is None:
+        return torch.full((batch,), tokens, dtype=torch.int32, device=device), None
+    lengths = torch.as_tensor(lengths)
+    assert lengths.shape == (batch,) and not lengths.is_floating_point() and lengths.dtype != torch.bool, \
+        "lengths are a number of tokens for each prompt"
+    if lengths.is_cuda:
+        counts = lengths.to(device).clamp(1, tokens)
+        return counts.to(torch.int32), counts != lengths.to(device)
+    assert batch == 0 or (int(lengths.min()) >= 1 and int(lengths.max()) <= tokens), \
+        f"a prompt has from 1 to {tokens} tokens, the columns that there are"
+    return lengths.to(device=device, dtype=torch.int32), None
 
 
 class Generator:
@@ -63,12 +78,12 @@ class Generator:
     @torch.autocast("cuda", enabled=False)
     def prefill(self, prompts, lengths=None):
         """Starts the sequences: prompts (batch, T) int64, the first lengths[b] of each (all by default).  Returns the logits
-        (batch, vocab) of the tokens that follow."""
+        (batch, vocab) of the tokens that follow.  Lengths are from 1 to T; those that are on the GPU are not waited for, but
+        taken as the nearest ones that are, and `_lib.check_status()` says so."""
         b, t = prompts.shape
         assert b == self.batch and 1 <= t <= self.max_tokens, "prompts are (batch, up to max_tokens) token ids"
         device = self.tables.device
-        lengths = torch.full((b,), t, device=device) if lengths is None else torch.as_tensor(lengths, device=device)
-        counts = lengths.to(torch.int32)
+        counts, bad = _prompt_lengths(lengths, b, t, device)
         padded = -(-t // 64) * 64  # the training attention takes whole tiles of 64
         positions = self.model.embed_positions.weight if self.model.embed_positions is not None else None
         assert padded <= self.model.config.max_position_embeddings, "the prompt, in whole tiles of 64, exceeds the model's positions"
@@ -107,7 +122,11 @@ class Generator:
         self.next.copy_(counts)
         self.longest = t if self.budget is None else min(t, self.budget)
         self.position = t
-        return self._logits(last)
+        logits = self._logits(last)
+        if bad is not None:  # once the work is done, because the matrix products stop while there is a report
+            none = torch.zeros((b, self.heads, 1, self.head_dim), dtype=x.dtype, device=device)
+            cache_append(self.caches[0].k, self.caches[0].v, self.tables, start, none, none, torch.where(bad, -1, 0).to(torch.int32))
+        return logits
 
     def _logits(self, x):
         return self.model.logits_out(self.model.final_layernorm(x.unsqueeze(1))).squeeze(1)
