@@ -3,8 +3,9 @@ import pytest
 import torch
 
 import tritonformer_b200._lib as L
-from test_generate import _model
+from test_generate import _model, _teacher
 from tritonformer_b200.generate import Generator, _prompt_lengths
+from util import norm_rel
 
 gpu = pytest.mark.gpu
 
@@ -42,3 +43,19 @@ def test_lengths_on_the_gpu_that_do_not_fit(budget):
         logits = gen.step(ids[:, 0])
     assert logits.isfinite().all() and gen.next.tolist() == [15, 64, 64, 21]
     L.check_status()
+
+
+@gpu
+@pytest.mark.parametrize("pad", [-1, -100, 1 << 40])
+def test_padding_may_be_any_number(pad):
+    model = _model(layers=1)
+    ids = torch.randint(0, 1000, (3, 70), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    lengths = [70, 33, 1]
+    for at in (lengths, torch.tensor(lengths, device="cuda")):
+        gen = Generator(model, 3, 128, budget=24)
+        want = gen.prefill(ids, lengths)
+        padded = ids.clone()
+        for b, n in enumerate(lengths):
+            padded[b, n:] = pad
+        assert torch.equal(want, gen.prefill(padded, at)) and L.device_status() == 0
+        assert torch.equal(want, gen.prefill(padded.cpu(), at)) and L.device_status() == 0

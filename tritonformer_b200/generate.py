@@ -77,8 +77,8 @@ class Generator:
     @torch.no_grad()
     @torch.autocast("cuda", enabled=False)
     def prefill(self, prompts, lengths=None):
-        """Starts the sequences: prompts (batch, T) int64, the first lengths[b] of each (all by default).  Returns the logits
-        (batch, vocab) of the tokens that follow.  Lengths are from 1 to T; those that are on the GPU are not waited for, but
+        """Starts the sequences: prompts (batch, T) int64, the first lengths[b] of each (all by default); what follows those may be
+        any number.  Returns the logits (batch, vocab) of the tokens that follow.  Lengths are from 1 to T; those that are on the GPU are not waited for, but
         taken as the nearest ones that are, and `_lib.check_status()` says so."""
         b, t = prompts.shape
         assert b == self.batch and 1 <= t <= self.max_tokens, "prompts are (batch, up to max_tokens) token ids"
@@ -88,7 +88,8 @@ class Generator:
         positions = self.model.embed_positions.weight if self.model.embed_positions is not None else None
         assert padded <= self.model.config.max_position_embeddings, "the prompt, in whole tiles of 64, exceeds the model's positions"
         ids = torch.zeros((b, padded), dtype=torch.int64, device=device)
-        ids[:, :t] = prompts
+        behind = torch.arange(t, device=device) >= counts[:, None]
+        ids[:, :t] = prompts.to(device).masked_fill(behind, 0)  # padding may be no token at all
         x = Embedding.apply(ids, self.model.embed_tokens.weight, positions)
         start = torch.zeros_like(counts)
         # a prompt that is longer than what its sequence has pages for passes through pages of its own
