@@ -59,3 +59,31 @@ def test_padding_may_be_any_number(pad):
             padded[b, n:] = pad
         assert torch.equal(want, gen.prefill(padded, at)) and L.device_status() == 0
         assert torch.equal(want, gen.prefill(padded.cpu(), at)) and L.device_status() == 0
+
+
+@gpu
+@pytest.mark.parametrize("heads", [4, 12])
+@pytest.mark.parametrize("budget", [None, 128])
+def test_alibi_models_moved_to_bf16(heads, budget):
+    """Their table was made in fp16 and rounded again; the logits are the model's own."""
+    model = _model(heads=heads, alibi=True).to(torch.bfloat16).fuse_projection_weights()
+    assert model.attn_bias.dtype is torch.bfloat16
+    ids = torch.randint(0, 1000, (2, 128), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    with torch.no_grad():
+        want = model(ids, None)[:, 99:]
+    got = _teacher(model, ids, 100, Generator(model, 2, 128, budget=budget))
+    assert norm_rel(got, want) < 2e-2  # as in test_generate.py
+    graph = _teacher(model, ids, 100, Generator(model, 2, 128, budget=budget, graph=True))
+    assert torch.equal(got, graph)
+    L.check_status()
+
+
+@gpu
+def test_a_bias_that_is_not_alibi_is_refused():
+    model = _model(heads=12, alibi=True)
+    model.attn_bias = model.attn_bias * 1.05
+    ids = torch.randint(0, 1000, (1, 10), device="cuda")
+    gen = Generator(model, 1, 64)
+    with pytest.raises(AssertionError, match="no other bias"):
+        gen.prefill(ids)
+        gen.step(ids[:, 0])

@@ -60,6 +60,8 @@ class _Bias:
 def _resolve_bias(attn_bias, heads, seq, dtype):
     if attn_bias is None:
         return _Bias()
+    if isinstance(attn_bias, _Bias):
+        return attn_bias
     if attn_bias.dim() == 1:
         assert attn_bias.shape[0] == heads, \
             f"Expected attention bias to have leading dimension equal to number of heads ({heads})"

@@ -11,10 +11,11 @@ head of every layer keeps the `recent` last keys and those that have got most at
 """
 import torch
 
-from .attention import _resolve_bias
+from .attention import _Bias, _resolve_bias
 from .embedding import Embedding
 from .fused import LinearResidual, MLPResidual, QKVProjection
 from .kvcache import PagedKVCache, cache_append, cache_evict, prompt_attention, prompt_mass
+from .transformer import get_slopes
 
 
 def _prompt_lengths(lengths, batch, tokens, device):
@@ -30,6 +31,22 @@ def _prompt_lengths(lengths, batch, tokens, device):
     assert batch == 0 or (int(lengths.min()) >= 1 and int(lengths.max()) <= tokens), \
         f"a prompt has from 1 to {tokens} tokens, the columns that there are"
     return lengths.to(device=device, dtype=torch.int32), None
+
+
+def _bias_of(table, heads):
+    bias = _resolve_bias(table, heads, 0, table.dtype)
+    if bias.table is None or table.dtype is not torch.bfloat16:
+        return bias
+    # A model that was moved to bf16 has an ALiBi table that was rounded twice (to fp16 as it was made: slopes, distances and
+    # products), and so is no table of bf16 slopes.  The slopes themselves are what it stands for.
+    slopes = torch.tensor(get_slopes(heads), dtype=torch.float16).float().to(table.device)
+    at = torch.arange(table.shape[1], device=table.device)
+    back = (at[:, None] - at).clamp(min=0).float()
+    for h in range(heads):
+        want = back * slopes[h]
+        if not bool(((table[h].float() + want).abs() <= (2.0 ** -8 + 2.0 ** -9) * want)[back > 0].all()):
+            return bias
+    return _Bias(slopes=slopes)
 
 
 class Generator:
@@ -60,9 +77,16 @@ class Generator:
         self.logits = torch.zeros((batch, config.vocab_size), dtype=weight.dtype, device=device)
         self.longest = self.position = 0  # upper bounds of `lengths` and `next` that the host knows
         self.want_graph, self.graph = graph, None
+        self.bias = None  # the model's table, its version, and what _bias_of found
 
     def _bias(self):
-        return self.model.attn_bias
+        """The model's bias in the operators' form; a table that is new here is looked over, which waits for the host."""
+        table = self.model.attn_bias
+        if table is None:
+            return None
+        if self.bias is None or self.bias[0] is not table or self.bias[1] != table._version:
+            self.bias = table, table._version, _bias_of(table, self.heads)
+        return self.bias[2]
 
     def _block(self, layer, x, attend):
         """One layer on (batch, tokens, hidden) without gradients; `attend` maps q, k, v to the context."""
@@ -178,8 +202,7 @@ class Generator:
         # a step ahead of the capture makes the workspaces; the sequences then go back to where they were
         before = self.lengths.clone(), self.next.clone()
         masses = [c.mass.clone() if c.mass is not None else None for c in self.caches]
-        if self._bias() is not None:
-            _resolve_bias(self._bias(), self.heads, 0, self.logits.dtype)  # looks the table over, which waits for the host
+        self._bias()  # may wait for the host
 
         def back():
             self.lengths.copy_(before[0])

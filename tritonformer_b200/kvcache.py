@@ -20,15 +20,11 @@ and writes nothing out of bounds and shows in `_lib.check_status()`.
 import torch
 
 from . import _host
-from .attention import _Bias, _resolve_bias, attention_forward
-
-_NO_BIAS = _Bias()
+from .attention import _resolve_bias, attention_forward
 
 
 def _slopes(attn_bias, heads):
-    if attn_bias is None:
-        return _NO_BIAS
-    bias = _resolve_bias(attn_bias, heads, 0, attn_bias.dtype)
+    bias = _resolve_bias(attn_bias, heads, 0, getattr(attn_bias, "dtype", None))
     assert bias.table is None, "the cache takes ALiBi slopes or an ALiBi table, no other bias"
     return bias
 
@@ -40,7 +36,7 @@ def paged_attention(query, k_pages, v_pages, tables, lengths, key=None, value=No
     stays).  A sequence without keys gets zeros.  With `mass` every key's weights, summed over the query heads of its head, are
     added to it, in place or into `mass_out` (no page may then be part of two sequences); with `positions` the new key's entry is set.  The query's position is
     query_positions[b], or the number of the last slot."""
-    bias = _NO_BIAS if attn_bias is None else _slopes(attn_bias, query.shape[1])
+    bias = _slopes(attn_bias, query.shape[1])
     return _host.paged_attention(query, k_pages, v_pages, tables, lengths, key, value, bias.slopes, int(bias.rounded),
                                  query_positions, mass, positions, mass_out)
 
@@ -55,7 +51,7 @@ def prompt_mass(query, key, lse, counts=None, attn_bias=None):
     """(batch, cache heads, T) fp32: what each key of a prompt gets of the causal attention of its first counts[b] tokens, summed
     over the queries and over the query heads of its head.  query (batch, heads, T, head_dim), key (batch, cache heads, T,
     head_dim), lse (batch, heads, T) of the scaled and biased scores; any T."""
-    bias = _NO_BIAS if attn_bias is None else _slopes(attn_bias, query.shape[1])
+    bias = _slopes(attn_bias, query.shape[1])
     return _host.prompt_mass(query, key, lse, counts, bias.slopes, int(bias.rounded))
 
 
