@@ -87,3 +87,17 @@ def test_a_bias_that_is_not_alibi_is_refused():
     with pytest.raises(AssertionError, match="no other bias"):
         gen.prefill(ids)
         gen.step(ids[:, 0])
+
+
+@gpu
+@pytest.mark.parametrize("alibi", [False, True])
+def test_prompts_up_to_the_last_position(alibi):
+    """Whole tiles of 64 may be more than the model's positions: 100 of them here."""
+    model = _model(layers=2, alibi=alibi, positions=100)
+    ids = torch.randint(0, 1000, (2, 100), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    steps = _teacher(model, ids, 60, Generator(model, 2, 100))
+    for t in (65, 99, 100):
+        for budget in (None, 100):
+            got = Generator(model, 2, 100, budget=budget).prefill(ids[:, :t])
+            assert norm_rel(got, steps[:, t - 60]) < 2e-2  # as in test_generate.py
+    L.check_status()

@@ -110,11 +110,13 @@ class Generator:
         counts, bad = _prompt_lengths(lengths, b, t, device)
         padded = -(-t // 64) * 64  # the training attention takes whole tiles of 64
         positions = self.model.embed_positions.weight if self.model.embed_positions is not None else None
-        assert padded <= self.model.config.max_position_embeddings, "the prompt, in whole tiles of 64, exceeds the model's positions"
         ids = torch.zeros((b, padded), dtype=torch.int64, device=device)
         behind = torch.arange(t, device=device) >= counts[:, None]
         ids[:, :t] = prompts.to(device).masked_fill(behind, 0)  # padding may be no token at all
-        x = Embedding.apply(ids, self.model.embed_tokens.weight, positions)
+        known = min(padded, self.model.config.max_position_embeddings)
+        x = Embedding.apply(ids[:, :known], self.model.embed_tokens.weight, positions)
+        if known < padded:  # rows behind the model's last position, which no other row sees
+            x = torch.nn.functional.pad(x, (0, 0, 0, padded - known))
         start = torch.zeros_like(counts)
         # a prompt that is longer than what its sequence has pages for passes through pages of its own
         room = self.width * self.page
