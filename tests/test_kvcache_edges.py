@@ -97,3 +97,77 @@ def test_mass_does_not_see_what_lies_behind_a_prompt(T, counts, hd, alibi):
         bad[:, :, 40:60] = value
         assert torch.equal(want, kvcache.prompt_mass(bad, k, lse, n, attn_bias=slopes))
     assert want.isfinite().all() and L.device_status() == 0
+
+
+# --------------------------------------------------------------------------------------------------- append and evict
+
+
+def _pool(c):
+    return [x.clone() for x in (c.k, c.v, c.mass, c.positions)]
+
+
+def _equal(a, b):
+    return all(torch.equal(x.nan_to_num(7), y.nan_to_num(7)) for x, y in zip(a, b))
+
+
+@gpu
+@pytest.mark.parametrize("hd,off", [(32, 0), (64, 1), (128, 0)])
+def test_append_of_more_keys_than_there_is_room_for(hd, off):
+    """Those that fit are written, nothing else is, and it is reported; the other sequence gets all of its own."""
+    c = Cache([46, 10], 2, hd, 16, torch.float16, room=2)
+    c.tables = torch.arange(6, dtype=torch.int32, device="cuda").view(2, 3).flip(0).contiguous()  # two full tables of 48 slots
+    flat = torch.randn((2 * 2 * 9 * hd + 8,), device="cuda", generator=_gen(1)).half()
+    keys = flat[off:off + 2 * 2 * 9 * hd].view(2, 2, 9, hd)
+    want = c.copy()
+    for b, n in ((0, 2), (1, 9)):
+        p, r = c.at(b, c.lengths[b] + torch.arange(n, device="cuda"))
+        want.k[p, :, r], want.v[p, :, r] = keys[b, :, :n].transpose(0, 1), -keys[b, :, :n].transpose(0, 1)
+        want.mass[p, :, r] = 0.0
+        want.positions[p, :, r] = (c.lengths[b] + torch.arange(n, device="cuda", dtype=torch.int32))[:, None]
+    kvcache.cache_append(c.k, c.v, c.tables, c.len, keys, -keys, mass=c.mass, positions=c.positions)
+    assert L.device_status(reset=True) == 0x7201
+    assert _equal(_pool(c), _pool(want))
+    for counts, lengths in (([0, 0], [-3, 10]), ([-1, 0], [46, 10]), ([0, 0], [49, 10])):
+        kvcache.cache_append(c.k, c.v, c.tables, torch.tensor(lengths, dtype=torch.int32, device="cuda"), keys, -keys,
+                             torch.tensor(counts, dtype=torch.int32, device="cuda"), c.mass, c.positions)
+        assert L.device_status(reset=True) == 0x7201
+        assert _equal(_pool(c), _pool(want))
+    tables = c.tables.clone()
+    tables[0, 2] = c.pages
+    kvcache.cache_append(c.k, c.v, tables, c.len, keys[:, :, :2], keys[:, :, :2], torch.tensor([2, 0], dtype=torch.int32, device="cuda"),
+                         c.mass, c.positions)
+    assert L.device_status(reset=True) == 0x7200
+    assert _equal(_pool(c), _pool(want))
+
+
+@gpu
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("lengths,keep", [([100, 100], 50), ([9000, 9000], 3000)])  # one block a head, and clusters
+def test_evict_leaves_the_others_alone(lengths, keep, in_place):
+    """A bad page or length of one sequence is reported; the other one is cut as ever, and no row of anybody else changes."""
+    def evict(c, tables, n):
+        out = None if in_place else tuple(torch.zeros_like(x) for x in (c.k, c.v, c.mass, c.positions))
+        left = kvcache.cache_evict(c.k, c.v, c.mass, c.positions, tables, n, keep, 0, out=out, out_tables=None if in_place else c.tables)
+        return left, _pool(c) if in_place else [x.clone() for x in out]
+
+    good = Cache(lengths, 2, 64, 16, torch.float16)
+    clean = _pool(good)
+    own = torch.zeros(good.pages, dtype=torch.bool, device="cuda")
+    own[good.tables[0].long()] = True  # pages of the sequence with the fault
+    left, want = evict(good, good.tables, good.len)
+    assert L.device_status() == 0 and left.tolist() == [keep, keep]
+    for bad in (-1, good.pages, 2 ** 31 - 1):
+        c = Cache(lengths, 2, 64, 16, torch.float16)
+        tables = c.tables.clone()
+        tables[0, 2] = bad
+        left, got = evict(c, tables, c.len)
+        assert L.device_status(reset=True) == 0x7200 and left.tolist() == [keep, keep]
+        assert _equal([x[~own] for x in got], [x[~own] for x in want])
+    c = Cache(lengths, 2, 64, 16, torch.float16)
+    n = c.len.clone()
+    n[0] = -1
+    left, got = evict(c, c.tables, n)
+    assert L.device_status(reset=True) == 0x7201 and left.tolist() == [0, keep]
+    assert _equal([x[~own] for x in got], [x[~own] for x in want])
+    untouched = clean if in_place else [torch.zeros_like(x) for x in clean]
+    assert _equal([x[own] for x in got], [x[own] for x in untouched])
