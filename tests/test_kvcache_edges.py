@@ -1,5 +1,6 @@
 """The paged key-value cache where values, lengths and layouts are at their limits.  Bounds as in test_kvcache.py, unless a test
 says otherwise."""
+import ctypes
 import math
 
 import pytest
@@ -171,3 +172,23 @@ def test_evict_leaves_the_others_alone(lengths, keep, in_place):
     assert _equal([x[~own] for x in got], [x[~own] for x in want])
     untouched = clean if in_place else [torch.zeros_like(x) for x in clean]
     assert _equal([x[own] for x in got], [x[own] for x in untouched])
+
+
+def test_evict_in_place_is_slot_by_slot():
+    """The input's own buffers under another shape are no output: their slots are not the input's."""
+    def strides(*s):
+        return (ctypes.c_int64 * len(s))(*s)
+
+    one, two, three = ctypes.c_void_p(256), ctypes.c_void_p(512), strides(1024, 1024, 64)
+
+    def evict(page=16, pages=4, width=2, out=three, k_out=one, mass_out=one):
+        return L.lib.tfb_cache_evict(one, one, one, None, one, one, None, k_out, k_out, mass_out, None, one, two, 1, 1, 64, 4, 0, 16, 4,
+                                     2, 2, three, page, pages, width, 2, out, one, 8, 0, None)
+
+    assert evict() == -1 and b"scratch" in L.lib.tfb_last_error()  # looked at last: nothing is launched here
+    for bad in (dict(page=32, pages=2), dict(out=strides(2048, 1024, 64)), dict(out=strides(1024, 1024, 128)), dict(page=8, mass_out=two),
+                dict(page=8, k_out=two)):
+        assert evict(**bad) == -1 and b"other shape" in L.lib.tfb_last_error(), bad
+    for good in (dict(page=8, k_out=two, mass_out=two), dict(out=strides(2048, 1024, 64), k_out=two), dict(out=strides(1024, 7 * 8, 64)),
+                 dict(pages=3)):  # buffers of their own, a stride that says nothing, fewer of the pages
+        assert evict(**good) == -1 and b"scratch" in L.lib.tfb_last_error(), good

@@ -621,6 +621,12 @@ extern "C" int tfb_cache_evict(const void* k_pages, const void* v_pages, const f
   TFB_REQUIRE(left && left != lengths, "cache_evict: the new lengths need an array of their own");
   TFB_REQUIRE((positions == nullptr) == (positions_out == nullptr), "cache_evict: positions come with positions for the output");
   TFB_REQUIRE((k_out == k_pages) == (v_out == v_pages), "cache_evict: keys in place and values not, or the other way round");
+  const bool stats_shared = mass_out == mass || (positions && positions_out == positions);
+  TFB_REQUIRE(out_page == page || (k_out != k_pages && !stats_shared), "cache_evict: the input's own buffers in other shape are no output");
+  const int64_t extents[3] = {num_pages < out_num_pages ? num_pages : out_num_pages, kv_heads, page};
+  for (int i = 0; i < 3; ++i)
+    TFB_REQUIRE(k_out != k_pages || extents[i] == 1 || out_page_strides[i] == page_strides[i],
+                "cache_evict: the input's own pages in other shape are no output");
   if (B == 0) return TFB_OK;
   TFB_REQUIRE(aligned16(k_pages) && aligned16(v_pages) && aligned16(k_out) && aligned16(v_out),
               "cache_evict: the pages are not 16-byte aligned");
