@@ -43,7 +43,8 @@ const char* tfb_last_error(void);
 int64_t tfb_launch_count(void);
 /* Device-side status word of the library on the calling thread's CURRENT device (one word per GPU,
  * shared by every kernel of the library): 0, or the code of the first bounded wait that expired
- * (0x2xxx attention backward, 0x5xxx attention forward, 0x8xxx prompt mass, 0x9xxx paged attention, 0x1xxx / 0x3xxx GEMM, 0x7e00 the test probe)
+ * (0x2xxx attention backward, 0x5xxx attention forward, 0x8xxx prompt mass, 0x9xxx paged attention,
+ * 0x1xxx / 0x3xxx GEMM, 0x7e00 the test probe)
  * or 0x7100 for a token id outside the embedding table, 0x7200 / 0x7201 for a page id / a length that
  * does not fit a paged cache (below).  While it is non-zero the tcgen05 kernels
  * (GEMM, attention) return at once without writing their outputs; the other kernels still run.
@@ -323,7 +324,8 @@ int tfb_loss_scale_update(float* state4, int* found_inf, float growth, float bac
  * No keys: zeros.  slopes and alibi_round as in tfb_attention_fwd, with distance query_positions[b] - position of the key
  * (query_positions NULL: the number of the last slot); a new key's position is the query's.  With mass and mass_out (the same
  * buffer, or another one of its shape) mass_out = mass + the key's weights, summed over the query heads of its key head, in the
- * slots in use; a new key starts from zero; no page may then be part of two sequences.  group <= 128.  Strides {b, h} in elements, unit stride on hd, any alignment.
+ * slots in use; a new key starts from zero; no page may then be part of two sequences.  group <= 128.  Strides {b, h} in
+ * elements, unit stride on hd, any alignment.
  * workspace: at least tfb_paged_attention_workspace_bytes(), 16-byte aligned, its first 8192 bytes ZERO on entry and zero again
  * when the kernel has finished (the GEMM's workspace, where that is large enough, serves both); calls that share one must be
  * stream-ordered.  scratch is for masses only and needs no initialisation; capacity = width * page.            */
@@ -352,7 +354,8 @@ int tfb_cache_append(const void* key, const void* value, void* k_pages, void* v_
  * the queries i with j <= i < counts[b] (NULL: T) of exp(s_hij - lse[b,h,i]), s the scaled and biased scores of
  * tfb_attention_fwd and lse (strides {b, h}, unit stride on T) its log-sum-exp; zero for keys from counts[b] on.  q (B, kv_heads *
  * group, T, hd) and k (B, kv_heads, T, hd) with strides {b, h, t}, positive multiples of 8, and 16-byte aligned bases.
- * Any T from 1 to 2^23.  workspace as in tfb_paged_attention, of at least tfb_prompt_mass_workspace_bytes().       */
+ * Any T from 1 to 2^23.  What q, k and lse hold from counts[b] on may be anything, and a row whose lse is -infinity gives
+ * nothing.  workspace as in tfb_paged_attention, of at least tfb_prompt_mass_workspace_bytes().                  */
 int64_t tfb_prompt_mass_workspace_bytes(void);
 int tfb_prompt_mass(const void* q, const void* k, const float* lse, const int* counts, const float* slopes,
                     int alibi_round, float* out, int64_t B, int64_t kv_heads, int64_t group, int64_t T, int64_t hd,
@@ -363,8 +366,9 @@ int tfb_prompt_mass(const void* q, const void* k, const float* lse, const int* c
  * is at least next_positions[b] - recent (NULL: lengths[b] - recent) counts as one of infinite mass and a mass that is no number as
  * one of -infinity; ties go to the lower slot.  Keys that stay and lie before slot `keep` stay in their slots; those from behind fill
  * the slots that become free, in the order of their slots.  left[b] = min(lengths[b], keep) is the new length (in an array of
- * its own: lengths is still read).  The outputs, each with its statistics, are either the inputs (and out_tables = tables: in place; no page may then be
- * part of two sequences) or other buffers of the same kv_heads and hd, which get every slot that is left.  keep >= recent. */
+ * its own: lengths is still read).  The outputs, each with its statistics, are either the inputs (in the same shape, and out_tables =
+ * tables: in place; no page may then be part of two sequences) or other buffers of the same kv_heads and hd, which get every
+ * slot that is left.  keep >= recent. */
 int64_t tfb_cache_evict_scratch_bytes(int64_t B, int64_t kv_heads, int64_t keep);
 int tfb_cache_evict(const void* k_pages, const void* v_pages, const float* mass, const int* positions,
                     const int* tables, const int* lengths, const int* next_positions, void* k_out, void* v_out,

@@ -8,6 +8,15 @@ namespace tfb {
 extern __device__ int g_dev_status;   // the library's status word (status.cu)
 constexpr int kBadPage = 0x7200;      // a page id outside the cache
 constexpr int kBadLength = 0x7201;    // a length that is negative or more than the sequence's table has room for
+constexpr int64_t kCounterBytes = 8192;  // head of a workspace: arrival counters, zero between kernels
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+inline int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 
 struct PageMap {
   const int* tables;  // (B, width) page ids, row pitch table_ld

@@ -35,7 +35,6 @@ namespace tfb {
 namespace {
 
 constexpr int PG_WARPS = 8;
-constexpr float kLog2e = 1.4426950408889634f;
 // Probabilities are kept relative to a reference that the running maximum may pass by 2^15 before everything is rescaled
 // (they then still fit fp16); a new reference is 2^4 below the maximum, so that small ones stay clear of fp16's subnormals.
 constexpr float kAhead = 15.f, kBelow = 4.f;
@@ -93,11 +92,6 @@ struct PgParams {
   int scores_stay;  // they fit the L2
 };
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {  // the rest of the 16 is zeros
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -1067,15 +1061,9 @@ __global__ void __launch_bounds__(MASS_THREADS) paged_mass_kernel(const PgParams
   }
 }
 
-int encode_tmap_sw128(CUtensorMap* out, const void* base, int dtype, int rank, const uint64_t* dims,
-                      const uint64_t* strides_bytes, const uint32_t* box);
-
 namespace {
 
-int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
-
 // Workspace: counters, then the pieces of blocks and warps for the widest rows.  Scratch, for the masses: log-sum-exps, scores.
-constexpr int64_t kCounterBytes = 8192;
 struct PgWorkspace {
   int64_t ml, acc, heads_acc, bytes;
 };

@@ -41,9 +41,10 @@ constexpr int AP_ROWS = 64;  // rows of a block
 
 // One block: AP_ROWS rows of a (sequence, key head); neighbouring blocks take neighbouring heads, which lie side by side in a
 // projection's output.  VEC: 16-byte chunks; otherwise element by element.
-template <typename E, int HD, bool VEC>
+template <int HD, bool VEC>
 __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
-  constexpr int W = VEC ? 8 : 1, LANES = HD / 8, PER = 256 / LANES, N = AP_ROWS / PER;
+  using E = uint16_t;  // a copy: of the type only the size matters
+  constexpr int LANES = HD / 8, PER = 256 / LANES, N = AP_ROWS / PER;
   __shared__ int sh_page[AP_ROWS], sh_row[AP_ROWS];
   grid_dependency_wait();
   allow_dependents();
@@ -97,7 +98,7 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
       if (sh_page[r] < 0) continue;
       const int64_t o = row_offset(p.map, sh_page[r], h, sh_row[r]) + c;
 #pragma unroll
-      for (int e = 0; e < 8; e += W) {
+      for (int e = 0; e < 8; ++e) {
         static_cast<E*>(p.k)[o + e] = key[(t0 + r) * p.k_t + c + e];
         static_cast<E*>(p.v)[o + e] = value[(t0 + r) * p.v_t + c + e];
       }
@@ -505,8 +506,6 @@ __global__ void __launch_bounds__(256, 4) evict_move_kernel(const EvictParams p)
   move_rows<HD, 256>(p, item, b, item % p.kv_heads, p.moves[item], p.left[b], blockIdx.y, gridDim.y);
 }
 
-int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
-
 constexpr int EV_SMEM = 200 * 1024;  // worths, beside the kernel's own arrays
 
 template <int MOVE>
@@ -531,10 +530,10 @@ int evict_select(const EvictParams& p, int64_t smem, cudaStream_t st) {
   return launched("cache_evict");
 }
 
-template <typename E, int HD, bool VEC>
+template <int HD, bool VEC>
 int append_launch(const AppendParams& p, cudaStream_t st) {
   const dim3 grid((unsigned)(p.B * p.kv_heads), (unsigned)ceil_div(p.T, AP_ROWS));
-  launch_overlapped(append_kernel<E, HD, VEC>, grid, dim3(256), 0, st, p);
+  launch_overlapped(append_kernel<HD, VEC>, grid, dim3(256), 0, st, p);
   return launched("cache_append");
 }
 
@@ -584,10 +583,9 @@ extern "C" int tfb_cache_append(const void* key, const void* value, void* k_page
   cudaStream_t st = (cudaStream_t)stream;
   bool vec = aligned16(key) && aligned16(value);
   for (int i = 0; i < 3; ++i) vec = vec && key_strides[i] % 8 == 0 && value_strides[i] % 8 == 0;
-  // a copy: the type does not matter beyond its size
-  if (hd == 32) return vec ? append_launch<uint16_t, 32, true>(p, st) : append_launch<uint16_t, 32, false>(p, st);
-  if (hd == 64) return vec ? append_launch<uint16_t, 64, true>(p, st) : append_launch<uint16_t, 64, false>(p, st);
-  return vec ? append_launch<uint16_t, 128, true>(p, st) : append_launch<uint16_t, 128, false>(p, st);
+  if (hd == 32) return vec ? append_launch<32, true>(p, st) : append_launch<32, false>(p, st);
+  if (hd == 64) return vec ? append_launch<64, true>(p, st) : append_launch<64, false>(p, st);
+  return vec ? append_launch<128, true>(p, st) : append_launch<128, false>(p, st);
 }
 
 extern "C" int64_t tfb_cache_evict_scratch_bytes(int64_t B, int64_t kv_heads, int64_t keep) {
@@ -664,7 +662,8 @@ extern "C" int tfb_cache_evict(const void* k_pages, const void* v_pages, const f
   cudaStream_t st = (cudaStream_t)stream;
   // as many blocks for a (sequence, key head) as the SMs have room for, none with fewer than 2048 slots of a full table
   p.cluster = 1;
-  while (p.cluster < 8 && B * kv_heads * p.cluster * 2 <= sm_count() * 2 && p.map.capacity() >= (int64_t)p.cluster * 2 * 2048) p.cluster *= 2;
+  while (p.cluster < 8 && B * kv_heads * p.cluster * 2 <= sm_count() * 2 && p.map.capacity() >= (int64_t)p.cluster * 2 * 2048)
+    p.cluster *= 2;
   int64_t smem = (ceil_div(ceil_div(p.map.capacity(), 32), p.cluster) * 32 * 4 + 15) / 16 * 16;
   if (smem > EV_SMEM) smem = EV_SMEM;
   p.room = (int)(smem / 4);

@@ -15,11 +15,13 @@
 // takes an equal stretch of it: the causal triangle and prompts of different lengths leave no CTA with more than one tile
 // over another.  Key tiles that several CTAs share leave their sums in a workspace; the last of the CTAs adds them, in order.
 //
-// Bound: the exponentials, one per score, 16 a clock and SM: 2048 clocks for a tile of 128 x 256, against 512 of the product at
+// Floor: the exponentials, one per score, 16 a clock and SM: 2048 clocks for a tile of 128 x 256, against 512 of the product at
 // head_dim 64.  One pair in four goes to the FMA pipe (a polynomial of degree 5 for 2^f, |f| <= 1/2, relative error 2.1e-7 in 32
-// bits, the SFU's own being 2.4e-7).  A tile of 128 x 128, with a warp for the terms, was bound by the
-// issuing warps' 1.2 k clocks a tile instead.  Measured: 4 prompts of 2048 tokens, 16 heads of 64, exact slopes 62 us (89 with
-// 128 x 128); one of 8192, 12 query heads of 128 on 4 key heads 152 us (264).
+// bits, the SFU's own being 2.4e-7), which leaves the SFU 1536.  A tile takes about twice that: 42 to 58% of the SFU's and 62 to
+// 67% of the issue slots are in use, so nothing is full, and what is waited for (the scores' way out of tensor memory, which a warp
+// has nothing to do beside, is the likely cause) has not been measured.  A tile of 128 x 128, with a warp for the terms, took
+// longer: the issuing warps' 1.2 k clocks a tile.  Measured: 4 prompts of 2048 tokens, 16 heads of 64, exact slopes 62 us (89 with
+// 128 x 128); one of 8192, 12 query heads of 128 on 4 key heads 153 us (264).
 #include "attn.cuh"
 #include "paged.cuh"
 #include "tc05.cuh"
@@ -36,7 +38,6 @@ constexpr int PM_COLS = PM_QUERIES / PM_PARTS;
 // A warp is at most two tiles ahead of another, which may still read the sums of the key tile that ended before those: each of
 // the last PM_TURNS key tiles has a place and a barrier of its own.
 constexpr int PM_TURNS = 4;
-constexpr float kLog2e = 1.4426950408889634f;
 
 template <int HD> struct PmCfg {
   static constexpr int PANELS = HD / 64;
@@ -113,11 +114,6 @@ struct PmCursor {
   }
 };
 
-__device__ __forceinline__ float pm_ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ float at_least(float x, float low) {  // NaN stays
   float y;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(low));
@@ -138,7 +134,8 @@ __device__ __forceinline__ uint64_t pm_ex2_fma(uint64_t xp) {
   q = f2_fma(q, f, both(1.0000001192092896f));
   float n0, n1;
   f2_unpack(xr, n0, n1);
-  return f2_mul(q, f2_pack(__int_as_float((__float_as_int(n0) << 23) + 0x3f800000), __int_as_float((__float_as_int(n1) << 23) + 0x3f800000)));
+  auto power = [](float n) { return __int_as_float((__float_as_int(n) << 23) + 0x3f800000); };
+  return f2_mul(q, f2_pack(power(n0), power(n1)));
 }
 
 }  // namespace
@@ -419,7 +416,7 @@ __global__ void __launch_bounds__(PmCfg<HD>::THREADS, 1) prompt_mass_kernel(cons
                 } else {
                   float x0, x1;
                   f2_unpack(x, x0, x1);
-                  x = f2_pack(pm_ex2(x0), pm_ex2(x1));
+                  x = f2_pack(ex2(x0), ex2(x1));
                 }
                 acc[a] = f2_add(acc[a], x);
               }
@@ -435,7 +432,7 @@ __global__ void __launch_bounds__(PmCfg<HD>::THREADS, 1) prompt_mass_kernel(cons
                 f2_unpack(term[c], t0, t1);
                 if (d < 0 || t0 == -INFINITY) x0 = -INFINITY;
                 if (d + 1 < 0 || t1 == -INFINITY) x1 = -INFINITY;
-                acc[a] = f2_add(acc[a], f2_pack(pm_ex2(x0), pm_ex2(x1)));
+                acc[a] = f2_add(acc[a], f2_pack(ex2(x0), ex2(x1)));
               }
           }
         }
@@ -537,12 +534,7 @@ __global__ void __launch_bounds__(PmCfg<HD>::THREADS, 1) prompt_mass_kernel(cons
   }
 }
 
-int encode_tmap_sw128(CUtensorMap* out, const void* base, int dtype, int rank, const uint64_t* dims,
-                      const uint64_t* strides_bytes, const uint32_t* box);
-
 namespace {
-
-constexpr int64_t kCounterBytes = 8192;  // of the workspace; the pieces follow
 
 template <typename T, int HD, int MODE>
 int pm_launch(const CUtensorMap& tq, const CUtensorMap& tk, const PmParams& p, cudaStream_t st) {

@@ -5,9 +5,13 @@
     logits = gen.prefill(prompts, lengths); logits = gen.step(tokens) # or token by token
 
 The prompts' attention is the training forward; their keys and values (and with a budget their attention masses) go into the
-cache's pages.  Everything runs in the model's own type, also inside an autocast region.  A step writes each sequence's new key and value and attends over its pages in one call per layer.  With a budget every
-head of every layer keeps the `recent` last keys and those that have got most attention, after the prompt and then every
-`interval` tokens.  The reference has no counterpart: it trains only.
+cache's pages.  Everything runs in the model's own type, also inside an autocast region, on the layers' weights: forward hooks
+on a layer or a projection are not called.  A step writes each sequence's new key and value and attends over its pages in one call
+per layer.  With a budget every head of every layer keeps the `recent` last keys and those that have got most attention, after
+the prompt and then every `interval` tokens.  The reference has no counterpart: it trains only.
+
+A model without ALiBi has a learned position for each token; with it, the slopes come from its table, also where the model was
+moved to bf16 after the table was made in fp16.  A captured step (`graph=True`) reads the weights that the model had in memory then.
 """
 import torch
 
@@ -102,8 +106,8 @@ class Generator:
     @torch.autocast("cuda", enabled=False)
     def prefill(self, prompts, lengths=None):
         """Starts the sequences: prompts (batch, T) int64, the first lengths[b] of each (all by default); what follows those may be
-        any number.  Returns the logits (batch, vocab) of the tokens that follow.  Lengths are from 1 to T; those that are on the GPU are not waited for, but
-        taken as the nearest ones that are, and `_lib.check_status()` says so."""
+        any number.  Returns the logits (batch, vocab) of the tokens that follow.  Lengths are from 1 to T; those that are on the
+        GPU are not waited for, but taken as the nearest ones that are, and `_lib.check_status()` says so."""
         b, t = prompts.shape
         assert b == self.batch and 1 <= t <= self.max_tokens, "prompts are (batch, up to max_tokens) token ids"
         device = self.tables.device

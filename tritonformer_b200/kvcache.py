@@ -3,7 +3,7 @@
 The keys and values of a layer lie in a pool of pages, (pages, heads, page, head_dim).  Slot s of sequence b is row s % page of
 page `tables[b, s // page]`; what a table holds beyond the slots in use does not matter.  `tables` (batch, pages of a sequence)
 and `lengths` (batch,) are int32 tensors on the GPU, so no call waits for the host and all of them can be captured in a CUDA
-graph.  For eviction every (page, head, slot) has two statistics: the attention that its key has got so far (`mass`, fp32), and
+graph, which has its own scratch and may be replayed beside other calls and graphs.  For eviction every (page, head, slot) has two statistics: the attention that its key has got so far (`mass`, fp32), and
 the position of its token (`positions`, int32), because a key that moves to another slot keeps its distance for ALiBi.
 
   * `paged_attention`   one new token per sequence: writes its key and value, attends to all keys, adds to the masses
@@ -34,8 +34,9 @@ def paged_attention(query, k_pages, v_pages, tables, lengths, key=None, value=No
     """Attention of one query per sequence, (batch, heads, head_dim), over the lengths[b] keys in its pages; with `key` and
     `value` (batch, cache heads, head_dim) over those and the new key, which is written into slot lengths[b] (`lengths` itself
     stays).  A sequence without keys gets zeros.  With `mass` every key's weights, summed over the query heads of its head, are
-    added to it, in place or into `mass_out` (no page may then be part of two sequences); with `positions` the new key's entry is set.  The query's position is
-    query_positions[b], or the number of the last slot."""
+    added to it, in place or into `mass_out` (no page may then be part of two sequences); the call then takes 4 bytes of scratch per
+    query head and slot of the tables, whatever the lengths are.  With `positions` the new key's entry is set.  The query's
+    position is query_positions[b], or the number of the last slot."""
     bias = _slopes(attn_bias, query.shape[1])
     return _host.paged_attention(query, k_pages, v_pages, tables, lengths, key, value, bias.slopes, int(bias.rounded),
                                  query_positions, mass, positions, mass_out)
@@ -50,7 +51,7 @@ def prompt_attention(query, key, value, attn_bias=None):
 def prompt_mass(query, key, lse, counts=None, attn_bias=None):
     """(batch, cache heads, T) fp32: what each key of a prompt gets of the causal attention of its first counts[b] tokens, summed
     over the queries and over the query heads of its head.  query (batch, heads, T, head_dim), key (batch, cache heads, T,
-    head_dim), lse (batch, heads, T) of the scaled and biased scores; any T."""
+    head_dim), lse (batch, heads, T) of the scaled and biased scores; any T.  What lies behind a prompt's end may be anything."""
     bias = _slopes(attn_bias, query.shape[1])
     return _host.prompt_mass(query, key, lse, counts, bias.slopes, int(bias.rounded))
 
