@@ -5,7 +5,7 @@
 //
 // Measured: prompts of up to 4096 keys, 16 x 8 heads of 128 with statistics, 272 MB in and out, 46.0 us (5.9 TB/s; rows stored so that
 // they leave the caches first, 48.9 without).  Eviction in place of 4 x 8 heads of 128 from 32768 to 8192 keys 66 us, of which the
-// selection takes 32; of 16 x 16 heads of 64 from up to 2048 to 512 keys into other pages 23.6; from 1088 to 1024 keys 10.6.
+// selection takes 31; of 16 x 16 heads of 64 from up to 2048 to 512 keys into other pages 23.7; from 1088 to 1024 keys 10.7.
 //
 // Eviction has a selection before its copies.  A key's worth is its mass, or infinite while its position is among the
 // `recent` last ones; each (sequence, key head) keeps the `keep` worthiest, ties to the lower slot.  With the worth in the upper and
