@@ -101,3 +101,22 @@ def test_prompts_up_to_the_last_position(alibi):
             got = Generator(model, 2, 100, budget=budget).prefill(ids[:, :t])
             assert norm_rel(got, steps[:, t - 60]) < 2e-2  # as in test_generate.py
     L.check_status()
+
+
+@gpu
+def test_a_captured_step_follows_the_models_bias():
+    """A table of other slopes, in another tensor and in the same one; the step that was captured before has gone."""
+    model = _model(alibi=True)
+    ids = torch.randint(0, 1000, (2, 60), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    gen = Generator(model, 2, 128, graph=True)
+    seen = []
+    for change in (lambda: None, lambda: setattr(model, "attn_bias", model.attn_bias * 0.25), lambda: model.attn_bias.mul_(8)):
+        change()
+        want = _teacher(model, ids, 40, Generator(model, 2, 128))
+        assert torch.equal(want, _teacher(model, ids, 40, gen))
+        assert all(not torch.equal(want, x) for x in seen)
+        seen.append(want)
+    graph = gen.graph
+    _teacher(model, ids, 40, gen)
+    assert gen.graph is graph  # nothing has changed
+    L.check_status()

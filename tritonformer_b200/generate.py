@@ -81,15 +81,15 @@ class Generator:
         self.logits = torch.zeros((batch, config.vocab_size), dtype=weight.dtype, device=device)
         self.longest = self.position = 0  # upper bounds of `lengths` and `next` that the host knows
         self.want_graph, self.graph = graph, None
-        self.bias = None  # the model's table, its version, and what _bias_of found
+        self.bias = None, None, None  # the model's table, its version, and what _bias_of found
 
     def _bias(self):
         """The model's bias in the operators' form; a table that is new here is looked over, which waits for the host."""
         table = self.model.attn_bias
-        if table is None:
-            return None
-        if self.bias is None or self.bias[0] is not table or self.bias[1] != table._version:
-            self.bias = table, table._version, _bias_of(table, self.heads)
+        version = None if table is None else table._version
+        if self.bias[0] is not table or self.bias[1] != version:
+            self.bias = table, version, None if table is None else _bias_of(table, self.heads)
+            self.graph = None  # a captured step reads the slopes that it was captured with
         return self.bias[2]
 
     def _block(self, layer, x, attend):
@@ -187,6 +187,7 @@ class Generator:
         if self.longest == self.width * self.page or (self.budget is not None and self.longest >= self.budget + self.interval):
             self._evict()
         self.tokens.copy_(tokens)
+        self._bias()
         if self.want_graph and self.graph is None:
             self._capture()
         if self.graph is not None:
@@ -208,7 +209,6 @@ class Generator:
         # a step ahead of the capture makes the workspaces; the sequences then go back to where they were
         before = self.lengths.clone(), self.next.clone()
         masses = [c.mass.clone() if c.mass is not None else None for c in self.caches]
-        self._bias()  # may wait for the host
 
         def back():
             self.lengths.copy_(before[0])
