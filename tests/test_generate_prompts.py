@@ -120,3 +120,23 @@ def test_a_captured_step_follows_the_models_bias():
     _teacher(model, ids, 40, gen)
     assert gen.graph is graph  # nothing has changed
     L.check_status()
+
+
+@gpu
+def test_a_captured_step_follows_the_models_weights():
+    """Weights that are written to in place, and weights that have moved."""
+    model = _model()
+    ids = torch.randint(0, 1000, (2, 60), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    gen = Generator(model, 2, 128, graph=True)
+    _teacher(model, ids, 40, gen)
+    graph = gen.graph
+    with torch.no_grad():
+        model.layer_list[0].attention.v_proj.weight.mul_(0.5)
+    want = _teacher(model, ids, 40, Generator(model, 2, 128))
+    assert torch.equal(want, _teacher(model, ids, 40, gen)) and gen.graph is graph
+    model.fuse_projection_weights()
+    with torch.no_grad():
+        model.layer_list[1].attention.v_proj.weight.mul_(0.5)
+    want = _teacher(model, ids, 40, Generator(model, 2, 128))
+    assert torch.equal(want, _teacher(model, ids, 40, gen)) and gen.graph is not graph
+    L.check_status()

@@ -11,7 +11,8 @@ per layer.  With a budget every head of every layer keeps the `recent` last keys
 the prompt and then every `interval` tokens.  The reference has no counterpart: it trains only.
 
 A model without ALiBi has a learned position for each token; with it, the slopes come from its table, also where the model was
-moved to bf16 after the table was made in fp16.  A captured step (`graph=True`) reads the weights that the model had in memory then.
+moved to bf16 after the table was made in fp16.  A captured step (`graph=True`) reads the weights where they were in memory;
+if they lie elsewhere when the next prompts come, it is captured again.  They must not move between a prompt and its steps.
 """
 import torch
 
@@ -81,6 +82,7 @@ class Generator:
         self.logits = torch.zeros((batch, config.vocab_size), dtype=weight.dtype, device=device)
         self.longest = self.position = 0  # upper bounds of `lengths` and `next` that the host knows
         self.want_graph, self.graph = graph, None
+        self.weights = None  # where the captured step reads them
         self.bias = None, None, None  # the model's table, its version, and what _bias_of found
 
     def _bias(self):
@@ -112,6 +114,8 @@ class Generator:
         assert b == self.batch and 1 <= t <= self.max_tokens, "prompts are (batch, up to max_tokens) token ids"
         device = self.tables.device
         counts, bad = _prompt_lengths(lengths, b, t, device)
+        if self.graph is not None and self.weights != self._addresses():
+            self.graph = None
         padded = -(-t // 64) * 64  # the training attention takes whole tiles of 64
         positions = self.model.embed_positions.weight if self.model.embed_positions is not None else None
         ids = torch.zeros((b, padded), dtype=torch.int64, device=device)
@@ -205,6 +209,9 @@ class Generator:
         self.lengths.copy_(left)
         self.longest = min(self.longest, self.budget)
 
+    def _addresses(self):
+        return [p.data_ptr() for p in self.model.parameters()]
+
     def _capture(self):
         # a step ahead of the capture makes the workspaces; the sequences then go back to where they were
         before = self.lengths.clone(), self.next.clone()
@@ -226,6 +233,7 @@ class Generator:
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph, stream=side):
             self._forward()
+        self.weights = self._addresses()
 
     def generate(self, prompts, lengths=None, new_tokens=1, choose=None):
         """(batch, new_tokens) token ids that follow the prompts; `choose` maps logits to tokens (the largest by default)."""
