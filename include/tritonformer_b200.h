@@ -378,6 +378,40 @@ int tfb_cache_evict(const void* k_pages, const void* v_pages, const float* mass,
                     int64_t out_num_pages, int64_t out_width, int64_t out_table_ld, const int64_t* out_page_strides,
                     void* scratch, int64_t scratch_bytes, int dtype, void* stream);
 
+/* ------------------------------------------------------------------- weights in 4 bits
+ * No counterpart in the reference, which trains only.  A weight W (K, N), y = x W, is held as W[k,n] = s[k / group, n] * c[k,n]: c a
+ * whole number from -7 to 7, s of the 16-bit type `dtype`, groups of 32, 64 or 128 rows of a column.  Rows are padded to units of 64
+ * and columns to strips of 16.  codes: tfb_int4_codes() words (strip, unit, 4 r + j, t), each with columns 16 strip + r and 16 strip +
+ * r + 8 at rows 64 unit + 32 (t / 2) + 8 j + 4 (t % 2) + 0..3; row offset 2 p + e of column half c lies at bits 4 (c + 2 p) + 16 e, as c + 8.
+ * scales: tfb_int4_scales() values (strip, group of the padded rows, r, column half).  Both 16-byte aligned.
+ *
+ * tfb_int4_quantize: codes and scales of w, element strides w_k, w_n.  s = (largest magnitude of the group) / 7, rounded to the type, and NaN where
+ * a weight is not finite; c = W / s rounded to the nearest whole number, ties to even.
+ * tfb_int4_expand: s * c rounded to the type, transposed: out (16 * strips, 64 * units), 16-byte aligned.
+ * tfb_int4_linear: out = act(x W + bias) + addend for M rows of x (pitch x_ld, unit stride, any alignment), out and addend of pitch
+ * out_ld, addend_ld; bias (N) and addend may be NULL, the addend may be the output.  For few rows: every 64 of them read the weights again.  */
+int64_t tfb_int4_codes(int64_t K, int64_t N);
+int64_t tfb_int4_scales(int64_t K, int64_t N, int group);
+int tfb_int4_quantize(const void* w, int64_t w_k, int64_t w_n, int64_t K, int64_t N, int group, void* codes,
+                      void* scales, int dtype, void* stream);
+int tfb_int4_expand(const void* codes, const void* scales, int64_t K, int64_t N, int group, void* out, int dtype,
+                    void* stream);
+int tfb_int4_linear(const void* x, int64_t x_ld, const void* codes, const void* scales, const void* bias,
+                    const void* addend, int64_t addend_ld, void* out, int64_t out_ld, int64_t M, int64_t K, int64_t N,
+                    int group, int relu, int dtype, void* stream);
+
+/* ------------------------------------------------------------------- drawing tokens
+ * No counterpart in the reference.  One token per row of logits (B, vocab), pitch ld, fp32, fp16 or bf16: with w_i = exp((l_i - max l) / t)
+ * and the order of larger logits first, equal ones by index, kept are the first top_k (0: all), of those the ones whose predecessors
+ * weigh less than top_p times the sum of the top_k, of those the ones with w_i >= min_p; out[b] is the first index j at which the sum of
+ * the kept weights up to j exceeds uniforms[b] times their sum.  Weights and sums in 64 bits.  A logit that is NaN counts as -infinity, all
+ * +infinite ones share the weight; a row of -infinity gives -1.  temperature 0: the first of the largest.  Each setting is an array with one
+ * value per row, or where that is NULL the number behind it; values outside their range (temperature >= 0, top_k >= 0, top_p and min_p from
+ * 0 to 1, uniforms from 0 to below 1) are taken as the nearest, NaN as 0 or, for top_p, as 1.                                   */
+int tfb_sample(const void* logits, int64_t ld, const float* uniforms, const float* temperature,
+               float temperature_all, const int* top_k, int top_k_all, const float* top_p, float top_p_all,
+               const float* min_p, float min_p_all, int64_t* out, int64_t B, int64_t vocab, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -68,6 +68,12 @@ _SIGNATURES = {
     "tfb_prompt_mass": (_i32, [_vp] * 5 + [_i32, _vp] + [_i64] * 5 + [_pi64] * 3 + [_vp, _i64, _i32, _vp]),
     "tfb_cache_evict_scratch_bytes": (_i64, [_i64] * 3),
     "tfb_cache_evict": (_i32, [_vp] * 13 + [_i64] * 9 + [_pi64] + [_i64] * 4 + [_pi64, _vp, _i64, _i32, _vp]),
+    "tfb_int4_codes": (_i64, [_i64] * 2),
+    "tfb_int4_scales": (_i64, [_i64] * 2 + [_i32]),
+    "tfb_int4_quantize": (_i32, [_vp] + [_i64] * 4 + [_i32, _vp, _vp, _i32, _vp]),
+    "tfb_int4_expand": (_i32, [_vp] * 2 + [_i64] * 2 + [_i32, _vp, _i32, _vp]),
+    "tfb_int4_linear": (_i32, [_vp, _i64] + [_vp] * 4 + [_i64, _vp] + [_i64] * 4 + [_i32, _i32, _i32, _vp]),
+    "tfb_sample": (_i32, [_vp, _i64, _vp, _vp, _f32, _vp, _i32, _vp, _f32, _vp, _f32, _vp, _i64, _i64, _i32, _vp]),
 }
 
 EXPORTS = tuple(sorted(_SIGNATURES))

@@ -49,6 +49,24 @@ Tensor cross_entropy(const Tensor& logits, const Tensor& labels, bool f32);
 Tensor lm_loss(const Tensor& logits, const Tensor& labels);
 Tensor embedding(const Tensor& ids, const Tensor& tok, const Tensor& pos);
 
+// Raises unless the defined ones of the inputs of an operator without gradients are CUDA tensors of one device that want none.
+void check_plain(const char* what, std::initializer_list<const Tensor*> inputs);
+
+// Weights in 4 bits, and drawing tokens (decode.cpp).
+struct Int4 {
+  Tensor codes, scales;
+  int64_t in, out, group;
+};
+Int4 int4_quantize(const Tensor& weight, int64_t group);
+Tensor int4_expand(const Int4& w);
+Tensor int4_linear(const Tensor& x, const Int4& w, const Tensor& bias, bool relu, const Tensor& addend);
+struct Setting {  // one number per row, or one for all
+  Tensor each;
+  double all;
+};
+Tensor sample(const Tensor& logits, const Tensor& uniforms, const Setting& temperature, const Setting& top_k, const Setting& top_p,
+              const Setting& min_p);
+
 // The paged key-value cache (kvcache.cpp).
 Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& tables, const Tensor& lengths,
                        const Tensor& key, const Tensor& value, const Tensor& slopes, int64_t rounded,

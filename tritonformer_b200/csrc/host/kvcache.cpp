@@ -3,7 +3,7 @@
 
 namespace tfb_host {
 
-static void check_plain(const char* what, std::initializer_list<const Tensor*> inputs) {
+void check_plain(const char* what, std::initializer_list<const Tensor*> inputs) {
   if (needs_node(inputs)) throw ArgumentError(std::string(what) + ": no gradients: call it under torch.no_grad()");
   const Tensor* first = nullptr;
   for (const Tensor* t : inputs) {

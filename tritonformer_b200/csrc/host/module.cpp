@@ -219,6 +219,62 @@ TFB_PY(py_cache_evict) {
     });
   });
 }
+Int4 int4_of(Args& a) {  // codes, scales, rows, columns, group
+  Int4 w;
+  w.codes = a.tensor();
+  w.scales = a.tensor();
+  w.in = a.integer();
+  w.out = a.integer();
+  w.group = a.integer();
+  return w;
+}
+TFB_PY(py_int4_quantize) {  // weight, group -> (codes, scales)
+  return guarded([&]() -> PyObject* {
+    refuse_tracing("quantize_int4");
+    Args a(argv, argc, 2, "quantize_int4");
+    const Tensor& w = a.tensor();
+    const int64_t group = a.integer();
+    Int4 q;
+    {
+      pybind11::gil_scoped_release no_gil;
+      q = int4_quantize(w, group);
+    }
+    return Py_BuildValue("(NN)", THPVariable_Wrap(q.codes), THPVariable_Wrap(q.scales));
+  });
+}
+TFB_PY(py_int4_expand) {  // a packed weight
+  return guarded([&]() -> PyObject* {
+    refuse_tracing("Int4Weight.dequantize");
+    Args a(argv, argc, 5, "Int4Weight.dequantize");
+    const Int4 w = int4_of(a);
+    return tensor_result([&] { return int4_expand(w); });
+  });
+}
+TFB_PY(py_int4_linear) {  // x, a packed weight, bias, relu, addend
+  return guarded([&]() -> PyObject* {
+    refuse_tracing("linear_int4");
+    Args a(argv, argc, 9, "linear_int4");
+    const Tensor& x = a.tensor();
+    const Int4 w = int4_of(a);
+    const Tensor& bias = a.tensor();
+    const bool relu = a.truth();
+    const Tensor& addend = a.tensor();
+    return tensor_result([&] { return int4_linear(x, w, bias, relu, addend); });
+  });
+}
+TFB_PY(py_sample) {  // logits, uniforms, and of temperature, top_k, top_p, min_p each: one per row or None, one for all
+  return guarded([&]() -> PyObject* {
+    refuse_tracing("sample_tokens");
+    Args a(argv, argc, 10, "sample_tokens");
+    const Tensor &logits = a.tensor(), &uniforms = a.tensor();
+    Setting s[4];
+    for (Setting& x : s) {
+      x.each = a.tensor();
+      x.all = a.real();
+    }
+    return tensor_result([&] { return sample(logits, uniforms, s[0], s[1], s[2], s[3]); });
+  });
+}
 TFB_PY(py_set_grad_mode) {  // accumulating, overwrite, defer, fork
   return guarded([&]() -> PyObject* {
     Args a(argv, argc, 4, "set_grad_mode");
@@ -273,6 +329,7 @@ PyMethodDef methods[] = {TFB_METHOD(linear), TFB_METHOD(layernorm), TFB_METHOD(a
                          TFB_METHOD(cross_entropy), TFB_METHOD(lm_loss), TFB_METHOD(embedding), TFB_METHOD(layer),
                          TFB_METHOD(layer_and_activations),
                          TFB_METHOD(paged_attention), TFB_METHOD(cache_append), TFB_METHOD(prompt_mass), TFB_METHOD(cache_evict),
+                         TFB_METHOD(int4_quantize), TFB_METHOD(int4_expand), TFB_METHOD(int4_linear), TFB_METHOD(sample),
                          TFB_METHOD(set_grad_mode), TFB_METHOD(take_written), TFB_METHOD(join_weight_grads),
                          TFB_METHOD(gemm_workspace), TFB_METHOD(reset_workspaces), TFB_METHOD(set_recorder), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Native host path of tritonformer_b200.", -1, methods,

@@ -1,0 +1,585 @@
+// One token per row of logits, drawn with a given uniform number (sm_100a).
+//
+//   w_i = exp((l_i - max l) / t);  order: larger logits first, equal ones by index;  kept: the first k in that order, of those the
+//   first whose predecessors weigh less than p times the sum, of those the ones with w_i >= m;
+//   token = the first index j with  sum of the kept w_i, i <= j,  >  u * sum of the kept w_i.
+//
+// What is kept is a beginning of the order, so it is all logits above a value and some of those equal to it.  That value is searched
+// for, with nothing sorted: a round takes the count and weight above 8 values at once and goes on in the ninth part that holds the
+// border.  All sums are in 64 bits, weights to some 2^-48: a token is the drawn one or it is not, and where a sum meets the border
+// between two of 50 thousand tokens, 32 bits would now and then give the neighbour.
+// A cluster of 1 to 8 blocks has a row in its shared memory; blocks, warps and lanes hold it in the order of its columns, so that the
+// last sums, by warps, say which warp has the token.  Sums are taken in a fixed order: the same call gives the same token.
+#include <cooperative_groups.h>
+#include "common.cuh"
+
+namespace tfb {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int SM_WARPS = 16, SM_THREADS = SM_WARPS * 32, SM_CLUSTER = 8;
+constexpr int SM_CUTS = 8;  // values that a round looks at
+constexpr double kLog2eD = 1.4426950408889634074;
+
+struct SampleParams {
+  const void* logits;
+  int64_t ld;
+  const float* uniforms;
+  const float *temperature, *top_p, *min_p;  // null: the number below for all rows
+  const int* top_k;
+  float temperature_all, top_p_all, min_p_all;
+  int top_k_all;
+  int64_t* out;
+  int vocab;
+  int warp_units;  // 16-byte units of a warp
+};
+
+// Whole numbers in the order of a type's values; -0 and 0 have one.
+template <typename T> struct Keys {
+  static constexpr uint32_t kSign = 0x8000u;
+  static __device__ __forceinline__ uint32_t of(float x) {  // x rounded to the type
+    const T v = Num<T>::from_f(x + 0.f);
+    const uint32_t u = *reinterpret_cast<const uint16_t*>(&v);
+    return (u & kSign ? 0u - u : u | kSign) & 0xffffu;
+  }
+  static __device__ __forceinline__ float value(uint32_t k) {
+    const uint16_t u = (uint16_t)(k & kSign ? k ^ kSign : 0u - k);
+    return Num<T>::to_f(*reinterpret_cast<const T*>(&u));
+  }
+};
+template <> struct Keys<float> {
+  static __device__ __forceinline__ uint32_t of(float x) {
+    const uint32_t u = __float_as_uint(x + 0.f);
+    return u & 0x80000000u ? 0u - u : u | 0x80000000u;
+  }
+  static __device__ __forceinline__ float value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : 0u - k); }
+};
+
+template <typename T> constexpr int kPerUnit = 16 / sizeof(T);
+template <typename T> __device__ __forceinline__ void unpack_unit(const uint4& v, float (&x)[kPerUnit<T>]) {
+  if constexpr (sizeof(T) == 4) {
+    x[0] = __uint_as_float(v.x); x[1] = __uint_as_float(v.y); x[2] = __uint_as_float(v.z); x[3] = __uint_as_float(v.w);
+  } else {
+    unpack8<T>(v, x);
+  }
+}
+
+// 2^y for y <= 0, by Tang's method (ACM TOMS 15, 1989): 2^(i / 32) from a table, one entry in each lane, times a polynomial for the rest.
+// All lanes of the warp take part.
+__device__ __forceinline__ double weight_of(double y, double table) {
+  constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
+  constexpr double l = 0.69314718055994530942;
+  y = fmax(y, -1021.0);
+  const double k = __fma_rn(y, 32.0, kMagic);
+  const int n = __double2loint(k);
+  const double r = __fma_rn(k - kMagic, -1.0 / 32, y);  // at most 1/64
+  double p = __fma_rn(r, l * l * l * l * l / 120, l * l * l * l / 24);
+  p = __fma_rn(r, p, l * l * l / 6);
+  p = __fma_rn(r, p, l * l / 2);
+  p = __fma_rn(r, p, l);
+  p = __fma_rn(r, p, 1.0);
+  const double s = __shfl_sync(0xffffffffu, table, n & 31) * p;
+  return y < -1000.0 ? 0.0 : __hiloint2double(__double2hiint(s) + ((n >> 5) << 20), __double2loint(s));
+}
+
+template <typename V> __device__ __forceinline__ V sum_lanes(V v, int from) {
+#pragma unroll
+  for (int o = from; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+struct Shared {
+  double sums[2][SM_CLUSTER][SM_CUTS];
+  int counts[2][SM_CLUSTER][SM_CUTS];
+  double warp_sums[SM_WARPS][SM_CUTS];
+  int warp_counts[SM_WARPS][SM_CUTS];
+  float tops[SM_CLUSTER][2];
+  int any[SM_CLUSTER];
+  float warp_tops[SM_WARPS][2];
+  int warp_any[SM_WARPS];
+  double all_sums[SM_CLUSTER * SM_WARPS];
+  int all_ties[SM_CLUSTER * SM_WARPS];
+};
+
+}  // namespace
+
+template <typename T>
+__global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams p) {
+  constexpr int W = kPerUnit<T>;
+  extern __shared__ uint4 units[];
+  __shared__ Shared sh;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t row = blockIdx.x / blocks;
+  const double table = exp2(lane / 32.0);
+  if (blocks > 1) cluster.barrier_arrive();  // waited for before the first access to another block's memory
+  auto sync = [&]() {
+    if (blocks == 1) __syncthreads();
+    else cluster.sync();
+  };
+  grid_dependency_wait();
+  allow_dependents();
+
+  // ---- the row's settings
+  float t = p.temperature ? p.temperature[row] : p.temperature_all;
+  float top_p = p.top_p ? p.top_p[row] : p.top_p_all, min_p = p.min_p ? p.min_p[row] : p.min_p_all;
+  int k = p.top_k ? p.top_k[row] : p.top_k_all;
+  float u = p.uniforms[row];
+  if (!(t > 0.f) || top_p <= 0.f) {
+    k = 1;
+    t = 1.f;
+  }
+  if (k <= 0 || k >= p.vocab) k = 0;
+  const bool nucleus = top_p < 1.f && k != 1;
+  if (!(min_p > 0.f)) min_p = 0.f;
+  min_p = fminf(min_p, 1.f);
+  u = !(u > 0.f) ? 0.f : fminf(u, 0.99999994f);
+  const double per = kLog2eD / (double)t;
+
+  // ---- the warp's part of the row: 16-byte units of memory, with what is not the row's as -infinity
+  const T* logits = static_cast<const T*>(p.logits) + row * p.ld;
+  const int shift = (int)((reinterpret_cast<uintptr_t>(logits) & 15) / sizeof(T));
+  const uint4* source = reinterpret_cast<const uint4*>(logits - shift);
+  const int row_units = (p.vocab + shift + W - 1) / W;
+  const int first = (rank * SM_WARPS + warp) * p.warp_units;
+  const int mine = max(0, min(p.warp_units, row_units - first));  // of these units there are
+  uint4* part = units + warp * p.warp_units;
+  const T none = Num<T>::from_f(-INFINITY);
+  float top = -INFINITY, bottom = INFINITY;
+  int finite = 0;
+  for (int i = lane; i < mine; i += 32) {
+    uint4 v = ld_stream16(source + first + i);
+    if (first + i == 0 || first + i == row_units - 1) {
+      T* e = reinterpret_cast<T*>(&v);
+#pragma unroll
+      for (int q = 0; q < W; ++q) {
+        const int c = (first + i) * W + q - shift;
+        if (c < 0 || c >= p.vocab) e[q] = none;
+      }
+    }
+    part[i] = v;
+    float x[W];
+    unpack_unit<T>(v, x);
+#pragma unroll
+    for (int q = 0; q < W; ++q) {
+      top = fmaxf(top, x[q]);
+      if (x[q] > -INFINITY) {
+        bottom = fminf(bottom, x[q]);
+        ++finite;
+      }
+    }
+  }
+  __syncwarp();
+  top = warp_max(top);
+  bottom = -warp_max(-bottom);
+  finite = sum_lanes(finite, 16);
+  if (lane == 0) {
+    sh.warp_tops[warp][0] = top;
+    sh.warp_tops[warp][1] = bottom;
+    sh.warp_any[warp] = finite;
+  }
+  __syncthreads();
+  if (blocks > 1) cluster.barrier_wait();
+  if (warp == 0) {
+    top = warp_max(lane < SM_WARPS ? sh.warp_tops[lane][0] : -INFINITY);
+    bottom = -warp_max(lane < SM_WARPS ? -sh.warp_tops[lane][1] : -INFINITY);
+    finite = sum_lanes(lane < SM_WARPS ? sh.warp_any[lane] : 0, 16);
+    if (lane < blocks) {
+      Shared* to = cluster.map_shared_rank(&sh, lane);
+      to->tops[rank][0] = top;
+      to->tops[rank][1] = bottom;
+      to->any[rank] = finite;
+    }
+  }
+  sync();
+  top = -INFINITY;
+  bottom = INFINITY;
+  finite = 0;
+  for (int i = 0; i < blocks; ++i) {
+    top = fmaxf(top, sh.tops[i][0]);
+    bottom = fminf(bottom, sh.tops[i][1]);
+    finite += sh.any[i];
+  }
+  if (finite == 0) {  // nothing is allowed
+    if (rank == 0 && tid == 0) p.out[row] = -1;
+    return;
+  }
+  const double peak = (double)top;
+  auto weigh = [&](float x) {  // all lanes
+    const double w = weight_of(((double)x - peak) * per, table);
+    return x == top ? 1.0 : w;
+  };
+
+  // Sums over the cluster; every thread gets them.  Two sets of places in turn: one barrier separates the uses of each.
+  int parity = 0;
+  auto reduce = [&](double (&s)[SM_CUTS], int (&c)[SM_CUTS]) {
+    // lanes first: each step halves the values that a lane has
+#pragma unroll
+    for (int n = SM_CUTS / 2, mask = 16; n > 0; n /= 2, mask /= 2) {
+      const bool upper = (lane & mask) != 0;
+#pragma unroll
+      for (int i = 0; i < n; ++i) {
+        const double send = upper ? s[i] : s[i + n];
+        const int send_c = upper ? c[i] : c[i + n];
+        s[i] = (upper ? s[i + n] : s[i]) + __shfl_xor_sync(0xffffffffu, send, mask);
+        c[i] = (upper ? c[i + n] : c[i]) + __shfl_xor_sync(0xffffffffu, send_c, mask);
+      }
+    }
+    s[0] = sum_lanes(s[0], 2);
+    c[0] = sum_lanes(c[0], 2);
+    if ((lane & 3) == 0) {
+      const int i = (lane & 16) / 4 + (lane & 8) / 4 + (lane & 4) / 4;
+      sh.warp_sums[warp][i] = s[0];
+      sh.warp_counts[warp][i] = c[0];
+    }
+    __syncthreads();
+    if (tid < SM_CUTS * blocks) {
+      const int i = tid % SM_CUTS;
+      double v = 0.0;
+      int n = 0;
+#pragma unroll
+      for (int w = 0; w < SM_WARPS; ++w) {
+        v += sh.warp_sums[w][i];
+        n += sh.warp_counts[w][i];
+      }
+      Shared* to = cluster.map_shared_rank(&sh, tid / SM_CUTS);
+      to->sums[parity][rank][i] = v;
+      to->counts[parity][rank][i] = n;
+    }
+    sync();
+#pragma unroll
+    for (int i = 0; i < SM_CUTS; ++i) {
+      s[i] = 0.0;
+      c[i] = 0;
+    }
+    for (int b = 0; b < blocks; ++b)
+#pragma unroll
+      for (int i = 0; i < SM_CUTS; ++i) {
+        s[i] += sh.sums[parity][b][i];
+        c[i] += sh.counts[parity][b][i];
+      }
+    parity ^= 1;
+  };
+
+  // The cut: all logits above `cut` and the first `ties` of those equal to it.  Below every logit: all of them.
+  const uint32_t over = Keys<T>::of(top) + 1;
+  uint32_t low = Keys<T>::of(bottom) - 1, high = over;  // the search's borders: reached at `low`, not at `high`
+  const uint32_t under = low;
+  int count_low = finite, count_high = 0;  // logits at or above the two
+  double sum_high = 0.0;
+  int ties = 0;
+  float cuts[SM_CUTS];
+  auto place = [&](int round) {  // 8 values between the borders, descending
+    const float a = Keys<T>::value(low), b = Keys<T>::value(high);
+    const bool even = high - low <= SM_CUTS + 1 || (round & 1) != 0 || !isfinite(b - a);
+#pragma unroll
+    for (int i = 0; i < SM_CUTS; ++i) {
+      uint32_t key;
+      if (even) key = high - max((uint32_t)(((uint64_t)(high - low) * (i + 1)) / (SM_CUTS + 1)), 1u);
+      else key = Keys<T>::of(b - (b - a) * ((i + 1) / (float)(SM_CUTS + 1)));
+      cuts[i] = Keys<T>::value(min(max(key, low + 1), high - 1));
+    }
+  };
+  auto narrow = [&](int i_low, const double (&s)[SM_CUTS], const int (&c)[SM_CUTS]) {  // the first of the cuts that reaches the goal
+    double sum = sum_high;
+    int count = count_high;
+    uint32_t h = high;
+#pragma unroll
+    for (int i = 0; i < SM_CUTS; ++i) {
+      if (i < i_low) {
+        sum = sum_high + s[i];
+        count = count_high + c[i];
+        h = Keys<T>::of(cuts[i]);
+      }
+      if (i == i_low) {
+        low = Keys<T>::of(cuts[i]);
+        count_low = count_high + c[i];
+      }
+    }
+    high = h;
+    sum_high = sum;
+    count_high = count;
+  };
+
+  if (k == 1) {
+    low = Keys<T>::of(top);
+    ties = 1;
+  } else if (k > 0 && k < finite) {
+    for (int round = 0; high - low > 1 && round < 64; ++round) {
+      place(round);
+      const float a = Keys<T>::value(low), b = Keys<T>::value(high);
+      const bool open = high == over;  // whose value may be none
+      double s[SM_CUTS];
+      int c[SM_CUTS];
+#pragma unroll
+      for (int i = 0; i < SM_CUTS; ++i) {
+        s[i] = 0.0;
+        c[i] = 0;
+      }
+      for (int i = lane; i < mine; i += 32) {
+        float x[W];
+        unpack_unit<T>(part[i], x);
+#pragma unroll
+        for (int q = 0; q < W; ++q)
+          if (x[q] > a && (open || x[q] < b))
+#pragma unroll
+            for (int j = 0; j < SM_CUTS; ++j) c[j] += x[q] >= cuts[j];
+      }
+      reduce(s, c);
+      int reached = SM_CUTS;
+#pragma unroll
+      for (int i = SM_CUTS - 1; i >= 0; --i)
+        if (count_high + c[i] >= k) reached = i;
+      narrow(reached, s, c);
+    }
+    ties = k - count_high;
+  } else {
+    low = under;
+  }
+
+  if (nucleus) {
+    // of what is left the first whose predecessors weigh less than p times the sum
+    const int tied = ties;
+    const double low_weight = __shfl_sync(0xffffffffu, weigh(Keys<T>::value(low)), 0);
+    const uint32_t floor = low;
+    high = over;
+    count_high = 0;
+    sum_high = 0.0;
+    double goal = 0.0;
+    for (int round = 0; round == 0 || (high - low > 1 && round < 64); ++round) {
+      if (round == 0) {  // by weights, and the last is the sum of all
+        const float steps[SM_CUTS] = {0.7f, 1.5f, 2.5f, 4.f, 6.f, 8.5f, 12.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < SM_CUTS; ++i)
+          cuts[i] = Keys<T>::value(min(max(Keys<T>::of(isfinite(top) ? top - steps[i] * t : top), low + 1), high - 1));
+      } else {
+        place(round);
+      }
+      const float a = Keys<T>::value(low), b = Keys<T>::value(high);
+      const bool open = high == over;  // whose value may be none
+      double s[SM_CUTS];
+      int c[SM_CUTS];
+#pragma unroll
+      for (int i = 0; i < SM_CUTS; ++i) {
+        s[i] = 0.0;
+        c[i] = 0;
+      }
+      const int steps = (mine + 31) / 32;
+      for (int step = 0; step < steps; ++step) {
+        const int i = step * 32 + lane;
+        float x[W];
+        unpack_unit<T>(part[min(i, mine - 1)], x);
+#pragma unroll
+        for (int q = 0; q < W; ++q) {
+          const bool in = i < mine && x[q] > a && (open || x[q] < b);
+          if (!__any_sync(0xffffffffu, in)) continue;
+          const double w = weigh(x[q]);
+          if (in) {
+#pragma unroll
+            for (int j = 0; j < SM_CUTS; ++j)
+              if (x[q] >= cuts[j] || (round == 0 && j == SM_CUTS - 1)) {
+                s[j] += w;
+                ++c[j];
+              }
+          }
+        }
+      }
+      reduce(s, c);
+      if (round == 0) {
+        goal = (double)top_p * (s[SM_CUTS - 1] + tied * low_weight);
+        cuts[SM_CUTS - 1] = Keys<T>::value(low);  // what lies at `low` or above it reaches the goal
+      }
+      int reached = SM_CUTS;
+#pragma unroll
+      for (int i = SM_CUTS - 1; i >= 0; --i)
+        if (sum_high + s[i] >= goal && !(round == 0 && i == SM_CUTS - 1)) reached = i;
+      if (round == 0 && reached == SM_CUTS) {  // between the last of the cuts and `low`
+        const uint32_t keep = low;
+        const int had = count_low;
+        narrow(SM_CUTS - 1, s, c);
+        low = keep;
+        count_low = had;
+      } else {
+        narrow(reached, s, c);
+      }
+    }
+    const double w = __shfl_sync(0xffffffffu, weigh(Keys<T>::value(low)), 0);
+    const double fit = ceil((goal - sum_high) / w);
+    const int there = low == floor ? tied : count_low - count_high;
+    ties = fit < there ? max((int)fit, 1) : there;  // (w = 0: infinite, or NaN)
+    if (low == floor && tied == 0) ties = 0;
+  }
+
+  // ---- the kept weights of each warp, then the warp that has the token
+  const float cut = Keys<T>::value(low);
+  const double cut_weight = __shfl_sync(0xffffffffu, weigh(cut), 0);
+  const bool ties_kept = ties > 0 && cut_weight >= (double)min_p;
+  const int steps = (mine + 31) / 32;
+  double sum = 0.0;
+  int equal = 0;
+  for (int step = 0; step < steps; ++step) {
+    const int i = step * 32 + lane;
+    float x[W];
+    unpack_unit<T>(part[min(i, mine - 1)], x);
+#pragma unroll
+    for (int q = 0; q < W; ++q) {
+      const bool in = i < mine && x[q] > cut;
+      equal += i < mine && x[q] == cut;
+      if (!__any_sync(0xffffffffu, in)) continue;
+      const double w = weigh(x[q]);
+      if (in && w >= (double)min_p) sum += w;
+    }
+  }
+  sum = sum_lanes(sum, 16);
+  equal = sum_lanes(equal, 16);
+  if (lane < blocks) {
+    Shared* to = cluster.map_shared_rank(&sh, lane);
+    to->all_sums[rank * SM_WARPS + warp] = sum;
+    to->all_ties[rank * SM_WARPS + warp] = equal;
+  }
+  sync();
+  // each warp for itself, in the order of the warps
+  double before = 0.0, total = 0.0, here = 0.0;
+  int tie_base = 0, last = -1;
+  int seen = 0;
+  const int me = rank * SM_WARPS + warp;
+  for (int i = 0; i < blocks * SM_WARPS; ++i) {
+    const int n = sh.all_ties[i], kept = ties_kept ? max(0, min(n, ties - seen)) : 0;
+    const double w = sh.all_sums[i] + kept * cut_weight;
+    if (i == me) {
+      before = total;
+      here = w;
+      tie_base = seen;
+    }
+    if (w > 0.0) last = i;
+    seen += n;
+    total += w;
+  }
+  const double goal = (double)u * total;
+  const bool found = here > 0.0 && before <= goal && (before + here > goal || last == me);
+  if (!found) return;
+  double base = before;
+  int token = -1, rank_base = tie_base;
+  for (int step = 0; step < steps; ++step) {
+    const int i = step * 32 + lane;
+    float x[W];
+    unpack_unit<T>(part[min(i, mine - 1)], x);
+    int n = 0;
+#pragma unroll
+    for (int q = 0; q < W; ++q) n += i < mine && x[q] == cut;
+    int upto_n = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto_n, o);
+      if (lane >= o) upto_n += v;
+    }
+    int at = rank_base + upto_n - n;
+    rank_base += __shfl_sync(0xffffffffu, upto_n, 31);
+    double w[W], mine_sum = 0.0;
+#pragma unroll
+    for (int q = 0; q < W; ++q) {
+      const bool in = i < mine && x[q] > cut;
+      double v = 0.0;
+      if (__any_sync(0xffffffffu, in)) v = weigh(x[q]);
+      if (!in || v < (double)min_p) v = 0.0;
+      if (i < mine && x[q] == cut && ties_kept && at++ < ties) v = cut_weight;
+      w[q] = v;
+      mine_sum += v;
+    }
+    double upto = mine_sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    double line = base + (upto - mine_sum);
+    int hit = -1, back = -1;
+#pragma unroll
+    for (int q = 0; q < W; ++q) {
+      line += w[q];
+      if (w[q] > 0.0) {
+        back = q;
+        if (hit < 0 && line > goal) hit = q;
+      }
+    }
+    const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0), backs = __ballot_sync(0xffffffffu, back >= 0);
+    if (hits) {
+      const int who = __ffs(hits) - 1;
+      token = (first + step * 32 + who) * W + __shfl_sync(0xffffffffu, hit, who) - shift;
+      break;
+    }
+    if (backs) {  // where rounding leaves the goal behind the last kept one, that one
+      const int who = 31 - __clz(backs);
+      token = (first + step * 32 + who) * W + __shfl_sync(0xffffffffu, back, who) - shift;
+    }
+    base += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  if (lane == 0) p.out[row] = token;
+}
+
+namespace {
+
+template <typename T>
+int sample_launch(SampleParams p, int64_t B, cudaStream_t st) {
+  constexpr int W = kPerUnit<T>;
+  const int64_t row_units = ceil_div((int64_t)p.vocab + W - 1, W);
+  // blocks of a row: what the SMs have room for, and as many as its logits need
+  int blocks = 1;
+  while (blocks < SM_CLUSTER && (B * blocks < sm_count() || ceil_div(row_units, (int64_t)SM_WARPS * blocks) * SM_WARPS * 16 > 104 * 1024) &&
+         row_units > (int64_t)SM_THREADS * blocks)
+    blocks *= 2;
+  p.warp_units = (int)ceil_div(row_units, (int64_t)SM_WARPS * blocks);
+  const int64_t smem = (int64_t)p.warp_units * SM_WARPS * 16;
+  if (smem > 212 * 1024) return fail(TFB_ERR_UNSUPPORTED, "sample: %d logits in a row are more than a cluster has room for", p.vocab);
+  static std::atomic<uint64_t> done{0};
+  if (int rc = ensure_dynamic_smem(sample_kernel<T>, 212 * 1024, done, "sample")) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(B * blocks));
+  cfg.blockDim = dim3(SM_THREADS);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = blocks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = g_plain_launch.load(std::memory_order_relaxed) ? 1 : 2;
+  (void)cudaLaunchKernelEx(&cfg, sample_kernel<T>, p);
+  return launched("sample");
+}
+
+}  // namespace
+}  // namespace tfb
+
+using namespace tfb;
+
+extern "C" int tfb_sample(const void* logits, int64_t ld, const float* uniforms, const float* temperature, float temperature_all,
+                          const int* top_k, int top_k_all, const float* top_p, float top_p_all, const float* min_p, float min_p_all,
+                          int64_t* out, int64_t B, int64_t vocab, int dtype, void* stream) {
+  TFB_REQUIRE(B >= 0 && B < (1 << 24) && vocab >= 1 && vocab < (1 << 24), "sample: bad shape");
+  TFB_REQUIRE(B <= 1 || ld >= 0, "sample: negative row stride");
+  if (B == 0) return TFB_OK;
+  TFB_REQUIRE(logits && uniforms && out, "sample: null buffer");
+  SampleParams p = {};
+  p.logits = logits;
+  p.ld = ld;
+  p.uniforms = uniforms;
+  p.temperature = temperature;
+  p.temperature_all = temperature_all;
+  p.top_k = top_k;
+  p.top_k_all = top_k_all;
+  p.top_p = top_p;
+  p.top_p_all = top_p_all;
+  p.min_p = min_p;
+  p.min_p_all = min_p_all;
+  p.out = out;
+  p.vocab = (int)vocab;
+  if (dtype == TFB_F32) return sample_launch<float>(p, B, (cudaStream_t)stream);
+  if (dtype == TFB_F16) return sample_launch<__half>(p, B, (cudaStream_t)stream);
+  if (dtype == TFB_BF16) return sample_launch<__nv_bfloat16>(p, B, (cudaStream_t)stream);
+  return fail(TFB_ERR_ARG, "sample: dtype %d", dtype);
+}
