@@ -378,6 +378,29 @@ int tfb_cache_evict(const void* k_pages, const void* v_pages, const float* mass,
                     int64_t out_num_pages, int64_t out_width, int64_t out_table_ld, const int64_t* out_page_strides,
                     void* scratch, int64_t scratch_bytes, int dtype, void* stream);
 
+/* The same cache in 4 bits: pages (num_pages, kv_heads, page, hd / 2) of bytes, page_strides in bytes (multiples of 16, 16-byte aligned bases),
+ * and contiguous scales (num_pages, kv_heads, page, 2) of the 16-bit type, a row's of its key and of its value.  A value is its row's
+ * scale times a whole number c from -7 to 7: the scale is the row's largest magnitude over 7, rounded to the type (NaN where a value is not finite),
+ * c the nearest to value / scale, ties to even.  The 32-bit word w of a row holds dims 8 w .. 8 w + 7, dim 8 w + 2 n + e at
+ * bits 4 n + 16 e, as c + 8.  Such a cache has no statistics: a key's position is its slot's number.
+ *
+ * tfb_paged_attention_int4: tfb_paged_attention on it; q, the new rows and out are of the 16-bit type; the new row is attended to as it is stored.
+ * workspace as there.
+ * tfb_cache_append_int4: tfb_cache_append into it.  k_stored and v_stored (B, kv_heads, T, hd), strides {b, h, t} (multiples of 8,
+ * 16-byte aligned bases; both NULL: none) get what the cache now has for the rows, rounded to the type, and zeros from counts[b] on.    */
+int tfb_paged_attention_int4(const void* q, const void* k_new, const void* v_new, void* out, void* k_pages,
+                             void* v_pages, void* scales, const int* tables, const int* lengths, const float* slopes,
+                             int alibi_round, int64_t B, int64_t kv_heads, int64_t group, int64_t hd,
+                             int64_t num_pages, int64_t page, int64_t width, int64_t table_ld,
+                             const int64_t* page_strides, const int64_t* q_strides, const int64_t* k_new_strides,
+                             const int64_t* v_new_strides, const int64_t* o_strides, void* workspace,
+                             int64_t workspace_bytes, int dtype, void* stream);
+int tfb_cache_append_int4(const void* key, const void* value, void* k_pages, void* v_pages, void* scales,
+                          const int* tables, const int* lengths, const int* counts, void* k_stored, void* v_stored,
+                          int64_t B, int64_t kv_heads, int64_t T, int64_t hd, int64_t num_pages, int64_t page,
+                          int64_t width, int64_t table_ld, const int64_t* page_strides, const int64_t* key_strides,
+                          const int64_t* value_strides, const int64_t* stored_strides, int dtype, void* stream);
+
 /* ------------------------------------------------------------------- weights in 4 bits
  * No counterpart in the reference, which trains only.  A weight W (K, N), y = x W, is held as W[k,n] = s[k / group, n] * c[k,n]: c a
  * whole number from -7 to 7, s of the 16-bit type `dtype`, groups of 32, 64 or 128 rows of a column.  Rows are padded to units of 64

@@ -68,6 +68,8 @@ _SIGNATURES = {
     "tfb_prompt_mass": (_i32, [_vp] * 5 + [_i32, _vp] + [_i64] * 5 + [_pi64] * 3 + [_vp, _i64, _i32, _vp]),
     "tfb_cache_evict_scratch_bytes": (_i64, [_i64] * 3),
     "tfb_cache_evict": (_i32, [_vp] * 13 + [_i64] * 9 + [_pi64] + [_i64] * 4 + [_pi64, _vp, _i64, _i32, _vp]),
+    "tfb_paged_attention_int4": (_i32, [_vp] * 10 + [_i32] + [_i64] * 8 + [_pi64] * 5 + [_vp, _i64, _i32, _vp]),
+    "tfb_cache_append_int4": (_i32, [_vp] * 10 + [_i64] * 8 + [_pi64] * 4 + [_i32, _vp]),
     "tfb_int4_codes": (_i64, [_i64] * 2),
     "tfb_int4_scales": (_i64, [_i64] * 2 + [_i32]),
     "tfb_int4_quantize": (_i32, [_vp] + [_i64] * 4 + [_i32, _vp, _vp, _i32, _vp]),

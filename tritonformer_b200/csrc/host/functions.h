@@ -74,6 +74,14 @@ Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_p
 void cache_append(const Tensor& k_pages, const Tensor& v_pages, const Tensor& tables, const Tensor& lengths, const Tensor& key,
                   const Tensor& value, const Tensor& counts, const Tensor& mass, const Tensor& positions, const Tensor& key_mass,
                   const Tensor& first_positions);
+// On a cache in 4 bits: k_pages and v_pages of bytes, with a pair of scales for each row.
+Tensor paged_attention_int4(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& scales, const Tensor& tables,
+                            const Tensor& lengths, const Tensor& key, const Tensor& value, const Tensor& slopes, int64_t rounded);
+struct Stored {  // what the cache has for the rows, if wanted
+  Tensor key, value;
+};
+Stored cache_append_int4(const Tensor& k_pages, const Tensor& v_pages, const Tensor& scales, const Tensor& tables, const Tensor& lengths,
+                         const Tensor& key, const Tensor& value, const Tensor& counts, bool stored);
 Tensor prompt_mass(const Tensor& q, const Tensor& k, const Tensor& lse, const Tensor& counts, const Tensor& slopes, int64_t rounded);
 Tensor cache_evict(const Tensor& k, const Tensor& v, const Tensor& mass, const Tensor& positions, const Tensor& tables,
                    const Tensor& lengths, const Tensor& next_positions, const Tensor& k_out, const Tensor& v_out,

@@ -158,6 +158,105 @@ void cache_append(const Tensor& k_pages, const Tensor& v_pages, const Tensor& ta
                          dtype_code(key.scalar_type()), current_stream(key)));
 }
 
+// A pool in 4 bits; its head_dim is that of the values, its strides are in bytes.
+static Pool pool_int4_of(const Tensor& k, const Tensor& v, const Tensor& scales) {
+  TFB_ASSERT(k.defined() && v.defined() && k.dim() == 4 && k.sizes() == v.sizes() && k.scalar_type() == at::kByte &&
+                 v.scalar_type() == at::kByte,
+             "key and value pages in 4 bits are (pages, heads, page, head_dim / 2) uint8 tensors of one shape");
+  TFB_ASSERT(k.size(3) == 16 || k.size(3) == 32 || k.size(3) == 64, "Only head_dims of [32,64,128] are supported.");
+  TFB_ASSERT(k.size(0) > 0 && k.size(1) > 0 && k.size(2) > 0, "the cache has no pages");
+  TFB_ASSERT(k.stride(3) == 1 && v.stride(3) == 1, "the pages need a unit stride on head_dim");
+  Pool p{k.size(0), k.size(1), k.size(2), 2 * k.size(3), {step(k, 0), step(k, 1), step(k, 2)}};
+  for (int i = 0; i < 3; ++i) {
+    TFB_ASSERT(step(v, i) == p.strides[i], "key and value pages need the same strides");
+    TFB_ASSERT(k.size(i) == 1 || p.strides[i] > 0, "the pages overlap");
+  }
+  TFB_ASSERT(scales.dim() == 4 && scales.size(0) == p.pages && scales.size(1) == p.heads && scales.size(2) == p.page &&
+                 scales.size(3) == 2 && scales.is_contiguous() &&
+                 (scales.scalar_type() == at::kHalf || scales.scalar_type() == at::kBFloat16),
+             "the scales are a contiguous (pages, heads, page, 2) fp16/bf16 tensor");
+  return p;
+}
+
+Tensor paged_attention_int4(const Tensor& q_, const Tensor& k_pages, const Tensor& v_pages, const Tensor& scales, const Tensor& tables,
+                            const Tensor& lengths, const Tensor& key_, const Tensor& value_, const Tensor& slopes, int64_t rounded) {
+  check_plain("paged_attention", {&q_, &k_pages, &v_pages, &scales, &tables, &lengths, &key_, &value_, &slopes});
+  BodyGuard guard;
+  const Pool pool = pool_int4_of(k_pages, v_pages, scales);
+  TFB_ASSERT(q_.defined() && q_.dim() == 3 && q_.size(2) == pool.hd, "the query is a (batch, heads, head_dim) tensor");
+  TFB_ASSERT(q_.scalar_type() == scales.scalar_type(), "the query has the scales' type");
+  const int64_t B = q_.size(0), heads = q_.size(1);
+  TFB_ASSERT(heads > 0 && heads % pool.heads == 0, "the query heads are a multiple of the cache's heads");
+  const Table table = table_of(tables, B);
+  TFB_ASSERT(lengths.defined(), "lengths: expected a contiguous (batch,) int32 tensor");
+  check_per_sequence(lengths, B, "lengths");
+  TFB_ASSERT(key_.defined() == value_.defined(), "a new key comes with a value");
+  Tensor key, value;
+  if (key_.defined()) {
+    TFB_ASSERT(key_.dim() == 3 && key_.size(0) == B && key_.size(1) == pool.heads && key_.size(2) == pool.hd &&
+                   value_.sizes() == key_.sizes(),
+               "new keys and values are (batch, cache heads, head_dim) tensors");
+    TFB_ASSERT(key_.scalar_type() == q_.scalar_type() && value_.scalar_type() == q_.scalar_type(),
+               "new keys and values have the scales' type");
+    key = unit_inner(key_);
+    value = unit_inner(value_);
+  }
+  TFB_ASSERT(!slopes.defined() || (slopes.dim() == 1 && slopes.size(0) == heads && slopes.scalar_type() == at::kFloat &&
+                                   slopes.is_contiguous()),
+             "the slopes are a contiguous (heads,) fp32 tensor");
+  const c10::cuda::CUDAGuard device(q_.device());
+  const Tensor q = unit_inner(q_);
+  Tensor out = at::empty({B, heads, pool.hd}, q.options());
+  if (B == 0) return out;
+  const cudaStream_t stream = current_stream(q);
+  const Tensor ws = gemm_workspace(q.device(), stream);
+  const int64_t sq[2] = {step(q, 0), step(q, 1)}, so[2] = {heads * pool.hd, pool.hd};
+  int64_t sk[2] = {0, 0}, sv[2] = {0, 0};
+  if (key.defined())
+    for (int i = 0; i < 2; ++i) {
+      sk[i] = step(key, i);
+      sv[i] = step(value, i);
+    }
+  check(tfb_paged_attention_int4(q.data_ptr(), key.defined() ? key.data_ptr() : nullptr, value.defined() ? value.data_ptr() : nullptr,
+                                 out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), scales.data_ptr(), table.p, ints(lengths),
+                                 floats(slopes), (int)rounded, B, pool.heads, heads / pool.heads, pool.hd, pool.pages, pool.page,
+                                 table.width, table.ld, pool.strides, sq, sk, sv, so, ws.data_ptr(), ws.numel(),
+                                 dtype_code(q.scalar_type()), stream));
+  return out;
+}
+
+Stored cache_append_int4(const Tensor& k_pages, const Tensor& v_pages, const Tensor& scales, const Tensor& tables, const Tensor& lengths,
+                         const Tensor& key_, const Tensor& value_, const Tensor& counts, bool stored) {
+  check_plain("cache_append", {&k_pages, &v_pages, &scales, &tables, &lengths, &key_, &value_, &counts});
+  BodyGuard guard;
+  const Pool pool = pool_int4_of(k_pages, v_pages, scales);
+  TFB_ASSERT(key_.defined() && value_.defined() && key_.dim() == 4 && key_.sizes() == value_.sizes() &&
+                 key_.size(1) == pool.heads && key_.size(3) == pool.hd,
+             "keys and values are (batch, cache heads, T, head_dim) tensors");
+  TFB_ASSERT(key_.scalar_type() == scales.scalar_type() && value_.scalar_type() == scales.scalar_type(),
+             "keys and values have the scales' type");
+  const int64_t B = key_.size(0), T = key_.size(2);
+  const Table table = table_of(tables, B);
+  TFB_ASSERT(lengths.defined(), "lengths: expected a contiguous (batch,) int32 tensor");
+  check_per_sequence(lengths, B, "lengths");
+  check_per_sequence(counts, B, "counts");
+  const c10::cuda::CUDAGuard device(key_.device());
+  Stored out;
+  if (stored) {  // as a projection's output lies
+    out.key = at::empty({B, T, pool.heads, pool.hd}, key_.options()).transpose(1, 2);
+    out.value = at::empty({B, T, pool.heads, pool.hd}, key_.options()).transpose(1, 2);
+  }
+  if (B == 0 || T == 0) return out;
+  const Tensor key = unit_inner(key_), value = unit_inner(value_);
+  const int64_t sk[3] = {step(key, 0), step(key, 1), step(key, 2)}, sv[3] = {step(value, 0), step(value, 1), step(value, 2)};
+  const int64_t ss[3] = {T * pool.heads * pool.hd, pool.hd, pool.heads * pool.hd};
+  check(tfb_cache_append_int4(key.data_ptr(), value.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), scales.data_ptr(), table.p,
+                              ints(lengths), ints(counts), stored ? out.key.data_ptr() : nullptr,
+                              stored ? out.value.data_ptr() : nullptr, B, pool.heads, T, pool.hd, pool.pages, pool.page, table.width,
+                              table.ld, pool.strides, sk, sv, ss, dtype_code(key.scalar_type()), current_stream(key)));
+  return out;
+}
+
 // What a tensor map can describe: 16-byte aligned rows, no repetition; strides of dimensions of one entry made to fit.
 static bool mapped(const Tensor& t, int64_t (&s)[3]) {
   bool ok = t.stride(3) == 1 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;

@@ -196,6 +196,34 @@ TFB_PY(py_cache_append) {
     Py_RETURN_NONE;
   });
 }
+// q, k_pages, v_pages, scales, tables, lengths, key, value, slopes, rounded
+TFB_PY(py_paged_attention_int4) {
+  return guarded([&]() -> PyObject* {
+    refuse_tracing("paged_attention");
+    Args a(argv, argc, 10, "paged_attention");
+    const Tensor &q = a.tensor(), &k = a.tensor(), &v = a.tensor(), &scales = a.tensor(), &tables = a.tensor(), &lengths = a.tensor(),
+                 &key = a.tensor(), &value = a.tensor(), &slopes = a.tensor();
+    const int64_t rounded = a.integer();
+    return tensor_result([&] { return paged_attention_int4(q, k, v, scales, tables, lengths, key, value, slopes, rounded); });
+  });
+}
+// k_pages, v_pages, scales, tables, lengths, key, value, counts, stored -> (key, value), or None
+TFB_PY(py_cache_append_int4) {
+  return guarded([&]() -> PyObject* {
+    refuse_tracing("cache_append");
+    Args a(argv, argc, 9, "cache_append");
+    const Tensor &k = a.tensor(), &v = a.tensor(), &scales = a.tensor(), &tables = a.tensor(), &lengths = a.tensor(), &key = a.tensor(),
+                 &value = a.tensor(), &counts = a.tensor();
+    const bool wanted = a.truth();
+    Stored got;
+    {
+      pybind11::gil_scoped_release no_gil;
+      got = cache_append_int4(k, v, scales, tables, lengths, key, value, counts, wanted);
+    }
+    if (!wanted) Py_RETURN_NONE;
+    return Py_BuildValue("(NN)", THPVariable_Wrap(got.key), THPVariable_Wrap(got.value));
+  });
+}
 TFB_PY(py_prompt_mass) {  // q, k, lse, counts, slopes, rounded
   return guarded([&]() -> PyObject* {
     refuse_tracing("prompt_mass");
@@ -329,7 +357,7 @@ PyMethodDef methods[] = {TFB_METHOD(linear), TFB_METHOD(layernorm), TFB_METHOD(a
                          TFB_METHOD(cross_entropy), TFB_METHOD(lm_loss), TFB_METHOD(embedding), TFB_METHOD(layer),
                          TFB_METHOD(layer_and_activations),
                          TFB_METHOD(paged_attention), TFB_METHOD(cache_append), TFB_METHOD(prompt_mass), TFB_METHOD(cache_evict),
-                         TFB_METHOD(int4_quantize), TFB_METHOD(int4_expand), TFB_METHOD(int4_linear), TFB_METHOD(sample),
+                         TFB_METHOD(paged_attention_int4), TFB_METHOD(cache_append_int4), TFB_METHOD(int4_quantize), TFB_METHOD(int4_expand), TFB_METHOD(int4_linear), TFB_METHOD(sample),
                          TFB_METHOD(set_grad_mode), TFB_METHOD(take_written), TFB_METHOD(join_weight_grads),
                          TFB_METHOD(gemm_workspace), TFB_METHOD(reset_workspaces), TFB_METHOD(set_recorder), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Native host path of tritonformer_b200.", -1, methods,

@@ -8,7 +8,7 @@
 // subtracting; products of codes are exact and their sum over a group meets the scale in 32 bits, so no weight is rounded.
 // The warps of a block share the contraction and join their sums in shared memory, in their order: the result does not depend on
 // timing.  More rows than that go to the tensor cores of the library's own matrix product, on weights expanded to 16 bits.
-#include "common.cuh"
+#include "nibbles.cuh"
 
 namespace tfb {
 namespace {
@@ -28,46 +28,6 @@ struct Int4Params {
   int out_vec;  // rows of the output and the addend 4 bytes at a time
   int relu;
 };
-
-template <typename T> __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
-template <> __device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-template <>
-__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ uint32_t masked_or(uint32_t v, uint32_t mask, uint32_t bits) {  // (v & mask) | bits in one instruction
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(v), "r"(mask), "r"(bits));
-  return r;
-}
-
-// The four pairs of codes of a word, as exact 16-bit numbers: pair i is nibbles i and i + 4.
-template <typename T> __device__ __forceinline__ void expand(uint32_t w, uint32_t (&a)[4]);
-template <> __device__ __forceinline__ void expand<__half>(uint32_t w, uint32_t (&a)[4]) {
-  const __half2 off = __float2half2_rn(-1032.f), sixteenth = __float2half2_rn(0.0625f), off16 = __float2half2_rn(-72.f);
-#pragma unroll
-  for (int i = 0; i < 2; ++i, w >>= 8) {
-    const uint32_t lo = masked_or(w, 0x000f000fu, 0x64006400u), hi = masked_or(w, 0x00f000f0u, 0x64006400u);
-    const __half2 x = __hadd2(*reinterpret_cast<const __half2*>(&lo), off);
-    const __half2 y = __hfma2(*reinterpret_cast<const __half2*>(&hi), sixteenth, off16);
-    a[2 * i] = *reinterpret_cast<const uint32_t*>(&x);
-    a[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&y);
-  }
-}
-template <> __device__ __forceinline__ void expand<__nv_bfloat16>(uint32_t w, uint32_t (&a)[4]) {
-  const __nv_bfloat162 off = __float2bfloat162_rn(-136.f);
-#pragma unroll
-  for (int i = 0; i < 4; ++i, w >>= 4) {
-    const uint32_t v = masked_or(w, 0x000f000fu, 0x43004300u);
-    const __nv_bfloat162 x = __hadd2(*reinterpret_cast<const __nv_bfloat162*>(&v), off);
-    a[i] = *reinterpret_cast<const uint32_t*>(&x);
-  }
-}
 
 // Eight values of a row from column k on, zeros from column K on.
 __device__ __forceinline__ uint4 load_x8(const uint16_t* row, int k, int K, int vec) {
@@ -145,12 +105,12 @@ __global__ void __launch_bounds__(kMaxWarps * 32) int4_linear_kernel(const Int4P
             for (int e = 0; e < 4; ++e) part[t][e] = 0.f;
         }
         uint32_t a[4];
-        expand<T>(h ? now[s].z : now[s].x, a);
+        expand_nibbles<T>(h ? now[s].z : now[s].x, a);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) mma16816<T>(part[t], a, b[t][h].x, b[t][h].y);
-        expand<T>(h ? now[s].w : now[s].y, a);
+        for (int t = 0; t < NT; ++t) mma<T>(part[t], a, b[t][h].x, b[t][h].y);
+        expand_nibbles<T>(h ? now[s].w : now[s].y, a);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) mma16816<T>(part[t], a, b[t][h].z, b[t][h].w);
+        for (int t = 0; t < NT; ++t) mma<T>(part[t], a, b[t][h].z, b[t][h].w);
         if (SMALL || h == 1) {
           const float2 f = Num<T>::to_f2(*reinterpret_cast<const typename Num<T>::T2*>(&scale[s][SMALL ? h : 0]));
 #pragma unroll
@@ -223,8 +183,7 @@ __global__ void __launch_bounds__(256) int4_quantize_kernel(const T* __restrict_
     const int n = threadIdx.x % QC, part = threadIdx.x / QC, first = part / per * per;
     uint16_t top = 0;
     for (int q = 0; q < per; ++q) top = most[first + q][n] > top ? most[first + q][n] : top;
-    const float f = Num<T>::to_f(*reinterpret_cast<const T*>(&top));
-    const T s = Num<T>::from_f(isfinite(f) ? __fdiv_rn(f, 7.f) : NAN);
+    const T s = scale_of<T>(top);
     scale[part][n] = s;
     const int g = (k0 + part * 32) / group, column = n0 + n;
     if (part == first && g < groups && column < strips * 16)
@@ -239,9 +198,7 @@ __global__ void __launch_bounds__(256) int4_quantize_kernel(const T* __restrict_
     for (int e = 0; e < 8; ++e) {
       const int k = unit * kUnit + t / 2 * 32 + j * 8 + t % 2 * 4 + (e % 4 / 2) * 2 + e / 4, n = strip * 16 + e % 2 * 8 + r;
       const float s = Num<T>::to_f(scale[k / 32][n]);
-      int c = 0;
-      if (s > 0.f) c = max(-7, min(7, __float2int_rn(__fdiv_rn(Num<T>::to_f(*reinterpret_cast<const T*>(&tile[k][n])), s))));
-      v |= (uint32_t)(c + 8) << (4 * e);
+      v |= (uint32_t)(code_of(Num<T>::to_f(*reinterpret_cast<const T*>(&tile[k][n])), s) + 8) << (4 * e);
     }
     codes[(((int64_t)(n0 / 16 + strip) * units + k0 / kUnit + unit) * 128) + word] = v;
   }
@@ -264,8 +221,8 @@ __global__ void __launch_bounds__(256) int4_expand_kernel(const uint4* __restric
       const uint32_t s2 = scales[((int64_t)strip * groups + at) * 8 + r];
       const float2 f = Num<T>::to_f2(*reinterpret_cast<const typename Num<T>::T2*>(&s2));
       uint32_t a[2][4];
-      expand<T>(h ? w.z : w.x, a[0]);
-      expand<T>(h ? w.w : w.y, a[1]);
+      expand_nibbles<T>(h ? w.z : w.x, a[0]);
+      expand_nibbles<T>(h ? w.w : w.y, a[1]);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         float v[8];

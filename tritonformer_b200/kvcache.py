@@ -13,7 +13,9 @@ the position of its token (`positions`, int32), because a key that moves to anot
   * `cache_evict`       each head keeps `keep` keys: the recent ones, then those of the largest mass
 
 The query heads may be a multiple of the cache's heads (query head h uses key head h // group).  head_dim is 32, 64 or 128, the
-type fp16 or bf16.  `attn_bias` is None, the (heads,) ALiBi slopes, or the model's (heads, T, T) ALiBi table, from which only
+type fp16 or bf16.  A cache in 4 bits has pages of bytes, (pages, heads, page, head_dim / 2), and `scales` (pages, heads, page, 2) of the 16-bit
+type, one for each row of keys and one for its row of values: a value is a whole number from -7 to 7 times its row's scale (the row's largest
+magnitude over 7).  `paged_attention` and `cache_append` take either; nothing is evicted from a cache in 4 bits.  `attn_bias` is None, the (heads,) ALiBi slopes, or the model's (heads, T, T) ALiBi table, from which only
 the slopes and the rounding are taken.  None of these has a gradient.  A page id or a length that does not fit the cache reads
 and writes nothing out of bounds and shows in `_lib.check_status()`.
 """
@@ -23,6 +25,9 @@ from . import _host
 from .attention import _resolve_bias, attention_forward
 
 
+_NO_STATISTICS = "a cache in 4 bits has no masses and positions"
+
+
 def _slopes(attn_bias, heads):
     bias = _resolve_bias(attn_bias, heads, 0, getattr(attn_bias, "dtype", None))
     assert bias.table is None, "the cache takes ALiBi slopes or an ALiBi table, no other bias"
@@ -30,14 +35,18 @@ def _slopes(attn_bias, heads):
 
 
 def paged_attention(query, k_pages, v_pages, tables, lengths, key=None, value=None, attn_bias=None, query_positions=None,
-                    mass=None, positions=None, mass_out=None):
+                    mass=None, positions=None, mass_out=None, scales=None):
     """Attention of one query per sequence, (batch, heads, head_dim), over the lengths[b] keys in its pages; with `key` and
     `value` (batch, cache heads, head_dim) over those and the new key, which is written into slot lengths[b] (`lengths` itself
     stays).  A sequence without keys gets zeros.  With `mass` every key's weights, summed over the query heads of its head, are
     added to it, in place or into `mass_out` (no page may then be part of two sequences); the call then takes 4 bytes of scratch per
     query head and slot of the tables, whatever the lengths are.  With `positions` the new key's entry is set.  The query's
-    position is query_positions[b], or the number of the last slot."""
+    position is query_positions[b], or the number of the last slot.  With `scales` the cache is one in 4 bits, which has neither masses nor
+    positions; the new row is quantized and attended to as it is stored."""
     bias = _slopes(attn_bias, query.shape[1])
+    if scales is not None:
+        assert all(x is None for x in (query_positions, mass, positions, mass_out)), _NO_STATISTICS
+        return _host.paged_attention_int4(query, k_pages, v_pages, scales, tables, lengths, key, value, bias.slopes, int(bias.rounded))
     return _host.paged_attention(query, k_pages, v_pages, tables, lengths, key, value, bias.slopes, int(bias.rounded),
                                  query_positions, mass, positions, mass_out)
 
@@ -57,10 +66,16 @@ def prompt_mass(query, key, lse, counts=None, attn_bias=None):
 
 
 def cache_append(k_pages, v_pages, tables, lengths, key, value, counts=None, mass=None, positions=None, key_mass=None,
-                 first_positions=None):
+                 first_positions=None, scales=None, stored=False):
     """Writes the first counts[b] (None: all) of the keys and values (batch, cache heads, T, head_dim) into the slots from
     lengths[b] on (`lengths` itself stays).  `mass` gets `key_mass` (batch, cache heads, T), or zeros; `positions`
-    first_positions[b] + t, or the slots' numbers."""
+    first_positions[b] + t, or the slots' numbers.  With `scales` the cache is one in 4 bits, without masses and positions; with `stored` the call then
+    returns (keys, values) like those that were given, as the cache now has them (zeros behind the counts), so that a prompt's own attention
+    can see what later tokens will."""
+    if scales is not None:
+        assert all(x is None for x in (mass, positions, key_mass, first_positions)), _NO_STATISTICS
+        return _host.cache_append_int4(k_pages, v_pages, scales, tables, lengths, key, value, counts, bool(stored))
+    assert not stored, "stored: a cache in 16 bits has the keys and values that it is given"
     _host.cache_append(k_pages, v_pages, tables, lengths, key, value, counts, mass, positions, key_mass, first_positions)
 
 
@@ -78,20 +93,30 @@ def cache_evict(k_pages, v_pages, mass, positions, tables, lengths, keep, recent
 
 class PagedKVCache:
     """The pages of one layer and their statistics.  `statistics=False` leaves out what only eviction (and, where keys have been
-    evicted, ALiBi) needs."""
+    evicted, ALiBi) needs.  `bits=4`: keys and values in 4 bits, without statistics; `dtype` is that of queries and scales."""
 
-    def __init__(self, pages, heads, head_dim, page=64, dtype=torch.float16, device="cuda", statistics=True):
-        self.k = torch.zeros((pages, heads, page, head_dim), device=device, dtype=dtype)
+    def __init__(self, pages, heads, head_dim, page=64, dtype=torch.float16, device="cuda", statistics=True, bits=16):
+        assert bits in (4, 16), "a cache holds 16 or 4 bits"
+        assert bits == 16 or not statistics, _NO_STATISTICS
+        row, kind = (head_dim, dtype) if bits == 16 else (head_dim // 2, torch.uint8)
+        self.k = torch.zeros((pages, heads, page, row), device=device, dtype=kind)
         self.v = torch.zeros_like(self.k)
+        self.scales = torch.zeros((pages, heads, page, 2), device=device, dtype=dtype) if bits == 4 else None
         self.mass = torch.zeros((pages, heads, page), device=device) if statistics else None
         self.positions = torch.zeros((pages, heads, page), device=device, dtype=torch.int32) if statistics else None
 
     def attend(self, query, tables, lengths, key=None, value=None, attn_bias=None, query_positions=None):
+        if self.scales is not None:
+            return paged_attention(query, self.k, self.v, tables, lengths, key, value, attn_bias, query_positions, scales=self.scales)
         return paged_attention(query, self.k, self.v, tables, lengths, key, value, attn_bias, query_positions, self.mass,
                                self.positions)
 
-    def append(self, tables, lengths, key, value, counts=None, key_mass=None, first_positions=None):
+    def append(self, tables, lengths, key, value, counts=None, key_mass=None, first_positions=None, stored=False):
+        if self.scales is not None:
+            return cache_append(self.k, self.v, tables, lengths, key, value, counts, None, None, key_mass, first_positions, self.scales, stored)
+        assert not stored, "stored: a cache in 16 bits has the keys and values that it is given"
         cache_append(self.k, self.v, tables, lengths, key, value, counts, self.mass, self.positions, key_mass, first_positions)
 
     def evict(self, tables, lengths, keep, recent=0, next_positions=None):
+        assert self.scales is None, _NO_STATISTICS
         return cache_evict(self.k, self.v, self.mass, self.positions, tables, lengths, keep, recent, next_positions)
