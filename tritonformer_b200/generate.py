@@ -2,6 +2,7 @@
 
     gen = Generator(model, batch=8, max_tokens=2048)                  # or budget=512: at most 512 + 64 keys a head
     tokens = gen.generate(prompts, lengths, new_tokens=100)           # (8, 100), greedy
+    tokens = gen.generate(prompts, lengths, 100, temperature=0.8, top_k=40, top_p=0.95)   # drawn
     logits = gen.prefill(prompts, lengths); logits = gen.step(tokens) # or token by token
 
 The prompts' attention is the training forward; their keys and values (and with a budget their attention masses) go into the
@@ -13,13 +14,19 @@ the prompt and then every `interval` tokens.  The reference has no counterpart: 
 A model without ALiBi has a learned position for each token; with it, the slopes come from its table, also where the model was
 moved to bf16 after the table was made in fp16.  A captured step (`graph=True`) reads the weights where they were in memory;
 if they lie elsewhere when the next prompts come, it is captured again.  They must not move between a prompt and its steps.
+
+`weight_bits=4` packs the linear weights as they are at that moment (`pack_weights()` does so again, after more training); embeddings, norms and
+biases stay the model's own.  `cache_bits=4` holds keys and values in 4 bits; a prompt's own attention then works on them as they are stored, so
+that its logits are those of its tokens one by one.  Nothing is evicted from such a cache.
 """
 import torch
 
 from .attention import _Bias, _resolve_bias
 from .embedding import Embedding
 from .fused import LinearResidual, MLPResidual, QKVProjection
+from .int4 import linear_int4, quantize_int4
 from .kvcache import PagedKVCache, cache_append, cache_evict, prompt_attention, prompt_mass
+from .sampling import sample_tokens
 from .transformer import get_slopes
 
 
@@ -56,14 +63,18 @@ def _bias_of(table, heads):
 
 class Generator:
     """State of `batch` sequences on one model.  `max_tokens`: prompt and generated tokens of a sequence together.  All tensors are
-    made here, so steps can be captured in a CUDA graph (`graph=True`)."""
+    made here, so steps can be captured in a CUDA graph (`graph=True`).  `weight_bits` and `cache_bits` are 16 or 4; `weight_group`: rows of
+    a column that share a scale."""
 
-    def __init__(self, model, batch, max_tokens, page=64, budget=None, recent=None, interval=64, graph=False):
+    def __init__(self, model, batch, max_tokens, page=64, budget=None, recent=None, interval=64, graph=False, weight_bits=16,
+                 cache_bits=16, weight_group=64):
         config = model.config
         weight = model.embed_tokens.weight
         assert weight.is_cuda and weight.dtype in (torch.float16, torch.bfloat16), "Generator expects a CUDA fp16/bf16 model"
         assert max_tokens <= config.max_position_embeddings, "more tokens than the model has positions"
         assert budget is None or (budget >= 1 and interval >= 1), "the budget and the interval are at least 1"
+        assert weight_bits in (4, 16) and cache_bits in (4, 16), "weights and cache have 16 or 4 bits"
+        assert cache_bits == 16 or budget is None, "nothing is evicted from a cache in 4 bits"
         self.model, self.batch, self.max_tokens, self.page = model, batch, max_tokens, page
         self.heads = config.num_attention_heads
         self.head_dim = config.hidden_size // config.num_attention_heads
@@ -74,7 +85,7 @@ class Generator:
         device = weight.device
         # every sequence owns its pages, the same ones in every layer's pool
         self.tables = torch.arange(batch * self.width, dtype=torch.int32, device=device).view(batch, self.width)
-        self.caches = [PagedKVCache(batch * self.width, self.heads, self.head_dim, page, weight.dtype, device, budget is not None)
+        self.caches = [PagedKVCache(batch * self.width, self.heads, self.head_dim, page, weight.dtype, device, budget is not None, cache_bits)
                        for _ in model.layer_list]
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)  # keys in the cache
         self.next = torch.zeros(batch, dtype=torch.int32, device=device)     # position of the token that comes next
@@ -84,6 +95,23 @@ class Generator:
         self.want_graph, self.graph = graph, None
         self.weights = None  # where the captured step reads them
         self.bias = None, None, None  # the model's table, its version, and what _bias_of found
+        self.weight_group, self.packed, self.packed_head = weight_group, None, None
+        if weight_bits == 4:
+            self.pack_weights()
+
+    @torch.no_grad()
+    def pack_weights(self):
+        """Takes the model's linear weights as they are now, in 4 bits."""
+        def pack(*weights):
+            return quantize_int4(weights[0] if len(weights) == 1 else torch.cat(weights, 1), self.weight_group)
+
+        self.packed = {}
+        for layer in self.model.layer_list:
+            att, mlp = layer.attention, layer.mlp
+            self.packed[layer] = (pack(att.q_proj.weight, att.k_proj.weight, att.v_proj.weight), pack(att.out_proj.weight),
+                                  pack(mlp.dense_h_to_4h.weight), pack(mlp.dense_4h_to_h.weight))
+        self.packed_head = pack(self.model.logits_out.weight)
+        self.graph = None  # a captured step reads the weights that it was captured with
 
     def _bias(self):
         """The model's bias in the operators' form; a table that is new here is looked over, which waits for the host."""
@@ -98,6 +126,11 @@ class Generator:
         """One layer on (batch, tokens, hidden) without gradients; `attend` maps q, k, v to the context."""
         att, mlp = layer.attention, layer.mlp
         normed = layer.input_layernorm(x)
+        if self.packed is not None:
+            qkv, out, first, second = self.packed[layer]
+            x = linear_int4(attend(*linear_int4(normed, qkv).chunk(3, dim=-1)), out, addend=x)
+            hidden = linear_int4(layer.post_attention_layernorm(x), first, mlp.dense_h_to_4h.bias, relu=True)
+            return linear_int4(hidden, second, mlp.dense_4h_to_h.bias, addend=x)
         q, k, v = QKVProjection.apply(normed, att.q_proj.weight, att.k_proj.weight, att.v_proj.weight)
         x = LinearResidual.apply(attend(q, k, v), att.out_proj.weight, None, x)
         normed = layer.post_attention_layernorm(x)
@@ -139,6 +172,10 @@ class Generator:
 
             def attend(q, k, v):
                 q, k, v = (layer.attention._heads(y) for y in (q, k, v))
+                if cache.scales is not None:
+                    k, v = cache.append(tables, start, k, v, counts, stored=True)
+                    out, _ = prompt_attention(q, k, v, self._bias())
+                    return out.transpose(1, 2).reshape(b, padded, -1)
                 out, lse = prompt_attention(q, k, v, self._bias())
                 masses = prompt_mass(q, k, lse, counts, self._bias()) if self.budget is not None else None
                 into.append(tables, start, k, v, counts, masses)
@@ -160,11 +197,13 @@ class Generator:
         logits = self._logits(last)
         if bad is not None:  # once the work is done, because the matrix products stop while there is a report
             none = torch.zeros((b, self.heads, 1, self.head_dim), dtype=x.dtype, device=device)
-            cache_append(self.caches[0].k, self.caches[0].v, self.tables, start, none, none, torch.where(bad, -1, 0).to(torch.int32))
+            cache_append(self.caches[0].k, self.caches[0].v, self.tables, start, none, none, torch.where(bad, -1, 0).to(torch.int32),
+                         scales=self.caches[0].scales)
         return logits
 
     def _logits(self, x):
-        return self.model.logits_out(self.model.final_layernorm(x.unsqueeze(1))).squeeze(1)
+        x = self.model.final_layernorm(x.unsqueeze(1))
+        return (self.model.logits_out(x) if self.packed is None else linear_int4(x, self.packed_head)).squeeze(1)
 
     def _forward(self):
         model = self.model
@@ -174,7 +213,8 @@ class Generator:
 
             def attend(q, k, v):
                 q, k, v = (y.view(self.batch, self.heads, self.head_dim) for y in (q, k, v))
-                out = cache.attend(q, self.tables, self.lengths, k, v, self._bias(), self.next)
+                # without eviction a token's position is its slot
+                out = cache.attend(q, self.tables, self.lengths, k, v, self._bias(), self.next if cache.scales is None else None)
                 return out.view(self.batch, 1, -1)
 
             x = self._block(layer, x, attend)
@@ -235,12 +275,26 @@ class Generator:
             self._forward()
         self.weights = self._addresses()
 
-    def generate(self, prompts, lengths=None, new_tokens=1, choose=None):
-        """(batch, new_tokens) token ids that follow the prompts; `choose` maps logits to tokens (the largest by default)."""
-        choose = choose or (lambda logits: logits.argmax(-1))
+    def generate(self, prompts, lengths=None, new_tokens=1, choose=None, temperature=None, top_k=0, top_p=1.0, min_p=0.0,
+                 uniforms=None, generator=None):
+        """(batch, new_tokens) token ids that follow the prompts.  With a `temperature` they are drawn as `sample_tokens` does, from
+        `uniforms` (batch, new_tokens) in [0, 1) or else from numbers of `generator`; without one `choose` maps logits to tokens (the
+        largest by default)."""
+        if temperature is None:
+            plain = all(not isinstance(x, torch.Tensor) and x == y for x, y in ((top_k, 0), (top_p, 1.0), (min_p, 0.0)))
+            assert plain and uniforms is None and generator is None, "drawing tokens takes a temperature"
+            choose = choose or (lambda logits: logits.argmax(-1))
+        else:
+            assert choose is None, "tokens are drawn with a temperature, or chosen"
+            if uniforms is None:
+                uniforms = torch.rand((self.batch, new_tokens), device=self.tables.device, generator=generator)
+            assert uniforms.shape == (self.batch, new_tokens), "uniforms: one number for each sequence and token"
         logits, out = self.prefill(prompts, lengths), []
         for i in range(new_tokens):
-            out.append(choose(logits))
+            if temperature is None:
+                out.append(choose(logits))
+            else:
+                out.append(sample_tokens(logits, uniforms[:, i], temperature, top_k, top_p, min_p))
             if i + 1 < new_tokens:
                 logits = self.step(out[-1])
         return torch.stack(out, 1) if out else prompts[:, :0]
