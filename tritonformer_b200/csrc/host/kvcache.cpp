@@ -243,8 +243,9 @@ Stored cache_append_int4(const Tensor& k_pages, const Tensor& v_pages, const Ten
   const c10::cuda::CUDAGuard device(key_.device());
   Stored out;
   if (stored) {  // as a projection's output lies
-    out.key = at::empty({B, T, pool.heads, pool.hd}, key_.options()).transpose(1, 2);
-    out.value = at::empty({B, T, pool.heads, pool.hd}, key_.options()).transpose(1, 2);
+    const int64_t sizes[4] = {B, pool.heads, T, pool.hd}, strides[4] = {T * pool.heads * pool.hd, pool.hd, pool.heads * pool.hd, 1};
+    out.key = at::empty_strided(sizes, strides, key_.options());
+    out.value = at::empty_strided(sizes, strides, key_.options());
   }
   if (B == 0 || T == 0) return out;
   const Tensor key = unit_inner(key_), value = unit_inner(value_);

@@ -1,37 +1,43 @@
 // Products with weights held in 4 bits (sm_100a): y = act(x W + bias) + addend with W[k, n] = s[k / group, n] c[k, n], c a whole
 // number from -7 to 7 and s a 16-bit number.
 //
-// Single tokens and small batches are bound by reading W once, 4.25 bits a weight at groups of 64.  The packed layout is the
+// Single tokens and small batches would be bound by reading W once, 4.25 bits a weight at groups of 64.  The packed layout is the
 // operand layout of mma.sync m16n8k16: the 16 bytes that a lane loads are its share of 16 columns (along M) by 64 rows (along
 // the contraction), so that weights go from global memory to the instruction without shared memory, and 8 rows of x lie along N.
-// A nibble becomes a 16-bit number by being put below a power of two's exponent (1024 + c in fp16, 128 + c in bf16, exactly) and
-// subtracting; products of codes are exact and their sum over a group meets the scale in 32 bits, so no weight is rounded.
-// The warps of a block share the contraction and join their sums in shared memory, in their order: the result does not depend on
-// timing.  More rows than that go to the tensor cores of the library's own matrix product, on weights expanded to 16 bits.
+// Products of codes are exact and their sum over a group meets the scale in 32 bits, so no weight is rounded.
+// A warp has a strip of 16 columns and a stretch of the contraction; up to 8 warps of a block share a strip where there are few, and join their
+// sums in shared memory, in their order: the result does not depend on timing.  More rows go to the tensor cores of the library's own matrix
+// product, on weights expanded to 16 bits.
+//
+// What bounds it is the whole-number pipe: a word of 8 codes takes five of its instructions to become 16-bit numbers, at two cycles each, 70 cycles of
+// a scheduler for a unit (512 bytes) with all else, where a copy would take 12 SM cycles for it.  Measured in graphs, weights not in the L2, fp16:
+// 1 x 1024 x 1024 1.45 us; 1 x 4096 x 1024 3.9; 4 x 1024 x 50304 8.5 (27.7 MB, 3.3 TB/s); 24 x 2048 x 8192 in groups of 32 9.3; 16 x 4096 x 12288 12.7.
+// Two units in flight at a time for up to 8 rows and one for more, in 16 warps an SM at least, were the fastest of 1, 2 and 4 with 8 to 32 warps (4 units:
+// 11.5 us for the 50304 columns, one 11.4).  Rings in shared memory, filled by cp.async or bulk copies for a block or a warp, were slower
+// throughout (12 to 20 us for the 50304 columns): the copies hide, their bookkeeping is what the pipe has no room for.
 #include "nibbles.cuh"
 
 namespace tfb {
 namespace {
 
-constexpr int kUnit = 64;     // rows of a unit: what a lane's 16 bytes cover
-constexpr int kMaxWarps = 16;
+constexpr int kUnit = 64;  // rows of a unit: what a lane's 16 bytes cover
+constexpr int kWarps = 8;  // of a block
 
 struct Int4Params {
   const void* x;
-  const uint4* codes;   // (strips, units, 32)
+  const uint4* codes;      // (strips, units, 32)
   const uint32_t* scales;  // (strips, groups, 8): of columns r and r + 8
   const void *bias, *addend;
   void* out;
   int64_t x_ld, addend_ld, out_ld;
-  int M, K, N, units, groups, group_log2, strips;
-  int x_vec;    // rows of x can be read 16 bytes at a time
-  int out_vec;  // rows of the output and the addend 4 bytes at a time
+  int M, K, N, units, groups, strips;
+  int parts_log2;  // warps of a strip, which share the contraction
+  int x_vec;       // rows of x can be read 16 bytes at a time
   int relu;
 };
 
-// Eight values of a row from column k on, zeros from column K on.
-__device__ __forceinline__ uint4 load_x8(const uint16_t* row, int k, int K, int vec) {
-  if (vec && k + 8 <= K) return *reinterpret_cast<const uint4*>(row + k);
+// Eight values of a row of x from column k on, zeros from column K on.
+__device__ __forceinline__ uint4 load_x8(const uint16_t* row, int k, int K) {
   uint32_t v[4] = {0, 0, 0, 0};
 #pragma unroll
   for (int e = 0; e < 8; ++e)
@@ -39,111 +45,139 @@ __device__ __forceinline__ uint4 load_x8(const uint16_t* row, int k, int K, int 
   return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-// One block: S strips of 16 columns by NT * 8 rows of x; its warps take the units of the contraction in turn.
-// SMALL: groups of 32, two to a unit.
-template <typename T, int NT, int S, bool SMALL>
-__global__ void __launch_bounds__(kMaxWarps * 32) int4_linear_kernel(const Int4Params p) {
-  extern __shared__ float sums[];  // [warps][NT * 8][S * 16 + 1]
-  constexpr int LD = S * 16 + 1, GR = SMALL ? 2 : 1;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  const int r = lane >> 2, j = lane & 3;
-  const int strip0 = blockIdx.x * S, m0 = blockIdx.y * (NT * 8);
+// A warp: a strip of 16 columns, a stretch of its units, NT * 8 rows of x.  U units at a time: their loads are on their way together, the next
+// ones' beside the products.  Rows of x that there are none of repeat the last: a column of the product is a row of x, and theirs go nowhere.
+// GROUP_LOG2: 5, 6 or 7; groups of 32 are two to a unit, of 128 one for two.
+template <typename T, int NT, int GROUP_LOG2>
+__global__ void __launch_bounds__(kWarps * 32, 2) int4_linear_kernel(const Int4Params p) {
+  constexpr int U = NT == 1 ? 2 : 1, GR = GROUP_LOG2 == 5 ? 2 : 1;
+  __shared__ float sums[kWarps][NT * 8][17];  // of the warps that share a strip, columns padded by one
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, j = lane & 3;
+  const int m0 = blockIdx.y * (NT * 8), parts = 1 << p.parts_log2, part = warp & (parts - 1);
+  const int strip = (blockIdx.x << (3 - p.parts_log2)) + (warp >> p.parts_log2);
+  const int share = (p.units + parts - 1) >> p.parts_log2;
+  int u = part * share;
+  const int end = strip < p.strips ? min(u + share, p.units) : u;
+  const uint4* codes = p.codes + ((int64_t)min(strip, p.strips - 1) * p.units + u) * 32 + lane;
+  const uint32_t* scales = p.scales + (int64_t)min(strip, p.strips - 1) * p.groups * 8 + r;
+  if (u < end) asm volatile("prefetch.global.L2 [%0];" ::"l"(codes));
   grid_dependency_wait();
   allow_dependents();
 
-  float acc[S][NT][4];
+  const uint16_t* rows[NT];
 #pragma unroll
-  for (int s = 0; s < S; ++s)
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[s][t][e] = 0.f;
+  for (int t = 0; t < NT; ++t) rows[t] = static_cast<const uint16_t*>(p.x) + (int64_t)min(m0 + t * 8 + r, p.M - 1) * p.x_ld + 8 * j;
 
-  uint4 w[S];
-  uint32_t sc[S][GR];
-  auto load = [&](int u) {
+  float acc[NT][4];
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-      const int strip = min(strip0 + s, p.strips - 1);
-      w[s] = ld_stream16(p.codes + ((int64_t)strip * p.units + u) * 32 + lane);
+  for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int g = 0; g < GR; ++g) {
-        const int at = SMALL ? 2 * u + g : (u * kUnit) >> p.group_log2;
-        sc[s][g] = p.scales[((int64_t)strip * p.groups + at) * 8 + r];
+    for (int e = 0; e < 4; ++e) acc[t][e] = 0.f;
+  // a unit's products, added to acc; b: the lane's two chunks of each row
+  auto multiply = [&](const uint4& w, const uint32_t (&sc)[GR], const uint4 (&b)[NT][2]) {
+    float sum[GR][NT][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t a[2][4];
+      expand_nibbles<T>(h ? w.z : w.x, a[0]);
+      expand_nibbles<T>(h ? w.w : w.y, a[1]);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        if (GR == 2 || h == 0) mma_first<T>(sum[GR == 2 ? h : 0][t], a[0], b[t][h].x, b[t][h].y);
+        else mma<T>(sum[0][t], a[0], b[t][h].x, b[t][h].y);
+        mma<T>(sum[GR == 2 ? h : 0][t], a[1], b[t][h].z, b[t][h].w);
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < GR; ++g) {
+      const float2 f = Num<T>::to_f2(*reinterpret_cast<const typename Num<T>::T2*>(&sc[g]));
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        acc[t][0] = fmaf(f.x, sum[g][t][0], acc[t][0]);
+        acc[t][1] = fmaf(f.x, sum[g][t][1], acc[t][1]);
+        acc[t][2] = fmaf(f.y, sum[g][t][2], acc[t][2]);
+        acc[t][3] = fmaf(f.y, sum[g][t][3], acc[t][3]);
       }
     }
   };
-  int u = warp;
-  if (u < p.units) load(u);
-  for (; u < p.units; u += warps) {
-    uint4 b[NT][2];
+  auto load_scales = [&](int unit, uint32_t (&sc)[GR]) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int m = m0 + t * 8 + r;
-      const uint16_t* row = static_cast<const uint16_t*>(p.x) + (int64_t)m * p.x_ld;
+    for (int g = 0; g < GR; ++g) sc[g] = scales[(GROUP_LOG2 == 5 ? 2 * unit + g : GROUP_LOG2 == 6 ? unit : unit >> 1) * 8];
+  };
+  uint4 w[U];
+  uint32_t sc[U][GR];
+  auto load = [&]() {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) b[t][h] = m < p.M ? load_x8(row, u * kUnit + 32 * h + 8 * j, p.K, p.x_vec) : make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < U; ++i) {
+      w[i] = ld_stream16(codes + i * 32);
+      load_scales(u + i, sc[i]);
     }
-    uint4 now[S];
-    uint32_t scale[S][GR];
+  };
+  const int quick = p.x_vec ? min(end, p.K / kUnit) : u;  // units whose rows of x are whole vectors
+  if (u + U <= quick) load();
+#pragma unroll 1
+  while (u + U <= quick) {
+    uint4 now[U], b[U][NT][2];
+    uint32_t sn[U][GR];
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-      now[s] = w[s];
+    for (int i = 0; i < U; ++i) {
+      now[i] = w[i];
 #pragma unroll
-      for (int g = 0; g < GR; ++g) scale[s][g] = sc[s][g];
+      for (int g = 0; g < GR; ++g) sn[i][g] = sc[i][g];
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) b[i][t][h] = *reinterpret_cast<const uint4*>(rows[t] + (u + i) * kUnit + h * 32);
     }
-    if (u + warps < p.units) load(u + warps);
+    u += U;
+    codes += U * 32;
+    if (u + U <= quick) load();
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-      float part[NT][4];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (SMALL || h == 0) {
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) part[t][e] = 0.f;
-        }
-        uint32_t a[4];
-        expand_nibbles<T>(h ? now[s].z : now[s].x, a);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) mma<T>(part[t], a, b[t][h].x, b[t][h].y);
-        expand_nibbles<T>(h ? now[s].w : now[s].y, a);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) mma<T>(part[t], a, b[t][h].z, b[t][h].w);
-        if (SMALL || h == 1) {
-          const float2 f = Num<T>::to_f2(*reinterpret_cast<const typename Num<T>::T2*>(&scale[s][SMALL ? h : 0]));
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            acc[s][t][0] = fmaf(f.x, part[t][0], acc[s][t][0]);
-            acc[s][t][1] = fmaf(f.x, part[t][1], acc[s][t][1]);
-            acc[s][t][2] = fmaf(f.y, part[t][2], acc[s][t][2]);
-            acc[s][t][3] = fmaf(f.y, part[t][3], acc[s][t][3]);
-          }
-        }
-      }
-    }
+    for (int i = 0; i < U; ++i) multiply(now[i], sn[i], b[i]);
   }
-  float* mine = sums + warp * (NT * 8) * LD;
-#pragma unroll
-  for (int s = 0; s < S; ++s)
+  for (; u < end; ++u, codes += 32) {
+    uint4 b[NT][2];
+    uint32_t sn[GR];
+    load_scales(u, sn);
+    const uint4 now = ld_stream16(codes);
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) mine[(t * 8 + 2 * j + (e & 1)) * LD + s * 16 + r + 8 * (e >> 1)] = acc[s][t][e];
-  __syncthreads();
+      for (int h = 0; h < 2; ++h) {
+        const int k = u * kUnit + h * 32;
+        b[t][h] = p.x_vec && k + 8 * j + 8 <= p.K ? *reinterpret_cast<const uint4*>(rows[t] + k) : load_x8(rows[t], k, p.K - 8 * j);
+      }
+    multiply(now, sn, b);
+  }
+
   const T* bias = static_cast<const T*>(p.bias);
   const T* addend = static_cast<const T*>(p.addend);
   T* out = static_cast<T*>(p.out);
-  for (int i = threadIdx.x; i < NT * 8 * S * 16; i += blockDim.x) {
-    const int m = i / (S * 16), c = i % (S * 16), n = strip0 * 16 + c;
-    if (m0 + m >= p.M || n >= p.N) continue;
-    float v = 0.f;
-    for (int k = 0; k < warps; ++k) v += sums[(k * NT * 8 + m) * LD + c];
+  auto finish = [&](float v, int m, int n) {
+    if (m >= p.M || n >= p.N) return;
     if (bias) v += Num<T>::to_f(bias[n]);
     if (p.relu) v = v < 0.f ? 0.f : v;  // NaN stays
-    if (addend) v += Num<T>::to_f(addend[(int64_t)(m0 + m) * p.addend_ld + n]);
-    out[(int64_t)(m0 + m) * p.out_ld + n] = Num<T>::from_f(v);
+    if (addend) v += Num<T>::to_f(addend[(int64_t)m * p.addend_ld + n]);
+    out[(int64_t)m * p.out_ld + n] = Num<T>::from_f(v);
+  };
+  if (parts == 1) {
+    if (strip < p.strips)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) finish(acc[t][e], m0 + t * 8 + 2 * j + (e & 1), strip * 16 + r + 8 * (e >> 1));
+    return;
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sums[warp][t * 8 + 2 * j + (e & 1)][r + 8 * (e >> 1)] = acc[t][e];
+  __syncthreads();
+  for (int i = threadIdx.x; i < (NT * 128) << (3 - p.parts_log2); i += kWarps * 32) {
+    const int s = i / (NT * 128), m = i / 16 % (NT * 8), n = i % 16;
+    float v = 0.f;
+    for (int k = 0; k < parts; ++k) v += sums[(s << p.parts_log2) + k][m][n];
+    finish(v, m0 + m, ((blockIdx.x << (3 - p.parts_log2)) + s) * 16 + n);
   }
 }
 
@@ -240,29 +274,23 @@ __global__ void __launch_bounds__(256) int4_expand_kernel(const uint4* __restric
   }
 }
 
-template <typename T, int NT, int S>
-int int4_launch(const Int4Params& p, int warps, cudaStream_t st) {
-  const dim3 grid((unsigned)ceil_div(p.strips, S), (unsigned)ceil_div(p.M, NT * 8));
-  const size_t smem = (size_t)warps * NT * 8 * (S * 16 + 1) * 4;
-  const auto kernel = p.group_log2 == 5 ? int4_linear_kernel<T, NT, S, true> : int4_linear_kernel<T, NT, S, false>;
-  launch_overlapped(kernel, grid, dim3(warps * 32), smem, st, p);
+template <typename T, int NT>
+int int4_launch(Int4Params p, int group, cudaStream_t st) {
+  const int64_t row_tiles = ceil_div(p.M, NT * 8);
+  // warps of a strip: as many as there are SMs for (12 warps each; with 24 the 50304 columns take 9.8 us instead of 8.5), with a unit each at least
+  p.parts_log2 = 0;
+  while (p.parts_log2 < 3 && (2 << p.parts_log2) <= p.units && ((int64_t)p.strips * row_tiles << p.parts_log2) < sm_count() * 12) ++p.parts_log2;
+  const dim3 grid((unsigned)ceil_div(p.strips, kWarps >> p.parts_log2), (unsigned)row_tiles);
+  const auto kernel = group == 32   ? int4_linear_kernel<T, NT, 5>
+                      : group == 64 ? int4_linear_kernel<T, NT, 6>
+                                    : int4_linear_kernel<T, NT, 7>;
+  launch_overlapped(kernel, grid, dim3(kWarps * 32), 0, st, p);
   return launched("int4_linear");
 }
 
 template <typename T>
-int int4_dispatch(const Int4Params& p, cudaStream_t st) {
-  const int nt = p.M <= 8 ? 1 : p.M <= 16 ? 2 : p.M <= 32 ? 4 : 8;
-  // strips of a warp: more share their loads of x, as long as there are blocks for all SMs
-  int s = nt == 1 ? 4 : nt == 2 ? 2 : 1;
-  while (s > 1 && ceil_div(p.strips, s) < 2 * sm_count()) s /= 2;
-  const int64_t blocks = ceil_div(p.strips, s) * ceil_div(p.M, nt * 8);
-  int warps = 1;
-  while (warps < kMaxWarps && warps * 2 <= p.units && blocks * warps < sm_count() * 16) warps *= 2;
-  while (warps > 1 && (size_t)warps * nt * 8 * (s * 16 + 1) * 4 > 48 * 1024) warps /= 2;
-  if (nt == 1) return s == 4 ? int4_launch<T, 1, 4>(p, warps, st) : s == 2 ? int4_launch<T, 1, 2>(p, warps, st) : int4_launch<T, 1, 1>(p, warps, st);
-  if (nt == 2) return s == 2 ? int4_launch<T, 2, 2>(p, warps, st) : int4_launch<T, 2, 1>(p, warps, st);
-  if (nt == 4) return int4_launch<T, 4, 1>(p, warps, st);
-  return int4_launch<T, 8, 1>(p, warps, st);
+int int4_dispatch(const Int4Params& p, int group, cudaStream_t st) {
+  return p.M <= 8 ? int4_launch<T, 1>(p, group, st) : p.M <= 16 ? int4_launch<T, 2>(p, group, st) : int4_launch<T, 4>(p, group, st);
 }
 
 int check_int4(const char* what, int64_t K, int64_t N, int group) {
@@ -314,10 +342,10 @@ extern "C" int tfb_int4_linear(const void* x, int64_t x_ld, const void* codes, c
                                int64_t addend_ld, void* out, int64_t out_ld, int64_t M, int64_t K, int64_t N, int group, int relu,
                                int dtype, void* stream) {
   if (int rc = check_int4("int4_linear", K, N, group)) return rc;
-  TFB_REQUIRE(M >= 0 && M <= 64 * 65535, "int4_linear: bad row count");
+  TFB_REQUIRE(M >= 0 && M <= 32 * 65535, "int4_linear: bad row count");
   if (M == 0) return TFB_OK;
   TFB_REQUIRE(x && codes && scales && out && aligned16(codes) && aligned16(scales), "int4_linear: the weights are not 16-byte aligned");
-  TFB_REQUIRE((M == 1 || x_ld >= 0) && out_ld >= N, "int4_linear: row stride smaller than the row");
+  TFB_REQUIRE((M == 1 || (x_ld >= 0 && x_ld < (1LL << 40))) && out_ld >= N, "int4_linear: row stride smaller than the row");
   Int4Params p = {};
   p.x = x;
   p.codes = static_cast<const uint4*>(codes);
@@ -333,9 +361,8 @@ extern "C" int tfb_int4_linear(const void* x, int64_t x_ld, const void* codes, c
   p.N = (int)N;
   p.units = (int)ceil_div(K, kUnit);
   p.groups = (int)int4_groups(K, group);
-  p.group_log2 = group == 32 ? 5 : group == 64 ? 6 : 7;
   p.strips = (int)ceil_div(N, 16);
   p.x_vec = aligned16(x) && (M == 1 || x_ld % 8 == 0);
   p.relu = relu;
-  TFB_DISPATCH_16(dtype, T, { return int4_dispatch<T>(p, (cudaStream_t)stream); })
+  TFB_DISPATCH_16(dtype, T, { return int4_dispatch<T>(p, group, (cudaStream_t)stream); })
 }

@@ -25,10 +25,10 @@ constexpr int A4_ROWS = 64;  // rows of a block
 
 // What codes stand for, rounded to the type.
 template <typename T>
-__device__ __forceinline__ uint4 restore8(uint32_t word, float scale) {
+__device__ __forceinline__ uint4 restore8(const float (&whole)[8], float scale) {
   float x[8];
 #pragma unroll
-  for (int d = 0; d < 8; ++d) x[d] = (float)((int)(word >> (4 * (d / 2) + 16 * (d % 2)) & 15) - 8) * scale;
+  for (int d = 0; d < 8; ++d) x[d] = whole[d] * scale;
   return pack8<T>(x);
 }
 
@@ -47,7 +47,7 @@ __device__ __forceinline__ uint4 load_row8(const T* p, bool vec) {
 // One block: A4_ROWS rows of a (sequence, key head); neighbouring blocks take neighbouring heads, which lie side by side in a
 // projection's output.
 template <typename T, int HD, bool VEC>
-__global__ void __launch_bounds__(256) append_int4_kernel(const Append4Params p) {
+__global__ void __launch_bounds__(256, 4) append_int4_kernel(const Append4Params p) {
   constexpr int LANES = HD / 8, PER = 256 / LANES, N = A4_ROWS / PER;
   __shared__ int sh_page[A4_ROWS], sh_row[A4_ROWS];
   grid_dependency_wait();
@@ -59,7 +59,15 @@ __global__ void __launch_bounds__(256) append_int4_kernel(const Append4Params p)
   const int t0 = blockIdx.y * A4_ROWS;
   if (blockIdx.y == 0 && h == 0 && threadIdx.x == 0 && (len < 0 || want < 0 || want > p.T || (int64_t)len + want > cap))
     atomicCAS(&g_dev_status, 0, kBadLength);
-  if (t0 >= count && !p.k_stored) return;
+  if (t0 >= count) {  // nothing to write but zeros behind the sequence's keys
+    if (p.k_stored)
+      for (int r = threadIdx.x / LANES; r < A4_ROWS && t0 + r < p.T; r += PER) {
+        const int64_t o = b * p.s_b + h * p.s_h + (t0 + r) * p.s_t + threadIdx.x % LANES * 8;
+        st_stream16(static_cast<T*>(p.k_stored) + o, make_uint4(0, 0, 0, 0));
+        st_stream16(static_cast<T*>(p.v_stored) + o, make_uint4(0, 0, 0, 0));
+      }
+    return;
+  }
   if (threadIdx.x < A4_ROWS) {
     int page = -1, row = 0;
     const int t = t0 + threadIdx.x;
@@ -85,7 +93,8 @@ __global__ void __launch_bounds__(256) append_int4_kernel(const Append4Params p)
   for (int i = 0; i < N; ++i) {
     const int r = i * PER + threadIdx.x / LANES, t = t0 + r;
     T ks, vs;
-    const uint32_t kw = quantize8<T, LANES>(kr[i], ks), vw = quantize8<T, LANES>(vr[i], vs);
+    float kc[8], vc[8];
+    const uint32_t kw = quantize8<T, LANES>(kr[i], ks, kc), vw = quantize8<T, LANES>(vr[i], vs, vc);
     if (sh_page[r] >= 0) {
       const int64_t o = row_offset(p.map, sh_page[r], h, sh_row[r]) + c * 4;
       *reinterpret_cast<uint32_t*>(p.k + o) = kw;
@@ -94,10 +103,10 @@ __global__ void __launch_bounds__(256) append_int4_kernel(const Append4Params p)
         p.scales[stat_offset(p.map, sh_page[r], p.kv_heads, h, sh_row[r])] =
             *reinterpret_cast<const uint16_t*>(&ks) | (uint32_t)*reinterpret_cast<const uint16_t*>(&vs) << 16;
     }
-    if (p.k_stored && t < p.T) {  // zeros behind the sequence's keys
+    if (p.k_stored && t < p.T) {
       const int64_t o = b * p.s_b + h * p.s_h + t * p.s_t + c * 8;
-      st_stream16(static_cast<T*>(p.k_stored) + o, restore8<T>(kw, t < count ? Num<T>::to_f(ks) : 0.f));
-      st_stream16(static_cast<T*>(p.v_stored) + o, restore8<T>(vw, t < count ? Num<T>::to_f(vs) : 0.f));
+      st_stream16(static_cast<T*>(p.k_stored) + o, restore8<T>(kc, Num<T>::to_f(ks)));
+      st_stream16(static_cast<T*>(p.v_stored) + o, restore8<T>(vc, Num<T>::to_f(vs)));
     }
   }
 }

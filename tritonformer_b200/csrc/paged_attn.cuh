@@ -590,7 +590,8 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
         if (cu.keys.fresh >= 0 && kk < C::KEYS) {
           const int kv = cu.hr / p.row_tiles, c = lane % (HD / 8);
           T scale;
-          const uint32_t word = quantize8<T, HD / 8>(now.fresh, scale);
+          float whole[8];
+          const uint32_t word = quantize8<T, HD / 8>(now.fresh, scale, whole);
           const uint32_t mine = *reinterpret_cast<const uint16_t*>(&scale);
           const uint32_t pair = __shfl_sync(0xffffffffu, mine, 0) | __shfl_sync(0xffffffffu, mine, HD / 8) << 16;
           if (lane < HD / 4)
