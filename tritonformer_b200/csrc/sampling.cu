@@ -519,25 +519,467 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams p
   if (lane == 0) p.out[row] = token;
 }
 
+// ---------------------------------------------------------------------------------------------------------- 16 bits
+// Logits of 16 bits have 2^16 values, and equal logits weigh the same: a histogram over all values is all that the cut needs.  Blocks count their
+// part of the row (a counter of 16 bits for each value, 128 KB of shared memory), the blocks of a cluster add theirs up where there is
+// something to add, and a scan over rows of 64 values gives the cut, with an exponential for each value that occurs instead of each logit.
+// Then the weights of what is kept are summed in the order of the columns.
 namespace {
 
+constexpr int H_THREADS = 1024, H_WARPS = 32, H_ROWS = 1024;  // rows of 64 values, two to a word
+constexpr int H_UNITS = 8;                                    // 16-byte units of a lane
+constexpr int kMostCounted = H_THREADS * H_UNITS * 8 - 8;     // logits of a block: a counter holds as many
+
+// Values in descending order: bin 0 is the last positive NaN, then infinity, .., the lowest, -infinity and the negative NaNs.
+template <typename T> struct Bins;
+template <> struct Bins<__half> { static constexpr int kTop = 0x03ff, kEnd = 0xfc00; };         // of infinity, of -infinity
+template <> struct Bins<__nv_bfloat16> { static constexpr int kTop = 0x007f, kEnd = 0xff80; };
+// the two bins of a word of logits; -0 has 0's
+template <typename T> __device__ __forceinline__ uint32_t bins_of(uint32_t word) {
+  using T2 = typename Num<T>::T2;
+  const T2 v = __hadd2(*reinterpret_cast<const T2*>(&word), Num<T>::from_f2(0.f, 0.f));
+  const uint32_t u = *reinterpret_cast<const uint32_t*>(&v);
+  return u ^ (0x7fff7fffu - ((u >> 15) & 0x00010001u) * 0x7fffu);
+}
+template <typename T> __device__ __forceinline__ float value_of(int bin) {
+  const uint16_t u = (uint16_t)(bin & 0x8000 ? bin : bin ^ 0x7fff);
+  return Num<T>::to_f(*reinterpret_cast<const T*>(&u));
+}
+
+struct HistShared {
+  uint32_t rows[H_WARPS];  // bit i of word w: row 32 i + w has logits
+  int counts[H_ROWS];      // of the whole row of logits
+  double weights[H_ROWS];
+  int warp_counts[H_WARPS];
+  double warp_weights[H_WARPS];
+  int found, cut, ties;
+  double before, sum;
+  double all_sums[SM_CLUSTER * H_WARPS];
+  int all_ties[SM_CLUSTER * H_WARPS];
+};
+
+}  // namespace
+
 template <typename T>
-int sample_launch(SampleParams p, int64_t B, cudaStream_t st) {
-  constexpr int W = kPerUnit<T>;
-  const int64_t row_units = ceil_div((int64_t)p.vocab + W - 1, W);
-  // blocks of a row: what the SMs have room for, and as many as its logits need
-  int blocks = 1;
-  while (blocks < SM_CLUSTER && (B * blocks < sm_count() || ceil_div(row_units, (int64_t)SM_WARPS * blocks) * SM_WARPS * 16 > 104 * 1024) &&
-         row_units > (int64_t)SM_THREADS * blocks)
-    blocks *= 2;
-  p.warp_units = (int)ceil_div(row_units, (int64_t)SM_WARPS * blocks);
-  const int64_t smem = (int64_t)p.warp_units * SM_WARPS * 16;
-  if (smem > 212 * 1024) return fail(TFB_ERR_UNSUPPORTED, "sample: %d logits in a row are more than a cluster has room for", p.vocab);
-  static std::atomic<uint64_t> done{0};
-  if (int rc = ensure_dynamic_smem(sample_kernel<T>, 212 * 1024, done, "sample")) return rc;
+__global__ void __launch_bounds__(H_THREADS, 1) sample_hist_kernel(const SampleParams p) {
+  constexpr int W = 8;
+  extern __shared__ uint4 smem_units[];
+  uint32_t* hist = reinterpret_cast<uint32_t*>(smem_units);
+  __shared__ HistShared sh;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t row = blockIdx.x / blocks;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) smem_units[i * H_THREADS + tid] = make_uint4(0, 0, 0, 0);
+  sh.counts[tid] = 0;
+  sh.weights[tid] = 0.0;
+  if (tid == 0) sh.found = H_ROWS;
+  const double table = exp2(lane / 32.0);
+  auto sync = [&]() {
+    if (blocks == 1) __syncthreads();
+    else cluster.sync();
+  };
+  grid_dependency_wait();
+  allow_dependents();
+
+  // ---- the warp's part of the row, counted
+  const T* logits = static_cast<const T*>(p.logits) + row * p.ld;
+  const int shift = (int)((reinterpret_cast<uintptr_t>(logits) & 15) / sizeof(T));
+  const uint4* source = reinterpret_cast<const uint4*>(logits - shift);
+  const int row_units = (p.vocab + shift + W - 1) / W;
+  const int first = (rank * H_WARPS + warp) * p.warp_units;
+  const int mine = max(0, min(p.warp_units, row_units - first));  // of these units there are
+  uint4 v[H_UNITS];
+#pragma unroll
+  for (int i = 0; i < H_UNITS; ++i) {
+    const T none = Num<T>::from_f(-INFINITY);
+    const uint32_t nones = *reinterpret_cast<const uint16_t*>(&none) * 0x10001u;
+    v[i] = make_uint4(nones, nones, nones, nones);
+    if (i * 32 + lane < mine) v[i] = __ldg(source + first + i * 32 + lane);
+  }
+  float t = p.temperature ? p.temperature[row] : p.temperature_all;
+  float top_p = p.top_p ? p.top_p[row] : p.top_p_all, min_p = p.min_p ? p.min_p[row] : p.min_p_all;
+  int k = p.top_k ? p.top_k[row] : p.top_k_all;
+  float u = p.uniforms[row];
+  if (!(t > 0.f) || top_p <= 0.f) {
+    k = 1;
+    t = 1.f;
+  }
+  if (k <= 0 || k >= p.vocab) k = 0;
+  const bool nucleus = top_p < 1.f && k != 1;
+  if (!(min_p > 0.f)) min_p = 0.f;
+  min_p = fminf(min_p, 1.f);
+  u = !(u > 0.f) ? 0.f : fminf(u, 0.99999994f);
+  const double per = kLog2eD / (double)t;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < H_UNITS; ++i) {
+    const int at = first + i * 32 + lane;
+    if (i * 32 + lane < mine) {
+      const uint32_t words[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+      const bool edge = at == 0 || at == row_units - 1;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint32_t b = bins_of<T>(words[q]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t bin = e ? b >> 16 : b & 0xffffu;
+          const int c = at * W + 2 * q + e - shift;
+          if (bin < Bins<T>::kEnd && (!edge || (c >= 0 && c < p.vocab))) atomicAdd(hist + (bin >> 1), 1u << (16 * (bin & 1)));
+        }
+      }
+    }
+  }
+  __syncthreads();
+  {
+    uint32_t bits = 0;
+    for (int i = 0; i < 32; ++i) {
+      const int r = i * 32 + warp;
+      uint32_t word = hist[r * 32 + lane];
+      if (r <= Bins<T>::kTop / 64 && word != 0) {  // NaNs
+        const int b = r * 64 + 2 * lane;
+        word &= (b < Bins<T>::kTop ? 0u : 0xffffu) | (b + 1 < Bins<T>::kTop ? 0u : 0xffff0000u);
+        hist[r * 32 + lane] = word;
+      }
+      bits |= (uint32_t)(__any_sync(0xffffffffu, word != 0) != 0) << i;
+    }
+    if (lane == 0) sh.rows[warp] = bits;
+  }
+  sync();
+  // counts of a row's two bins of a lane, over the cluster
+  auto counts_of = [&](int r, int (&c)[2]) {
+    c[0] = c[1] = 0;
+    for (int b = 0; b < blocks; ++b) {
+      const uint32_t word = cluster.map_shared_rank(hist, b)[r * 32 + lane];
+      c[0] += word & 0xffffu;
+      c[1] += word >> 16;
+    }
+  };
+  uint32_t set = 0;  // of word `lane`
+  for (int b = 0; b < blocks; ++b) set |= cluster.map_shared_rank(&sh, b)->rows[lane];
+  const int top_row = __reduce_min_sync(0xffffffffu, set ? (__ffs(set) - 1) * 32 + lane : H_ROWS);
+  if (top_row == H_ROWS) {  // nothing is allowed
+    if (rank == 0 && tid == 0) p.out[row] = -1;
+    if (blocks > 1) cluster.sync();
+    return;
+  }
+  int c[2];
+  counts_of(top_row, c);
+  const int top_lane = __ffs(__ballot_sync(0xffffffffu, (c[0] | c[1]) != 0)) - 1;
+  const int top_bin = top_row * 64 + 2 * top_lane + (__shfl_sync(0xffffffffu, c[0], top_lane) == 0);
+  const float top = value_of<T>(top_bin);
+  const double peak = (double)top;
+  auto weigh = [&](float x) {  // all lanes
+    const double w = weight_of(((double)x - peak) * per, table);
+    return x == top ? 1.0 : w;
+  };
+
+  // ---- counts and weights of the rows, each from one warp of the cluster to all blocks
+  uint32_t todo = __shfl_sync(0xffffffffu, set, warp);
+  while (todo != 0) {
+    const int i = __ffs(todo) - 1, r = i * 32 + warp;
+    todo &= todo - 1;
+    if ((i & (blocks - 1)) != rank) continue;
+    counts_of(r, c);
+    const double w0 = weigh(value_of<T>(r * 64 + 2 * lane)), w1 = weigh(value_of<T>(r * 64 + 2 * lane + 1));
+    const double sum = sum_lanes((c[0] ? c[0] * w0 : 0.0) + (c[1] ? c[1] * w1 : 0.0), 16);
+    const int n = __reduce_add_sync(0xffffffffu, c[0] + c[1]);
+    if (lane < blocks) {
+      HistShared* to = cluster.map_shared_rank(&sh, lane);
+      to->counts[r] = n;
+      to->weights[r] = sum;
+    }
+  }
+  sync();
+
+  // ---- their sums up to each row, thread by thread
+  int upto = sh.counts[tid];
+  double mass = sh.weights[tid];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int n = __shfl_up_sync(0xffffffffu, upto, o);
+    const double w = __shfl_up_sync(0xffffffffu, mass, o);
+    if (lane >= o) {
+      upto += n;
+      mass += w;
+    }
+  }
+  if (lane == 31) {
+    sh.warp_counts[warp] = upto;
+    sh.warp_weights[warp] = mass;
+  }
+  __syncthreads();
+  int all_upto = sh.warp_counts[lane];
+  double all_mass = sh.warp_weights[lane];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int n = __shfl_up_sync(0xffffffffu, all_upto, o);
+    const double w = __shfl_up_sync(0xffffffffu, all_mass, o);
+    if (lane >= o) {
+      all_upto += n;
+      all_mass += w;
+    }
+  }
+  const int finite = __shfl_sync(0xffffffffu, all_upto, 31);
+  double sum = __shfl_sync(0xffffffffu, all_mass, 31);
+  if (warp > 0) {
+    upto += __shfl_sync(0xffffffffu, all_upto, warp - 1);
+    mass += __shfl_sync(0xffffffffu, all_mass, warp - 1);
+  }
+  // The first row whose sums reach a goal, and what lies before it; a warp looks at its bins.
+  auto find_row = [&](bool reached, double before) {
+    const unsigned ones = __ballot_sync(0xffffffffu, reached);
+    if (ones && lane == __ffs(ones) - 1) atomicMin(&sh.found, tid);
+    __syncthreads();
+    const int r = sh.found;
+    if (tid == r) sh.before = before;
+    __syncthreads();
+    return r;
+  };
+  int cut = Bins<T>::kEnd, ties = 0;  // all bins before `cut` are kept, and of it so many
+  if (k == 1) {
+    cut = top_bin;
+    ties = 1;
+  } else if (k > 0 && k < finite) {
+    const int n = sh.counts[tid];
+    const int r = find_row(upto >= k, mass - sh.weights[tid]);
+    if (tid == r) sh.ties = k - (upto - n);  // wanted of the row
+    __syncthreads();
+    if (warp == 0) {
+      counts_of(r, c);
+      int lanes = c[0] + c[1];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v_ = __shfl_up_sync(0xffffffffu, lanes, o);
+        if (lane >= o) lanes += v_;
+      }
+      const int want = sh.ties, who = __ffs(__ballot_sync(0xffffffffu, lanes >= want)) - 1;
+      const double w0 = weigh(value_of<T>(r * 64 + 2 * lane)), w1 = weigh(value_of<T>(r * 64 + 2 * lane + 1));
+      const int ahead = lanes - c[0] - c[1];  // of the row before this lane's
+      const bool second = want > ahead + c[0];
+      const int left = want - ahead - (second ? c[0] : 0);
+      double part = lane < who ? (c[0] ? c[0] * w0 : 0.0) + (c[1] ? c[1] * w1 : 0.0)
+                    : lane == who ? (second ? (c[0] ? c[0] * w0 : 0.0) + left * w1 : left * w0) : 0.0;
+      part = sum_lanes(part, 16);
+      if (lane == who) {
+        sh.cut = r * 64 + 2 * lane + second;
+        sh.ties = left;
+        sh.sum = sh.before + part;
+        sh.found = H_ROWS;
+      }
+    }
+    __syncthreads();
+    cut = sh.cut;
+    ties = sh.ties;
+    sum = sh.sum;
+  }
+  if (nucleus) {
+    const double goal = (double)top_p * sum;
+    const int r = find_row(mass >= goal && sh.counts[tid] > 0, mass - sh.weights[tid]);
+    if (r < H_ROWS) {  // (else rounding alone has put the goal behind the last)
+      if (warp == 0) {
+        counts_of(r, c);
+        const double w0 = weigh(value_of<T>(r * 64 + 2 * lane)), w1 = weigh(value_of<T>(r * 64 + 2 * lane + 1));
+        const double m0 = c[0] ? c[0] * w0 : 0.0, m1 = c[1] ? c[1] * w1 : 0.0;
+        double lanes = m0 + m1;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double v_ = __shfl_up_sync(0xffffffffu, lanes, o);
+          if (lane >= o) lanes += v_;
+        }
+        const double ahead = sh.before + (lanes - (m0 + m1));
+        const unsigned has = __ballot_sync(0xffffffffu, (c[0] | c[1]) != 0);
+        const unsigned over = __ballot_sync(0xffffffffu, (c[0] | c[1]) != 0 && ahead + (m0 + m1) >= goal);
+        const int who = over ? __ffs(over) - 1 : 31 - __clz(has);  // by rounding the row's last
+        if (lane == who) {
+          const bool second = c[0] == 0 || (c[1] != 0 && ahead + m0 < goal);
+          const int there = second ? c[1] : c[0];
+          const double fit = ceil((goal - ahead - (second ? m0 : 0.0)) / (second ? w1 : w0));
+          sh.cut = r * 64 + 2 * lane + second;
+          sh.ties = fit < there ? max((int)fit, 1) : there;  // (no weight: infinite, or NaN)
+        }
+      }
+      __syncthreads();
+      const int bin = sh.cut;
+      if (bin < cut || (bin == cut && sh.ties < ties)) {
+        cut = bin;
+        ties = sh.ties;
+      }
+    }
+  }
+
+  // ---- the kept weights of each warp, then the warp that has the token
+  const double cut_weight = __shfl_sync(0xffffffffu, weigh(cut < Bins<T>::kEnd ? value_of<T>(cut) : -INFINITY), 0);
+  const bool ties_kept = ties > 0 && cut_weight >= (double)min_p;
+  const int steps = (mine + 31) / 32;
+  auto unit_at = [&](int step) {  // a unit's bins, those that are not the row's at the end
+    const int i = step * 32 + lane;
+    uint4 x = make_uint4(0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu);
+    if (i < mine) {
+      x = __ldg(source + first + i);
+      x = make_uint4(bins_of<T>(x.x), bins_of<T>(x.y), bins_of<T>(x.z), bins_of<T>(x.w));
+      if (first + i == 0 || first + i == row_units - 1) {
+        uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int q = 0; q < W; ++q) {
+          const int col = (first + i) * W + q - shift;
+          if (col < 0 || col >= p.vocab) w[q / 2] |= 0xffffu << (16 * (q % 2));
+        }
+        x = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+    return x;
+  };
+  // of NaNs the bins are before infinity's
+  auto kept = [&](int bin) { return bin < cut && bin >= Bins<T>::kTop; };
+  double total_here = 0.0;
+  int equal = 0;
+  uint4 next = unit_at(0);
+#pragma unroll 1
+  for (int step = 0; step < steps; ++step) {
+    const uint32_t w[4] = {next.x, next.y, next.z, next.w};
+    if (step + 1 < steps) next = unit_at(step + 1);
+#pragma unroll
+    for (int q = 0; q < W; ++q) {
+      const int bin = q & 1 ? w[q / 2] >> 16 : w[q / 2] & 0xffffu;
+      equal += bin == cut;
+      if (!__any_sync(0xffffffffu, kept(bin))) continue;
+      const double x = weigh(value_of<T>(bin));
+      if (kept(bin) && x >= (double)min_p) total_here += x;
+    }
+  }
+  total_here = sum_lanes(total_here, 16);
+  equal = __reduce_add_sync(0xffffffffu, equal);
+  const int me = rank * H_WARPS + warp;
+  if (lane < blocks) {
+    HistShared* to = cluster.map_shared_rank(&sh, lane);
+    to->all_sums[me] = total_here;
+    to->all_ties[me] = equal;
+  }
+  sync();
+  // each warp for itself: `blocks` neighbours to a lane
+  int tied = 0;
+  for (int q = 0; q < blocks; ++q) tied += sh.all_ties[lane * blocks + q];
+  int tie_base = tied;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int n = __shfl_up_sync(0xffffffffu, tie_base, o);
+    if (lane >= o) tie_base += n;
+  }
+  tie_base -= tied;
+  double weight = 0.0;
+  int seen = tie_base;
+  auto weight_at = [&](int i, int& ties_before) {  // of a warp of the cluster
+    const int n = sh.all_ties[i], some = ties_kept ? max(0, min(n, ties - ties_before)) : 0;
+    ties_before += n;
+    return sh.all_sums[i] + some * cut_weight;
+  };
+  for (int q = 0; q < blocks; ++q) weight += weight_at(lane * blocks + q, seen);
+  double line = weight;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double n = __shfl_up_sync(0xffffffffu, line, o);
+    if (lane >= o) line += n;
+  }
+  const double goal = (double)u * __shfl_sync(0xffffffffu, line, 31);
+  line -= weight;
+  int owner = 1 << 30, last = -1;
+  double owner_before = 0.0;
+  seen = tie_base;
+  int owner_ties = 0;
+  for (int q = 0; q < blocks; ++q) {
+    const int i = lane * blocks + q, ties_before = seen;
+    const double w = weight_at(i, seen);
+    if (w > 0.0) {
+      last = i;
+      if (owner == 1 << 30 && line + w > goal) {
+        owner = i;
+        owner_before = line;
+        owner_ties = ties_before;
+      }
+    }
+    line += w;
+  }
+  const unsigned owners = __ballot_sync(0xffffffffu, owner < 1 << 30);
+  if (owners) {
+    const int who = __ffs(owners) - 1;
+    owner = __shfl_sync(0xffffffffu, owner, who);
+    owner_before = __shfl_sync(0xffffffffu, owner_before, who);
+    owner_ties = __shfl_sync(0xffffffffu, owner_ties, who);
+  } else {  // by rounding: the last that has any; its last kept one
+    owner = __reduce_max_sync(0xffffffffu, last);
+    for (int i = 0; i < owner; ++i) owner_ties += sh.all_ties[i];
+    owner_before = -INFINITY;
+  }
+  if (owner != me) return;
+  const bool to_last = owners == 0;
+  double base = owner_before;
+  int token = -1, rank_base = owner_ties;
+#pragma unroll 1
+  for (int step = 0; step < steps; ++step) {
+    const uint4 x = unit_at(step);
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    int n = 0;
+#pragma unroll
+    for (int q = 0; q < W; ++q) n += (int)(q & 1 ? w[q / 2] >> 16 : w[q / 2] & 0xffffu) == cut;
+    int upto_n = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v_ = __shfl_up_sync(0xffffffffu, upto_n, o);
+      if (lane >= o) upto_n += v_;
+    }
+    int at = rank_base + upto_n - n;
+    rank_base += __shfl_sync(0xffffffffu, upto_n, 31);
+    double ws[W], here = 0.0;
+#pragma unroll
+    for (int q = 0; q < W; ++q) {
+      const int bin = q & 1 ? w[q / 2] >> 16 : w[q / 2] & 0xffffu;
+      double y = 0.0;
+      if (__any_sync(0xffffffffu, kept(bin))) y = weigh(value_of<T>(bin));
+      if (!kept(bin) || y < (double)min_p) y = 0.0;
+      if (bin == cut && ties_kept && at++ < ties) y = cut_weight;
+      ws[q] = y;
+      here += y;
+    }
+    double sums = here;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double v_ = __shfl_up_sync(0xffffffffu, sums, o);
+      if (lane >= o) sums += v_;
+    }
+    double run = base + (sums - here);
+    int hit = -1, back = -1;
+#pragma unroll
+    for (int q = 0; q < W; ++q) {
+      run += ws[q];
+      if (ws[q] > 0.0) {
+        back = q;
+        if (hit < 0 && !to_last && run > goal) hit = q;
+      }
+    }
+    const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0), backs = __ballot_sync(0xffffffffu, back >= 0);
+    if (hits) {
+      const int who = __ffs(hits) - 1;
+      token = (first + step * 32 + who) * W + __shfl_sync(0xffffffffu, hit, who) - shift;
+      break;
+    }
+    if (backs) {  // where rounding leaves the goal behind the last kept one, that one
+      const int who = 31 - __clz(backs);
+      token = (first + step * 32 + who) * W + __shfl_sync(0xffffffffu, back, who) - shift;
+    }
+    base += __shfl_sync(0xffffffffu, sums, 31);
+  }
+  if (lane == 0) p.out[row] = token;
+}
+
+namespace {
+
+template <typename K>
+int sample_start(K kernel, const SampleParams& p, int64_t B, int blocks, int threads, int64_t smem, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(B * blocks));
-  cfg.blockDim = dim3(SM_THREADS);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
@@ -548,8 +990,37 @@ int sample_launch(SampleParams p, int64_t B, cudaStream_t st) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = g_plain_launch.load(std::memory_order_relaxed) ? 1 : 2;
-  (void)cudaLaunchKernelEx(&cfg, sample_kernel<T>, p);
+  (void)cudaLaunchKernelEx(&cfg, kernel, p);
   return launched("sample");
+}
+
+template <typename T>
+int sample_launch(SampleParams p, int64_t B, cudaStream_t st) {
+  constexpr int W = kPerUnit<T>;
+  const int64_t row_units = ceil_div((int64_t)p.vocab + W - 1, W);
+  int blocks = 1;
+  if constexpr (sizeof(T) == 2) {
+    // blocks of a row: what their counters hold, and more where the SMs have room
+    while (blocks < SM_CLUSTER && ((int64_t)p.vocab > (int64_t)kMostCounted * blocks || (B * blocks * 2 <= sm_count() && row_units > H_THREADS / 2 * blocks)))
+      blocks *= 2;
+    if ((int64_t)p.vocab > (int64_t)kMostCounted * blocks)
+      return fail(TFB_ERR_UNSUPPORTED, "sample: %d logits in a row are more than a cluster has room for", p.vocab);
+    p.warp_units = (int)ceil_div(row_units, (int64_t)H_WARPS * blocks);
+    static std::atomic<uint64_t> done{0};
+    if (int rc = ensure_dynamic_smem(sample_hist_kernel<T>, H_ROWS * 128, done, "sample")) return rc;
+    return sample_start(sample_hist_kernel<T>, p, B, blocks, H_THREADS, H_ROWS * 128, st);
+  } else {
+    // blocks of a row: what the SMs have room for, and as many as its logits need
+    while (blocks < SM_CLUSTER && (B * blocks < sm_count() || ceil_div(row_units, (int64_t)SM_WARPS * blocks) * SM_WARPS * 16 > 104 * 1024) &&
+           row_units > (int64_t)SM_THREADS * blocks)
+      blocks *= 2;
+    p.warp_units = (int)ceil_div(row_units, (int64_t)SM_WARPS * blocks);
+    const int64_t smem = (int64_t)p.warp_units * SM_WARPS * 16;
+    if (smem > 212 * 1024) return fail(TFB_ERR_UNSUPPORTED, "sample: %d logits in a row are more than a cluster has room for", p.vocab);
+    static std::atomic<uint64_t> done{0};
+    if (int rc = ensure_dynamic_smem(sample_kernel<T>, 212 * 1024, done, "sample")) return rc;
+    return sample_start(sample_kernel<T>, p, B, blocks, SM_THREADS, smem, st);
+  }
 }
 
 }  // namespace
