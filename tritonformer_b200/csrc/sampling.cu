@@ -552,8 +552,9 @@ struct HistShared {
   double weights[H_ROWS];
   int warp_counts[H_WARPS];
   double warp_weights[H_WARPS];
-  int found, cut, ties;
-  double before, sum;
+  float warp_tops[H_WARPS], warp_lows[H_WARPS], tops[SM_CLUSTER];
+  int found, cut, ties, owner, owner_ties, to_last;
+  double before, owner_before, goal;
   double all_sums[SM_CLUSTER * H_WARPS];
   int all_ties[SM_CLUSTER * H_WARPS];
 };
@@ -562,6 +563,7 @@ struct HistShared {
 
 template <typename T>
 __global__ void __launch_bounds__(H_THREADS, 1) sample_hist_kernel(const SampleParams p) {
+  using T2 = typename Num<T>::T2;
   constexpr int W = 8;
   extern __shared__ uint4 smem_units[];
   uint32_t* hist = reinterpret_cast<uint32_t*>(smem_units);
@@ -572,8 +574,6 @@ __global__ void __launch_bounds__(H_THREADS, 1) sample_hist_kernel(const SampleP
   const int64_t row = blockIdx.x / blocks;
 #pragma unroll
   for (int i = 0; i < 8; ++i) smem_units[i * H_THREADS + tid] = make_uint4(0, 0, 0, 0);
-  sh.counts[tid] = 0;
-  sh.weights[tid] = 0.0;
   if (tid == 0) sh.found = H_ROWS;
   const double table = exp2(lane / 32.0);
   auto sync = [&]() {
@@ -583,20 +583,40 @@ __global__ void __launch_bounds__(H_THREADS, 1) sample_hist_kernel(const SampleP
   grid_dependency_wait();
   allow_dependents();
 
-  // ---- the warp's part of the row, counted
+  // ---- the warp's part of the row: 16-byte units of memory, with what is not the row's as -infinity
   const T* logits = static_cast<const T*>(p.logits) + row * p.ld;
   const int shift = (int)((reinterpret_cast<uintptr_t>(logits) & 15) / sizeof(T));
   const uint4* source = reinterpret_cast<const uint4*>(logits - shift);
   const int row_units = (p.vocab + shift + W - 1) / W;
   const int first = (rank * H_WARPS + warp) * p.warp_units;
-  const int mine = max(0, min(p.warp_units, row_units - first));  // of these units there are
+  const int mine = max(0, min(p.warp_units, row_units - first)), steps = (mine + 31) / 32;  // of these units there are
+  const T none = Num<T>::from_f(-INFINITY);
+  const uint32_t nones = *reinterpret_cast<const uint16_t*>(&none) * 0x10001u;
+  const bool edges = first == 0 || first + mine == row_units;  // the row's first or last unit is among them
+  auto load_unit = [&](int step) { return step * 32 + lane < mine ? __ldg(source + first + step * 32 + lane) : make_uint4(nones, nones, nones, nones); };
+  auto trim = [&](uint4& x, int step) {
+    const int at = first + step * 32 + lane;
+    if (at == 0 || at == row_units - 1) {
+      uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int q = 0; q < W; ++q) {
+        const int col = at * W + q - shift;
+        if (col < 0 || col >= p.vocab) w[q / 2] = q % 2 ? (w[q / 2] & 0xffffu) | (nones & 0xffff0000u) : (w[q / 2] & 0xffff0000u) | (nones & 0xffffu);
+      }
+      x = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  };
+  auto unit_at = [&](int step) {
+    uint4 x = load_unit(step);
+    if (edges) trim(x, step);
+    return x;
+  };
   uint4 v[H_UNITS];
 #pragma unroll
-  for (int i = 0; i < H_UNITS; ++i) {
-    const T none = Num<T>::from_f(-INFINITY);
-    const uint32_t nones = *reinterpret_cast<const uint16_t*>(&none) * 0x10001u;
-    v[i] = make_uint4(nones, nones, nones, nones);
-    if (i * 32 + lane < mine) v[i] = __ldg(source + first + i * 32 + lane);
+  for (int i = 0; i < H_UNITS; ++i) v[i] = load_unit(i);
+  if (edges) {
+#pragma unroll
+    for (int i = 0; i < H_UNITS; ++i) trim(v[i], i);
   }
   float t = p.temperature ? p.temperature[row] : p.temperature_all;
   float top_p = p.top_p ? p.top_p[row] : p.top_p_all, min_p = p.min_p ? p.min_p[row] : p.min_p_all;
@@ -611,175 +631,300 @@ __global__ void __launch_bounds__(H_THREADS, 1) sample_hist_kernel(const SampleP
   if (!(min_p > 0.f)) min_p = 0.f;
   min_p = fminf(min_p, 1.f);
   u = !(u > 0.f) ? 0.f : fminf(u, 0.99999994f);
-  const double per = kLog2eD / (double)t;
-  __syncthreads();
+
+  // ---- the largest logit of each thread (NaN is none) and of all
+  T2 most = *reinterpret_cast<const T2*>(&v[0].x);
 #pragma unroll
   for (int i = 0; i < H_UNITS; ++i) {
-    const int at = first + i * 32 + lane;
-    if (i * 32 + lane < mine) {
+    most = __hmax2(most, *reinterpret_cast<const T2*>(&v[i].x));
+    most = __hmax2(most, *reinterpret_cast<const T2*>(&v[i].y));
+    most = __hmax2(most, *reinterpret_cast<const T2*>(&v[i].z));
+    most = __hmax2(most, *reinterpret_cast<const T2*>(&v[i].w));
+  }
+  const float2 pair = Num<T>::to_f2(most);
+  const float mine_top = fmaxf(fmaxf(pair.x, pair.y), -INFINITY);
+  float top = warp_max(mine_top);
+  const float low = -warp_max(-mine_top);  // the smallest of them
+  if (lane == 0) {
+    sh.warp_tops[warp] = top;
+    sh.warp_lows[warp] = low;
+  }
+  __syncthreads();
+  top = warp_max(sh.warp_tops[lane]);
+  if (blocks > 1) {
+    cluster.sync();  // the others are there
+    if (tid < blocks) cluster.map_shared_rank(&sh, tid)->tops[rank] = top;
+    cluster.sync();
+    for (int b = 0; b < blocks; ++b) top = fmaxf(top, sh.tops[b]);
+  }
+  if (top == -INFINITY) {  // nothing is allowed
+    if (rank == 0 && tid == 0) p.out[row] = -1;
+    return;
+  }
+  auto bin_of = [&](float x) {  // of a value of the type
+    const T y = Num<T>::from_f(x + 0.f);
+    const int b = *reinterpret_cast<const uint16_t*>(&y);
+    return b & 0x8000 ? b : b ^ 0x7fff;
+  };
+  const int top_bin = bin_of(top);
+
+  // Weights relative to 2^(R / 32), R the whole number next to 32 log2(e) top / t: a logit's whole part and rest are then three sums away.  Where
+  // those numbers are too large for 64 bits to tell neighbours apart, or infinite, relative to the top one, from the difference to it.
+  const double per = kLog2eD / (double)t, per32 = per * 32.0, peak = (double)top;
+  constexpr double kMagic = 6755399441055744.0;  // as in weight_of
+  const bool near_by = fabs(peak * per32) < 16384.0;
+  const double magic = kMagic - (near_by ? rint(peak * per32) : 0.0);
+  const float lowest = top - 680.f * t;  // from there on 2^-981: nothing
+  auto weigh_near = [&](float x) {       // all lanes
+    constexpr double l = 0.69314718055994530942 / 32;
+    const double xd = (double)fmaxf(x, lowest), k_ = __fma_rn(xd, per32, magic);
+    const int n = __double2loint(k_);
+    const double r = __fma_rn(xd, per32, magic - k_);  // at most 1/2; the polynomial leaves 2^-39 of the weight
+    const double q = __fma_rn(r, __fma_rn(r, __fma_rn(r, l * l * l * l / 24, l * l * l / 6), l * l / 2), l);
+    const double base = __shfl_sync(0xffffffffu, table, n), w = __fma_rn(base, r * q, base);
+    return __hiloint2double(__double2hiint(w) + ((n << 15) & 0xfff00000), __double2loint(w));
+  };
+  auto weigh_far = [&](float x) {
+    const double w = weight_of(((double)x - peak) * per, table);
+    return x == top ? 1.0 : w;
+  };
+  auto weigh = [&](float x) { return near_by ? weigh_near(x) : weigh_far(x); };
+  // The weights of the warp's logits above a value, and how many are equal to it.
+  auto sweep = [&](float above, bool count, int& equal) {
+    double sum = 0.0;
+    equal = 0;
+    uint4 next = unit_at(0);
+#pragma unroll 1
+    for (int step = 0; step < steps; ++step) {
+      const uint32_t w[4] = {next.x, next.y, next.z, next.w};
+      if (step + 1 < steps) next = unit_at(step + 1);
+      float x[W];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float2 f = Num<T>::to_f2(*reinterpret_cast<const T2*>(&w[q]));
+        x[2 * q] = f.x;
+        x[2 * q + 1] = f.y;
+      }
+      float high = x[0];
+#pragma unroll
+      for (int q = 1; q < W; ++q) high = fmaxf(high, x[q]);
+      if (!__any_sync(0xffffffffu, high >= above)) continue;
+      if (count) {
+#pragma unroll
+        for (int q = 0; q < W; ++q) equal += x[q] == above;
+      }
+      if (!__any_sync(0xffffffffu, high > above)) continue;
+#pragma unroll 1
+      for (int half = 0; half < 2; ++half) {  // (eight at once do not fit the registers)
+        float z[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) z[q] = half ? x[4 + q] : x[q];
+        if (near_by) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const double y = weigh_near(z[q]);
+            if (z[q] > above) sum += y;
+          }
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const double y = weigh_far(z[q]);
+            if (z[q] > above) sum += y;
+          }
+        }
+      }
+    }
+    sum = sum_lanes(sum, 16);
+    equal = __reduce_add_sync(0xffffffffu, equal);
+    return sum;
+  };
+  const int me = rank * H_WARPS + warp;
+  auto share = [&](double sum, int equal) {  // each warp's with all blocks
+    if (lane < blocks) {
+      HistShared* to = cluster.map_shared_rank(&sh, lane);
+      to->all_sums[me] = sum;
+      to->all_ties[me] = equal;
+    }
+    sync();
+  };
+
+  // ---- Only what may be above the cut is counted: of the k largest none is below the k-th largest of the threads' largest ones.
+  int limit = Bins<T>::kEnd - 1;
+  if (k > 1 && k <= H_THREADS) {
+    const int own = mine_top > -INFINITY ? bin_of(mine_top) : Bins<T>::kEnd;
+    const float low = -warp_max(-sh.warp_lows[lane]);
+    int lo = top_bin - 1;  // too few up to there
+    if (low > -INFINITY) limit = bin_of(low);
+    while (limit - lo > 1) {
+      const int mid = (lo + limit) / 2;
+      if (__syncthreads_count(own <= mid) >= k) limit = mid;
+      else lo = mid;
+    }
+  }
+
+  uint32_t set = 0;  // bit i: row 32 i + lane has logits
+  int c[2];
+  // counts of a row's two bins of a lane, over the cluster
+  auto counts_of = [&](int r) {
+    uint32_t word = hist[r * 32 + lane];
+    c[0] = word & 0xffffu;
+    c[1] = word >> 16;
+    for (int b = 1; b < blocks; ++b) {
+      word = cluster.map_shared_rank(hist, b == rank ? 0 : b)[r * 32 + lane];
+      c[0] += word & 0xffffu;
+      c[1] += word >> 16;
+    }
+  };
+  auto row_weight = [&](int r) {  // of the lane's two bins
+    const double w0 = weigh(value_of<T>(r * 64 + 2 * lane)), w1 = weigh(value_of<T>(r * 64 + 2 * lane + 1));
+    return (c[0] ? c[0] * w0 : 0.0) + (c[1] ? c[1] * w1 : 0.0);
+  };
+  const bool all_weights = nucleus && k == 0;
+  // the logits' counts, and of each row of values how many there are in the cluster; for a nucleus of all logits their weights too
+  if (k > 1 || all_weights) {
+#pragma unroll
+    for (int i = 0; i < H_UNITS; ++i) {
+      if (i * 32 >= mine) break;
       const uint32_t words[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-      const bool edge = at == 0 || at == row_units - 1;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const uint32_t b = bins_of<T>(words[q]);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const uint32_t bin = e ? b >> 16 : b & 0xffffu;
-          const int c = at * W + 2 * q + e - shift;
-          if (bin < Bins<T>::kEnd && (!edge || (c >= 0 && c < p.vocab))) atomicAdd(hist + (bin >> 1), 1u << (16 * (bin & 1)));
+          if (bin - Bins<T>::kTop <= (uint32_t)(limit - Bins<T>::kTop)) atomicAdd(hist + (bin >> 1), 1u + (bin & 1) * 0xffffu);
         }
       }
     }
-  }
-  __syncthreads();
-  {
+    sh.counts[tid] = 0;
+    sh.weights[tid] = 0.0;
+    __syncthreads();
     uint32_t bits = 0;
-    for (int i = 0; i < 32; ++i) {
+    for (int i = 0; i * 32 + warp <= limit / 64; ++i) {
       const int r = i * 32 + warp;
-      uint32_t word = hist[r * 32 + lane];
-      if (r <= Bins<T>::kTop / 64 && word != 0) {  // NaNs
-        const int b = r * 64 + 2 * lane;
-        word &= (b < Bins<T>::kTop ? 0u : 0xffffu) | (b + 1 < Bins<T>::kTop ? 0u : 0xffff0000u);
-        hist[r * 32 + lane] = word;
+      const uint32_t word = hist[r * 32 + lane];
+      if (!__any_sync(0xffffffffu, word != 0)) continue;
+      bits |= 1u << i;
+      if (blocks == 1) {
+        counts_of(r);
+        const int n = __reduce_add_sync(0xffffffffu, c[0] + c[1]);
+        const double sum = all_weights ? sum_lanes(row_weight(r), 16) : 0.0;
+        if (lane == 0) {
+          sh.counts[r] = n;
+          sh.weights[r] = sum;
+        }
       }
-      bits |= (uint32_t)(__any_sync(0xffffffffu, word != 0) != 0) << i;
     }
     if (lane == 0) sh.rows[warp] = bits;
-  }
-  sync();
-  // counts of a row's two bins of a lane, over the cluster
-  auto counts_of = [&](int r, int (&c)[2]) {
-    c[0] = c[1] = 0;
-    for (int b = 0; b < blocks; ++b) {
-      const uint32_t word = cluster.map_shared_rank(hist, b)[r * 32 + lane];
-      c[0] += word & 0xffffu;
-      c[1] += word >> 16;
-    }
-  };
-  uint32_t set = 0;  // of word `lane`
-  for (int b = 0; b < blocks; ++b) set |= cluster.map_shared_rank(&sh, b)->rows[lane];
-  const int top_row = __reduce_min_sync(0xffffffffu, set ? (__ffs(set) - 1) * 32 + lane : H_ROWS);
-  if (top_row == H_ROWS) {  // nothing is allowed
-    if (rank == 0 && tid == 0) p.out[row] = -1;
-    if (blocks > 1) cluster.sync();
-    return;
-  }
-  int c[2];
-  counts_of(top_row, c);
-  const int top_lane = __ffs(__ballot_sync(0xffffffffu, (c[0] | c[1]) != 0)) - 1;
-  const int top_bin = top_row * 64 + 2 * top_lane + (__shfl_sync(0xffffffffu, c[0], top_lane) == 0);
-  const float top = value_of<T>(top_bin);
-  const double peak = (double)top;
-  auto weigh = [&](float x) {  // all lanes
-    const double w = weight_of(((double)x - peak) * per, table);
-    return x == top ? 1.0 : w;
-  };
-
-  // ---- counts and weights of the rows, each from one warp of the cluster to all blocks
-  uint32_t todo = __shfl_sync(0xffffffffu, set, warp);
-  while (todo != 0) {
-    const int i = __ffs(todo) - 1, r = i * 32 + warp;
-    todo &= todo - 1;
-    if ((i & (blocks - 1)) != rank) continue;
-    counts_of(r, c);
-    const double w0 = weigh(value_of<T>(r * 64 + 2 * lane)), w1 = weigh(value_of<T>(r * 64 + 2 * lane + 1));
-    const double sum = sum_lanes((c[0] ? c[0] * w0 : 0.0) + (c[1] ? c[1] * w1 : 0.0), 16);
-    const int n = __reduce_add_sync(0xffffffffu, c[0] + c[1]);
-    if (lane < blocks) {
-      HistShared* to = cluster.map_shared_rank(&sh, lane);
-      to->counts[r] = n;
-      to->weights[r] = sum;
+    sync();
+    set = 0;
+    for (int b = 0; b < blocks; ++b) set |= cluster.map_shared_rank(&sh, b)->rows[lane];
+    if (blocks > 1) {
+      for (uint32_t todo = __shfl_sync(0xffffffffu, set, warp); todo != 0; todo &= todo - 1) {
+        const int i = __ffs(todo) - 1, r = i * 32 + warp;
+        if ((i & (blocks - 1)) != rank) continue;
+        counts_of(r);
+        const double sum = all_weights ? sum_lanes(row_weight(r), 16) : 0.0;
+        const int n = __reduce_add_sync(0xffffffffu, c[0] + c[1]);
+        if (lane < blocks) {
+          HistShared* other = cluster.map_shared_rank(&sh, lane);
+          other->counts[r] = n;
+          other->weights[r] = sum;
+        }
+      }
+      cluster.sync();
     }
   }
-  sync();
-
-  // ---- their sums up to each row, thread by thread
-  int upto = sh.counts[tid];
-  double mass = sh.weights[tid];
+  // sums up to each row, thread by thread
+  auto scan = [&](auto upto, auto* warps) {
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int n = __shfl_up_sync(0xffffffffu, upto, o);
-    const double w = __shfl_up_sync(0xffffffffu, mass, o);
-    if (lane >= o) {
-      upto += n;
-      mass += w;
+    for (int o = 1; o < 32; o <<= 1) {
+      const auto n = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += n;
     }
-  }
-  if (lane == 31) {
-    sh.warp_counts[warp] = upto;
-    sh.warp_weights[warp] = mass;
-  }
-  __syncthreads();
-  int all_upto = sh.warp_counts[lane];
-  double all_mass = sh.warp_weights[lane];
+    if (lane == 31) warps[warp] = upto;
+    __syncthreads();
+    auto all = warps[lane];
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int n = __shfl_up_sync(0xffffffffu, all_upto, o);
-    const double w = __shfl_up_sync(0xffffffffu, all_mass, o);
-    if (lane >= o) {
-      all_upto += n;
-      all_mass += w;
+    for (int o = 1; o < 32; o <<= 1) {
+      const auto n = __shfl_up_sync(0xffffffffu, all, o);
+      if (lane >= o) all += n;
     }
-  }
-  const int finite = __shfl_sync(0xffffffffu, all_upto, 31);
-  double sum = __shfl_sync(0xffffffffu, all_mass, 31);
-  if (warp > 0) {
-    upto += __shfl_sync(0xffffffffu, all_upto, warp - 1);
-    mass += __shfl_sync(0xffffffffu, all_mass, warp - 1);
-  }
-  // The first row whose sums reach a goal, and what lies before it; a warp looks at its bins.
-  auto find_row = [&](bool reached, double before) {
+    const auto before = __shfl_sync(0xffffffffu, all, warp ? warp - 1 : 0);
+    if (warp) upto += before;
+    return upto;
+  };
+  // the first row whose sum reaches a goal
+  auto find_row = [&](bool reached) {
     const unsigned ones = __ballot_sync(0xffffffffu, reached);
     if (ones && lane == __ffs(ones) - 1) atomicMin(&sh.found, tid);
     __syncthreads();
-    const int r = sh.found;
-    if (tid == r) sh.before = before;
-    __syncthreads();
-    return r;
+    return sh.found;
   };
   int cut = Bins<T>::kEnd, ties = 0;  // all bins before `cut` are kept, and of it so many
   if (k == 1) {
     cut = top_bin;
     ties = 1;
-  } else if (k > 0 && k < finite) {
-    const int n = sh.counts[tid];
-    const int r = find_row(upto >= k, mass - sh.weights[tid]);
-    if (tid == r) sh.ties = k - (upto - n);  // wanted of the row
-    __syncthreads();
-    if (warp == 0) {
-      counts_of(r, c);
-      int lanes = c[0] + c[1];
+  } else if (k > 0) {
+    const int n = sh.counts[tid], upto = scan(n, sh.warp_counts);
+    const int r = find_row(upto >= k);
+    if (r < H_ROWS) {
+      if (tid == r) sh.ties = k - (upto - n);  // wanted of the row
+      __syncthreads();
+      if (warp == 0) {
+        counts_of(r);
+        int lanes = c[0] + c[1];
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v_ = __shfl_up_sync(0xffffffffu, lanes, o);
-        if (lane >= o) lanes += v_;
+        for (int o = 1; o < 32; o <<= 1) {
+          const int v_ = __shfl_up_sync(0xffffffffu, lanes, o);
+          if (lane >= o) lanes += v_;
+        }
+        const int left = sh.ties - (lanes - c[0] - c[1]);  // wanted of this lane's and those behind it
+        __syncwarp();
+        if (lane == __ffs(__ballot_sync(0xffffffffu, left <= c[0] + c[1])) - 1) {
+          const bool second = left > c[0];
+          sh.cut = r * 64 + 2 * lane + second;
+          sh.ties = left - (second ? c[0] : 0);
+          sh.found = H_ROWS;
+        }
       }
-      const int want = sh.ties, who = __ffs(__ballot_sync(0xffffffffu, lanes >= want)) - 1;
-      const double w0 = weigh(value_of<T>(r * 64 + 2 * lane)), w1 = weigh(value_of<T>(r * 64 + 2 * lane + 1));
-      const int ahead = lanes - c[0] - c[1];  // of the row before this lane's
-      const bool second = want > ahead + c[0];
-      const int left = want - ahead - (second ? c[0] : 0);
-      double part = lane < who ? (c[0] ? c[0] * w0 : 0.0) + (c[1] ? c[1] * w1 : 0.0)
-                    : lane == who ? (second ? (c[0] ? c[0] * w0 : 0.0) + left * w1 : left * w0) : 0.0;
-      part = sum_lanes(part, 16);
-      if (lane == who) {
-        sh.cut = r * 64 + 2 * lane + second;
-        sh.ties = left;
-        sh.sum = sh.before + part;
-        sh.found = H_ROWS;
-      }
+      __syncthreads();
+      cut = sh.cut;
+      ties = sh.ties;
     }
-    __syncthreads();
-    cut = sh.cut;
-    ties = sh.ties;
-    sum = sh.sum;
   }
   if (nucleus) {
-    const double goal = (double)top_p * sum;
-    const int r = find_row(mass >= goal && sh.counts[tid] > 0, mass - sh.weights[tid]);
+    // of a row's counts what is left
+    auto cut_off = [&](int r) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int bin = r * 64 + 2 * lane + e;
+        c[e] = bin < cut ? c[e] : bin == cut ? ties : 0;
+      }
+    };
+    if (!all_weights) {
+      const int last = min(cut / 64, H_ROWS - 1);
+      for (uint32_t todo = __shfl_sync(0xffffffffu, set, warp); todo != 0; todo &= todo - 1) {
+        const int r = (__ffs(todo) - 1) * 32 + warp;
+        if (r > last) break;
+        counts_of(r);
+        cut_off(r);
+        const double sum = sum_lanes(row_weight(r), 16);
+        if (lane == 0) sh.weights[r] = sum;
+      }
+      __syncthreads();
+    }
+    const double own = sh.weights[tid], mass = scan(own, sh.warp_weights);
+    if (tid == H_THREADS - 1) sh.goal = (double)top_p * mass;
+    __syncthreads();
+    const double goal = sh.goal;
+    const int r = find_row(mass >= goal && own > 0.0);
     if (r < H_ROWS) {  // (else rounding alone has put the goal behind the last)
+      if (tid == r) sh.before = mass - own;
+      __syncthreads();
       if (warp == 0) {
-        counts_of(r, c);
+        counts_of(r);
+        cut_off(r);
         const double w0 = weigh(value_of<T>(r * 64 + 2 * lane)), w1 = weigh(value_of<T>(r * 64 + 2 * lane + 1));
         const double m0 = c[0] ? c[0] * w0 : 0.0, m1 = c[1] ? c[1] * w1 : 0.0;
         double lanes = m0 + m1;
@@ -801,128 +946,118 @@ __global__ void __launch_bounds__(H_THREADS, 1) sample_hist_kernel(const SampleP
         }
       }
       __syncthreads();
-      const int bin = sh.cut;
-      if (bin < cut || (bin == cut && sh.ties < ties)) {
-        cut = bin;
-        ties = sh.ties;
+      cut = sh.cut;
+      ties = sh.ties;
+    }
+  }
+  if (min_p > 0.f) {  // the last value that weighs enough, 32 at a time
+    if (warp == 0) {
+      const double enough = (double)min_p * weigh(top);
+      int lo = top_bin, hi = Bins<T>::kEnd;  // enough, not enough
+      while (hi - lo > 1) {
+        const int step = (hi - lo + 32) / 33, bin = min(lo + step * (lane + 1), hi - 1);
+        const double w = weigh(value_of<T>(bin));
+        const unsigned yes = __ballot_sync(0xffffffffu, w >= enough);
+        const int n = yes == 0xffffffffu ? 32 : __ffs(~yes) - 1;  // a beginning of the lanes
+        const int next = min(lo + step * (n + 1), hi - 1);
+        if (n > 0) lo = min(lo + step * n, hi - 1);
+        if (n < 32) hi = next;
       }
+      if (lane == 0) sh.cut = lo;
+    }
+    __syncthreads();
+    if (sh.cut < cut) {
+      cut = sh.cut + 1;
+      ties = 0;
     }
   }
 
   // ---- the kept weights of each warp, then the warp that has the token
-  const double cut_weight = __shfl_sync(0xffffffffu, weigh(cut < Bins<T>::kEnd ? value_of<T>(cut) : -INFINITY), 0);
-  const bool ties_kept = ties > 0 && cut_weight >= (double)min_p;
-  const int steps = (mine + 31) / 32;
-  auto unit_at = [&](int step) {  // a unit's bins, those that are not the row's at the end
-    const int i = step * 32 + lane;
-    uint4 x = make_uint4(0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu);
-    if (i < mine) {
-      x = __ldg(source + first + i);
-      x = make_uint4(bins_of<T>(x.x), bins_of<T>(x.y), bins_of<T>(x.z), bins_of<T>(x.w));
-      if (first + i == 0 || first + i == row_units - 1) {
-        uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  // as a value (-0 is no bin of any logit: what is above it is above the next one)
+  const float above = cut < Bins<T>::kEnd ? value_of<T>(cut == 0x8000 ? 0x8001 : cut) : -INFINITY;
+  const double cut_weight = __shfl_sync(0xffffffffu, weigh(above), 0);
+  const bool ties_kept = ties > 0;
+  {
+    int equal;
+    const double sum = sweep(above, ties_kept, equal);
+    share(sum, equal);
+  }
+  if (warp == 0) {  // `blocks` neighbours to a lane
+    int tied = 0;
+    for (int q = 0; q < blocks; ++q) tied += sh.all_ties[lane * blocks + q];
+    int tie_base = tied;
 #pragma unroll
-        for (int q = 0; q < W; ++q) {
-          const int col = (first + i) * W + q - shift;
-          if (col < 0 || col >= p.vocab) w[q / 2] |= 0xffffu << (16 * (q % 2));
+    for (int o = 1; o < 32; o <<= 1) {
+      const int n = __shfl_up_sync(0xffffffffu, tie_base, o);
+      if (lane >= o) tie_base += n;
+    }
+    tie_base -= tied;
+    double weight = 0.0;
+    int seen = tie_base;
+    auto weight_at = [&](int i, int& ties_before) {  // of a warp of the cluster
+      const int n = sh.all_ties[i], some = ties_kept ? max(0, min(n, ties - ties_before)) : 0;
+      ties_before += n;
+      return sh.all_sums[i] + some * cut_weight;
+    };
+    for (int q = 0; q < blocks; ++q) weight += weight_at(lane * blocks + q, seen);
+    double line = weight;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double n = __shfl_up_sync(0xffffffffu, line, o);
+      if (lane >= o) line += n;
+    }
+    const double goal = (double)u * __shfl_sync(0xffffffffu, line, 31);
+    line -= weight;
+    int owner = 1 << 30, last = -1;
+    double owner_before = 0.0;
+    seen = tie_base;
+    int owner_ties = 0;
+    for (int q = 0; q < blocks; ++q) {
+      const int i = lane * blocks + q, ties_before = seen;
+      const double w = weight_at(i, seen);
+      if (w > 0.0) {
+        last = i;
+        if (owner == 1 << 30 && line + w > goal) {
+          owner = i;
+          owner_before = line;
+          owner_ties = ties_before;
         }
-        x = make_uint4(w[0], w[1], w[2], w[3]);
       }
+      line += w;
     }
-    return x;
-  };
-  // of NaNs the bins are before infinity's
-  auto kept = [&](int bin) { return bin < cut && bin >= Bins<T>::kTop; };
-  double total_here = 0.0;
-  int equal = 0;
-  uint4 next = unit_at(0);
+    const unsigned owners = __ballot_sync(0xffffffffu, owner < 1 << 30);
+    if (owners) {
+      const int who = __ffs(owners) - 1;
+      owner = __shfl_sync(0xffffffffu, owner, who);
+      owner_before = __shfl_sync(0xffffffffu, owner_before, who);
+      owner_ties = __shfl_sync(0xffffffffu, owner_ties, who);
+    } else {  // by rounding: the last that has any; its last kept one
+      owner = __reduce_max_sync(0xffffffffu, last);
+      for (int i = 0; i < owner; ++i) owner_ties += sh.all_ties[i];
+      owner_before = -INFINITY;
+    }
+    if (lane == 0) {
+      sh.owner = owner;
+      sh.owner_before = owner_before;
+      sh.owner_ties = owner_ties;
+      sh.goal = goal;
+      sh.to_last = owners == 0;
+    }
+  }
+  __syncthreads();
+  if (sh.owner != me) return;
+  const bool to_last = sh.to_last != 0;
+  const double aim = sh.goal;
+  double base = sh.owner_before;
+  int token = -1, rank_base = sh.owner_ties;
 #pragma unroll 1
   for (int step = 0; step < steps; ++step) {
-    const uint32_t w[4] = {next.x, next.y, next.z, next.w};
-    if (step + 1 < steps) next = unit_at(step + 1);
-#pragma unroll
-    for (int q = 0; q < W; ++q) {
-      const int bin = q & 1 ? w[q / 2] >> 16 : w[q / 2] & 0xffffu;
-      equal += bin == cut;
-      if (!__any_sync(0xffffffffu, kept(bin))) continue;
-      const double x = weigh(value_of<T>(bin));
-      if (kept(bin) && x >= (double)min_p) total_here += x;
-    }
-  }
-  total_here = sum_lanes(total_here, 16);
-  equal = __reduce_add_sync(0xffffffffu, equal);
-  const int me = rank * H_WARPS + warp;
-  if (lane < blocks) {
-    HistShared* to = cluster.map_shared_rank(&sh, lane);
-    to->all_sums[me] = total_here;
-    to->all_ties[me] = equal;
-  }
-  sync();
-  // each warp for itself: `blocks` neighbours to a lane
-  int tied = 0;
-  for (int q = 0; q < blocks; ++q) tied += sh.all_ties[lane * blocks + q];
-  int tie_base = tied;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int n = __shfl_up_sync(0xffffffffu, tie_base, o);
-    if (lane >= o) tie_base += n;
-  }
-  tie_base -= tied;
-  double weight = 0.0;
-  int seen = tie_base;
-  auto weight_at = [&](int i, int& ties_before) {  // of a warp of the cluster
-    const int n = sh.all_ties[i], some = ties_kept ? max(0, min(n, ties - ties_before)) : 0;
-    ties_before += n;
-    return sh.all_sums[i] + some * cut_weight;
-  };
-  for (int q = 0; q < blocks; ++q) weight += weight_at(lane * blocks + q, seen);
-  double line = weight;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const double n = __shfl_up_sync(0xffffffffu, line, o);
-    if (lane >= o) line += n;
-  }
-  const double goal = (double)u * __shfl_sync(0xffffffffu, line, 31);
-  line -= weight;
-  int owner = 1 << 30, last = -1;
-  double owner_before = 0.0;
-  seen = tie_base;
-  int owner_ties = 0;
-  for (int q = 0; q < blocks; ++q) {
-    const int i = lane * blocks + q, ties_before = seen;
-    const double w = weight_at(i, seen);
-    if (w > 0.0) {
-      last = i;
-      if (owner == 1 << 30 && line + w > goal) {
-        owner = i;
-        owner_before = line;
-        owner_ties = ties_before;
-      }
-    }
-    line += w;
-  }
-  const unsigned owners = __ballot_sync(0xffffffffu, owner < 1 << 30);
-  if (owners) {
-    const int who = __ffs(owners) - 1;
-    owner = __shfl_sync(0xffffffffu, owner, who);
-    owner_before = __shfl_sync(0xffffffffu, owner_before, who);
-    owner_ties = __shfl_sync(0xffffffffu, owner_ties, who);
-  } else {  // by rounding: the last that has any; its last kept one
-    owner = __reduce_max_sync(0xffffffffu, last);
-    for (int i = 0; i < owner; ++i) owner_ties += sh.all_ties[i];
-    owner_before = -INFINITY;
-  }
-  if (owner != me) return;
-  const bool to_last = owners == 0;
-  double base = owner_before;
-  int token = -1, rank_base = owner_ties;
-#pragma unroll 1
-  for (int step = 0; step < steps; ++step) {
-    const uint4 x = unit_at(step);
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    const uint4 unit = unit_at(step);
+    float x[W];
+    unpack8<T>(unit, x);
     int n = 0;
 #pragma unroll
-    for (int q = 0; q < W; ++q) n += (int)(q & 1 ? w[q / 2] >> 16 : w[q / 2] & 0xffffu) == cut;
+    for (int q = 0; q < W; ++q) n += x[q] == above;
     int upto_n = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -934,11 +1069,10 @@ __global__ void __launch_bounds__(H_THREADS, 1) sample_hist_kernel(const SampleP
     double ws[W], here = 0.0;
 #pragma unroll
     for (int q = 0; q < W; ++q) {
-      const int bin = q & 1 ? w[q / 2] >> 16 : w[q / 2] & 0xffffu;
       double y = 0.0;
-      if (__any_sync(0xffffffffu, kept(bin))) y = weigh(value_of<T>(bin));
-      if (!kept(bin) || y < (double)min_p) y = 0.0;
-      if (bin == cut && ties_kept && at++ < ties) y = cut_weight;
+      if (__any_sync(0xffffffffu, x[q] > above)) y = weigh(x[q]);
+      if (!(x[q] > above)) y = 0.0;
+      if (x[q] == above && ties_kept && at++ < ties) y = cut_weight;
       ws[q] = y;
       here += y;
     }
@@ -955,7 +1089,7 @@ __global__ void __launch_bounds__(H_THREADS, 1) sample_hist_kernel(const SampleP
       run += ws[q];
       if (ws[q] > 0.0) {
         back = q;
-        if (hit < 0 && !to_last && run > goal) hit = q;
+        if (hit < 0 && !to_last && run > aim) hit = q;
       }
     }
     const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0), backs = __ballot_sync(0xffffffffu, back >= 0);
@@ -1000,15 +1134,17 @@ int sample_launch(SampleParams p, int64_t B, cudaStream_t st) {
   const int64_t row_units = ceil_div((int64_t)p.vocab + W - 1, W);
   int blocks = 1;
   if constexpr (sizeof(T) == 2) {
-    // blocks of a row: what their counters hold, and more where the SMs have room
-    while (blocks < SM_CLUSTER && ((int64_t)p.vocab > (int64_t)kMostCounted * blocks || (B * blocks * 2 <= sm_count() && row_units > H_THREADS / 2 * blocks)))
+    // blocks of a row: what their counters hold, and more where they find half of the SMs free (16 rows of 131071: 22 to 34 us with 2 or 4
+    // blocks; with 8, whose clusters do not all find room at once, 28 to 51)
+    while (blocks < SM_CLUSTER && ((int64_t)p.vocab > (int64_t)kMostCounted * blocks || (B * blocks * 4 <= sm_count() && row_units > H_THREADS / 2 * blocks)))
       blocks *= 2;
     if ((int64_t)p.vocab > (int64_t)kMostCounted * blocks)
       return fail(TFB_ERR_UNSUPPORTED, "sample: %d logits in a row are more than a cluster has room for", p.vocab);
     p.warp_units = (int)ceil_div(row_units, (int64_t)H_WARPS * blocks);
     static std::atomic<uint64_t> done{0};
-    if (int rc = ensure_dynamic_smem(sample_hist_kernel<T>, H_ROWS * 128, done, "sample")) return rc;
-    return sample_start(sample_hist_kernel<T>, p, B, blocks, H_THREADS, H_ROWS * 128, st);
+    constexpr int smem = H_ROWS * 128;
+    if (int rc = ensure_dynamic_smem(sample_hist_kernel<T>, smem, done, "sample")) return rc;
+    return sample_start(sample_hist_kernel<T>, p, B, blocks, H_THREADS, smem, st);
   } else {
     // blocks of a row: what the SMs have room for, and as many as its logits need
     while (blocks < SM_CLUSTER && (B * blocks < sm_count() || ceil_div(row_units, (int64_t)SM_WARPS * blocks) * SM_WARPS * 16 > 104 * 1024) &&
