@@ -412,7 +412,7 @@ int tfb_cache_append_int4(const void* key, const void* value, void* k_pages, voi
  * a weight is not finite; c = W / s rounded to the nearest whole number, ties to even.
  * tfb_int4_expand: s * c rounded to the type, transposed: out (16 * strips, 64 * units), 16-byte aligned.
  * tfb_int4_linear: out = act(x W + bias) + addend for M rows of x (pitch x_ld, unit stride, any alignment), out and addend of pitch
- * out_ld, addend_ld; bias (N) and addend may be NULL, the addend may be the output.  For few rows: every 64 of them read the weights again.  */
+ * out_ld, addend_ld; bias (N) and addend may be NULL, the addend may be the output.  For few rows: every 32 of them read the weights again.  */
 int64_t tfb_int4_codes(int64_t K, int64_t N);
 int64_t tfb_int4_scales(int64_t K, int64_t N, int group);
 int tfb_int4_quantize(const void* w, int64_t w_k, int64_t w_n, int64_t K, int64_t N, int group, void* codes,

@@ -44,22 +44,22 @@ constexpr int PG_WARPS = 8;
 constexpr float kAhead = 15.f, kBelow = 4.f;
 constexpr float kNone = -INFINITY;
 
-// What beginning a row of scores costs a warp, in tiles: rows of a tile or two would otherwise pile up in a few warps.
-constexpr int kRowCost = 4;
-
 // G: query heads that a warp takes at once, 4, 8 or 16.  Q4: pages in 4 bits.
 template <int HD, int G, int BIAS, bool Q4> struct PgCfg {
   static constexpr int NT = G == 16 ? 2 : 1;   // blocks of 8 columns in the products
-  static constexpr int KEYS = Q4 ? (HD == 128 ? 32 : 64) : 2048 / HD;  // keys of a tile
+  static constexpr int KEYS = Q4 ? 64 : 2048 / HD;  // keys of a tile
   static constexpr int MT = KEYS / 16;
   static constexpr int R = 8 * NT;             // query heads of a head tile
   static constexpr int CHUNKS = HD / (Q4 ? 32 : 8);  // 16-byte chunks of a row
   static constexpr int RPI = 32 / CHUNKS;      // rows that a warp copies with one cp.async
   static constexpr int ITERS = KEYS / RPI;     // 8, and in 4 bits 2 or 4
   static constexpr int OWN = (KEYS + 31) / 32; // keys whose place a lane looks up
-  static constexpr int TILE = KEYS * CHUNKS * 16;  // bytes of the keys of a tile (4096, and in 4 bits 1024 or 2048)
+  static constexpr int TILE = KEYS * CHUNKS * 16;  // bytes of the keys of a tile (4096, and in 4 bits 1024 to 4096)
   static constexpr int PANELS = HD == 128 ? 2 : 1;  // parts of a row of at most 128 bytes, one after the other
   static constexpr int STAGES = 3;             // what 227 KB hold
+  // What beginning a row of scores costs a warp, in tiles: rows of a tile or two would otherwise pile up in a few warps.  (In 4 bits a tile
+  // has more keys and takes longer: 24 sequences of up to 2048 keys 22.2 us, with 4 24.3.)
+  static constexpr int ROW_COST = Q4 ? 1 : 4;
   static constexpr int OFF_POS = PG_WARPS * STAGES * 2 * TILE;   // [warp][stage][KEYS] positions, or scales
   static constexpr int OFF_ML = OFF_POS + (BIAS || Q4 ? PG_WARPS * STAGES * KEYS * 4 : 0);  // [warp][2][R] reference and sum of a piece
   static constexpr int OFF_BAR = OFF_ML + PG_WARPS * 2 * R * 8;  // [warp][stage]
@@ -162,7 +162,7 @@ __device__ __forceinline__ SeqKeys keys_of(const PgParams& p, int len) {
 }
 
 // A place in the line: sequence, (key head, head tile), tile, and its distance from the stretch's beginning.
-template <int KEYS>
+template <int KEYS, int ROW_COST>
 struct Cursor {
   int b, hr, j, tiles, at;
   SeqKeys keys;
@@ -172,7 +172,7 @@ struct Cursor {
   }
   // to the first tile of the next row of scores; false if there is none
   __device__ __forceinline__ bool next_row(const PgParams& p) {
-    at += kRowCost;
+    at += ROW_COST;
     j = 0;
     if (++hr < p.kv_heads * p.row_tiles) return true;
     hr = 0;
@@ -192,7 +192,7 @@ struct Cursor {
 __device__ __forceinline__ int64_t divide(int64_t n, int64_t d) {  // of values that are not negative
   return ((n | d) >> 32) == 0 ? (int64_t)((uint32_t)n / (uint32_t)d) : n / d;
 }
-// The line has kRowCost units and one for each tile of a row, and is cut into equal stretches, one for each warp (with fewer
+// The line has ROW_COST units and one for each tile of a row, and is cut into equal stretches, one for each warp (with fewer
 // units than warps, of one unit): the first `more` have a unit more than `each`.
 struct Line {
   int64_t units, each, more, parts;
@@ -207,7 +207,7 @@ struct Line {
     return (int)((t < wide ? divide(t, each + 1) : more + divide(t - wide, each)) / PG_WARPS);
   }
 };
-__device__ __forceinline__ int row_units(int tiles) { return tiles ? tiles + kRowCost : 0; }
+template <int ROW_COST> __device__ __forceinline__ int row_units(int tiles) { return tiles ? tiles + ROW_COST : 0; }
 
 __device__ __forceinline__ float alibi_rounded_log2(int mode, float slope, float dist) {  // slope already rounded
   const int drop = mode == 2 ? 13 : 16;
@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
   if (p.B <= 32) {         // each warp by itself: no barrier, one load (one user 10.0 us, with the scan below 10.9)
     const int len = lane < p.B ? p.lengths[lane] : 0;
     const int tiles = lane < p.B ? (keys_of(p, len).n + C::KEYS - 1) / C::KEYS : 0;
-    const uint32_t mine = row_units(tiles);
+    const uint32_t mine = row_units<C::ROW_COST>(tiles);
     uint32_t upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
     const int per = (p.B + PG_WARPS * 32 - 1) / (PG_WARPS * 32);
     const int b_lo = min((int)threadIdx.x * per, p.B), b_hi = min(b_lo + per, p.B);
     int64_t mine = 0;
-    for (int b = b_lo; b < b_hi; ++b) mine += row_units((keys_of(p, p.lengths[b]).n + C::KEYS - 1) / C::KEYS);
+    for (int b = b_lo; b < b_hi; ++b) mine += row_units<C::ROW_COST>((keys_of(p, p.lengths[b]).n + C::KEYS - 1) / C::KEYS);
     int64_t upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -312,12 +312,12 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
 #pragma unroll 1
       for (int w = 0; w < PG_WARPS; ++w) {
         const int64_t f = line.begin((int64_t)blockIdx.x * PG_WARPS + w);
-        if (f >= base * heads && f < (base + row_units(tiles)) * heads) {
+        if (f >= base * heads && f < (base + row_units<C::ROW_COST>(tiles)) * heads) {
           sh_b[w] = b;
           sh_base[w] = base * heads;
         }
       }
-      base += row_units(tiles);
+      base += row_units<C::ROW_COST>(tiles);
     }
     __syncthreads();
     start_b = sh_b[warp];
@@ -350,20 +350,20 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
     return c * 32 + 8 * (g8 >> 1) + 2 * n + (g8 & 1);
   };
 
-  Cursor<C::KEYS> cu;
+  Cursor<C::KEYS, C::ROW_COST> cu;
   cu.at = length;
   if (length > 0) {
     cu.b = start_b;
     cu.load(p);
     const int64_t in = from - start_base;  // units of the sequence before the stretch
-    const int units = row_units(cu.tiles);
+    const int units = row_units<C::ROW_COST>(cu.tiles);
     cu.hr = in < (1LL << 31) ? (int)((uint32_t)in / (uint32_t)units) : (int)(in / units);
-    cu.j = (int)(in - (int64_t)cu.hr * units) - kRowCost;
+    cu.j = (int)(in - (int64_t)cu.hr * units) - C::ROW_COST;
     cu.at = max(-cu.j, 0);
     cu.j = max(cu.j, 0);
   }
   if (cu.at < length) {
-    Cursor<C::KEYS> ld = cu;
+    Cursor<C::KEYS, C::ROW_COST> ld = cu;
 
     // Page and row of what this lane looks up, one tile ahead of the copies: box `lane` of the tile, or keys lane, lane + 32.
     int page[C::OWN], row[C::OWN];
@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
       int here, page;
       uint4 fresh;
     };
-    auto fetch = [&](const Cursor<C::KEYS>& c, Row& w) {
+    auto fetch = [&](const Cursor<C::KEYS, C::ROW_COST>& c, Row& w) {
       const int kv = c.hr / p.row_tiles, r0 = (c.hr - kv * p.row_tiles) * R;
       const T* q = static_cast<const T*>(p.q) + c.b * p.q_b;
 #pragma unroll
@@ -518,7 +518,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
       }
     };
     Row now, ahead;
-    Cursor<C::KEYS> rows = cu;  // the row of `ahead`
+    Cursor<C::KEYS, C::ROW_COST> rows = cu;  // the row of `ahead`
 
     // where ldmatrix reads: chunk 0 of the lane's row; the chunk number's higher bits are xor-ed in
     const int mi = lane >> 3, l8 = lane & 7;
@@ -544,7 +544,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
 #pragma unroll 1
         for (; fetches > 0; --fetches) {
           now = ahead;
-          if (fetches == 2 || (cu.at + cu.tiles - cu.j + kRowCost < length && rows.next_row(p))) fetch(rows, ahead);
+          if (fetches == 2 || (cu.at + cu.tiles - cu.j + C::ROW_COST < length && rows.next_row(p))) fetch(rows, ahead);
         }
         fetches = 1;
 #pragma unroll

@@ -593,7 +593,7 @@ __global__ void __launch_bounds__(H_THREADS, 1) sample_hist_kernel(const SampleP
   const T none = Num<T>::from_f(-INFINITY);
   const uint32_t nones = *reinterpret_cast<const uint16_t*>(&none) * 0x10001u;
   const bool edges = first == 0 || first + mine == row_units;  // the row's first or last unit is among them
-  auto load_unit = [&](int step) { return step * 32 + lane < mine ? __ldg(source + first + step * 32 + lane) : make_uint4(nones, nones, nones, nones); };
+  auto load_unit = [&](int step) { return step * 32 + lane < mine ? source[first + step * 32 + lane] : make_uint4(nones, nones, nones, nones); };
   auto trim = [&](uint4& x, int step) {
     const int at = first + step * 32 + lane;
     if (at == 0 || at == row_units - 1) {
@@ -714,23 +714,17 @@ __global__ void __launch_bounds__(H_THREADS, 1) sample_hist_kernel(const SampleP
         for (int q = 0; q < W; ++q) equal += x[q] == above;
       }
       if (!__any_sync(0xffffffffu, high > above)) continue;
-#pragma unroll 1
-      for (int half = 0; half < 2; ++half) {  // (eight at once do not fit the registers)
-        float z[4];
+      if (near_by) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) z[q] = half ? x[4 + q] : x[q];
-        if (near_by) {
+        for (int q = 0; q < W; ++q) {
+          const double y = weigh_near(x[q]);
+          if (x[q] > above) sum += y;
+        }
+      } else {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const double y = weigh_near(z[q]);
-            if (z[q] > above) sum += y;
-          }
-        } else {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const double y = weigh_far(z[q]);
-            if (z[q] > above) sum += y;
-          }
+        for (int q = 0; q < W; ++q) {
+          const double y = weigh_far(x[q]);
+          if (x[q] > above) sum += y;
         }
       }
     }
