@@ -83,6 +83,24 @@ def test_equal_logits(dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("batch,vocab", [(1, 50304), (3, 2049), (150, 1500), (17, 131071), (2, 300)])
+def test_few_and_many_candidates(batch, vocab, dtype):
+    """Numbers of candidates around those at which they are found in another way, alone and with many equal logits among them."""
+    for i, k in enumerate((2, 31, 32, 33, 64, 200, 255, 256, 257, 1023, 1024, 1025)):
+        for x in (_logits(batch, vocab, dtype, i), _logits(batch, vocab, dtype, i, 2.0).round()):
+            _check(x[:5] if i % 3 else x, {"top_k": k, "top_p": (1.0, 0.9)[i % 2], "min_p": (0.0, 0.0, 0.01)[i % 3]}, i)
+    for i, least in enumerate((0.9, 0.3, 0.01, 1e-3, 1e-5, 1e-8)):
+        _check(_logits(batch, vocab, dtype, i)[:5], {"min_p": least, "temperature": (0.5, 1.0, 4.0)[i % 3]}, i)
+    # all that is left of a row is few: the rest is ruled out, in one place or all over
+    x = _logits(batch, vocab, dtype)
+    x[:, 40:] = -math.inf
+    _check(x[:5], {"top_k": 39}), _check(x[:5], {"top_k": 40, "top_p": 0.8}), _check(x[:5], {"top_k": 41}), _check(x[:5], {"min_p": 1e-4})
+    x = _logits(batch, vocab, dtype).masked_fill(torch.rand((batch, vocab), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda") < 0.97, -math.inf)
+    _check(x[:5], {"top_k": 20}), _check(x[:5], {"top_p": 0.7}), _check(x[:5], {"top_k": 100, "min_p": 0.1})
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
 def test_what_is_not_finite(dtype):
     for i, settings in enumerate(SETTINGS):
         x = _logits(8, 2500, dtype, i)

@@ -4,12 +4,21 @@
 //   first whose predecessors weigh less than p times the sum, of those the ones with w_i >= m;
 //   token = the first index j with  sum of the kept w_i, i <= j,  >  u * sum of the kept w_i.
 //
-// What is kept is a beginning of the order, so it is all logits above a value and some of those equal to it.  That value is searched
-// for, with nothing sorted: a round takes the count and weight above 8 values at once and goes on in the ninth part that holds the
-// border.  All sums are in 64 bits, weights to some 2^-48: a token is the drawn one or it is not, and where a sum meets the border
-// between two of 50 thousand tokens, 32 bits would now and then give the neighbour.
-// A cluster of 1 to 8 blocks has a row in its shared memory; blocks, warps and lanes hold it in the order of its columns, so that the
-// last sums, by warps, say which warp has the token.  Sums are taken in a fixed order: the same call gives the same token.
+// What is kept is a beginning of the order, so it is all logits above a value and some of those equal to it: that cut is what is looked for, and
+// nothing is sorted.  All sums are in 64 bits, weights to some 2^-39: a token is the drawn one or it is not, and where a sum meets the
+// border between two of 50 thousand tokens, 32 bits would now and then give the neighbour.  Sums are taken in a fixed order: the same call gives the same
+// token.
+//
+// A block or a cluster of blocks has a row; blocks, warps and lanes hold it in the order of its columns, so that the last sums, by warps, say which
+// warp has the token.  The cut comes from a list of candidates that are all compared (few of the largest, or of the heaviest), from a histogram over
+// all values (16 bits), or from a search (32 bits), below.
+//
+// Reading the logits is the least of it (13 MB for 128 rows of 50304: 2 us).  What bounds a call is the chain of its steps, each a barrier of 32 warps or
+// of a cluster (some 2000 cycles) with little between, and the exponentials where many logits are kept: 33 cycles of a scheduler each, nine sums and
+// products in 64 bits at two cycles, conversions and the table beside them.  Measured in graphs, fp16 logits: one row of 50304, top_k 40 and top_p 0.95,
+// 15.5 us; 128 rows of 50304, temperature alone 27.5, top_k 40 15.5, min_p 0.05 18.7, top_p 0.9 47; bf16, 16 rows of 131071, top_p 0.9 35.
+// fp32: 8 rows of 32000, temperature alone 14, top_k 40 31, top_p 0.9 59.
+#include <cfloat>
 #include <cooperative_groups.h>
 #include "common.cuh"
 
@@ -35,34 +44,17 @@ struct SampleParams {
   int warp_units;  // 16-byte units of a warp
 };
 
-// Whole numbers in the order of a type's values; -0 and 0 have one.
-template <typename T> struct Keys {
-  static constexpr uint32_t kSign = 0x8000u;
-  static __device__ __forceinline__ uint32_t of(float x) {  // x rounded to the type
-    const T v = Num<T>::from_f(x + 0.f);
-    const uint32_t u = *reinterpret_cast<const uint16_t*>(&v);
-    return (u & kSign ? 0u - u : u | kSign) & 0xffffu;
-  }
-  static __device__ __forceinline__ float value(uint32_t k) {
-    const uint16_t u = (uint16_t)(k & kSign ? k ^ kSign : 0u - k);
-    return Num<T>::to_f(*reinterpret_cast<const T*>(&u));
-  }
-};
-template <> struct Keys<float> {
-  static __device__ __forceinline__ uint32_t of(float x) {
-    const uint32_t u = __float_as_uint(x + 0.f);
-    return u & 0x80000000u ? 0u - u : u | 0x80000000u;
-  }
-  static __device__ __forceinline__ float value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : 0u - k); }
-};
-
-template <typename T> constexpr int kPerUnit = 16 / sizeof(T);
-template <typename T> __device__ __forceinline__ void unpack_unit(const uint4& v, float (&x)[kPerUnit<T>]) {
-  if constexpr (sizeof(T) == 4) {
-    x[0] = __uint_as_float(v.x); x[1] = __uint_as_float(v.y); x[2] = __uint_as_float(v.z); x[3] = __uint_as_float(v.w);
-  } else {
-    unpack8<T>(v, x);
-  }
+// Whole numbers in the order of 32-bit values; -0 and 0 have one.
+__device__ __forceinline__ uint32_t key_of(float x) {
+  const uint32_t u = __float_as_uint(x + 0.f);
+  return u & 0x80000000u ? 0u - u : u | 0x80000000u;
+}
+__device__ __forceinline__ float value_of_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : 0u - k); }
+__device__ __forceinline__ void unpack4(const uint4& v, float (&x)[4]) {
+  x[0] = __uint_as_float(v.x);
+  x[1] = __uint_as_float(v.y);
+  x[2] = __uint_as_float(v.z);
+  x[3] = __uint_as_float(v.w);
 }
 
 // 2^y for y <= 0, by Tang's method (ACM TOMS 15, 1989): 2^(i / 32) from a table, one entry in each lane, times a polynomial for the rest.
@@ -104,9 +96,11 @@ struct Shared {
 
 }  // namespace
 
-template <typename T>
-__global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams p) {
-  constexpr int W = kPerUnit<T>;
+// ---------------------------------------------------------------------------------------------------------- 32 bits
+// The search: a round takes the count and weight above 8 values at once and goes on in the ninth part that holds the border, in steps of value and of
+// representation in turn.  The row lies in the cluster's shared memory.
+__global__ void __launch_bounds__(SM_THREADS) sample_search_kernel(const SampleParams p) {
+  constexpr int W = 4;
   extern __shared__ uint4 units[];
   __shared__ Shared sh;
   cg::cluster_group cluster = cg::this_cluster();
@@ -139,29 +133,28 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams p
   const double per = kLog2eD / (double)t;
 
   // ---- the warp's part of the row: 16-byte units of memory, with what is not the row's as -infinity
-  const T* logits = static_cast<const T*>(p.logits) + row * p.ld;
-  const int shift = (int)((reinterpret_cast<uintptr_t>(logits) & 15) / sizeof(T));
+  const float* logits = static_cast<const float*>(p.logits) + row * p.ld;
+  const int shift = (int)((reinterpret_cast<uintptr_t>(logits) & 15) / sizeof(float));
   const uint4* source = reinterpret_cast<const uint4*>(logits - shift);
   const int row_units = (p.vocab + shift + W - 1) / W;
   const int first = (rank * SM_WARPS + warp) * p.warp_units;
   const int mine = max(0, min(p.warp_units, row_units - first));  // of these units there are
   uint4* part = units + warp * p.warp_units;
-  const T none = Num<T>::from_f(-INFINITY);
   float top = -INFINITY, bottom = INFINITY;
   int finite = 0;
   for (int i = lane; i < mine; i += 32) {
     uint4 v = ld_stream16(source + first + i);
     if (first + i == 0 || first + i == row_units - 1) {
-      T* e = reinterpret_cast<T*>(&v);
+      float* e = reinterpret_cast<float*>(&v);
 #pragma unroll
       for (int q = 0; q < W; ++q) {
         const int c = (first + i) * W + q - shift;
-        if (c < 0 || c >= p.vocab) e[q] = none;
+        if (c < 0 || c >= p.vocab) e[q] = -INFINITY;
       }
     }
     part[i] = v;
     float x[W];
-    unpack_unit<T>(v, x);
+    unpack4(v, x);
 #pragma unroll
     for (int q = 0; q < W; ++q) {
       top = fmaxf(top, x[q]);
@@ -264,22 +257,22 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams p
   };
 
   // The cut: all logits above `cut` and the first `ties` of those equal to it.  Below every logit: all of them.
-  const uint32_t over = Keys<T>::of(top) + 1;
-  uint32_t low = Keys<T>::of(bottom) - 1, high = over;  // the search's borders: reached at `low`, not at `high`
+  const uint32_t over = key_of(top) + 1;
+  uint32_t low = key_of(bottom) - 1, high = over;  // the search's borders: reached at `low`, not at `high`
   const uint32_t under = low;
   int count_low = finite, count_high = 0;  // logits at or above the two
   double sum_high = 0.0;
   int ties = 0;
   float cuts[SM_CUTS];
   auto place = [&](int round) {  // 8 values between the borders, descending
-    const float a = Keys<T>::value(low), b = Keys<T>::value(high);
+    const float a = value_of_key(low), b = value_of_key(high);
     const bool even = high - low <= SM_CUTS + 1 || (round & 1) != 0 || !isfinite(b - a);
 #pragma unroll
     for (int i = 0; i < SM_CUTS; ++i) {
       uint32_t key;
       if (even) key = high - max((uint32_t)(((uint64_t)(high - low) * (i + 1)) / (SM_CUTS + 1)), 1u);
-      else key = Keys<T>::of(b - (b - a) * ((i + 1) / (float)(SM_CUTS + 1)));
-      cuts[i] = Keys<T>::value(min(max(key, low + 1), high - 1));
+      else key = key_of(b - (b - a) * ((i + 1) / (float)(SM_CUTS + 1)));
+      cuts[i] = value_of_key(min(max(key, low + 1), high - 1));
     }
   };
   auto narrow = [&](int i_low, const double (&s)[SM_CUTS], const int (&c)[SM_CUTS]) {  // the first of the cuts that reaches the goal
@@ -291,10 +284,10 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams p
       if (i < i_low) {
         sum = sum_high + s[i];
         count = count_high + c[i];
-        h = Keys<T>::of(cuts[i]);
+        h = key_of(cuts[i]);
       }
       if (i == i_low) {
-        low = Keys<T>::of(cuts[i]);
+        low = key_of(cuts[i]);
         count_low = count_high + c[i];
       }
     }
@@ -304,12 +297,12 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams p
   };
 
   if (k == 1) {
-    low = Keys<T>::of(top);
+    low = key_of(top);
     ties = 1;
   } else if (k > 0 && k < finite) {
     for (int round = 0; high - low > 1 && round < 64; ++round) {
       place(round);
-      const float a = Keys<T>::value(low), b = Keys<T>::value(high);
+      const float a = value_of_key(low), b = value_of_key(high);
       const bool open = high == over;  // whose value may be none
       double s[SM_CUTS];
       int c[SM_CUTS];
@@ -320,7 +313,7 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams p
       }
       for (int i = lane; i < mine; i += 32) {
         float x[W];
-        unpack_unit<T>(part[i], x);
+        unpack4(part[i], x);
 #pragma unroll
         for (int q = 0; q < W; ++q)
           if (x[q] > a && (open || x[q] < b))
@@ -342,7 +335,7 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams p
   if (nucleus) {
     // of what is left the first whose predecessors weigh less than p times the sum
     const int tied = ties;
-    const double low_weight = __shfl_sync(0xffffffffu, weigh(Keys<T>::value(low)), 0);
+    const double low_weight = __shfl_sync(0xffffffffu, weigh(value_of_key(low)), 0);
     const uint32_t floor = low;
     high = over;
     count_high = 0;
@@ -353,11 +346,11 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams p
         const float steps[SM_CUTS] = {0.7f, 1.5f, 2.5f, 4.f, 6.f, 8.5f, 12.f, 0.f};
 #pragma unroll
         for (int i = 0; i < SM_CUTS; ++i)
-          cuts[i] = Keys<T>::value(min(max(Keys<T>::of(isfinite(top) ? top - steps[i] * t : top), low + 1), high - 1));
+          cuts[i] = value_of_key(min(max(key_of(isfinite(top) ? top - steps[i] * t : top), low + 1), high - 1));
       } else {
         place(round);
       }
-      const float a = Keys<T>::value(low), b = Keys<T>::value(high);
+      const float a = value_of_key(low), b = value_of_key(high);
       const bool open = high == over;  // whose value may be none
       double s[SM_CUTS];
       int c[SM_CUTS];
@@ -370,7 +363,7 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams p
       for (int step = 0; step < steps; ++step) {
         const int i = step * 32 + lane;
         float x[W];
-        unpack_unit<T>(part[min(i, mine - 1)], x);
+        unpack4(part[min(i, mine - 1)], x);
 #pragma unroll
         for (int q = 0; q < W; ++q) {
           const bool in = i < mine && x[q] > a && (open || x[q] < b);
@@ -389,7 +382,7 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams p
       reduce(s, c);
       if (round == 0) {
         goal = (double)top_p * (s[SM_CUTS - 1] + tied * low_weight);
-        cuts[SM_CUTS - 1] = Keys<T>::value(low);  // what lies at `low` or above it reaches the goal
+        cuts[SM_CUTS - 1] = value_of_key(low);  // what lies at `low` or above it reaches the goal
       }
       int reached = SM_CUTS;
 #pragma unroll
@@ -405,7 +398,7 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams p
         narrow(reached, s, c);
       }
     }
-    const double w = __shfl_sync(0xffffffffu, weigh(Keys<T>::value(low)), 0);
+    const double w = __shfl_sync(0xffffffffu, weigh(value_of_key(low)), 0);
     const double fit = ceil((goal - sum_high) / w);
     const int there = low == floor ? tied : count_low - count_high;
     ties = fit < there ? max((int)fit, 1) : there;  // (w = 0: infinite, or NaN)
@@ -413,7 +406,7 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams p
   }
 
   // ---- the kept weights of each warp, then the warp that has the token
-  const float cut = Keys<T>::value(low);
+  const float cut = value_of_key(low);
   const double cut_weight = __shfl_sync(0xffffffffu, weigh(cut), 0);
   const bool ties_kept = ties > 0 && cut_weight >= (double)min_p;
   const int steps = (mine + 31) / 32;
@@ -422,7 +415,7 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams p
   for (int step = 0; step < steps; ++step) {
     const int i = step * 32 + lane;
     float x[W];
-    unpack_unit<T>(part[min(i, mine - 1)], x);
+    unpack4(part[min(i, mine - 1)], x);
 #pragma unroll
     for (int q = 0; q < W; ++q) {
       const bool in = i < mine && x[q] > cut;
@@ -465,7 +458,7 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams p
   for (int step = 0; step < steps; ++step) {
     const int i = step * 32 + lane;
     float x[W];
-    unpack_unit<T>(part[min(i, mine - 1)], x);
+    unpack4(part[min(i, mine - 1)], x);
     int n = 0;
 #pragma unroll
     for (int q = 0; q < W; ++q) n += i < mine && x[q] == cut;
@@ -520,6 +513,10 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleParams p
 }
 
 // ---------------------------------------------------------------------------------------------------------- 16 bits
+// Few candidates.  The k-th largest of the threads' largest logits is not above the k-th largest logit, so what lies below it is out; the same holds for
+// each block of a cluster.  What is left, some more than k from each block, is put in a list; up to 256 of them are compared each with each,
+// which gives ranks and the weight ahead of each at once (one row, top_k 40: 20 us by the histogram, 15.5 so).
+//
 // Logits of 16 bits have 2^16 values, and equal logits weigh the same: a histogram over all values is all that the cut needs.  Blocks count their
 // part of the row (a counter of 16 bits for each value, 128 KB of shared memory), the blocks of a cluster add theirs up where there is
 // something to add, and a scan over rows of 64 values gives the cut, with an exponential for each value that occurs instead of each logit.
@@ -528,6 +525,7 @@ namespace {
 
 constexpr int H_THREADS = 1024, H_WARPS = 32, H_ROWS = 1024;  // rows of 64 values, two to a word
 constexpr int H_UNITS = 8;                                    // 16-byte units of a lane
+constexpr int H_FEW = 256;                                    // logits that are compared each with each
 constexpr int kMostCounted = H_THREADS * H_UNITS * 8 - 8;     // logits of a block: a counter holds as many
 
 // Values in descending order: bin 0 is the last positive NaN, then infinity, .., the lowest, -infinity and the negative NaNs.
@@ -555,6 +553,9 @@ struct HistShared {
   float warp_tops[H_WARPS], warp_lows[H_WARPS], tops[SM_CLUSTER];
   int found, cut, ties, owner, owner_ties, to_last;
   double before, owner_before, goal;
+  int few[SM_CLUSTER], limits[SM_CLUSTER], total;
+  int list_bin[H_FEW], list_col[H_FEW], part_count[4][H_FEW];
+  double list_weight[H_FEW], part_weight[4][H_FEW];
   double all_sums[SM_CLUSTER * H_WARPS];
   int all_ties[SM_CLUSTER * H_WARPS];
 };
@@ -754,6 +755,170 @@ __global__ void __launch_bounds__(H_THREADS, 1) sample_hist_kernel(const SampleP
       if (__syncthreads_count(own <= mid) >= k) limit = mid;
       else lo = mid;
     }
+  }
+
+  // ---- Few of them: a list in the order of the columns, each compared with all others.
+  const bool threshold = k == 0 && !nucleus && min_p > 0.f;
+  if ((k > 1 && k <= H_FEW) || threshold) {
+    if (threshold) {  // a little below what weighs enough
+      const float least = t * logf(min_p);
+      limit = min(bin_of(isfinite(top) ? fmaxf(top + least - 1e-5f * (fabsf(top) - least), -FLT_MAX) : top) + 1, limit);
+    }
+    uint2* raw = reinterpret_cast<uint2*>(smem_units + H_ROWS * 8);  // the first block's has (bin, column) of each block's, H_FEW to a block
+    uint2* to_first = cluster.map_shared_rank(raw, 0) + rank * H_FEW;
+    auto few = [&](uint32_t bin) { return bin - Bins<T>::kTop <= (uint32_t)(limit - Bins<T>::kTop); };
+    int mine_few = 0;
+    uint32_t some = 0;  // units with any in the warp
+#pragma unroll
+    for (int i = 0; i < H_UNITS; ++i) {
+      if (i * 32 >= mine) break;
+      const uint32_t words[4] = {bins_of<T>(v[i].x), bins_of<T>(v[i].y), bins_of<T>(v[i].z), bins_of<T>(v[i].w)};
+      int n = 0;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) n += few(words[q] & 0xffffu) + few(words[q] >> 16);
+      mine_few += n;
+      some |= (uint32_t)(__any_sync(0xffffffffu, n != 0) != 0) << i;
+    }
+    const int warp_few = __reduce_add_sync(0xffffffffu, mine_few);
+    if (lane == 0) sh.warp_counts[warp] = warp_few;
+    __syncthreads();
+    int upto = sh.warp_counts[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int n = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += n;
+    }
+    const int block_few = __shfl_sync(0xffffffffu, upto, 31);
+    int at = __shfl_sync(0xffffffffu, upto, warp) - warp_few;  // the warp's first place
+    if (block_few <= H_FEW) {
+#pragma unroll 1
+      for (; some != 0; some &= some - 1) {
+        const int step = __ffs(some) - 1;
+        const uint4 unit = unit_at(step);
+        const uint32_t words[4] = {bins_of<T>(unit.x), bins_of<T>(unit.y), bins_of<T>(unit.z), bins_of<T>(unit.w)};
+        int n = 0;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) n += few(words[q] & 0xffffu) + few(words[q] >> 16);
+        int lanes = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int m = __shfl_up_sync(0xffffffffu, lanes, o);
+          if (lane >= o) lanes += m;
+        }
+        int place = at + lanes - n;
+        at += __shfl_sync(0xffffffffu, lanes, 31);
+        if (n != 0) {
+#pragma unroll
+          for (int q = 0; q < W; ++q) {
+            const uint32_t bin = q & 1 ? words[q / 2] >> 16 : words[q / 2] & 0xffffu;
+            if (few(bin)) {
+              to_first[place++] = make_uint2(bin, (first + step * 32 + lane) * W + q - shift);
+            }
+          }
+        }
+      }
+    }
+    if (tid < blocks) {
+      HistShared* to = cluster.map_shared_rank(&sh, tid);
+      to->few[rank] = block_few;
+      to->limits[rank] = limit;
+    }
+    sync();
+    // The first block has those within all blocks' bounds, still in order; if they are too many it says so.
+    int total = 0;
+    if (rank == 0) {
+      bool in[2];
+      uint2 entry[2];
+      int most = 0, bound = Bins<T>::kEnd;
+      for (int b = 0; b < blocks; ++b) {
+        most = max(most, sh.few[b]);
+        bound = min(bound, sh.limits[b]);
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int place = 2 * tid + e;
+        in[e] = most <= H_FEW && place < blocks * H_FEW && (place & (H_FEW - 1)) < sh.few[place / H_FEW];
+        entry[e] = in[e] ? raw[place] : make_uint2(0, 0);
+        in[e] = in[e] && (int)entry[e].x <= bound;
+      }
+      const unsigned ones[2] = {__ballot_sync(0xffffffffu, in[0]), __ballot_sync(0xffffffffu, in[1])}, lt = (1u << lane) - 1;
+      if (lane == 0) sh.warp_counts[warp] = __popc(ones[0]) + __popc(ones[1]);
+      __syncthreads();
+      int warps = sh.warp_counts[lane];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int n = __shfl_up_sync(0xffffffffu, warps, o);
+        if (lane >= o) warps += n;
+      }
+      total = most <= H_FEW ? __shfl_sync(0xffffffffu, warps, 31) : H_FEW + 1;
+      int to = __shfl_sync(0xffffffffu, warps, warp) - (__popc(ones[0]) + __popc(ones[1])) + __popc(ones[0] & lt) + __popc(ones[1] & lt);
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (in[e] && to < H_FEW) {
+          sh.list_bin[to] = entry[e].x;
+          sh.list_col[to++] = entry[e].y;
+        }
+      if (tid < blocks) cluster.map_shared_rank(&sh, tid)->total = total;
+    }
+    sync();
+    total = sh.total;
+    if (total <= H_FEW) {
+      if (rank != 0) return;
+      const int i = tid & (H_FEW - 1), part = tid / H_FEW;
+      const bool real = i < total;
+      const int bin = real ? sh.list_bin[i] : Bins<T>::kEnd;
+      const double w = weigh(real ? value_of<T>(bin) : top);
+      if (part == 0) sh.list_weight[i] = real ? w : 0.0;
+      __syncthreads();
+      int before = 0;
+      double ahead = 0.0;
+      for (int j = part * (H_FEW / 4); j < min((part + 1) * (H_FEW / 4), total); ++j) {
+        const int other = sh.list_bin[j];
+        const bool is = other < bin || (other == bin && j < i);
+        before += is;
+        if (is) ahead += sh.list_weight[j];
+      }
+      sh.part_count[part][i] = before;
+      sh.part_weight[part][i] = ahead;
+      __syncthreads();
+      before = 0;
+      ahead = 0.0;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        before += sh.part_count[q][i];
+        ahead += sh.part_weight[q][i];
+      }
+      const int wanted = k > 0 ? min(k, total) : total;
+      if (part == 0 && real && before == wanted - 1) sh.before = ahead + w;
+      __syncthreads();
+      const double goal = (double)top_p * sh.before, enough = (double)min_p * weigh(top);
+      const bool keep = part == 0 && real && before < wanted && (!nucleus || before == 0 || ahead < goal) && w >= enough;
+      double line = keep ? w : 0.0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double n = __shfl_up_sync(0xffffffffu, line, o);
+        if (lane >= o) line += n;
+      }
+      if (lane == 31) sh.warp_weights[warp] = line;
+      if (tid == 0) sh.owner = -1;
+      __syncthreads();
+      double all = 0.0, base = 0.0;
+#pragma unroll
+      for (int q = 0; q < H_FEW / 32; ++q) {
+        if (q < warp) base += sh.warp_weights[q];
+        all += sh.warp_weights[q];
+      }
+      line += base;
+      // the first whose sum is above the goal; where rounding leaves none, the last
+      const double aim = (double)u * all;
+      if (keep && line > aim) atomicMin(&sh.found, i);
+      if (keep) atomicMax(&sh.owner, i);
+      __syncthreads();
+      if (tid == 0) p.out[row] = sh.list_col[sh.found < H_ROWS ? sh.found : sh.owner];
+      return;
+    }
+    // more than that: as any others, each block by its own bound
+    limit = k == 0 ? Bins<T>::kEnd - 1 : limit;
   }
 
   uint32_t set = 0;  // bit i: row 32 i + lane has logits
@@ -1122,35 +1287,41 @@ int sample_start(K kernel, const SampleParams& p, int64_t B, int blocks, int thr
   return launched("sample");
 }
 
+// 16 bits
 template <typename T>
-int sample_launch(SampleParams p, int64_t B, cudaStream_t st) {
-  constexpr int W = kPerUnit<T>;
-  const int64_t row_units = ceil_div((int64_t)p.vocab + W - 1, W);
+int sample_by_histogram(SampleParams p, int64_t B, cudaStream_t st) {
+  const int64_t row_units = ceil_div((int64_t)p.vocab + 7, 8);
   int blocks = 1;
-  if constexpr (sizeof(T) == 2) {
-    // blocks of a row: what their counters hold, and more where they find half of the SMs free (16 rows of 131071: 22 to 34 us with 2 or 4
-    // blocks; with 8, whose clusters do not all find room at once, 28 to 51)
-    while (blocks < SM_CLUSTER && ((int64_t)p.vocab > (int64_t)kMostCounted * blocks || (B * blocks * 4 <= sm_count() && row_units > H_THREADS / 2 * blocks)))
-      blocks *= 2;
-    if ((int64_t)p.vocab > (int64_t)kMostCounted * blocks)
-      return fail(TFB_ERR_UNSUPPORTED, "sample: %d logits in a row are more than a cluster has room for", p.vocab);
-    p.warp_units = (int)ceil_div(row_units, (int64_t)H_WARPS * blocks);
-    static std::atomic<uint64_t> done{0};
-    constexpr int smem = H_ROWS * 128;
-    if (int rc = ensure_dynamic_smem(sample_hist_kernel<T>, smem, done, "sample")) return rc;
-    return sample_start(sample_hist_kernel<T>, p, B, blocks, H_THREADS, smem, st);
-  } else {
-    // blocks of a row: what the SMs have room for, and as many as its logits need
-    while (blocks < SM_CLUSTER && (B * blocks < sm_count() || ceil_div(row_units, (int64_t)SM_WARPS * blocks) * SM_WARPS * 16 > 104 * 1024) &&
-           row_units > (int64_t)SM_THREADS * blocks)
-      blocks *= 2;
-    p.warp_units = (int)ceil_div(row_units, (int64_t)SM_WARPS * blocks);
-    const int64_t smem = (int64_t)p.warp_units * SM_WARPS * 16;
-    if (smem > 212 * 1024) return fail(TFB_ERR_UNSUPPORTED, "sample: %d logits in a row are more than a cluster has room for", p.vocab);
-    static std::atomic<uint64_t> done{0};
-    if (int rc = ensure_dynamic_smem(sample_kernel<T>, 212 * 1024, done, "sample")) return rc;
-    return sample_start(sample_kernel<T>, p, B, blocks, SM_THREADS, smem, st);
-  }
+  // blocks of a row: what their counters hold, and up to four where they find half of the SMs free (16 rows of 131071: 22 to 34 us with 2 or 4
+  // blocks; with 8, whose clusters do not all find room at once, 28 to 51.  One row of 50304, top_k 40: 15.5 us with 4 blocks, 22 with 8, whose
+  // own 40 largest are too many together for the list)
+  while (blocks < SM_CLUSTER && ((int64_t)p.vocab > (int64_t)kMostCounted * blocks ||
+                                 (blocks < 4 && B * blocks * 4 <= sm_count() && row_units > H_THREADS / 2 * blocks)))
+    blocks *= 2;
+  if ((int64_t)p.vocab > (int64_t)kMostCounted * blocks)
+    return fail(TFB_ERR_UNSUPPORTED, "sample: %d logits in a row are more than a cluster has room for", p.vocab);
+  p.warp_units = (int)ceil_div(row_units, (int64_t)H_WARPS * blocks);
+  static std::atomic<uint64_t> done{0};
+  constexpr int smem = H_ROWS * 128 + SM_CLUSTER * H_FEW * 8;
+  if (int rc = ensure_dynamic_smem(sample_hist_kernel<T>, smem, done, "sample")) return rc;
+  return sample_start(sample_hist_kernel<T>, p, B, blocks, H_THREADS, smem, st);
+}
+
+// 32 bits
+int sample_by_search(SampleParams p, int64_t B, cudaStream_t st) {
+  const int64_t row_units = ceil_div((int64_t)p.vocab + 3, 4);
+  int blocks = 1;
+  // blocks of a row: what the SMs have room for, and as many as its logits need
+  while (blocks < SM_CLUSTER && (B * blocks < sm_count() || ceil_div(row_units, (int64_t)SM_WARPS * blocks) * SM_WARPS * 16 > 104 * 1024) &&
+         row_units > (int64_t)SM_THREADS * blocks)
+    blocks *= 2;
+  p.warp_units = (int)ceil_div(row_units, (int64_t)SM_WARPS * blocks);
+  const int64_t smem = (int64_t)p.warp_units * SM_WARPS * 16;
+  if (smem > 212 * 1024)
+    return fail(TFB_ERR_UNSUPPORTED, "sample: %d logits in a row are more than a cluster has room for", p.vocab);
+  static std::atomic<uint64_t> done{0};
+  if (int rc = ensure_dynamic_smem(sample_search_kernel, 212 * 1024, done, "sample")) return rc;
+  return sample_start(sample_search_kernel, p, B, blocks, SM_THREADS, smem, st);
 }
 
 }  // namespace
@@ -1179,8 +1350,8 @@ extern "C" int tfb_sample(const void* logits, int64_t ld, const float* uniforms,
   p.min_p_all = min_p_all;
   p.out = out;
   p.vocab = (int)vocab;
-  if (dtype == TFB_F32) return sample_launch<float>(p, B, (cudaStream_t)stream);
-  if (dtype == TFB_F16) return sample_launch<__half>(p, B, (cudaStream_t)stream);
-  if (dtype == TFB_BF16) return sample_launch<__nv_bfloat16>(p, B, (cudaStream_t)stream);
+  if (dtype == TFB_F32) return sample_by_search(p, B, (cudaStream_t)stream);
+  if (dtype == TFB_F16) return sample_by_histogram<__half>(p, B, (cudaStream_t)stream);
+  if (dtype == TFB_BF16) return sample_by_histogram<__nv_bfloat16>(p, B, (cudaStream_t)stream);
   return fail(TFB_ERR_ARG, "sample: dtype %d", dtype);
 }
