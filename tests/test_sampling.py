@@ -83,6 +83,20 @@ def test_equal_logits(dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("batch,vocab", [(3, 65272), (2, 65535), (40, 65536), (40, 130544), (40, 130545), (40, 131056), (2, 522176 - 150000)])
+def test_more_equal_logits_than_a_short_counter_holds(batch, vocab, dtype):
+    """Equal weights: the kept ones are the first ones, and the token is the whole part of u times their number.  (i + 1/2) / n in 32 bits, times n
+    again, is within n 2^-24 < 1/32 of i + 1/2."""
+    x = torch.zeros((batch, vocab), device="cuda", dtype=dtype)  # weights of 1: exact sums
+    for settings, kept in (({}, vocab), ({"top_k": 30000}, 30000), ({"top_p": 0.5}, (vocab + 1) // 2), ({"min_p": 1.0}, vocab),
+                           ({"top_k": 50000, "top_p": 0.25}, 12500)):
+        want = torch.linspace(0, kept - 1, batch, dtype=torch.float64).round().long()
+        u = ((want + 0.5) / kept).float().cuda()
+        assert sample_tokens(x, u, **settings).tolist() == want.tolist()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("batch,vocab", [(1, 50304), (3, 2049), (150, 1500), (17, 131071), (2, 300)])
 def test_few_and_many_candidates(batch, vocab, dtype):
     """Numbers of candidates around those at which they are found in another way, alone and with many equal logits among them."""
@@ -206,7 +220,7 @@ def test_refusals():
     for call, text in ((lambda: sample_tokens(x[0], u), r"\(batch, vocab\)"), (lambda: sample_tokens(x, u[:2]), "uniform"),
                        (lambda: sample_tokens(x, u.double()), "uniform"), (lambda: sample_tokens(x.long(), u), "fp16, bf16 or fp32"),
                        (lambda: sample_tokens(x, u, temperature=-0.1), "temperature"), (lambda: sample_tokens(x, u, temperature=math.inf), "temperature"),
-                       (lambda: sample_tokens(x, u, top_k=-1), "top_k"), (lambda: sample_tokens(x, u, top_p=0.0), "top_p"),
+                       (lambda: sample_tokens(x, u, top_k=-1), "top_k"), (lambda: sample_tokens(x, u, top_k=2.5), "whole number"), (lambda: sample_tokens(x, u, top_p=0.0), "top_p"),
                        (lambda: sample_tokens(x, u, top_p=1.1), "top_p"), (lambda: sample_tokens(x, u, min_p=1.5), "min_p"),
                        (lambda: sample_tokens(x, u, top_k=u), "int32"), (lambda: sample_tokens(x, u, temperature=u[:1]), "fp32"),
                        (lambda: sample_tokens(x.cpu(), u), "CUDA"), (lambda: sample_tokens(x.clone().requires_grad_(), u), "no gradients")):

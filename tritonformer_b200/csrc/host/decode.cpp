@@ -128,7 +128,8 @@ Tensor sample(const Tensor& logits_, const Tensor& uniforms_, const Setting& tem
   const Tensor t = each_row(temperature, B, at::kFloat, "temperature"), k = each_row(top_k, B, at::kInt, "top_k"),
                p = each_row(top_p, B, at::kFloat, "top_p"), m = each_row(min_p, B, at::kFloat, "min_p");
   TFB_ASSERT(std::isfinite(temperature.all) && temperature.all >= 0, "sample_tokens: temperature: expected a finite number from 0 on");
-  TFB_ASSERT(top_k.all >= 0 && top_k.all < (1LL << 31), "sample_tokens: top_k: expected a number from 0 (all) on");
+  TFB_ASSERT(top_k.all >= 0 && top_k.all < (1LL << 31) && top_k.all == std::floor(top_k.all),
+             "sample_tokens: top_k: expected a whole number from 0 (all) on");
   TFB_ASSERT(top_p.all > 0 && top_p.all <= 1, "sample_tokens: top_p: expected a number above 0, up to 1");
   TFB_ASSERT(min_p.all >= 0 && min_p.all <= 1, "sample_tokens: min_p: expected a number from 0 to 1");
   const c10::cuda::CUDAGuard device(logits_.device());

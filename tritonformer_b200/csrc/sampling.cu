@@ -526,7 +526,8 @@ namespace {
 constexpr int H_THREADS = 1024, H_WARPS = 32, H_ROWS = 1024;  // rows of 64 values, two to a word
 constexpr int H_UNITS = 8;                                    // 16-byte units of a lane
 constexpr int H_FEW = 256;                                    // logits that are compared each with each
-constexpr int kMostCounted = H_THREADS * H_UNITS * 8 - 8;     // logits of a block: a counter holds as many
+// Logits of a block, at most: with one unit of a lane less than there is room for no block of a cluster has 2^16, which a counter does not hold.
+constexpr int kMostCounted = H_WARPS * (H_UNITS * 32 - 1) * 8 - 8;
 
 // Values in descending order: bin 0 is the last positive NaN, then infinity, .., the lowest, -infinity and the negative NaNs.
 template <typename T> struct Bins;
