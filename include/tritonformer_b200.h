@@ -380,8 +380,9 @@ int tfb_cache_evict(const void* k_pages, const void* v_pages, const float* mass,
 
 /* The same cache in 4 bits: pages (num_pages, kv_heads, page, hd / 2) of bytes, page_strides in bytes (multiples of 16, 16-byte aligned bases),
  * and contiguous scales (num_pages, kv_heads, page, 2) of the 16-bit type, a row's of its key and of its value.  A value is its row's
- * scale times a whole number c from -7 to 7: the scale is the row's largest magnitude over 7, rounded to the type (NaN where a value is not finite),
- * c the nearest to value / scale, ties to even.  The 32-bit word w of a row holds dims 8 w .. 8 w + 7, dim 8 w + 2 n + e at
+ * scale times a whole number c from -7 to 7: the scale is the row's largest magnitude over 7, rounded to the type, at most the largest whose
+ * sevenfold the type holds (9352 in fp16), NaN where a value is not finite; c is the nearest to value / scale, ties to even.
+ * The 32-bit word w of a row holds dims 8 w .. 8 w + 7, dim 8 w + 2 n + e at
  * bits 4 n + 16 e, as c + 8.  Such a cache has no statistics: a key's position is its slot's number.
  *
  * tfb_paged_attention_int4: tfb_paged_attention on it; q, the new rows and out are of the 16-bit type; the new row is attended to as it is stored.
@@ -408,8 +409,8 @@ int tfb_cache_append_int4(const void* key, const void* value, void* k_pages, voi
  * r + 8 at rows 64 unit + 32 (t / 2) + 8 j + 4 (t % 2) + 0..3; row offset 2 p + e of column half c lies at bits 4 (c + 2 p) + 16 e, as c + 8.
  * scales: tfb_int4_scales() values (strip, group of the padded rows, r, column half).  Both 16-byte aligned.
  *
- * tfb_int4_quantize: codes and scales of w, element strides w_k, w_n.  s = (largest magnitude of the group) / 7, rounded to the type, and NaN where
- * a weight is not finite; c = W / s rounded to the nearest whole number, ties to even.
+ * tfb_int4_quantize: codes and scales of w, element strides w_k, w_n.  s = (largest magnitude of the group) / 7, rounded to the type, at most
+ * the largest number whose sevenfold the type holds, and NaN where a weight is not finite; c = W / s rounded to the nearest whole number, ties to even.
  * tfb_int4_expand: s * c rounded to the type, transposed: out (16 * strips, 64 * units), 16-byte aligned.
  * tfb_int4_linear: out = act(x W + bias) + addend for M rows of x (pitch x_ld, unit stride, any alignment), out and addend of pitch
  * out_ld, addend_ld; bias (N) and addend may be NULL, the addend may be the output.  For few rows: every 32 of them read the weights again.  */

@@ -13,6 +13,7 @@ import tritonformer_b200._lib as L
 from tritonformer_b200 import Int4Weight, int4, linear_int4, quantize_int4
 
 U = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+LARGEST = {torch.float16: 9352.0, torch.bfloat16: 36.25 * 2.0 ** 120}  # the scales whose sevenfold is not above the largest value
 gpu = pytest.mark.gpu
 
 
@@ -32,7 +33,7 @@ def _definition(w, group):
     padded[:k] = w.double()
     blocks = padded.view(groups, group, n)
     top = blocks.abs().amax(1)
-    scales = torch.where(top.isfinite(), top / 7, torch.nan).to(w.dtype).double()
+    scales = torch.where(top.isfinite(), top / 7, torch.nan).to(w.dtype).double().clamp(max=LARGEST[w.dtype])
     codes = torch.where(scales[:, None] > 0, blocks / scales[:, None], 0.0).round().clamp(-7, 7)
     return codes.view(-1, n)[:k], scales.repeat_interleave(group, 0)[:k]
 
@@ -160,6 +161,37 @@ def test_linear_addend_and_bias_of_any_layout():
     q = quantize_int4(w)
     a, b = _randn(96, 4, seed=3, dtype=torch.float16).t(), _randn(96, 2, seed=4, dtype=torch.float16)[:, 0]
     assert torch.equal(linear_int4(x, q, b, False, a), linear_int4(x, q, b.contiguous(), False, a.contiguous()))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_the_largest_weights_stay_finite(dtype):
+    """7 LARGEST, rounded to the type, is what the type's largest value becomes.  Powers of two of it round alike."""
+    w = torch.zeros((64, 17), device="cuda", dtype=dtype)
+    w[3, 2], w[5, 16], w[6, 16] = torch.finfo(dtype).max, -torch.finfo(dtype).max, torch.finfo(dtype).max / 2
+    q = quantize_int4(w)
+    codes, scales = _definition(w, 64)
+    assert torch.equal(q.dequantize(), (codes * scales).to(dtype)) and q.dequantize().isfinite().all()
+    for m in (1, 70):
+        x = torch.zeros((m, 64), device="cuda", dtype=dtype)
+        x[0, 3], x[-1, 5] = 0.5, 0.25  # one row or two: the columns have one weight in each
+        got = linear_int4(x, q)
+        want = (codes * scales)[[3, 5], [2, 16]] * torch.tensor([0.5, 0.25], device="cuda")
+        assert torch.equal(torch.stack((got[0, 2], got[-1, 16])), want.to(dtype))
+
+
+@gpu
+@pytest.mark.parametrize("m", [1, 9, 30, 70, 300])
+def test_the_relu_of_nan_is_that_of_the_other_linears(m):
+    from tritonformer_b200.linear import LinearNoBiasReLU
+    w = _randn(128, 64, seed=1, dtype=torch.float16)
+    w[5, 7] = float("nan")
+    x = _randn(m, 128, seed=2, dtype=torch.float16)
+    q = quantize_int4(w)
+    got, plain = linear_int4(x, q, relu=True), linear_int4(x, q)
+    assert plain[:, 7].isnan().all() and not got[:, 7].any() and torch.equal(got[:, :7], plain[:, :7].clamp(min=0))
+    with torch.no_grad():
+        assert not LinearNoBiasReLU.apply(x, w)[:, 7].any()
 
 
 @gpu

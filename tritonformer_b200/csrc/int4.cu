@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) int4_linear_kernel(const Int4P
   auto finish = [&](float v, int m, int n) {
     if (m >= p.M || n >= p.N) return;
     if (bias) v += Num<T>::to_f(bias[n]);
-    if (p.relu) v = v < 0.f ? 0.f : v;  // NaN stays
+    if (p.relu) v = fmaxf(v, 0.f);  // as the matrix products of more rows
     if (addend) v += Num<T>::to_f(addend[(int64_t)m * p.addend_ld + n]);
     out[(int64_t)m * p.out_ld + n] = Num<T>::from_f(v);
   };

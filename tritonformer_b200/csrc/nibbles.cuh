@@ -67,9 +67,11 @@ template <typename T> __device__ __forceinline__ float pair_value(uint32_t w, in
 
 // Scale of a group of 16-bit values whose largest magnitude has the bits `top` (as whole numbers a NaN's are above infinity's), and
 // a value's code.  The quotients are rounded as divisions are; neither a scale nor a code then depends on more than the values.
+// A seventh of the type's largest values would be rounded up to a scale whose sevenfold is infinite; the one below it is theirs.
+template <typename T> constexpr float kLargestScale = std::is_same<T, __half>::value ? 9352.f : 36.25f * 0x1p120f;
 template <typename T> __device__ __forceinline__ T scale_of(uint32_t top) {
   const float f = pair_value<T>(top, 0);
-  return Num<T>::from_f(isfinite(f) ? __fdiv_rn(f, 7.f) : NAN);
+  return Num<T>::from_f(isfinite(f) ? fminf(__fdiv_rn(f, 7.f), kLargestScale<T>) : NAN);
 }
 __device__ __forceinline__ int code_of(float x, float scale) {
   return scale > 0.f ? max(-7, min(7, __float2int_rn(__fdiv_rn(x, scale)))) : 0;
@@ -88,7 +90,7 @@ __device__ __forceinline__ uint32_t quantize8(const uint4& v, T& scale, float (&
 #pragma unroll
   for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
   const float f = pair_value<T>(top, 0);
-  scale = Num<T>::from_f(isfinite(f) ? f * (1.f / 7.f) : NAN);
+  scale = Num<T>::from_f(isfinite(f) ? fminf(f * (1.f / 7.f), kLargestScale<T>) : NAN);
   const float s = Num<T>::to_f(scale);
   float x[8];
   unpack8<T>(v, x);

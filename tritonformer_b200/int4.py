@@ -2,7 +2,7 @@
 weights' bytes.  The reference has no counterpart: it trains only.
 
 A weight (in, out) is a 16-bit scale for each group of 32, 64 or 128 rows of a column, times a whole number from -7 to 7: the scale
-is the group's largest magnitude over 7, the number the nearest to weight / scale.  4.5, 4.25 or 4.125 bits a weight.
+is the group's largest magnitude over 7 (at most the largest number whose sevenfold the type holds), the number the nearest to weight / scale.  4.5, 4.25 or 4.125 bits a weight.
 
   * `quantize_int4`  packs a weight
   * `linear_int4`    act(x W + bias) + addend with a packed weight, any number of rows
@@ -39,5 +39,6 @@ def quantize_int4(weight, group=64):
 
 
 def linear_int4(x, weight, bias=None, relu=False, addend=None):
-    """act(x W + bias) + addend: x (.., in) of the type of the weight's scales, bias (out,), addend (.., out); sums in 32 bits, one rounding."""
+    """act(x W + bias) + addend: x (.., in) of the type of the weight's scales, bias (out,), addend (.., out); sums in 32 bits, one rounding.  The ReLU
+    of a NaN is 0, as in the other linears."""
     return _host.int4_linear(x, weight.codes, weight.scales, weight.in_features, weight.out_features, weight.group, bias, relu, addend)
