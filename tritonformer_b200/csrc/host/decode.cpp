@@ -53,7 +53,8 @@ Tensor int4_expand(const Int4& w) {
   return expanded(w).narrow(0, 0, w.out).narrow(1, 0, w.in).t();
 }
 
-// Up to how many rows the products read the packed weights themselves.
+// Up to how many rows the products read the packed weights themselves: each 32 rows read and unpack them again, while beyond it they are expanded once.
+// 64 and 65 rows, which take the one way and the other: 1024 x 4096 6.1 and 9.4 us, 2048 x 8192 15.8 and 18.2, 1024 x 50304 42.1 and 42.3.
 constexpr int64_t kFewRows = 64;
 
 Tensor int4_linear(const Tensor& x, const Int4& w, const Tensor& bias, bool relu, const Tensor& addend_) {

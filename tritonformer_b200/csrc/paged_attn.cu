@@ -76,7 +76,7 @@ int pg_split(const CUtensorMap& tk, const CUtensorMap& tv, const PgParams& p, cu
   using C = PgCfg<HD, G, BIAS, false>;
   static std::atomic<uint64_t> done{0};
   if (int rc = ensure_dynamic_smem(paged_attn_kernel<T, HD, G, BIAS, TMA, false>, C::SMEM, done, "paged_attention")) return rc;
-  launch_overlapped(paged_attn_kernel<T, HD, G, BIAS, TMA, false>, dim3(p.ctas), dim3(PG_WARPS * 32), C::SMEM, st, tk, tv, p);
+  launch_overlapped(paged_attn_kernel<T, HD, G, BIAS, TMA, false>, dim3(p.ctas), dim3(C::WARPS * 32), C::SMEM, st, tk, tv, p);
   return launched("paged_attention");
 }
 

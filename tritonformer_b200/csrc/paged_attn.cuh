@@ -38,7 +38,6 @@
 namespace tfb {
 namespace {
 
-constexpr int PG_WARPS = 8;
 // Probabilities are kept relative to a reference that the running maximum may pass by 2^15 before everything is rescaled
 // (they then still fit fp16); a new reference is 2^4 below the maximum, so that small ones stay clear of fp16's subnormals.
 constexpr float kAhead = 15.f, kBelow = 4.f;
@@ -46,6 +45,9 @@ constexpr float kNone = -INFINITY;
 
 // G: query heads that a warp takes at once, 4, 8 or 16.  Q4: pages in 4 bits.
 template <int HD, int G, int BIAS, bool Q4> struct PgCfg {
+  // In 4 bits a warp's time is that of making 16-bit numbers, and a third warp for each scheduler fills its waits: one user 9.6 -> 8.3 us, 24 sequences of
+  // up to 2048 keys 22.1 -> 20.6, long ones the same; 16 warps' registers do not hold a tile's work.
+  static constexpr int WARPS = Q4 ? 12 : 8;
   static constexpr int NT = G == 16 ? 2 : 1;   // blocks of 8 columns in the products
   static constexpr int KEYS = Q4 ? 64 : 2048 / HD;  // keys of a tile
   static constexpr int MT = KEYS / 16;
@@ -56,18 +58,18 @@ template <int HD, int G, int BIAS, bool Q4> struct PgCfg {
   static constexpr int OWN = (KEYS + 31) / 32; // keys whose place a lane looks up
   static constexpr int TILE = KEYS * CHUNKS * 16;  // bytes of the keys of a tile (4096, and in 4 bits 1024 to 4096)
   static constexpr int PANELS = HD == 128 ? 2 : 1;  // parts of a row of at most 128 bytes, one after the other
-  static constexpr int STAGES = 3;             // what 227 KB hold
+  static constexpr int STAGES = Q4 ? 2 : 3;    // what 227 KB hold
   // What beginning a row of scores costs a warp, in tiles: rows of a tile or two would otherwise pile up in a few warps.  (In 4 bits a tile
   // has more keys and takes longer: 24 sequences of up to 2048 keys 22.2 us, with 4 24.3.)
   static constexpr int ROW_COST = Q4 ? 1 : 4;
-  static constexpr int OFF_POS = PG_WARPS * STAGES * 2 * TILE;   // [warp][stage][KEYS] positions, or scales
-  static constexpr int OFF_ML = OFF_POS + (BIAS || Q4 ? PG_WARPS * STAGES * KEYS * 4 : 0);  // [warp][2][R] reference and sum of a piece
-  static constexpr int OFF_BAR = OFF_ML + PG_WARPS * 2 * R * 8;  // [warp][stage]
+  static constexpr int OFF_POS = WARPS * STAGES * 2 * TILE;   // [warp][stage][KEYS] positions, or scales
+  static constexpr int OFF_ML = OFF_POS + (BIAS || Q4 ? WARPS * STAGES * KEYS * 4 : 0);  // [warp][2][R] reference and sum of a piece
+  static constexpr int OFF_BAR = OFF_ML + WARPS * 2 * R * 8;  // [warp][stage]
   static constexpr int OFF_HEAD = OFF_BAR + 256;  // [warp][R][HD] the piece that a stretch begins in the middle of,
-  static constexpr bool HEAD_SMEM = OFF_HEAD + PG_WARPS * R * HD * 4 + 1024 <= 226 * 1024 + 256;  // if that fits (else in scratch)
-  static constexpr int SMEM = OFF_HEAD + (HEAD_SMEM ? PG_WARPS * R * HD * 4 : 0) + 1024;
+  static constexpr bool HEAD_SMEM = OFF_HEAD + WARPS * R * HD * 4 + 1024 <= 226 * 1024 + 256;  // if that fits (else in scratch)
+  static constexpr int SMEM = OFF_HEAD + (HEAD_SMEM ? WARPS * R * HD * 4 : 0) + 1024;
   static_assert(R * HD * 4 <= STAGES * 2 * TILE, "a piece fits its warp's ring");
-  static_assert(PG_WARPS * STAGES * 8 <= 256 && SMEM <= 227 * 1024 - 700, "shared memory");
+  static_assert(WARPS * STAGES * 8 <= 256 && SMEM <= 227 * 1024 - 700, "shared memory");
 };
 
 struct PgParams {
@@ -194,9 +196,9 @@ __device__ __forceinline__ int64_t divide(int64_t n, int64_t d) {  // of values 
 }
 // The line has ROW_COST units and one for each tile of a row, and is cut into equal stretches, one for each warp (with fewer
 // units than warps, of one unit): the first `more` have a unit more than `each`.
-struct Line {
+template <int WARPS> struct Line {
   int64_t units, each, more, parts;
-  __device__ __forceinline__ Line(int64_t units_, int ctas) : units(units_), parts(min(units_, (int64_t)ctas * PG_WARPS)) {
+  __device__ __forceinline__ Line(int64_t units_, int ctas) : units(units_), parts(min(units_, (int64_t)ctas * WARPS)) {
     each = parts ? divide(units, parts) : 0;
     more = units - each * parts;
   }
@@ -204,7 +206,7 @@ struct Line {
   // the block whose warps have unit t
   __device__ __forceinline__ int block_of(int64_t t) const {
     const int64_t wide = more * (each + 1);
-    return (int)((t < wide ? divide(t, each + 1) : more + divide(t - wide, each)) / PG_WARPS);
+    return (int)((t < wide ? divide(t, each + 1) : more + divide(t - wide, each)) / WARPS);
   }
 };
 template <int ROW_COST> __device__ __forceinline__ int row_units(int tiles) { return tiles ? tiles + ROW_COST : 0; }
@@ -215,25 +217,25 @@ __device__ __forceinline__ float alibi_rounded_log2(int mode, float slope, float
 }
 
 // What a block knows of its warps' pieces when it joins them.
-struct Pieces {
-  int64_t begin[PG_WARPS][2];  // the piece's row's first tile in the line
-  int b[PG_WARPS][2], hr[PG_WARPS][2], tiles[PG_WARPS][2];
-  uint8_t flags[PG_WARPS];  // bit 0: there is a piece [0], which began before the warp's stretch; 1: a piece [1], which goes on
+template <int WARPS> struct Pieces {
+  int64_t begin[WARPS][2];  // the piece's row's first tile in the line
+  int b[WARPS][2], hr[WARPS][2], tiles[WARPS][2];
+  uint8_t flags[WARPS];  // bit 0: there is a piece [0], which began before the warp's stretch; 1: a piece [1], which goes on
 };                          // behind it; 2: piece [0] is its row's last
 
 }  // namespace
 
 // BIAS: 0 none, 1 exact slopes, 2 slopes rounded as a table's
 template <typename T, int HD, int G, int BIAS, bool TMA, bool Q4>
-__global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __grid_constant__ CUtensorMap tmK,
-                                                                      const __grid_constant__ CUtensorMap tmV, const PgParams p) {
+__global__ void __launch_bounds__(PgCfg<HD, G, BIAS, Q4>::WARPS * 32, 1)
+    paged_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const PgParams p) {
   using C = PgCfg<HD, G, BIAS, Q4>;
-  constexpr int NT = C::NT, R = C::R, STAGES = C::STAGES, STAGE = 2 * C::TILE, KS = HD / 16;
+  constexpr int WARPS = C::WARPS, NT = C::NT, R = C::R, STAGES = C::STAGES, STAGE = 2 * C::TILE, KS = HD / 16;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ int64_t sh_scan[PG_WARPS], sh_base[PG_WARPS];
-  __shared__ int sh_b[PG_WARPS];
-  __shared__ __align__(8) Pieces sh;
+  __shared__ int64_t sh_scan[WARPS], sh_base[WARPS];
+  __shared__ int sh_b[WARPS];
+  __shared__ Pieces<WARPS> sh;
   __shared__ int sh_abort, sh_last[2], sh_first[2];
   volatile int* abort_flag = &sh_abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -265,8 +267,8 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
     }
   };
   // ---- the warps' stretches: a scan over the sequences' units
-  const int64_t part = (int64_t)blockIdx.x * PG_WARPS + warp;
-  Line line(0, 0);
+  const int64_t part = (int64_t)blockIdx.x * WARPS + warp;
+  Line<WARPS> line(0, 0);
   int start_b = 0;
   int64_t start_base = 0;  // the units before it
   if (p.B <= 32) {         // each warp by itself: no barrier, one load (one user 10.0 us, with the scan below 10.9)
@@ -279,13 +281,13 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
       const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += v;
     }
-    line = Line((int64_t)__shfl_sync(0xffffffffu, upto, 31) * heads, p.ctas);
+    line = Line<WARPS>((int64_t)__shfl_sync(0xffffffffu, upto, 31) * heads, p.ctas);
     const unsigned behind = __ballot_sync(0xffffffffu, (int64_t)upto * heads > line.begin(part));
     start_b = behind ? __ffs(behind) - 1 : 0;
     start_base = (int64_t)__shfl_sync(0xffffffffu, upto - mine, start_b) * heads;
     if (warp == 0 && lane < p.B) look_over(lane, len, tiles);
   } else {
-    const int per = (p.B + PG_WARPS * 32 - 1) / (PG_WARPS * 32);
+    const int per = (p.B + WARPS * 32 - 1) / (WARPS * 32);
     const int b_lo = min((int)threadIdx.x * per, p.B), b_hi = min(b_lo + per, p.B);
     int64_t mine = 0;
     for (int b = b_lo; b < b_hi; ++b) mine += row_units<C::ROW_COST>((keys_of(p, p.lengths[b]).n + C::KEYS - 1) / C::KEYS);
@@ -299,19 +301,19 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
     __syncthreads();
     int64_t base = upto - mine, total = 0;
 #pragma unroll
-    for (int w = 0; w < PG_WARPS; ++w) {
+    for (int w = 0; w < WARPS; ++w) {
       const int64_t v = sh_scan[w];
       if (w < warp) base += v;
       total += v;
     }
-    line = Line(total * heads, p.ctas);
+    line = Line<WARPS>(total * heads, p.ctas);
     for (int b = b_lo; b < b_hi; ++b) {
       const int len = p.lengths[b];
       const int tiles = (keys_of(p, len).n + C::KEYS - 1) / C::KEYS;
       look_over(b, len, tiles);
 #pragma unroll 1
-      for (int w = 0; w < PG_WARPS; ++w) {
-        const int64_t f = line.begin((int64_t)blockIdx.x * PG_WARPS + w);
+      for (int w = 0; w < WARPS; ++w) {
+        const int64_t f = line.begin((int64_t)blockIdx.x * WARPS + w);
         if (f >= base * heads && f < (base + row_units<C::ROW_COST>(tiles)) * heads) {
           sh_b[w] = b;
           sh_base[w] = base * heads;
@@ -323,7 +325,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
     start_b = sh_b[warp];
     start_base = sh_base[warp];
   }
-  if (line.begin((int64_t)blockIdx.x * PG_WARPS) >= line.units) return;  // nothing for this block
+  if (line.begin((int64_t)blockIdx.x * WARPS) >= line.units) return;  // nothing for this block
   const int64_t from = line.begin(part);
   const int length = (int)(line.begin(part + 1) - from);
 
@@ -333,7 +335,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
   float2* my_ml = reinterpret_cast<float2*>(smem + C::OFF_ML) + warp * 2 * R;
   auto head_piece = [&](int w) {
     return C::HEAD_SMEM ? reinterpret_cast<float*>(smem + C::OFF_HEAD) + w * (R * HD)
-                        : p.heads_acc + ((int64_t)blockIdx.x * PG_WARPS + w) * (R * HD);
+                        : p.heads_acc + ((int64_t)blockIdx.x * WARPS + w) * (R * HD);
   };
   const int g8 = lane >> 2, j2 = 2 * (lane & 3);  // row of an 8x8 block, first of its two columns
   // The second product takes the probabilities in two parts of 16 bits: rounded, and what that leaves (64 sequences of 8 query heads a
@@ -927,12 +929,9 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
     return;
   }
   const float2* ml = reinterpret_cast<const float2*>(smem + C::OFF_ML);
-  const uint64_t flags = *reinterpret_cast<const uint64_t*>(sh.flags);
+  const int flags = lane < WARPS ? sh.flags[lane] : 0;
   // bit w: of warp w
-  auto bits = [&](int bit) {  // bit `bit` of each byte, gathered
-    return (unsigned)(((flags >> bit & 0x0101010101010101ull) * 0x0102040810204080ull) >> 56);
-  };
-  const unsigned has0 = bits(0), has1 = bits(1), ends = bits(2);
+  const unsigned has0 = __ballot_sync(0xffffffffu, flags & 1), has1 = __ballot_sync(0xffffffffu, flags & 2), ends = __ballot_sync(0xffffffffu, flags & 4);
   // A chain of pieces starts with a piece [1], or with the piece [0] that has none before it in this block: only the first can.
   const unsigned lead = has0 & (0u - has0);                             // the first warp with a piece [0]
   const bool leads = lead != 0 && (has1 & (lead - 1u)) == 0;            // and nothing goes on into it
@@ -941,7 +940,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
   auto end_of = [&](int w, int slot) {  // a chain's last warp
     int end = w;
     bool ended = slot == 0 && (ends >> w & 1) != 0;
-    while (!ended && end + 1 < PG_WARPS && (has0 >> (end + 1) & 1) != 0) ended = (ends >> ++end & 1) != 0;
+    while (!ended && end + 1 < WARPS && (has0 >> (end + 1) & 1) != 0) ended = (ends >> ++end & 1) != 0;
     return ended ? end : end | 64;  // 64: the row goes on in the next block
   };
   if (leads) open0 = __ffs(lead) - 1;
@@ -949,7 +948,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
     const int w = 31 - __clz(has1);
     if (end_of(w, 1) & 64) open1 = w;
   }
-  for (int job = warp; job < chains * rows_most; job += PG_WARPS) {
+  for (int job = warp; job < chains * rows_most; job += WARPS) {
     const int chain = job / rows_most, r = job - chain * rows_most;
     const int slot = leads && chain == 0 ? 0 : 1;
     int w = open0;
@@ -1023,7 +1022,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 1) paged_attn_kernel(const __gr
     const int w = slot ? open1 : open0, b = sh.b[w][slot], hr = sh.hr[w][slot];
     const int kv = hr / p.row_tiles, r0 = (hr - kv * p.row_tiles) * R, rows = min(R, p.group - r0);
     // threads along (row, 4 columns), and what is left of them along the pieces, up to a share for 8 pieces
-    constexpr int N = 8, THREADS = PG_WARPS * 32;
+    constexpr int N = 8, THREADS = WARPS * 32;
     const int cols = rows * (HD / 4), shares = max(1, min(THREADS / cols, (pieces + N - 1) / N));
     float4* part = reinterpret_cast<float4*>(smem);            // [THREADS]
     float2* part_ml = reinterpret_cast<float2*>(part + THREADS);  // [THREADS]
@@ -1090,12 +1089,12 @@ struct PgWorkspace {
   int64_t ml, acc, heads_acc, bytes;
 };
 inline PgWorkspace pg_workspace() {
-  const int64_t n = sm_count(), R = 16, hd = 128;
+  const int64_t n = sm_count(), warps = 12, R = 16, hd = 128;
   PgWorkspace s;
   s.ml = kCounterBytes;
   s.acc = s.ml + up256(2 * n * R * 8);
   s.heads_acc = s.acc + up256(2 * n * R * hd * 4);
-  s.bytes = s.heads_acc + n * PG_WARPS * R * hd * 4;
+  s.bytes = s.heads_acc + n * warps * R * hd * 4;
   return s;
 }
 

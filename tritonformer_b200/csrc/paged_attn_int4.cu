@@ -8,6 +8,13 @@
 // probabilities before they are rounded (to two parts of bf16, so that the weights' rounding does not show).  A word of codes comes out of
 // ldmatrix as a lane's share of the instruction: for the keys 8 dims of a key, for the values (transposed as 16-bit units) 4 dims of two
 // neighbouring keys, which is the pair that the second product wants.  Tiles come by cp.async: a row is 16 to 64 bytes.
+//
+// What bounds it is no longer the reading but the instructions: 390 for 16 keys of 128 dims and 8 columns of queries, half of them to make
+// codes into numbers, issue slots 58% and the whole-number pipe 54% in use over a launch that lacks a tenth at both ends; the copies and the
+// softmax alone take 57 us of the 92 below.  Measured in graphs, in brackets the 16-bit cache: bf16, head_dim 128, 32 sequences of up to 16384 keys,
+// 8 key heads of 4 query heads 92 us (169); fp16, head_dim 64, 24 sequences of up to 2048 keys, 16 heads, slopes 20.4 (25.9); one
+// of 700 keys 8.3 (9.3).  Not kept for the long ones: two blocks an SM (113 us, registers spilled), tiles of 32 keys (95 to 109), 8 warps with
+// three tiles ahead (93, the short ones 9.6 and 22.1).
 #include "paged_attn.cuh"
 
 namespace tfb {
@@ -19,7 +26,7 @@ int pg4_split(const PgParams& p, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
   if (int rc = ensure_dynamic_smem(paged_attn_kernel<T, HD, G, BIAS, false, true>, C::SMEM, done, "paged_attention_int4")) return rc;
   const CUtensorMap none = {};
-  launch_overlapped(paged_attn_kernel<T, HD, G, BIAS, false, true>, dim3(p.ctas), dim3(PG_WARPS * 32), C::SMEM, st, none, none, p);
+  launch_overlapped(paged_attn_kernel<T, HD, G, BIAS, false, true>, dim3(p.ctas), dim3(C::WARPS * 32), C::SMEM, st, none, none, p);
   return launched("paged_attention_int4");
 }
 template <typename T, int HD, int G>
