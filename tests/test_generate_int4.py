@@ -11,8 +11,9 @@ import torch
 
 import tritonformer_b200._lib as L
 from test_generate import _model, _teacher
-from tritonformer_b200 import quantize_int4, sample_tokens
+from tritonformer_b200 import linear_int4, quantize_int4, sample_tokens
 from tritonformer_b200.generate import Generator
+from tritonformer_b200.kvcache import PagedKVCache
 from util import norm_rel
 
 gpu = pytest.mark.gpu
@@ -120,3 +121,46 @@ def test_a_length_that_does_not_fit_is_reported():
     with pytest.raises(RuntimeError, match="length"):
         L.check_status()
     assert L.device_status(reset=True) == 0x7201
+
+
+def test_two_streams_and_two_graphs_at_once():
+    """The operators' calls share no state: what runs beside them, eagerly or from graphs, changes nothing."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    randn = lambda *shape: torch.randn(shape, generator=g, device="cuda").half()  # noqa: E731
+    cache = PagedKVCache(64, 4, 64, 64, torch.float16, "cuda", False, 4)
+    tables = torch.arange(64, dtype=torch.int32, device="cuda").view(4, 16)
+    lengths = torch.tensor([1000, 3, 0, 512], dtype=torch.int32, device="cuda")
+    cache.append(tables, torch.zeros_like(lengths), randn(4, 4, 1000, 64), randn(4, 4, 1000, 64), lengths)
+    weight = quantize_int4(randn(200, 130))
+    sides = [(randn(40, 50304), torch.rand(40, generator=g, device="cuda"), {"top_p": 0.9}, randn(4, 4, 64), randn(1, 200)),
+             (randn(30, 30000), torch.rand(30, generator=g, device="cuda"), {"top_k": 300}, randn(4, 12, 64), randn(100, 200))]
+
+    def run(logits, u, settings, q, x):
+        return sample_tokens(logits, u, **settings), cache.attend(q, tables, lengths), linear_int4(x, weight)
+
+    want = [run(*side) for side in sides]
+    streams = [torch.cuda.Stream() for _ in sides]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = []
+        for stream, side in zip(streams, sides):
+            with torch.cuda.stream(stream):
+                got.append(run(*side))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for x, y in zip(got, want) for a, b in zip(x, y))
+    graphs, got = [], []
+    for side in sides:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            got.append(run(*side))
+    for _ in range(20):
+        for out in got:
+            for t in out:
+                t.zero_()
+        torch.cuda.synchronize()
+        for stream, graph in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for x, y in zip(got, want) for a, b in zip(x, y))
+    L.check_status()

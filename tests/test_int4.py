@@ -156,6 +156,24 @@ def test_linear_of_strided_inputs(m):
 
 
 @gpu
+@pytest.mark.parametrize("m", [10, 100])
+def test_linear_of_repeated_and_transposed_rows(m):
+    """The same numbers in another layout: the same bits."""
+    q = quantize_int4(_randn(200, 130, seed=1, dtype=torch.float16))
+    for x in (_randn(1, 200, seed=2, dtype=torch.float16).expand(m, 200), _randn(200, m, seed=3, dtype=torch.float16).t(),
+              _randn(m, 1, seed=4, dtype=torch.float16).expand(m, 200)):
+        assert torch.equal(linear_int4(x, q), linear_int4(x.contiguous(), q))
+    assert linear_int4(_randn(m, 200, seed=5, dtype=torch.float16)[:0], q).shape == (0, 130)
+
+
+@gpu
+def test_quantize_of_repeated_rows_and_columns():
+    for w in (_randn(1, 70, seed=1, dtype=torch.float16).expand(33, 70), _randn(33, 1, seed=2, dtype=torch.float16).expand(33, 70)):
+        a, b = quantize_int4(w), quantize_int4(w.contiguous())
+        assert torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales)
+
+
+@gpu
 def test_linear_addend_and_bias_of_any_layout():
     w, x = _randn(128, 96, seed=1, dtype=torch.float16), _randn(4, 128, seed=2, dtype=torch.float16)
     q = quantize_int4(w)
