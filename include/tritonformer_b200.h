@@ -412,6 +412,10 @@ int tfb_cache_append_int4(const void* key, const void* value, void* k_pages, voi
  * tfb_int4_quantize: codes and scales of w, element strides w_k, w_n.  s = (largest magnitude of the group) / 7, rounded to the type, at most
  * the largest number whose sevenfold the type holds, and NaN where a weight is not finite; c = W / s rounded to the nearest whole number, ties to even.
  * tfb_int4_expand: s * c rounded to the type, transposed: out (16 * strips, 64 * units), 16-byte aligned.
+ * tfb_int4_split: for many rows: s * c unrounded, as the sum of two numbers of the type.  Transposed, out (16 * strips, 2 * 64 * units): in a
+ * row's first half what rounding s * c leaves, in its second s * c rounded.  x_out (M, 2 * 64 * units): M rows of x (pitch x_ld, unit stride, any
+ * alignment) twice, zeros behind K; the first time what is not finite is zero, because an infinity times a rest of zero would be NaN.  tfb_gemm_fused of x_out and
+ * out is x W.  Both outputs 16-byte aligned.
  * tfb_int4_linear: out = act(x W + bias) + addend for M rows of x (pitch x_ld, unit stride, any alignment), out and addend of pitch
  * out_ld, addend_ld; bias (N) and addend may be NULL, the addend may be the output.  For few rows: every 32 of them read the weights again.  */
 int64_t tfb_int4_codes(int64_t K, int64_t N);
@@ -420,6 +424,8 @@ int tfb_int4_quantize(const void* w, int64_t w_k, int64_t w_n, int64_t K, int64_
                       void* scales, int dtype, void* stream);
 int tfb_int4_expand(const void* codes, const void* scales, int64_t K, int64_t N, int group, void* out, int dtype,
                     void* stream);
+int tfb_int4_split(const void* codes, const void* scales, int64_t K, int64_t N, int group, void* out, const void* x,
+                   int64_t x_ld, int64_t M, void* x_out, int dtype, void* stream);
 int tfb_int4_linear(const void* x, int64_t x_ld, const void* codes, const void* scales, const void* bias,
                     const void* addend, int64_t addend_ld, void* out, int64_t out_ld, int64_t M, int64_t K, int64_t N,
                     int group, int relu, int dtype, void* stream);

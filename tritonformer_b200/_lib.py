@@ -74,6 +74,7 @@ _SIGNATURES = {
     "tfb_int4_scales": (_i64, [_i64] * 2 + [_i32]),
     "tfb_int4_quantize": (_i32, [_vp] + [_i64] * 4 + [_i32, _vp, _vp, _i32, _vp]),
     "tfb_int4_expand": (_i32, [_vp] * 2 + [_i64] * 2 + [_i32, _vp, _i32, _vp]),
+    "tfb_int4_split": (_i32, [_vp] * 2 + [_i64] * 2 + [_i32] + [_vp] * 2 + [_i64] * 2 + [_vp, _i32, _vp]),
     "tfb_int4_linear": (_i32, [_vp, _i64] + [_vp] * 4 + [_i64, _vp] + [_i64] * 4 + [_i32, _i32, _i32, _vp]),
     "tfb_sample": (_i32, [_vp, _i64, _vp, _vp, _f32, _vp, _i32, _vp, _f32, _vp, _f32, _vp, _i64, _i64, _i32, _vp]),
 }

@@ -53,9 +53,10 @@ Tensor int4_expand(const Int4& w) {
   return expanded(w).narrow(0, 0, w.out).narrow(1, 0, w.in).t();
 }
 
-// Up to how many rows the products read the packed weights themselves: each 32 rows read and unpack them again, while beyond it they are expanded once.
-// 64 and 65 rows, which take the one way and the other: 1024 x 4096 6.1 and 9.4 us, 2048 x 8192 15.8 and 18.2, 1024 x 50304 42.1 and 42.3.
-constexpr int64_t kFewRows = 64;
+// Up to how many rows the products read the packed weights themselves: each 32 rows read and unpack them again, while beyond it they are unpacked once, into
+// two parts.  96 and 97 rows, which take the one way and the other: 1024 x 1024 3.9 and 8.2 us, 1024 x 4096 10.0 and 12.5, 2048 x 8192 28.6 and 27.5,
+// 1024 x 50304 56.3 and 77.4, 1536 x 6144 12.5 and 19.6; 32 rows more would add a third to the first of each pair.
+constexpr int64_t kFewRows = 96;
 
 Tensor int4_linear(const Tensor& x, const Int4& w, const Tensor& bias, bool relu, const Tensor& addend_) {
   check_plain("linear_int4", {&x, &w.codes, &w.scales, &bias, &addend_});
@@ -90,20 +91,18 @@ Tensor int4_linear(const Tensor& x, const Int4& w, const Tensor& bias, bool relu
                           (int)w.group, relu ? 1 : 0, dtype, stream));
     return out;
   }
-  const Tensor full = expanded(w);
-  Mat k;
-  k.keep = full;
-  k.p = full.data_ptr();
-  k.rows = w.in;
-  k.cols = w.out;
-  k.s0 = 1;
-  k.s1 = full.size(1);
+  // More: each weight as the sum of two numbers that it has 16 bits for, along a contraction of twice the length, in one product.
+  const int64_t inner = (w.in + 63) / 64 * 64 * 2;
+  const Tensor parts = at::empty({(w.out + 15) / 16 * 16, inner}, x.options()), twice = at::empty({a.rows, inner}, x.options());
+  check(tfb_int4_split(w.codes.data_ptr(), w.scales.data_ptr(), w.in, w.out, (int)w.group, parts.data_ptr(), a.p, a.s0, a.rows,
+                       twice.data_ptr(), dtype, stream));
+  Mat k = block(parts.data_ptr(), w.out, inner).t();
   Epilogue e;
   e.bias = b.defined() ? b.data_ptr() : nullptr;
   e.relu = relu;
   e.addend = addend.defined() ? addend.data_ptr() : nullptr;
   e.ld_addend = w.out;
-  gemm(tma_fit(a, x, dtype), k, out.data_ptr(), w.out, e, dtype, x.device(), stream);
+  gemm(block(twice.data_ptr(), a.rows, inner), k, out.data_ptr(), w.out, e, dtype, x.device(), stream);
   return out;
 }
 

@@ -7,7 +7,7 @@
 // Products of codes are exact and their sum over a group meets the scale in 32 bits, so no weight is rounded.
 // A warp has a strip of 16 columns and a stretch of the contraction; up to 8 warps of a block share a strip where there are few, and join their
 // sums in shared memory, in their order: the result does not depend on timing.  More rows go to the tensor cores of the library's own matrix
-// product, on weights expanded to 16 bits.
+// product, each weight as the sum of two 16-bit numbers: nothing of it is rounded there either.
 //
 // What bounds it is the whole-number pipe: a word of 8 codes takes five of its instructions to become 16-bit numbers, at two cycles each, 70 cycles of
 // a scheduler for a unit (512 bytes) with all else, where a copy would take 12 SM cycles for it.  Measured in graphs, weights not in the L2, fp16:
@@ -238,16 +238,54 @@ __global__ void __launch_bounds__(256) int4_quantize_kernel(const T* __restrict_
   }
 }
 
+// What the product of many rows takes beside the weights: its rows, twice.
+struct TwiceParams {
+  const void* x;
+  void* out;  // (M, 2 * units * 64)
+  int64_t ld;
+  int M, K, units, vec;  // vec: rows of x can be read 16 bytes at a time
+  int blocks;            // of the grid, the first ones
+};
+
+// The values of a vector that are finite, zeros for the others.
+template <typename T> __device__ __forceinline__ uint32_t finite_pair(uint32_t v) {
+  constexpr uint32_t kExponent = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  if ((v & kExponent) == kExponent) v &= 0xffff0000u;
+  if ((v >> 16 & kExponent) == kExponent) v &= 0xffffu;
+  return v;
+}
+
 // W in 16 bits, transposed: out (strips * 16, units * 64), so that a lane's codes are eight neighbours.  The product of code and scale
-// is rounded to 16 bits here: at most half a step of a weight, where the sums over a thousand rows are not exact to that either.
-// Bound by writing: 1536 x 6144 5.3 us, 1024 x 50304 22.8 (131 MB with the codes, 5.7 TB/s), beside products of 18 us and more.
-template <typename T, bool SMALL>
+// is rounded to 16 bits here.
+// SPLIT: unrounded, as the sum of two 16-bit numbers, out (strips * 16, 2 * units * 64): what the rounding leaves in a row's first half, the rounded value in its
+// second.  A scale has 11 significant bits (8 in bf16) and a code three, so the rest is three bits, on the grid of the scale: exact.  The rows
+// of x, repeated likewise, then make a product in which no weight is rounded, and the smaller sums come first.  Beside the rests what is not finite in x is
+// left out: an infinity times a rest of zero would be NaN.
+// Bound by writing: rounded, 1536 x 6144 5.3 us, 1024 x 50304 22.8 (131 MB with the codes, 5.7 TB/s).  A product of 1000 rows of 1536 x 6144 with weights in
+// two parts takes 36.8 us, with rounded ones it took 22.5, and was off by 2.7e-4 of the output's norm where the output's own rounding is 2.1e-4.
+template <typename T, bool SMALL, bool SPLIT>
 __global__ void __launch_bounds__(256) int4_expand_kernel(const uint4* __restrict__ codes, const uint32_t* __restrict__ scales, int units,
-                                                          int groups, int group_log2, int64_t pieces, T* __restrict__ out) {
+                                                          int groups, int group_log2, int64_t pieces, T* __restrict__ out, const TwiceParams x) {
   grid_dependency_wait();
   allow_dependents();
+  if (SPLIT && (int)blockIdx.x < x.blocks) {
+    const int per = x.units * 8;  // vectors of a row
+    const int64_t all = (int64_t)x.M * per;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)x.blocks * 256) {
+      const int64_t m = i / per;
+      const int k = (int)(i - m * per) * 8;
+      const uint16_t* row = static_cast<const uint16_t*>(x.x) + m * x.ld;
+      const uint4 v = x.vec && k + 8 <= x.K ? *reinterpret_cast<const uint4*>(row + k) : load_x8(row, k, x.K);
+      uint4* to = reinterpret_cast<uint4*>(static_cast<uint16_t*>(x.out) + m * per * 16 + k);
+      to[0] = make_uint4(finite_pair<T>(v.x), finite_pair<T>(v.y), finite_pair<T>(v.z), finite_pair<T>(v.w));
+      to[per] = v;
+    }
+    return;
+  }
+  const int block = SPLIT ? blockIdx.x - x.blocks : blockIdx.x, blocks = SPLIT ? gridDim.x - x.blocks : gridDim.x;
+  const int64_t pitch = (int64_t)units * kUnit * (SPLIT ? 2 : 1);
   const int lane = threadIdx.x & 31, r = lane >> 2, j = lane & 3;
-  for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < pieces; i += (int64_t)gridDim.x * 8) {
+  for (int64_t i = (int64_t)block * 8 + (threadIdx.x >> 5); i < pieces; i += (int64_t)blocks * 8) {
     const int strip = (int)(i / units), u = (int)(i - (int64_t)strip * units);
     const uint4 w = ld_stream16(codes + i * 32 + lane);
 #pragma unroll
@@ -269,7 +307,17 @@ __global__ void __launch_bounds__(256) int4_expand_kernel(const uint4* __restric
             v[t * 4 + q * 2] = c.x * (half ? f.y : f.x);
             v[t * 4 + q * 2 + 1] = c.y * (half ? f.y : f.x);
           }
-        *reinterpret_cast<uint4*>(out + ((int64_t)strip * 16 + half * 8 + r) * units * kUnit + u * kUnit + h * 32 + j * 8) = pack8<T>(v);
+        const uint4 rounded = pack8<T>(v);
+        T* to = out + ((int64_t)strip * 16 + half * 8 + r) * pitch + u * kUnit + h * 32 + j * 8;
+        if (SPLIT) {
+          float back[8];
+          unpack8<T>(rounded, back);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] -= back[e];
+          *reinterpret_cast<uint4*>(to) = pack8<T>(v);
+          to += (int64_t)units * kUnit;
+        }
+        *reinterpret_cast<uint4*>(to) = rounded;
       }
     }
   }
@@ -301,6 +349,18 @@ int check_int4(const char* what, int64_t K, int64_t N, int group) {
 }
 int64_t int4_groups(int64_t K, int group) { return ceil_div(ceil_div(K, kUnit) * kUnit, group); }
 
+template <typename T, bool SPLIT>
+int int4_expand_launch(const void* codes, const void* scales, int64_t K, int64_t N, int group, void* out, const TwiceParams& x,
+                       cudaStream_t st) {
+  const int64_t units = ceil_div(K, kUnit), pieces = units * ceil_div(N, 16);
+  const int64_t most = (int64_t)sm_count() * 16, blocks = ceil_div(pieces, 8);
+  const int log2 = group == 32 ? 5 : group == 64 ? 6 : 7;
+  launch_overlapped(group == 32 ? int4_expand_kernel<T, true, SPLIT> : int4_expand_kernel<T, false, SPLIT>,
+                    dim3((unsigned)((blocks < most ? blocks : most) + x.blocks)), dim3(256), 0, st, (const uint4*)codes, (const uint32_t*)scales,
+                    (int)units, (int)int4_groups(K, group), log2, pieces, (T*)out, x);
+  return launched("int4_expand");
+}
+
 }  // namespace
 }  // namespace tfb
 
@@ -328,15 +388,27 @@ extern "C" int tfb_int4_quantize(const void* w, int64_t w_k, int64_t w_n, int64_
 extern "C" int tfb_int4_expand(const void* codes, const void* scales, int64_t K, int64_t N, int group, void* out, int dtype, void* stream) {
   if (int rc = check_int4("int4_expand", K, N, group)) return rc;
   TFB_REQUIRE(codes && scales && out && aligned16(codes) && aligned16(scales) && aligned16(out), "int4_expand: the buffers are not 16-byte aligned");
-  const int64_t units = ceil_div(K, kUnit), pieces = units * ceil_div(N, 16);
-  const int64_t most = (int64_t)sm_count() * 16, blocks = ceil_div(pieces, 8);
-  const int log2 = group == 32 ? 5 : group == 64 ? 6 : 7;
-  TFB_DISPATCH_16(dtype, T, {
-    launch_overlapped(group == 32 ? int4_expand_kernel<T, true> : int4_expand_kernel<T, false>, dim3((unsigned)(blocks < most ? blocks : most)),
-                      dim3(256), 0, (cudaStream_t)stream, (const uint4*)codes, (const uint32_t*)scales, (int)units,
-                      (int)int4_groups(K, group), log2, pieces, (T*)out);
-    return launched("int4_expand");
-  })
+  TFB_DISPATCH_16(dtype, T, { return int4_expand_launch<T, false>(codes, scales, K, N, group, out, TwiceParams{}, (cudaStream_t)stream); })
+}
+
+extern "C" int tfb_int4_split(const void* codes, const void* scales, int64_t K, int64_t N, int group, void* out, const void* x, int64_t x_ld,
+                              int64_t M, void* x_out, int dtype, void* stream) {
+  if (int rc = check_int4("int4_split", K, N, group)) return rc;
+  TFB_REQUIRE(M >= 0 && M < (1LL << 31), "int4_split: bad row count");
+  TFB_REQUIRE(M <= 1 || (x_ld >= 0 && x_ld < (1LL << 40)), "int4_split: bad row stride");
+  TFB_REQUIRE(codes && scales && out && aligned16(codes) && aligned16(scales) && aligned16(out), "int4_split: the buffers are not 16-byte aligned");
+  TFB_REQUIRE(M == 0 || (x && x_out && aligned16(x_out)), "int4_split: the buffers are not 16-byte aligned");
+  TwiceParams p = {};
+  p.x = x;
+  p.out = x_out;
+  p.ld = x_ld;
+  p.M = (int)M;
+  p.K = (int)K;
+  p.units = (int)ceil_div(K, kUnit);
+  p.vec = aligned16(x) && (M <= 1 || x_ld % 8 == 0);
+  const int64_t most = (int64_t)sm_count() * 8, blocks = ceil_div(M * p.units * 8, 256);
+  p.blocks = (int)(blocks < most ? blocks : most);
+  TFB_DISPATCH_16(dtype, T, { return int4_expand_launch<T, true>(codes, scales, K, N, group, out, p, (cudaStream_t)stream); })
 }
 
 extern "C" int tfb_int4_linear(const void* x, int64_t x_ld, const void* codes, const void* scales, const void* bias, const void* addend,

@@ -8,8 +8,9 @@ is the group's largest magnitude over 7 (at most the largest number whose sevenf
   * `linear_int4`    act(x W + bias) + addend with a packed weight, any number of rows
   * `Int4Weight`     a packed weight; `dequantize()` gives what it stands for
 
-Up to 64 rows read the packed weights as they are, and no weight is rounded a second time; for more (a prompt) they are expanded to the
-16-bit type first, which rounds scale times number once, and go through the tensor-core product of the training.  No gradients.
+No product rounds a weight a second time.  Up to 96 rows read the packed weights as they are; for more (a prompt) each becomes the sum of two
+numbers of the 16-bit type, and the tensor-core product of the training takes both along a contraction of twice the length.  That call has
+two buffers beside its output: twice the weight in 16 bits, and twice its rows.  `dequantize` rounds, to give one number for a weight.  No gradients.
 """
 from . import _host
 
