@@ -553,6 +553,7 @@ struct HistShared {
   double warp_weights[H_WARPS];
   float warp_tops[H_WARPS], warp_lows[H_WARPS], tops[SM_CLUSTER];
   int found, cut, ties, owner, owner_ties, to_last;
+  int least;  // the last bin that weighs enough: not in `cut`, which other warps may still be reading while it is found
   double before, owner_before, goal;
   int few[SM_CLUSTER], limits[SM_CLUSTER], total;
   int list_bin[H_FEW], list_col[H_FEW], part_count[4][H_FEW];
@@ -1123,11 +1124,11 @@ __global__ void __launch_bounds__(H_THREADS, 1) sample_hist_kernel(const SampleP
         if (n > 0) lo = min(lo + step * n, hi - 1);
         if (n < 32) hi = next;
       }
-      if (lane == 0) sh.cut = lo;
+      if (lane == 0) sh.least = lo;
     }
     __syncthreads();
-    if (sh.cut < cut) {
-      cut = sh.cut + 1;
+    if (sh.least < cut) {
+      cut = sh.least + 1;
       ties = 0;
     }
   }
