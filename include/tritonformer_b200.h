@@ -434,7 +434,7 @@ int tfb_int4_linear(const void* x, int64_t x_ld, const void* codes, const void* 
  * No counterpart in the reference.  One token per row of logits (B, vocab), pitch ld, fp32, fp16 or bf16: with w_i = exp((l_i - max l) / t)
  * and the order of larger logits first, equal ones by index, kept are the first top_k (0: all), of those the ones whose predecessors
  * weigh less than top_p times the sum of the top_k, of those the ones with w_i >= min_p; out[b] is the first index j at which the sum of
- * the kept weights up to j exceeds uniforms[b] times their sum.  Weights and sums in 64 bits.  A logit that is NaN counts as -infinity, all
+ * the kept weights up to j exceeds uniforms[b] times their sum.  Weights and sums in 64 bits; what weighs less than 2^-960 of the sum counts as nothing.  A logit that is NaN counts as -infinity, all
  * +infinite ones share the weight; a row of -infinity gives -1.  temperature 0: the first of the largest.  Each setting is an array with one
  * value per row, or where that is NULL the number behind it; values outside their range (temperature >= 0, top_k >= 0, top_p and min_p from
  * 0 to 1, uniforms from 0 to below 1) are taken as the nearest, NaN as 0 or, for top_p, as 1.                                   */

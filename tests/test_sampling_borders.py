@@ -68,3 +68,18 @@ def test_the_same_logits_in_another_type_give_the_same_tokens(dtype):
     for i, settings in enumerate(SETTINGS):
         for x in (_logits(150, 4001, dtype, i).round(), _logits(150, 300, dtype, i, 0.4).round() + 1.375):
             assert torch.equal(sample_tokens(x, u, **settings), sample_tokens(x.float(), u, **settings))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [5, 900, 70000])
+def test_the_smallest_numbers_do_not_draw_what_weighs_nothing(vocab, dtype):
+    """At temperature 0.05 a logit of -30 below ten weighs e^-800, zero in 64 bits: not even u = 0 draws it, the first of its row and of many."""
+    x = _logits(6, vocab, dtype, 1, 0.5).clamp(-2, 2) + 8
+    x[:, 0] = -30.0
+    x[1::2, 1:vocab // 2] = -30.0
+    x[2, :-1], x[3, -1] = -30.0, -30.0
+    for u in (torch.zeros(6, device="cuda"), torch.full((6,), 2.0 ** -149, device="cuda"), torch.full((6,), 2.0 ** -24, device="cuda")):
+        for settings in ({}, {"top_k": 4}, {"top_k": 600}, {"top_p": 0.9}, {"min_p": 1e-30}, {"top_k": 200, "top_p": 0.999}):
+            got = _check(x, {"temperature": 0.05, **settings}, u=u)
+            assert (x.gather(1, got[:, None]) > 0).all()

@@ -30,6 +30,9 @@ namespace cg = cooperative_groups;
 constexpr int SM_WARPS = 16, SM_THREADS = SM_WARPS * 32, SM_CLUSTER = 8;
 constexpr int SM_CUTS = 8;  // values that a round looks at
 constexpr double kLog2eD = 1.4426950408889634074;
+// The smallest share of the sum that is looked for.  Logits far below the largest weigh some 2^-981 here where 64 bits have nothing, and not even a
+// uniform number of zero may draw them: 2^19 of them stay below this.
+constexpr double kLeastShare = 0x1p-960;
 
 struct SampleParams {
   const void* logits;
@@ -450,7 +453,7 @@ __global__ void __launch_bounds__(SM_THREADS) sample_search_kernel(const SampleP
     seen += n;
     total += w;
   }
-  const double goal = (double)u * total;
+  const double goal = fmax((double)u, kLeastShare) * total;
   const bool found = here > 0.0 && before <= goal && (before + here > goal || last == me);
   if (!found) return;
   double base = before;
@@ -913,7 +916,7 @@ __global__ void __launch_bounds__(H_THREADS, 1) sample_hist_kernel(const SampleP
       }
       line += base;
       // the first whose sum is above the goal; where rounding leaves none, the last
-      const double aim = (double)u * all;
+      const double aim = fmax((double)u, kLeastShare) * all;
       if (keep && line > aim) atomicMin(&sh.found, i);
       if (keep) atomicMax(&sh.owner, i);
       __syncthreads();
@@ -1168,7 +1171,7 @@ __global__ void __launch_bounds__(H_THREADS, 1) sample_hist_kernel(const SampleP
       const double n = __shfl_up_sync(0xffffffffu, line, o);
       if (lane >= o) line += n;
     }
-    const double goal = (double)u * __shfl_sync(0xffffffffu, line, 31);
+    const double goal = fmax((double)u, kLeastShare) * __shfl_sync(0xffffffffu, line, 31);
     line -= weight;
     int owner = 1 << 30, last = -1;
     double owner_before = 0.0;
