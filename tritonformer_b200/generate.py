@@ -279,7 +279,8 @@ class Generator:
                  uniforms=None, generator=None):
         """(batch, new_tokens) token ids that follow the prompts.  With a `temperature` they are drawn as `sample_tokens` does, from
         `uniforms` (batch, new_tokens) in [0, 1) or else from numbers of `generator`; without one `choose` maps logits to tokens (the
-        largest by default)."""
+        largest by default).  A drawn -1 marks a token whose logits were all NaN or -infinity; its sequence goes on with token 0, and the
+        others are not concerned."""
         if temperature is None:
             plain = all(not isinstance(x, torch.Tensor) and x == y for x, y in ((top_k, 0), (top_p, 1.0), (min_p, 0.0)))
             assert plain and uniforms is None and generator is None, "drawing tokens takes a temperature"
@@ -295,6 +296,6 @@ class Generator:
                 out.append(choose(logits))
             else:
                 out.append(sample_tokens(logits, uniforms[:, i], temperature, top_k, top_p, min_p))
-            if i + 1 < new_tokens:
-                logits = self.step(out[-1])
+            if i + 1 < new_tokens:  # -1 is no token of the embedding, whose report would stop the matrix products of all sequences
+                logits = self.step(out[-1] if temperature is None else out[-1].clamp(min=0))
         return torch.stack(out, 1) if out else prompts[:, :0]
