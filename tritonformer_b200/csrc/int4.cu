@@ -9,12 +9,13 @@
 // sums in shared memory, in their order: the result does not depend on timing.  More rows go to the tensor cores of the library's own matrix
 // product, each weight as the sum of two 16-bit numbers: nothing of it is rounded there either.
 //
-// What bounds it is the whole-number pipe: a word of 8 codes takes five of its instructions to become 16-bit numbers, at two cycles each, 70 cycles of
-// a scheduler for a unit (512 bytes) with all else, where a copy would take 12 SM cycles for it.  Measured in graphs, weights not in the L2, fp16:
-// 1 x 1024 x 1024 1.45 us; 1 x 4096 x 1024 3.9; 4 x 1024 x 50304 8.5 (27.7 MB, 3.3 TB/s); 24 x 2048 x 8192 in groups of 32 9.3; 16 x 4096 x 12288 12.7.
+// Measured in graphs, weights not in the L2, fp16: 1 x 1024 x 1024 1.5 us (1.7 with an addend); 1 x 4096 x 1024 4.2; 4 x 1024 x 50304 8.4 (27.7 MB,
+// 3.3 TB/s); 24 x 2048 x 8192 in groups of 32 9.2; 16 x 4096 x 12288 13.1.  No pipe is full there: for the 50304 columns and for 24 rows the counters
+// have issue slots at 52 and 33 %, the whole-number pipe, which makes codes into numbers, at 45 and 26 %, the tensor pipe at 19 and 21 %.  What is on its way is
+// little: 20 and 14 warps an SM with two units of 512 bytes and one, and the rows of x come from the L1 where they are used.
 // Two units in flight at a time for up to 8 rows and one for more, in 16 warps an SM at least, were the fastest of 1, 2 and 4 with 8 to 32 warps (4 units:
 // 11.5 us for the 50304 columns, one 11.4).  Rings in shared memory, filled by cp.async or bulk copies for a block or a warp, were slower
-// throughout (12 to 20 us for the 50304 columns): the copies hide, their bookkeeping is what the pipe has no room for.
+// throughout (12 to 20 us for the 50304 columns).
 #include "nibbles.cuh"
 
 namespace tfb {

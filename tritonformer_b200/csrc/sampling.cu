@@ -13,10 +13,11 @@
 // warp has the token.  The cut comes from a list of candidates that are all compared (few of the largest, or of the heaviest), from a histogram over
 // all values (16 bits), or from a search (32 bits), below.
 //
-// Reading the logits is the least of it (13 MB for 128 rows of 50304: 2 us).  What bounds a call is the chain of its steps, each a barrier of 32 warps or
-// of a cluster (some 2000 cycles) with little between, and the exponentials where many logits are kept: 33 cycles of a scheduler each, nine sums and
-// products in 64 bits at two cycles, conversions and the table beside them.  Measured in graphs, fp16 logits: one row of 50304, top_k 40 and top_p 0.95,
-// 15.5 us; 128 rows of 50304, temperature alone 27.5, top_k 40 15.5, min_p 0.05 18.7, top_p 0.9 47; bf16, 16 rows of 131071, top_p 0.9 35.
+// Reading the logits is the least of it (13 MB for 128 rows of 50304: 2 us), and no pipe is full: over rows with settings of their own issue slots are in
+// use 47 %, the whole-number pipe 30 %, the 64-bit one 8 %.  A call is a chain of steps with a barrier of the block or the cluster behind each.  Some are
+// one warp's, while the others wait or have gone (the search for min_p's border, the walk through the owner's logits); where many logits are kept
+// each has its exponential once more in the sums by warp, although the histogram has their total.  Measured in graphs, fp16 logits: one row of 50304, top_k 40 and
+// top_p 0.95, 14.6 us; 128 rows of 50304, temperature alone 28, top_k 40 15, min_p 0.05 18, top_p 0.9 48; bf16, 16 rows of 131071, top_p 0.9 35.
 // fp32: 8 rows of 32000, temperature alone 14, top_k 40 31, top_p 0.9 59.
 #include <cfloat>
 #include <cooperative_groups.h>
@@ -518,7 +519,7 @@ __global__ void __launch_bounds__(SM_THREADS) sample_search_kernel(const SampleP
 // ---------------------------------------------------------------------------------------------------------- 16 bits
 // Few candidates.  The k-th largest of the threads' largest logits is not above the k-th largest logit, so what lies below it is out; the same holds for
 // each block of a cluster.  What is left, some more than k from each block, is put in a list; up to 256 of them are compared each with each,
-// which gives ranks and the weight ahead of each at once (one row, top_k 40: 20 us by the histogram, 15.5 so).
+// which gives ranks and the weight ahead of each at once (one row, top_k 40: 20 us by the histogram, 14.6 so).
 //
 // Logits of 16 bits have 2^16 values, and equal logits weigh the same: a histogram over all values is all that the cut needs.  Blocks count their
 // part of the row (a counter of 16 bits for each value, 128 KB of shared memory), the blocks of a cluster add theirs up where there is
