@@ -412,10 +412,10 @@ int tfb_cache_append_int4(const void* key, const void* value, void* k_pages, voi
  * tfb_int4_quantize: codes and scales of w, element strides w_k, w_n.  s = (largest magnitude of the group) / 7, rounded to the type, at most
  * the largest number whose sevenfold the type holds, and NaN where a weight is not finite; c = W / s rounded to the nearest whole number, ties to even.
  * tfb_int4_expand: s * c rounded to the type, transposed: out (16 * strips, 64 * units), 16-byte aligned.
- * tfb_int4_split: for many rows: s * c unrounded, as the sum of two numbers of the type.  Transposed, out (16 * strips, 2 * 64 * units): in a
- * row's first half what rounding s * c leaves, in its second s * c rounded.  x_out (M, 2 * 64 * units): M rows of x (pitch x_ld, unit stride, any
- * alignment) twice, zeros behind K; the first time what is not finite is zero, because an infinity times a rest of zero would be NaN.  tfb_gemm_fused of x_out and
- * out is x W.  Both outputs 16-byte aligned.
+ * tfb_int4_split: for many rows: s * c unrounded, as the sum of two numbers of the type.  Transposed, out (16 * strips, 2 * 64 * units):
+ * in a row's first half what rounding s * c leaves, in its second s * c rounded.  x_out (M, 2 * 64 * units): M rows of x (pitch x_ld, unit
+ * stride, any alignment) twice, zeros behind K; the first time what is not finite is zero, because an infinity times a rest of zero would
+ * be NaN.  tfb_gemm_fused of x_out and out is x W.  Both outputs 16-byte aligned.
  * tfb_int4_linear: out = act(x W + bias) + addend for M rows of x (pitch x_ld, unit stride, any alignment), out and addend of pitch
  * out_ld, addend_ld; bias (N) and addend may be NULL, the addend may be the output.  For few rows: every 32 of them read the weights again.  */
 int64_t tfb_int4_codes(int64_t K, int64_t N);
@@ -434,8 +434,8 @@ int tfb_int4_linear(const void* x, int64_t x_ld, const void* codes, const void* 
  * No counterpart in the reference.  One token per row of logits (B, vocab), pitch ld, fp32, fp16 or bf16: with w_i = exp((l_i - max l) / t)
  * and the order of larger logits first, equal ones by index, kept are the first top_k (0: all), of those the ones whose predecessors
  * weigh less than top_p times the sum of the top_k, of those the ones with w_i >= min_p; out[b] is the first index j at which the sum of
- * the kept weights up to j exceeds uniforms[b] times their sum.  Weights and sums in 64 bits; what weighs less than 2^-960 of the sum counts as nothing.  A logit that is NaN counts as -infinity, all
- * +infinite ones share the weight; a row of -infinity gives -1.  temperature 0: the first of the largest.  Each setting is an array with one
+ * the kept weights up to j exceeds uniforms[b] times their sum.  Weights and sums in 64 bits; what weighs less than 2^-960 of the
+ * sum counts as nothing.  A logit that is NaN counts as -infinity, all +infinite ones share the weight; a row of -infinity gives -1.  temperature 0: the first of the largest.  Each setting is an array with one
  * value per row, or where that is NULL the number behind it; values outside their range (temperature >= 0, top_k >= 0, top_p and min_p from
  * 0 to 1, uniforms from 0 to below 1) are taken as the nearest, NaN as 0 or, for top_p, as 1.                                   */
 int tfb_sample(const void* logits, int64_t ld, const float* uniforms, const float* temperature,

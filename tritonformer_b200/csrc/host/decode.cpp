@@ -53,9 +53,10 @@ Tensor int4_expand(const Int4& w) {
   return expanded(w).narrow(0, 0, w.out).narrow(1, 0, w.in).t();
 }
 
-// Up to how many rows the products read the packed weights themselves: each 32 rows read and unpack them again, while beyond it they are unpacked once, into
-// two parts.  96 and 97 rows, which take the one way and the other: 1024 x 1024 3.9 and 8.2 us, 1024 x 4096 10.0 and 12.5, 2048 x 8192 28.6 and 27.5,
-// 1024 x 50304 56.3 and 77.4, 1536 x 6144 12.5 and 19.6; 32 rows more would add a third to the first of each pair.
+// Up to how many rows the products read the packed weights themselves: each 32 rows read and unpack them again, while beyond it
+// they are unpacked once, into two parts.  96 and 97 rows, which take the one way and the other: 1024 x 1024 3.9 and 8.2 us, 1024 x
+// 4096 10.0 and 12.5, 2048 x 8192 28.6 and 27.5, 1024 x 50304 56.3 and 77.4, 1536 x 6144 12.5 and 19.6; 32 rows more would add a
+// third to the first of each pair.
 constexpr int64_t kFewRows = 96;
 
 Tensor int4_linear(const Tensor& x, const Int4& w, const Tensor& bias, bool relu, const Tensor& addend_) {

@@ -5,17 +5,18 @@
 // operand layout of mma.sync m16n8k16: the 16 bytes that a lane loads are its share of 16 columns (along M) by 64 rows (along
 // the contraction), so that weights go from global memory to the instruction without shared memory, and 8 rows of x lie along N.
 // Products of codes are exact and their sum over a group meets the scale in 32 bits, so no weight is rounded.
-// A warp has a strip of 16 columns and a stretch of the contraction; up to 8 warps of a block share a strip where there are few, and join their
-// sums in shared memory, in their order: the result does not depend on timing.  More rows go to the tensor cores of the library's own matrix
-// product, each weight as the sum of two 16-bit numbers: nothing of it is rounded there either.
+// A warp has a strip of 16 columns and a stretch of the contraction; up to 8 warps of a block share a strip where there are few,
+// and join their sums in shared memory, in their order: the result does not depend on timing.  More rows go to the tensor cores of
+// the library's own matrix product, each weight as the sum of two 16-bit numbers: nothing of it is rounded there either.
 //
-// Measured in graphs, weights not in the L2, fp16: 1 x 1024 x 1024 1.5 us (1.7 with an addend); 1 x 4096 x 1024 4.2; 4 x 1024 x 50304 8.4 (27.7 MB,
-// 3.3 TB/s); 24 x 2048 x 8192 in groups of 32 9.2; 16 x 4096 x 12288 13.1.  No pipe is full there: for the 50304 columns and for 24 rows the counters
-// have issue slots at 52 and 33 %, the whole-number pipe, which makes codes into numbers, at 45 and 26 %, the tensor pipe at 19 and 21 %.  What is on its way is
-// little: 20 and 14 warps an SM with two units of 512 bytes and one, and the rows of x come from the L1 where they are used.
-// Two units in flight at a time for up to 8 rows and one for more, in 16 warps an SM at least, were the fastest of 1, 2 and 4 with 8 to 32 warps (4 units:
-// 11.5 us for the 50304 columns, one 11.4).  Rings in shared memory, filled by cp.async or bulk copies for a block or a warp, were slower
-// throughout (12 to 20 us for the 50304 columns).
+// Measured in graphs, weights not in the L2, fp16: 1 x 1024 x 1024 1.5 us (1.7 with an addend); 1 x 4096 x 1024 4.2; 4 x 1024 x
+// 50304 8.4 (27.7 MB, 3.3 TB/s); 24 x 2048 x 8192 in groups of 32 9.2; 16 x 4096 x 12288 13.1.  No pipe is full there: for the
+// 50304 columns and for 24 rows the counters have issue slots at 52 and 33 %, the whole-number pipe, which makes codes into
+// numbers, at 45 and 26 %, the tensor pipe at 19 and 21 %.  What is on its way is little: 20 and 14 warps an SM with two units of
+// 512 bytes and one, and the rows of x come from the L1 where they are used.
+// Two units in flight at a time for up to 8 rows and one for more, in 16 warps an SM at least, were the fastest of 1, 2 and 4 with
+// 8 to 32 warps (4 units: 11.5 us for the 50304 columns, one 11.4).  Rings in shared memory, filled by cp.async or bulk copies for
+// a block or a warp, were slower throughout (12 to 20 us for the 50304 columns).
 #include "nibbles.cuh"
 
 namespace tfb {
@@ -46,8 +47,9 @@ __device__ __forceinline__ uint4 load_x8(const uint16_t* row, int k, int K) {
   return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-// A warp: a strip of 16 columns, a stretch of its units, NT * 8 rows of x.  U units at a time: their loads are on their way together, the next
-// ones' beside the products.  Rows of x that there are none of repeat the last: a column of the product is a row of x, and theirs go nowhere.
+// A warp: a strip of 16 columns, a stretch of its units, NT * 8 rows of x.  U units at a time: their loads are on their way
+// together, the next ones' beside the products.  Rows of x that there are none of repeat the last: a column of the product is a row
+// of x, and theirs go nowhere.
 // GROUP_LOG2: 5, 6 or 7; groups of 32 are two to a unit, of 128 one for two.
 template <typename T, int NT, int GROUP_LOG2>
 __global__ void __launch_bounds__(kWarps * 32, 2) int4_linear_kernel(const Int4Params p) {
@@ -258,15 +260,17 @@ template <typename T> __device__ __forceinline__ uint32_t finite_pair(uint32_t v
 
 // W in 16 bits, transposed: out (strips * 16, units * 64), so that a lane's codes are eight neighbours.  The product of code and scale
 // is rounded to 16 bits here.
-// SPLIT: unrounded, as the sum of two 16-bit numbers, out (strips * 16, 2 * units * 64): what the rounding leaves in a row's first half, the rounded value in its
-// second.  A scale has 11 significant bits (8 in bf16) and a code three, so the rest is three bits, on the grid of the scale: exact.  The rows
-// of x, repeated likewise, then make a product in which no weight is rounded, and the smaller sums come first.  Beside the rests what is not finite in x is
-// left out: an infinity times a rest of zero would be NaN.
-// Bound by writing: rounded, 1536 x 6144 5.3 us, 1024 x 50304 22.8 (131 MB with the codes, 5.7 TB/s).  A product of 1000 rows of 1536 x 6144 with weights in
-// two parts takes 36.8 us, with rounded ones it took 22.5, and was off by 2.7e-4 of the output's norm where the output's own rounding is 2.1e-4.
+// SPLIT: unrounded, as the sum of two 16-bit numbers, out (strips * 16, 2 * units * 64): what the rounding leaves in a row's first
+// half, the rounded value in its second.  A scale has 11 significant bits (8 in bf16) and a code three, so the rest is three bits,
+// on the grid of the scale: exact.  The rows of x, repeated likewise, then make a product in which no weight is rounded, and the
+// smaller sums come first.  Beside the rests what is not finite in x is left out: an infinity times a rest of zero would be NaN.
+// Bound by writing: rounded, 1536 x 6144 5.3 us, 1024 x 50304 22.8 (131 MB with the codes, 5.7 TB/s).  A product of 1000 rows of
+// 1536 x 6144 with weights in two parts takes 36.8 us, with rounded ones it took 22.5, and was off by 2.7e-4 of the output's norm
+// where the output's own rounding is 2.1e-4.
 template <typename T, bool SMALL, bool SPLIT>
 __global__ void __launch_bounds__(256) int4_expand_kernel(const uint4* __restrict__ codes, const uint32_t* __restrict__ scales, int units,
-                                                          int groups, int group_log2, int64_t pieces, T* __restrict__ out, const TwiceParams x) {
+                                                          int groups, int group_log2, int64_t pieces, T* __restrict__ out,
+                                                          const TwiceParams x) {
   grid_dependency_wait();
   allow_dependents();
   if (SPLIT && (int)blockIdx.x < x.blocks) {
@@ -327,7 +331,8 @@ __global__ void __launch_bounds__(256) int4_expand_kernel(const uint4* __restric
 template <typename T, int NT>
 int int4_launch(Int4Params p, int group, cudaStream_t st) {
   const int64_t row_tiles = ceil_div(p.M, NT * 8);
-  // warps of a strip: as many as there are SMs for (12 warps each; with 24 the 50304 columns take 9.8 us instead of 8.5), with a unit each at least
+  // warps of a strip: as many as there are SMs for (12 warps each; with 24 the 50304 columns take 9.8 us instead of 8.5), with a
+  // unit each at least
   p.parts_log2 = 0;
   while (p.parts_log2 < 3 && (2 << p.parts_log2) <= p.units && ((int64_t)p.strips * row_tiles << p.parts_log2) < sm_count() * 12) ++p.parts_log2;
   const dim3 grid((unsigned)ceil_div(p.strips, kWarps >> p.parts_log2), (unsigned)row_tiles);
@@ -357,8 +362,8 @@ int int4_expand_launch(const void* codes, const void* scales, int64_t K, int64_t
   const int64_t most = (int64_t)sm_count() * 16, blocks = ceil_div(pieces, 8);
   const int log2 = group == 32 ? 5 : group == 64 ? 6 : 7;
   launch_overlapped(group == 32 ? int4_expand_kernel<T, true, SPLIT> : int4_expand_kernel<T, false, SPLIT>,
-                    dim3((unsigned)((blocks < most ? blocks : most) + x.blocks)), dim3(256), 0, st, (const uint4*)codes, (const uint32_t*)scales,
-                    (int)units, (int)int4_groups(K, group), log2, pieces, (T*)out, x);
+                    dim3((unsigned)((blocks < most ? blocks : most) + x.blocks)), dim3(256), 0, st, (const uint4*)codes,
+                    (const uint32_t*)scales, (int)units, (int)int4_groups(K, group), log2, pieces, (T*)out, x);
   return launched("int4_expand");
 }
 
@@ -388,16 +393,18 @@ extern "C" int tfb_int4_quantize(const void* w, int64_t w_k, int64_t w_n, int64_
 
 extern "C" int tfb_int4_expand(const void* codes, const void* scales, int64_t K, int64_t N, int group, void* out, int dtype, void* stream) {
   if (int rc = check_int4("int4_expand", K, N, group)) return rc;
-  TFB_REQUIRE(codes && scales && out && aligned16(codes) && aligned16(scales) && aligned16(out), "int4_expand: the buffers are not 16-byte aligned");
+  TFB_REQUIRE(codes && scales && out && aligned16(codes) && aligned16(scales) && aligned16(out),
+              "int4_expand: the buffers are not 16-byte aligned");
   TFB_DISPATCH_16(dtype, T, { return int4_expand_launch<T, false>(codes, scales, K, N, group, out, TwiceParams{}, (cudaStream_t)stream); })
 }
 
-extern "C" int tfb_int4_split(const void* codes, const void* scales, int64_t K, int64_t N, int group, void* out, const void* x, int64_t x_ld,
-                              int64_t M, void* x_out, int dtype, void* stream) {
+extern "C" int tfb_int4_split(const void* codes, const void* scales, int64_t K, int64_t N, int group, void* out, const void* x,
+                              int64_t x_ld, int64_t M, void* x_out, int dtype, void* stream) {
   if (int rc = check_int4("int4_split", K, N, group)) return rc;
   TFB_REQUIRE(M >= 0 && M < (1LL << 31), "int4_split: bad row count");
   TFB_REQUIRE(M <= 1 || (x_ld >= 0 && x_ld < (1LL << 40)), "int4_split: bad row stride");
-  TFB_REQUIRE(codes && scales && out && aligned16(codes) && aligned16(scales) && aligned16(out), "int4_split: the buffers are not 16-byte aligned");
+  TFB_REQUIRE(codes && scales && out && aligned16(codes) && aligned16(scales) && aligned16(out),
+              "int4_split: the buffers are not 16-byte aligned");
   TFB_REQUIRE(M == 0 || (x && x_out && aligned16(x_out)), "int4_split: the buffers are not 16-byte aligned");
   TwiceParams p = {};
   p.x = x;

@@ -35,8 +35,9 @@ __device__ __forceinline__ uint32_t masked_or(uint32_t v, uint32_t mask, uint32_
   return r;
 }
 
-// The eight codes of a word as exact 16-bit numbers: a[i] holds nibbles i and i + 4.  A nibble below the exponent of a power of two is that power
-// plus it (1024 in fp16; 128 in bf16, whose seven bits have no room for a nibble four places up); what is added comes off again.
+// The eight codes of a word as exact 16-bit numbers: a[i] holds nibbles i and i + 4.  A nibble below the exponent of a power of two
+// is that power plus it (1024 in fp16; 128 in bf16, whose seven bits have no room for a nibble four places up); what is added comes
+// off again.
 template <typename T> __device__ __forceinline__ void expand_nibbles(uint32_t w, uint32_t (&a)[4]);
 template <> __device__ __forceinline__ void expand_nibbles<__half>(uint32_t w, uint32_t (&a)[4]) {
   const __half2 off = __float2half2_rn(-1032.f), sixteenth = __float2half2_rn(0.0625f), off16 = __float2half2_rn(-72.f);
@@ -77,11 +78,12 @@ __device__ __forceinline__ int code_of(float x, float scale) {
   return scale > 0.f ? max(-7, min(7, __float2int_rn(__fdiv_rn(x, scale)))) : 0;
 }
 
-// A row of a cache in 4 bits: LANES lanes in a line have 8 neighbouring values each.  Returns a lane's word, dim 2 n + e at bits 4 n + 16 e;
-// `whole` are its codes.  The same codes and scales as above, without a division (16 sequences of up to 4096 keys, 8 heads of 128, with what
-// is stored: 179 us with divisions, 84 so).  With values and scales of 11 significant bits, top / 7 is no nearer than 2^-15 (relative) to the border
-// between two scales, and a quotient is either half-way between two whole numbers or at least 2^-12 away from that: products with
-// reciprocals, 2^-19 off, round to the same, once what is nearer than 2^-14 to a half has been made one.
+// A row of a cache in 4 bits: LANES lanes in a line have 8 neighbouring values each.  Returns a lane's word, dim 2 n + e at bits 4
+// n + 16 e; `whole` are its codes.  The same codes and scales as above, without a division (16 sequences of up to 4096 keys, 8
+// heads of 128, with what is stored: 179 us with divisions, 84 so).  With values and scales of 11 significant bits, top / 7 is no
+// nearer than 2^-15 (relative) to the border between two scales, and a quotient is either half-way between two whole numbers or at
+// least 2^-12 away from that: products with reciprocals, 2^-19 off, round to the same, once what is nearer than 2^-14 to a half has
+// been made one.
 template <typename T, int LANES>
 __device__ __forceinline__ uint32_t quantize8(const uint4& v, T& scale, float (&whole)[8]) {
   constexpr float kGrid = 1.5f * (1 << 10), kWhole = 1.5f * (1 << 23);  // adding them rounds to multiples of 2^-13, and of 1

@@ -5,8 +5,9 @@
 // largest magnitude three to four shuffles away, and a lane's 8 codes are one word of the row.  On request the values that the cache now
 // stands for are written out beside it, so that a prompt's own attention can use what later tokens will find.
 //
-// Measured: 16 sequences of up to 4096 keys, 8 heads of 128, bf16, with what is stored, 84 us, 5.2 TB/s (79% of a copy); 24 warps an SM instead of 32
-// took 90, divisions instead of products 179.  One token: 4.7 us in a graph, the chain of length, table, row and scale.
+// Measured: 16 sequences of up to 4096 keys, 8 heads of 128, bf16, with what is stored, 84 us, 5.2 TB/s (79% of a copy); 24 warps
+// an SM instead of 32 took 90, divisions instead of products 179.  One token: 4.7 us in a graph, the chain of length, table, row
+// and scale.
 #include "nibbles.cuh"
 #include "paged.cuh"
 

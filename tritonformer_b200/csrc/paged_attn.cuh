@@ -45,8 +45,8 @@ constexpr float kNone = -INFINITY;
 
 // G: query heads that a warp takes at once, 4, 8 or 16.  Q4: pages in 4 bits.
 template <int HD, int G, int BIAS, bool Q4> struct PgCfg {
-  // In 4 bits a warp's time is that of making 16-bit numbers, and a third warp for each scheduler fills its waits: one user 9.6 -> 8.3 us, 24 sequences of
-  // up to 2048 keys 22.1 -> 20.6, long ones the same; 16 warps' registers do not hold a tile's work.
+  // In 4 bits a warp's time is that of making 16-bit numbers, and a third warp for each scheduler fills its waits: one user 9.6
+  // -> 8.3 us, 24 sequences of up to 2048 keys 22.1 -> 20.6, long ones the same; 16 warps' registers do not hold a tile's work.
   static constexpr int WARPS = Q4 ? 12 : 8;
   static constexpr int NT = G == 16 ? 2 : 1;   // blocks of 8 columns in the products
   static constexpr int KEYS = Q4 ? 64 : 2048 / HD;  // keys of a tile
@@ -674,14 +674,14 @@ __global__ void __launch_bounds__(PgCfg<HD, G, BIAS, Q4>::WARPS * 32, 1)
           }
       } else {
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-        for (int m = 0; m < C::MT; ++m) {
-          uint32_t a[4];
-          ldm4(a, tile + (k_at ^ ((ks % PER_PANEL) << 5)) + (ks / PER_PANEL) * PANEL + m * BLOCK16);
+          for (int m = 0; m < C::MT; ++m) {
+            uint32_t a[4];
+            ldm4(a, tile + (k_at ^ ((ks % PER_PANEL) << 5)) + (ks / PER_PANEL) * PANEL + m * BLOCK16);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma<T>(s[m][nt], a, now.q[nt][ks][0], now.q[nt][ks][1]);
-        }
+            for (int nt = 0; nt < NT; ++nt) mma<T>(s[m][nt], a, now.q[nt][ks][0], now.q[nt][ks][1]);
+          }
       }
       float top[NT][2];
 #pragma unroll
@@ -820,15 +820,15 @@ __global__ void __launch_bounds__(PgCfg<HD, G, BIAS, Q4>::WARPS * 32, 1)
           }
       } else {
 #pragma unroll
-      for (int m = 0; m < C::MT; ++m)
+        for (int m = 0; m < C::MT; ++m)
 #pragma unroll
-        for (int hm = 0; hm < KS; ++hm) {
-          uint32_t a[4];
-          ldm4t(a, tile + (v_at ^ ((hm % PER_PANEL) << 5)) + (hm / PER_PANEL) * PANEL + m * BLOCK16);
+          for (int hm = 0; hm < KS; ++hm) {
+            uint32_t a[4];
+            ldm4t(a, tile + (v_at ^ ((hm % PER_PANEL) << 5)) + (hm / PER_PANEL) * PANEL + m * BLOCK16);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma<T>(o[hm][nt], a, pt[m][nt][0], pt[m][nt][1]);
-          if (APART) mma<T>(o_rest[hm], a, rt[m][0][0], rt[m][0][1]);
-        }
+            for (int nt = 0; nt < NT; ++nt) mma<T>(o[hm][nt], a, pt[m][nt][0], pt[m][nt][1]);
+            if (APART) mma<T>(o_rest[hm], a, rt[m][0][0], rt[m][0][1]);
+          }
       }
       if (!APART && !FINE && !Q4) {
         // The rests' products on top, unless a value is infinite: a rest of zero or below would make NaN of that.

@@ -9,13 +9,14 @@
 // ldmatrix as a lane's share of the instruction: for the keys 8 dims of a key, for the values (transposed as 16-bit units) 4 dims of two
 // neighbouring keys, which is the pair that the second product wants.  Tiles come by cp.async: a row is 16 to 64 bytes.
 //
-// What bounds it is no longer the reading but the instructions: 390 for 16 keys of 128 dims and 8 columns of queries, half of them to make
-// codes into numbers, issue slots 58% and the whole-number pipe 54% in use over a launch that lacks a tenth at both ends; the copies and the
-// softmax alone take 57 us of the 92 below.  Measured in graphs, in brackets the 16-bit cache: bf16, head_dim 128, 32 sequences of up to 16384 keys,
-// 8 key heads of 4 query heads 92 us (169); fp16, head_dim 64, 24 sequences of up to 2048 keys, 16 heads, slopes 20.4 (25.9); one
-// of 700 keys 8.3 (9.3).  With the new token's row quantized
-// and written, as a generation step calls it, on the same inputs each time: 85.8 us for 85.5 without, 20.2 for 19.6, 9.3 for 8.4.  Not kept for the long ones: two blocks an SM (113 us, registers spilled), tiles of 32 keys (95 to 109), TMA
-// boxes for the copies (95), 8 warps with three tiles ahead (93, the short ones 9.6 and 22.1).
+// What bounds it is no longer the reading but the instructions: 390 for 16 keys of 128 dims and 8 columns of queries, half of them
+// to make codes into numbers, issue slots 58% and the whole-number pipe 54% in use over a launch that lacks a tenth at both ends;
+// the copies and the softmax alone take 57 us of the 92 below.  Measured in graphs, in brackets the 16-bit cache: bf16, head_dim
+// 128, 32 sequences of up to 16384 keys, 8 key heads of 4 query heads 92 us (169); fp16, head_dim 64, 24 sequences of up to 2048
+// keys, 16 heads, slopes 20.4 (25.9); one of 700 keys 8.3 (9.3).  With the new token's row quantized and written, as a generation
+// step calls it, on the same inputs each time: 85.8 us for 85.5 without, 20.2 for 19.6, 9.3 for 8.4.  Not kept for the long ones:
+// two blocks an SM (113 us, registers spilled), tiles of 32 keys (95 to 109), TMA boxes for the copies (95), 8 warps with three
+// tiles ahead (93, the short ones 9.6 and 22.1).
 #include "paged_attn.cuh"
 
 namespace tfb {

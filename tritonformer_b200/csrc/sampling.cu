@@ -4,20 +4,21 @@
 //   first whose predecessors weigh less than p times the sum, of those the ones with w_i >= m;
 //   token = the first index j with  sum of the kept w_i, i <= j,  >  u * sum of the kept w_i.
 //
-// What is kept is a beginning of the order, so it is all logits above a value and some of those equal to it: that cut is what is looked for, and
-// nothing is sorted.  All sums are in 64 bits, weights to some 2^-39, the largest exactly 1: a token is the drawn one or it is not, and where a sum meets the
-// border between two of 50 thousand tokens, 32 bits would now and then give the neighbour.  Sums are taken in a fixed order: the same call gives the same
-// token.
+// What is kept is a beginning of the order, so it is all logits above a value and some of those equal to it: that cut is what is
+// looked for, and nothing is sorted.  All sums are in 64 bits, weights to some 2^-39, the largest exactly 1: a token is the drawn
+// one or it is not, and where a sum meets the border between two of 50 thousand tokens, 32 bits would now and then give the
+// neighbour.  Sums are taken in a fixed order: the same call gives the same token.
 //
-// A block or a cluster of blocks has a row; blocks, warps and lanes hold it in the order of its columns, so that the last sums, by warps, say which
-// warp has the token.  The cut comes from a list of candidates that are all compared (few of the largest, or of the heaviest), from a histogram over
-// all values (16 bits), or from a search (32 bits), below.
+// A block or a cluster of blocks has a row; blocks, warps and lanes hold it in the order of its columns, so that the last sums, by
+// warps, say which warp has the token.  The cut comes from a list of candidates that are all compared (few of the largest, or of
+// the heaviest), from a histogram over all values (16 bits), or from a search (32 bits), below.
 //
-// Reading the logits is the least of it (13 MB for 128 rows of 50304: 2 us), and no pipe is full: over rows with settings of their own issue slots are in
-// use 47 %, the whole-number pipe 30 %, the 64-bit one 8 %.  A call is a chain of steps with a barrier of the block or the cluster behind each.  Some are
-// one warp's, while the others wait or have gone (the search for min_p's border, the walk through the owner's logits); where many logits are kept
-// each has its exponential once more in the sums by warp, although the histogram has their total.  Measured in graphs, fp16 logits: one row of 50304, top_k 40 and
-// top_p 0.95, 14.6 us; 128 rows of 50304, temperature alone 28, top_k 40 15, min_p 0.05 18, top_p 0.9 48; bf16, 16 rows of 131071, top_p 0.9 35.
+// Reading the logits is the least of it (13 MB for 128 rows of 50304: 2 us), and no pipe is full: over rows with settings of their
+// own issue slots are in use 47 %, the whole-number pipe 30 %, the 64-bit one 8 %.  A call is a chain of steps with a barrier of
+// the block or the cluster behind each.  Some are one warp's, while the others wait or have gone (the search for min_p's border,
+// the walk through the owner's logits); where many logits are kept each has its exponential once more in the sums by warp, although
+// the histogram has their total.  Measured in graphs, fp16 logits: one row of 50304, top_k 40 and top_p 0.95, 14.6 us; 128 rows of
+// 50304, temperature alone 28, top_k 40 15, min_p 0.05 18, top_p 0.9 48; bf16, 16 rows of 131071, top_p 0.9 35.
 // fp32: 8 rows of 32000, temperature alone 14, top_k 40 31, top_p 0.9 59.
 #include <cfloat>
 #include <cooperative_groups.h>
@@ -31,8 +32,8 @@ namespace cg = cooperative_groups;
 constexpr int SM_WARPS = 16, SM_THREADS = SM_WARPS * 32, SM_CLUSTER = 8;
 constexpr int SM_CUTS = 8;  // values that a round looks at
 constexpr double kLog2eD = 1.4426950408889634074;
-// The smallest share of the sum that is looked for.  Logits far below the largest weigh some 2^-981 here where 64 bits have nothing, and not even a
-// uniform number of zero may draw them: 2^19 of them stay below this.
+// The smallest share of the sum that is looked for.  Logits far below the largest weigh some 2^-981 here where 64 bits have
+// nothing, and not even a uniform number of zero may draw them: 2^19 of them stay below this.
 constexpr double kLeastShare = 0x1p-960;
 
 struct SampleParams {
@@ -101,8 +102,8 @@ struct Shared {
 }  // namespace
 
 // ---------------------------------------------------------------------------------------------------------- 32 bits
-// The search: a round takes the count and weight above 8 values at once and goes on in the ninth part that holds the border, in steps of value and of
-// representation in turn.  The row lies in the cluster's shared memory.
+// The search: a round takes the count and weight above 8 values at once and goes on in the ninth part that holds the border, in
+// steps of value and of representation in turn.  The row lies in the cluster's shared memory.
 __global__ void __launch_bounds__(SM_THREADS) sample_search_kernel(const SampleParams p) {
   constexpr int W = 4;
   extern __shared__ uint4 units[];
@@ -517,20 +518,23 @@ __global__ void __launch_bounds__(SM_THREADS) sample_search_kernel(const SampleP
 }
 
 // ---------------------------------------------------------------------------------------------------------- 16 bits
-// Few candidates.  The k-th largest of the threads' largest logits is not above the k-th largest logit, so what lies below it is out; the same holds for
-// each block of a cluster.  What is left, some more than k from each block, is put in a list; up to 256 of them are compared each with each,
-// which gives ranks and the weight ahead of each at once (one row, top_k 40: 20 us by the histogram, 14.6 so).
+// Few candidates.  The k-th largest of the threads' largest logits is not above the k-th largest logit, so what lies below it is
+// out; the same holds for each block of a cluster.  What is left, some more than k from each block, is put in a list; up to 256 of
+// them are compared each with each, which gives ranks and the weight ahead of each at once (one row, top_k 40: 20 us by the
+// histogram, 14.6 so).
 //
-// Logits of 16 bits have 2^16 values, and equal logits weigh the same: a histogram over all values is all that the cut needs.  Blocks count their
-// part of the row (a counter of 16 bits for each value, 128 KB of shared memory), the blocks of a cluster add theirs up where there is
-// something to add, and a scan over rows of 64 values gives the cut, with an exponential for each value that occurs instead of each logit.
+// Logits of 16 bits have 2^16 values, and equal logits weigh the same: a histogram over all values is all that the cut needs.
+// Blocks count their part of the row (a counter of 16 bits for each value, 128 KB of shared memory), the blocks of a cluster add
+// theirs up where there is something to add, and a scan over rows of 64 values gives the cut, with an exponential for each value
+// that occurs instead of each logit.
 // Then the weights of what is kept are summed in the order of the columns.
 namespace {
 
 constexpr int H_THREADS = 1024, H_WARPS = 32, H_ROWS = 1024;  // rows of 64 values, two to a word
 constexpr int H_UNITS = 8;                                    // 16-byte units of a lane
 constexpr int H_FEW = 256;                                    // logits that are compared each with each
-// Logits of a block, at most: with one unit of a lane less than there is room for no block of a cluster has 2^16, which a counter does not hold.
+// Logits of a block, at most: with one unit of a lane less than there is room for no block of a cluster has 2^16, which a counter
+// does not hold.
 constexpr int kMostCounted = H_WARPS * (H_UNITS * 32 - 1) * 8 - 8;
 
 // Values in descending order: bin 0 is the last positive NaN, then infinity, .., the lowest, -infinity and the negative NaNs.
@@ -675,10 +679,10 @@ __global__ void __launch_bounds__(H_THREADS, 1) sample_hist_kernel(const SampleP
   };
   const int top_bin = bin_of(top);
 
-  // Weights from the difference to the top logit, which is exact in 64 bits: the top one weighs exactly 1, so that sums of equal logits are whole numbers and
-  // a border that they meet exactly is met.  (128 rows of 50304 with settings of their own take 45.4 us; 45.7 with weights from the logit itself, one
-  // sum less each, whose rounding put one token too many into a nucleus of equal logits.)  In the other form where the top logit is infinite, or 32 bits
-  // do not tell `lowest` from it.
+  // Weights from the difference to the top logit, which is exact in 64 bits: the top one weighs exactly 1, so that sums of equal
+  // logits are whole numbers and a border that they meet exactly is met.  (128 rows of 50304 with settings of their own take 45.4
+  // us; 45.7 with weights from the logit itself, one sum less each, whose rounding put one token too many into a nucleus of equal
+  // logits.)  In the other form where the top logit is infinite, or 32 bits do not tell `lowest` from it.
   const double per = kLog2eD / (double)t, per32 = per * 32.0, peak = (double)top;
   constexpr double kMagic = 6755399441055744.0;  // as in weight_of
   const bool near_by = fabs(peak * per32) < 16384.0;
@@ -1299,9 +1303,9 @@ template <typename T>
 int sample_by_histogram(SampleParams p, int64_t B, cudaStream_t st) {
   const int64_t row_units = ceil_div((int64_t)p.vocab + 7, 8);
   int blocks = 1;
-  // blocks of a row: what their counters hold, and up to four where they find half of the SMs free (16 rows of 131071: 22 to 34 us with 2 or 4
-  // blocks; with 8, whose clusters do not all find room at once, 28 to 51.  One row of 50304, top_k 40: 15.5 us with 4 blocks, 22 with 8, whose
-  // own 40 largest are too many together for the list)
+  // blocks of a row: what their counters hold, and up to four where they find half of the SMs free (16 rows of 131071: 22 to 34
+  // us with 2 or 4 blocks; with 8, whose clusters do not all find room at once, 28 to 51.  One row of 50304, top_k 40: 14.6 us
+  // with 4 blocks, 22 with 8, whose own 40 largest are too many together for the list)
   while (blocks < SM_CLUSTER && ((int64_t)p.vocab > (int64_t)kMostCounted * blocks ||
                                  (blocks < 4 && B * blocks * 4 <= sm_count() && row_units > H_THREADS / 2 * blocks)))
     blocks *= 2;
